@@ -84,10 +84,9 @@ __device__ __forceinline__ float gelu_fast(float x) {
 
 typedef __bf16 bf16x2e __attribute__((ext_vector_type(2)));
 typedef float f32x2e __attribute__((ext_vector_type(2)));
-// gelu_fast on two values with packed math (v_pk_fma_f32 / v_pk_mul_f32 take both lanes of a
-// pair per instruction): 20 instructions per pair instead of ~30 -- the FFN1 epilogue's GELU
-// was all of its non-MFMA VALU (PMC: 5.4 VALU per MFMA, i.e. VALU-issue-bound).  The same
-// A-S 7.1.26 formula; only the operation grouping differs from gelu_fast.
+// gelu_fast on two values (built without packed FP32 instructions: two scalar streams that the
+// compiler interleaves).  The same A-S 7.1.26 formula; only the operation grouping differs from
+// gelu_fast.
 __device__ __forceinline__ f32x2e gelu2_fast(f32x2e x) {
   const f32x2e one = {1.0f, 1.0f};
   const f32x2e z = __builtin_elementwise_abs(x) * 0.70710678118654752f;
