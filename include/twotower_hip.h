@@ -607,6 +607,35 @@ int tt_convert_batch(const tt_convert_job* jobs, int32_t njobs, void* stream);
 int tt_adam_f32(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
                 float beta2, float eps, int32_t step, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Gated linear recurrence over event histories (tt_recur.hip): the order-aware aggregation of
+ * the buyer tower (BuyerTower(aggregation_method="recurrent")).
+ *   A_t = sigmoid(gate_t)^(w_t) ;  h_t = A_t h_{t-1} + (1 - A_t) x_t ;  h_{-1} = h0 (NULL: 0)
+ * x, gate [B, S, D] of dtype (f32 or bf16), channels contiguous, histories x_sb / g_sb and events
+ * x_ss / g_ss elements apart; w [B, S] f32 (rows w_sb apart; NULL: all 1).  A weight that is not
+ * above 0 marks padding: the state passes unchanged whatever x and gate hold there, and the
+ * gradients there are 0.  h [B, S, D] of dtype (NULL: not wanted), h_last [B, D] f32 (may be h0
+ * itself when S <= 1).  ckpt [B, ceil(S / TT_SCAN_CKPT), D] f32 (NULL: no backward pass follows):
+ * the state before every TT_SCAN_CKPT-th event, which tt_gated_scan_bwd takes.
+ * dh [B, S, D] of dtype and dh_last [B, D] f32 (either may be NULL: zero) -> dx, dgate [B, S, D]
+ * of dtype, dh0 [B, D] f32 (may be NULL); all contiguous.  States and gradients are carried in
+ * f32 and rounded once on output.  S = 0: h_last = h0, dh0 = dh_last.
+ * Workspace: tt_gated_scan_workspace_bytes (0 for all but few long histories).
+ * --------------------------------------------------------------------------------- */
+#define TT_DTYPE_F32 0
+#define TT_DTYPE_BF16 1
+#define TT_SCAN_CKPT 16
+int tt_gated_scan_workspace_bytes(int64_t B, int64_t S, int32_t D, int64_t* bytes);
+int tt_gated_scan_fwd(const void* x, const void* gate, int32_t dtype, int64_t B, int64_t S,
+                      int32_t D, int64_t x_sb, int64_t x_ss, int64_t g_sb, int64_t g_ss,
+                      const float* w, int64_t w_sb, const float* h0, void* h, float* h_last,
+                      float* ckpt, void* workspace, int64_t workspace_bytes, void* stream);
+int tt_gated_scan_bwd(const void* x, const void* gate, int32_t dtype, int64_t B, int64_t S,
+                      int32_t D, int64_t x_sb, int64_t x_ss, int64_t g_sb, int64_t g_ss,
+                      const float* w, int64_t w_sb, const float* ckpt, const void* dh,
+                      const float* dh_last, void* dx, void* dgate, float* dh0, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

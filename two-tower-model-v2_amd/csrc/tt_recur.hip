@@ -1,0 +1,653 @@
+// tt_recur.hip -- gated linear recurrence over event histories (gfx950).
+//
+//   A_t = sigmoid(g_t)^(w_t) = exp(-w_t softplus(-g_t))      (w absent: 1)
+//   h_t = A_t h_{t-1} + (1 - A_t) x_t                        (h_{-1} = h0, or 0)
+//
+// An event of weight w moves the state exactly as w equal events of weight 1 do.  An event whose
+// weight is not above 0 (padding; also NaN) leaves the state as it is, bit for bit, whatever its
+// x and g hold, and gets zero gradients.
+//
+// Backward, with R the gradient that reaches h_t from later events:
+//   G_t = dh_t + R ;  dx_t = (1 - A_t) G_t ;  dg_t = w_t A_t sigmoid(-g_t) (h_{t-1} - x_t) G_t
+//   R <- A_t G_t   (after event 0: the gradient of h0)
+// The state is needed in 32 bits there, so the forward pass saves it (f32) before every 16th
+// event, 1/16 of one f32 tensor, and the backward pass recomputes the 16 states between in
+// registers: cheaper to read than h itself (0.25 instead of 2 or 4 bytes an element) and the
+// rounding of h to bf16 does not reach the gradients.
+//
+// Bound: HBM.  Forward 3 tensors (x, gate, h), backward 5 (x, gate, dh, dx, dgate).  A lane owns
+// VEC neighbouring channels of one history and walks the events; a wave's unit is (history, 64
+// VEC channels, chunk of events).  The histories' own count fills the card in training batches
+// (one chunk: every tensor is read once).  Few long histories are split along the events: a
+// first launch reduces every chunk to (product of A, state reached from 0), a second joins the
+// chunks, the third runs the chunks from their true start states.  The split pass reads x and
+// gate twice (from the 256 MB last-level cache where they fit).
+#include "tt_common.hpp"
+
+namespace tt {
+
+constexpr int RC_CK = 16;   // events between saved states
+constexpr int RC_U = 8;     // events whose rows are loaded together (forward)
+constexpr int RC_SEG = 16;  // segments of the chunk join
+
+struct ScanArgs {
+  const void *x, *gate;
+  const float *w, *h0;      // w [B, S] rows wsb apart; h0 [B, D]; either may be null
+  void* h;                  // [B, S, D] or null
+  float *h_last, *ck;       // [B, D]; [B, ceil(S / 16), D] or null
+  const void* dh;           // backward: [B, S, D] or null
+  const float* dlast;       // [B, D] or null
+  void *dx, *dgate;
+  float* dh0;
+  int64_t B, S, xsb, xss, gsb, gss, wsb;
+  int D, nw, C;             // waves per row, chunks per history
+  int64_t T;                // events per chunk (a multiple of 16 unless C == 1)
+  float *sumA, *sumH, *carry;  // [B, C, D] each (C > 1)
+};
+
+template <typename T, int VEC>
+struct Pack;
+template <>
+struct Pack<float, 1> { typedef float type; };
+template <>
+struct Pack<float, 2> { typedef float type __attribute__((ext_vector_type(2))); };
+template <>
+struct Pack<float, 4> { typedef float type __attribute__((ext_vector_type(4))); };
+template <>
+struct Pack<uint16_t, 1> { typedef uint16_t type; };
+template <>
+struct Pack<uint16_t, 2> { typedef uint32_t type; };
+template <>
+struct Pack<uint16_t, 4> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
+
+__device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(typename Pack<T, VEC>::type p, float (&o)[VEC]) {
+  if constexpr (std::is_same<T, float>::value) {
+    if constexpr (VEC == 1) {
+      o[0] = p;
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] = p[i];
+    }
+  } else if constexpr (VEC == 1) {
+    o[0] = bf_lo(p);
+  } else if constexpr (VEC == 2) {
+    o[0] = bf_lo(p);
+    o[1] = bf_hi(p);
+  } else {
+    o[0] = bf_lo(p[0]);
+    o[1] = bf_hi(p[0]);
+    o[2] = bf_lo(p[1]);
+    o[3] = bf_hi(p[1]);
+  }
+}
+typedef __bf16 rc_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float rc_f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t rc_pack2(float a, float b) {  // round to nearest even
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(rc_f32x2{a, b}, rc_bf16x2));
+}
+template <typename T, int VEC>
+__device__ __forceinline__ typename Pack<T, VEC>::type pack(const float (&v)[VEC]) {
+  typename Pack<T, VEC>::type p;
+  if constexpr (std::is_same<T, float>::value) {
+    if constexpr (VEC == 1) {
+      p = v[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) p[i] = v[i];
+    }
+  } else if constexpr (VEC == 1) {
+    p = (uint16_t)rc_pack2(v[0], 0.0f);
+  } else if constexpr (VEC == 2) {
+    p = rc_pack2(v[0], v[1]);
+  } else {
+    p[0] = rc_pack2(v[0], v[1]);
+    p[1] = rc_pack2(v[2], v[3]);
+  }
+  return p;
+}
+
+// exp(-|g|) to about 1 ulp: the product |g| log2(e) in two parts, the low one (< 2^-20) applied
+// to first order.
+__device__ __forceinline__ float exp_neg_abs(float g) {
+  const float n = -fabsf(g);
+  const float hi = n * 1.44269504f;
+  const float lo = fmaf(n, 1.44269504f, -hi) + n * 1.92596299e-8f;  // log2(e) - f32(log2(e))
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return hi < -150.0f ? 0.0f : fmaf(e, lo * 0.693147181f, e);
+}
+// e = exp(-|g|), r = 1 / (1 + e): sigmoid(|g|) = r and sigmoid(-|g|) = e r, neither by a
+// difference, so 1 - A keeps its relative precision for long memories (A next to 1).
+struct Gate {
+  float a, na;  // A, 1 - A
+  float sn;     // sigmoid(-g)
+  bool hi;      // A is nearer 1 than 0
+};
+// A s and A h + (1 - A) x.  Near 1 the part that leaves is computed from 1 - A: a rounded A would
+// be off 1 - (1 - A) by up to 2^-25, which a memory of 1 / (1 - A) events multiplies.
+__device__ __forceinline__ float decay(const Gate& q, float s) {
+  return q.hi ? fmaf(-q.na, s, s) : q.a * s;
+}
+__device__ __forceinline__ float move(const Gate& q, float h, float x) {
+  return q.hi ? fmaf(q.na, x - h, h) : fmaf(q.a, h, q.na * x);
+}
+__device__ __forceinline__ Gate gate_one(float g) {
+  const float e = exp_neg_abs(g);
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
+  const float er = e * r;
+  Gate o;
+  o.hi = g >= 0.0f;
+  o.a = o.hi ? r : er;
+  o.na = o.hi ? er : r;
+  o.sn = o.na;
+  return o;
+}
+// A = exp(-w softplus(-g)).  softplus(-g) = max(-g, 0) + log1p(e), log1p(e) = 2 atanh(e / (2 +
+// e)) by its odd series (argument <= 1/3: terms to z^15); expm1 by its series below 0.35, by the
+// difference from 1 above (relative error < 2^-22 either way).
+__device__ __forceinline__ Gate gate_pow(float g, float w) {
+  const float e = exp_neg_abs(g);
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
+  const float z = e * __builtin_amdgcn_rcpf(2.0f + e), z2 = z * z;
+  float s = fmaf(z2, 1.0f / 15.0f, 1.0f / 13.0f);
+  s = fmaf(s, z2, 1.0f / 11.0f);
+  s = fmaf(s, z2, 1.0f / 9.0f);
+  s = fmaf(s, z2, 1.0f / 7.0f);
+  s = fmaf(s, z2, 0.2f);
+  s = fmaf(s, z2, 1.0f / 3.0f);
+  s = fmaf(s, z2, 1.0f);
+  const float sp = fmaxf(-g, 0.0f) + 2.0f * z * s;
+  const float y = sp * w;  // A = exp(-y)
+  float q = fmaf(y, -1.0f / 40320.0f, 1.0f / 5040.0f);  // (1 - exp(-y)) / y
+  q = fmaf(q, y, -1.0f / 720.0f);
+  q = fmaf(q, y, 1.0f / 120.0f);
+  q = fmaf(q, y, -1.0f / 24.0f);
+  q = fmaf(q, y, 1.0f / 6.0f);
+  q = fmaf(q, y, -0.5f);
+  q = fmaf(q, y, 1.0f);
+  const float nsmall = q * y;
+  const float big = exp_neg_abs(y);
+  Gate o;
+  o.hi = y < 0.35f;
+  o.a = o.hi ? 1.0f - nsmall : big;
+  o.na = o.hi ? nsmall : 1.0f - big;
+  o.sn = g >= 0.0f ? e * r : r;
+  return o;
+}
+
+// unit = ((b * C) + c) * nw + wave-of-row; uniform over the wave
+struct Unit {
+  int64_t b;
+  int c, ch;  // chunk, first channel of this lane
+};
+template <int VEC>
+__device__ __forceinline__ Unit unit_of(const ScanArgs& a, int64_t u, int lane) {
+  Unit o;
+  const int64_t bc = u / a.nw;
+  o.ch = ((int)(u - bc * a.nw) * 64 + lane) * VEC;
+  o.b = bc / a.C;
+  o.c = (int)(bc - o.b * a.C);
+  return o;
+}
+
+// One event for VEC channels; w uniform.
+template <bool WT, int VEC, typename F>
+__device__ __forceinline__ void with_gate(float w, const float (&g)[VEC], F&& f) {
+  if constexpr (!WT) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f(i, gate_one(g[i]));
+  } else {
+    if (!(w > 0.0f)) return;
+    if (w == 1.0f) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f(i, gate_one(g[i]));
+    } else {
+      const float wc = fminf(w, 3.0e38f);  // an infinite weight: the state becomes x
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f(i, gate_pow(g[i], wc));
+    }
+  }
+}
+
+// SUM: the chunk's (product of A, state from 0) only.  Else the chunk from its start state, with
+// h, h_last and the saved states as asked for.
+template <typename T, int VEC, bool WT, bool SUM>
+__global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
+  typedef typename Pack<T, VEC>::type P;
+  const int lane = threadIdx.x & 63;
+  const int64_t nunits = a.B * a.C * a.nw;
+  const int64_t nck = (a.S + RC_CK - 1) / RC_CK;
+  for (int64_t u0 = (int64_t)blockIdx.x * 4; u0 < nunits; u0 += (int64_t)gridDim.x * 4) {
+    const int64_t uu = u0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (uu >= nunits) break;
+    const Unit un = unit_of<VEC>(a, uu, lane);
+    if (SUM && un.c == a.C - 1) continue;  // the last chunk starts nothing
+    if (un.ch >= a.D) continue;
+    const int64_t t0 = (int64_t)un.c * a.T, t1 = t0 + a.T < a.S ? t0 + a.T : a.S;
+    const T* xp = (const T*)a.x + un.b * a.xsb + un.ch;
+    const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
+    const float* wp = WT ? a.w + un.b * a.wsb : nullptr;
+    float h[VEC], pa[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      pa[i] = 1.0f;
+      h[i] = SUM ? 0.0f
+             : a.C > 1 ? a.carry[(un.b * a.C + un.c) * a.D + un.ch + i]
+             : a.h0    ? a.h0[un.b * a.D + un.ch + i]
+                       : 0.0f;
+    }
+    P xn[RC_U], gn[RC_U];
+    float wn[RC_U];
+    auto load = [&](int64_t t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < RC_U; ++j) {
+        const int64_t tt = t + j < t1 ? t + j : t1 - 1;
+        xn[j] = *(const P*)(xp + tt * a.xss);
+        gn[j] = *(const P*)(gp + tt * a.gss);
+        if (WT) wn[j] = wp[tt];
+      }
+    };
+    if (t0 < t1) load(t0);
+    for (int64_t t = t0; t < t1; t += RC_U) {
+      P xc[RC_U], gc[RC_U];
+      float wc[RC_U];
+#pragma unroll
+      for (int j = 0; j < RC_U; ++j) {
+        xc[j] = xn[j];
+        gc[j] = gn[j];
+        wc[j] = WT ? wn[j] : 1.0f;
+      }
+      if (t + RC_U < t1) load(t + RC_U);
+      if (!SUM && a.ck && (t & (RC_CK - 1)) == 0) {
+        float* c = a.ck + (un.b * nck + t / RC_CK) * a.D + un.ch;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) c[i] = h[i];
+      }
+#pragma unroll
+      for (int j = 0; j < RC_U; ++j) {
+        if (t + j < t1) {
+          float xv[VEC], gv[VEC];
+          unpack<T, VEC>(xc[j], xv);
+          unpack<T, VEC>(gc[j], gv);
+          with_gate<WT, VEC>(wc[j], gv, [&](int i, const Gate& q) __attribute__((always_inline)) {
+            h[i] = move(q, h[i], xv[i]);
+            if (SUM) pa[i] = decay(q, pa[i]);
+          });
+          if (!SUM && a.h) *(P*)((T*)a.h + (un.b * a.S + t + j) * a.D + un.ch) = pack<T, VEC>(h);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if (SUM) {
+        a.sumA[(un.b * a.C + un.c) * a.D + un.ch + i] = pa[i];
+        a.sumH[(un.b * a.C + un.c) * a.D + un.ch + i] = h[i];
+      } else if (un.c == a.C - 1) {
+        a.h_last[un.b * a.D + un.ch + i] = h[i];
+      }
+    }
+  }
+}
+
+// Joins the chunks of one history: carry[c] = the state before chunk c (REV: the gradient that
+// reaches the end of chunk c from the chunks after it).  64 channels x 16 segments of chunks per
+// block: a segment is composed to one (A, H), the segments before it give its start, a second
+// walk writes.  s <- A s + H over chunks c = 0.. (REV: C - 1 .. 1).
+template <bool REV>
+__global__ __launch_bounds__(64 * RC_SEG) void k_scan_join(const float* __restrict__ sumA,
+                                                           const float* __restrict__ sumH,
+                                                           const float* __restrict__ init,
+                                                           float* __restrict__ carry, int64_t B,
+                                                           int C, int D) {
+  __shared__ float sa[RC_SEG][64], sh[RC_SEG][64];
+  const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6;
+  const int nd = (D + 63) / 64;
+  const int per = (C + RC_SEG - 1) / RC_SEG;
+  for (int64_t blk = blockIdx.x; blk < B * nd; blk += gridDim.x) {
+    const int64_t b = blk / nd;
+    const int ch = (int)(blk - b * nd) * 64 + lane;
+    const bool ok = ch < D;
+    const int i0 = seg * per < C ? seg * per : C, i1 = i0 + per < C ? i0 + per : C;
+    auto at = [&](int i) { return (b * C + (REV ? C - 1 - i : i)) * D + (ok ? ch : 0); };
+    float pa = 1.0f, ph = 0.0f;
+    // (the last step's summary starts nothing and is not written: i runs to C - 2)
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) {
+      if (i < C - 1) {
+        const float A = sumA[at(i)], H = sumH[at(i)];
+        ph = fmaf(A, ph, H);
+        pa *= A;
+      }
+    }
+    sa[seg][lane] = pa;
+    sh[seg][lane] = ph;
+    __syncthreads();
+    float s = init && ok ? init[b * D + ch] : 0.0f;
+    for (int j = 0; j < seg; ++j) s = fmaf(sa[j][lane], s, sh[j][lane]);
+    if (ok) {
+#pragma unroll 8
+      for (int i = i0; i < i1; ++i) {
+        carry[at(i)] = s;
+        if (i < C - 1) s = fmaf(sumA[at(i)], s, sumH[at(i)]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Reverse summary of a chunk: product of A, and the gradient that leaves its front when none
+// enters its end.
+template <typename T, int VEC, bool WT>
+__global__ __launch_bounds__(256) void k_scan_bwd_sum(const ScanArgs a) {
+  typedef typename Pack<T, VEC>::type P;
+  const int lane = threadIdx.x & 63;
+  const int64_t nunits = a.B * a.C * a.nw;
+  for (int64_t u0 = (int64_t)blockIdx.x * 4; u0 < nunits; u0 += (int64_t)gridDim.x * 4) {
+    const int64_t uu = u0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (uu >= nunits) break;
+    const Unit un = unit_of<VEC>(a, uu, lane);
+    if (un.c == 0 || un.ch >= a.D) continue;
+    const int64_t t0 = (int64_t)un.c * a.T, t1 = t0 + a.T < a.S ? t0 + a.T : a.S;
+    const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
+    const T* dp = a.dh ? (const T*)a.dh + un.b * a.S * a.D + un.ch : nullptr;
+    const float* wp = WT ? a.w + un.b * a.wsb : nullptr;
+    float R[VEC], pa[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      pa[i] = 1.0f;
+      R[i] = 0.0f;
+    }
+    P gn[RC_U], dn[RC_U];
+    float wn[RC_U];
+    auto load = [&](int64_t t) __attribute__((always_inline)) {  // events t, t - 1, ...
+#pragma unroll
+      for (int j = 0; j < RC_U; ++j) {
+        const int64_t tt = t - j > t0 ? t - j : t0;
+        gn[j] = *(const P*)(gp + tt * a.gss);
+        if (dp) dn[j] = *(const P*)(dp + tt * a.D);
+        if (WT) wn[j] = wp[tt];
+      }
+    };
+    load(t1 - 1);
+    for (int64_t t = t1 - 1; t >= t0; t -= RC_U) {
+      P gc[RC_U], dc[RC_U];
+      float wc[RC_U];
+#pragma unroll
+      for (int j = 0; j < RC_U; ++j) {
+        gc[j] = gn[j];
+        if (dp) dc[j] = dn[j];
+        wc[j] = WT ? wn[j] : 1.0f;
+      }
+      if (t - RC_U >= t0) load(t - RC_U);
+#pragma unroll
+      for (int j = 0; j < RC_U; ++j) {
+        if (t - j >= t0) {
+          float gv[VEC], dv[VEC];
+          unpack<T, VEC>(gc[j], gv);
+          if (dp) {
+            unpack<T, VEC>(dc[j], dv);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) R[i] += dv[i];
+          }
+          with_gate<WT, VEC>(wc[j], gv, [&](int i, const Gate& q) __attribute__((always_inline)) {
+            R[i] = decay(q, R[i]);
+            pa[i] = decay(q, pa[i]);
+          });
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      a.sumA[(un.b * a.C + un.c) * a.D + un.ch + i] = pa[i];
+      a.sumH[(un.b * a.C + un.c) * a.D + un.ch + i] = R[i];
+    }
+  }
+}
+
+template <typename T, int VEC, bool WT>
+__global__ __launch_bounds__(256) void k_scan_bwd(const ScanArgs a) {
+  typedef typename Pack<T, VEC>::type P;
+  const int lane = threadIdx.x & 63;
+  const int64_t nunits = a.B * a.C * a.nw;
+  const int64_t nck = (a.S + RC_CK - 1) / RC_CK;
+  for (int64_t u0 = (int64_t)blockIdx.x * 4; u0 < nunits; u0 += (int64_t)gridDim.x * 4) {
+    const int64_t uu = u0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (uu >= nunits) break;
+    const Unit un = unit_of<VEC>(a, uu, lane);
+    if (un.ch >= a.D) continue;
+    const int64_t t0 = (int64_t)un.c * a.T, t1 = t0 + a.T < a.S ? t0 + a.T : a.S;
+    const T* xp = (const T*)a.x + un.b * a.xsb + un.ch;
+    const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
+    const int64_t ob = un.b * a.S * a.D + un.ch;
+    const float* wp = WT ? a.w + un.b * a.wsb : nullptr;
+    float R[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      R[i] = a.C > 1 ? a.carry[(un.b * a.C + un.c) * a.D + un.ch + i]
+             : a.dlast ? a.dlast[un.b * a.D + un.ch + i]
+                       : 0.0f;
+    for (int64_t s0 = t1 > t0 ? (t1 - 1) / RC_CK * RC_CK : t0 - 1; s0 >= t0; s0 -= RC_CK) {
+      const int n = (int)(t1 - s0 < RC_CK ? t1 - s0 : RC_CK);
+      P xr[RC_CK], gr[RC_CK], dr[RC_CK];
+      float wr[RC_CK], h[VEC];
+#pragma unroll
+      for (int j = 0; j < RC_CK; ++j) {
+        const int64_t tt = s0 + (j < n ? j : n - 1);
+        xr[j] = *(const P*)(xp + tt * a.xss);
+        gr[j] = *(const P*)(gp + tt * a.gss);
+        if (a.dh) dr[j] = *(const P*)((const T*)a.dh + ob + tt * a.D);
+        wr[j] = WT ? wp[tt] : 1.0f;
+      }
+      const float* c = a.ck + (un.b * nck + s0 / RC_CK) * a.D + un.ch;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[i] = c[i];
+      // (A negative here: the decay is 1 - |A|, see decay())
+      float A[RC_CK][VEC], nA[RC_CK][VEC], q[RC_CK][VEC];
+#pragma unroll
+      for (int j = 0; j < RC_CK; ++j) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {  // padding: the gradient passes by
+          A[j][i] = -0.0f;
+          nA[j][i] = q[j][i] = 0.0f;
+        }
+        if (j < n) {
+          float xv[VEC], gv[VEC];
+          unpack<T, VEC>(xr[j], xv);
+          unpack<T, VEC>(gr[j], gv);
+          with_gate<WT, VEC>(wr[j], gv, [&](int i, const Gate& o) __attribute__((always_inline)) {
+            A[j][i] = o.hi ? -o.na : o.a;
+            nA[j][i] = o.na;
+            q[j][i] = (h[i] - xv[i]) * (WT ? wr[j] * o.a : o.a) * o.sn;
+            h[i] = move(o, h[i], xv[i]);
+          });
+        }
+      }
+#pragma unroll
+      for (int j = RC_CK - 1; j >= 0; --j) {
+        if (j < n) {
+          float G[VEC], dxv[VEC], dgv[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) G[i] = R[i];
+          if (a.dh) {
+            float dv[VEC];
+            unpack<T, VEC>(dr[j], dv);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) G[i] += dv[i];
+          }
+          const bool live = !WT || wr[j] > 0.0f;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            dxv[i] = live ? nA[j][i] * G[i] : 0.0f;
+            dgv[i] = live ? q[j][i] * G[i] : 0.0f;
+            R[i] = __float_as_int(A[j][i]) < 0 ? fmaf(A[j][i], G[i], G[i]) : A[j][i] * G[i];
+          }
+          const int64_t o = ob + (s0 + j) * a.D;
+          *(P*)((T*)a.dx + o) = pack<T, VEC>(dxv);
+          *(P*)((T*)a.dgate + o) = pack<T, VEC>(dgv);
+        }
+      }
+    }
+    if (a.dh0 && un.c == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) a.dh0[un.b * a.D + un.ch + i] = R[i];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- host side
+struct ScanPlan {
+  int vec, nw, C;
+  int64_t T;
+};
+// VEC: two channels a lane where D, the strides and the addresses allow (4- or 8-byte loads),
+// else one.  Chunks: as many as give the card about 2048 waves, none shorter than 64 events; one
+// chunk when the histories alone give 1024.
+static ScanPlan scan_plan(int64_t B, int64_t S, int D, bool vec_ok) {
+  ScanPlan p;
+  p.vec = vec_ok && D % 2 == 0 ? 2 : 1;
+  p.nw = (D + 64 * p.vec - 1) / (64 * p.vec);
+  p.C = 1;
+  p.T = S > 0 ? S : 1;
+  const int64_t waves = B * p.nw;
+  if (waves < 1024 && S >= 128) {
+    int64_t c = (2048 + waves - 1) / waves, cmax = (S + 63) / 64;
+    c = c < cmax ? c : cmax;
+    p.T = ((S + c - 1) / c + RC_CK - 1) / RC_CK * RC_CK;
+    p.C = (int)((S + p.T - 1) / p.T);
+  }
+  return p;
+}
+// workspace for either vector width (the caller of the size does not know the addresses)
+static int64_t scan_ws(int64_t B, int64_t S, int D) {
+  int64_t need = 0;
+  for (int v = 0; v < 2; ++v) {
+    const ScanPlan p = scan_plan(B, S, D, v != 0);
+    const int64_t n = p.C > 1 ? 3 * B * p.C * (int64_t)D * 4 : 0;
+    need = n > need ? n : need;
+  }
+  return need;
+}
+
+template <template <typename, int, bool> class K>
+static void scan_launch(int dtype, int vec, bool wt, unsigned grid, hipStream_t st,
+                        const ScanArgs& a) {
+#define RC_GO(T, V, W) hipLaunchKernelGGL((K<T, V, W>::fn), dim3(grid), dim3(256), 0, st, a)
+  if (dtype == TT_DTYPE_F32) {
+    if (vec == 2) { if (wt) RC_GO(float, 2, true); else RC_GO(float, 2, false); }
+    else { if (wt) RC_GO(float, 1, true); else RC_GO(float, 1, false); }
+  } else {
+    if (vec == 2) { if (wt) RC_GO(uint16_t, 2, true); else RC_GO(uint16_t, 2, false); }
+    else { if (wt) RC_GO(uint16_t, 1, true); else RC_GO(uint16_t, 1, false); }
+  }
+#undef RC_GO
+}
+template <typename T, int V, bool W>
+struct KFwd { static constexpr auto fn = k_scan_fwd<T, V, W, false>; };
+template <typename T, int V, bool W>
+struct KSum { static constexpr auto fn = k_scan_fwd<T, V, W, true>; };
+template <typename T, int V, bool W>
+struct KBwd { static constexpr auto fn = k_scan_bwd<T, V, W>; };
+template <typename T, int V, bool W>
+struct KBwdSum { static constexpr auto fn = k_scan_bwd_sum<T, V, W>; };
+
+static bool addr_ok(const void* p, int64_t bytes) { return ((uintptr_t)p % bytes) == 0; }
+
+// shared checks and plan; returns TT_OK with a.C == 0 when there is nothing to do
+static int scan_setup(ScanArgs& a, int32_t dtype, ScanPlan& p, void* workspace, int64_t ws_bytes,
+                      std::initializer_list<const void*> rows, const char* fn) {
+  const int64_t sz = dtype == TT_DTYPE_F32 ? 4 : 2;
+  bool vec = a.xsb % 2 == 0 && a.xss % 2 == 0 && a.gsb % 2 == 0 && a.gss % 2 == 0;
+  for (const void* r : rows) vec = vec && addr_ok(r, 2 * sz);
+  p = scan_plan(a.B, a.S, a.D, vec);
+  a.nw = p.nw;
+  a.C = p.C;
+  a.T = p.T;
+  if (p.C > 1) {
+    const int64_t one = a.B * p.C * (int64_t)a.D;
+    if (!workspace || ws_bytes < 3 * one * 4)
+      return fail(TT_ERR_WORKSPACE, std::string(fn) + ": workspace too small");
+    a.sumA = (float*)workspace;
+    a.sumH = a.sumA + one;
+    a.carry = a.sumH + one;
+  }
+  return TT_OK;
+}
+static unsigned scan_grid(const ScanArgs& a) {
+  const int64_t blocks = (a.B * a.C * a.nw + 3) / 4;
+  return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
+}
+static unsigned join_grid(const ScanArgs& a) {
+  const int64_t blocks = a.B * ((a.D + 63) / 64);
+  return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
+}
+
+}  // namespace tt
+
+using namespace tt;
+
+#define RC_SIZES()                                                                              \
+  TT_REQUIRE(dtype == TT_DTYPE_F32 || dtype == TT_DTYPE_BF16, "dtype must be f32 or bf16");     \
+  TT_REQUIRE(B >= 0 && S >= 0 && D >= 1, "need B >= 0, S >= 0, D >= 1");                        \
+  TT_REQUIRE(B < (1LL << 31) && S < (1LL << 40) && D <= (1 << 24), "sizes out of range")
+
+extern "C" int tt_gated_scan_workspace_bytes(int64_t B, int64_t S, int32_t D, int64_t* bytes) {
+  TT_REQUIRE(bytes, "null pointer");
+  TT_REQUIRE(B >= 0 && S >= 0 && D >= 1, "need B >= 0, S >= 0, D >= 1");
+  *bytes = B > 0 ? scan_ws(B, S, D) : 0;
+  return TT_OK;
+}
+
+extern "C" int tt_gated_scan_fwd(const void* x, const void* gate, int32_t dtype, int64_t B,
+                                 int64_t S, int32_t D, int64_t x_sb, int64_t x_ss, int64_t g_sb,
+                                 int64_t g_ss, const float* w, int64_t w_sb, const float* h0,
+                                 void* h, float* h_last, float* ckpt, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  RC_SIZES();
+  if (B == 0) return TT_OK;
+  TT_REQUIRE(h_last, "null pointer");
+  TT_REQUIRE(S == 0 || (x && gate), "null pointer");
+  ScanArgs a{};
+  a.x = x; a.gate = gate; a.w = w; a.h0 = h0; a.h = h; a.h_last = h_last; a.ck = ckpt;
+  a.B = B; a.S = S; a.D = D;
+  a.xsb = x_sb; a.xss = x_ss; a.gsb = g_sb; a.gss = g_ss; a.wsb = w_sb;
+  ScanPlan p;
+  if (int rc = scan_setup(a, dtype, p, workspace, workspace_bytes, {x, gate, h}, __func__)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (p.C > 1) {
+    scan_launch<KSum>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+    hipLaunchKernelGGL(k_scan_join<false>, dim3(join_grid(a)), dim3(64 * RC_SEG), 0, st, a.sumA,
+                       a.sumH, a.h0, a.carry, B, a.C, D);
+  }
+  scan_launch<KFwd>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+  return check_launch("tt_gated_scan_fwd");
+}
+
+extern "C" int tt_gated_scan_bwd(const void* x, const void* gate, int32_t dtype, int64_t B,
+                                 int64_t S, int32_t D, int64_t x_sb, int64_t x_ss, int64_t g_sb,
+                                 int64_t g_ss, const float* w, int64_t w_sb, const float* ckpt,
+                                 const void* dh, const float* dh_last, void* dx, void* dgate,
+                                 float* dh0, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  RC_SIZES();
+  if (B == 0) return TT_OK;
+  TT_REQUIRE(S == 0 || (x && gate && ckpt && dx && dgate), "null pointer");
+  ScanArgs a{};
+  a.x = x; a.gate = gate; a.w = w; a.ck = const_cast<float*>(ckpt);
+  a.dh = dh; a.dlast = dh_last; a.dx = dx; a.dgate = dgate; a.dh0 = dh0;
+  a.B = B; a.S = S; a.D = D;
+  a.xsb = x_sb; a.xss = x_ss; a.gsb = g_sb; a.gss = g_ss; a.wsb = w_sb;
+  ScanPlan p;
+  if (int rc = scan_setup(a, dtype, p, workspace, workspace_bytes, {x, gate, dh, dx, dgate}, __func__))
+    return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (p.C > 1) {
+    scan_launch<KBwdSum>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+    hipLaunchKernelGGL(k_scan_join<true>, dim3(join_grid(a)), dim3(64 * RC_SEG), 0, st, a.sumA,
+                       a.sumH, a.dlast, a.carry, B, a.C, D);
+  }
+  scan_launch<KBwd>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+  return check_launch("tt_gated_scan_bwd");
+}

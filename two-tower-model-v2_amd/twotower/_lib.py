@@ -7,6 +7,7 @@ if the library is missing or no HIP device is visible, every op raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import subprocess
@@ -36,6 +37,9 @@ TT_PREC_F32 = 0
 TT_PREC_BF16 = 1
 TT_PREC_X3 = 2  # f32 operands, split-bf16 (hi + lo) MFMA products
 TT_ACT_NONE, TT_ACT_GELU, TT_ACT_RELU = 0, 1, 2
+TT_DTYPE_F32, TT_DTYPE_BF16 = 0, 1
+TT_SCAN_CKPT = 16  # events between the states tt_gated_scan_fwd saves for the backward pass
+DTYPES = {torch.float32: TT_DTYPE_F32, torch.bfloat16: TT_DTYPE_BF16}
 
 
 class BertLayer(ctypes.Structure):
@@ -206,6 +210,12 @@ SIGNATURES = {
     "tt_convert_batch": (ctypes.c_int, [ctypes.POINTER(ConvertJob), _i32, _vp]),
     "tt_item_concat": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _i64,
                                       _vp, _vp]),
+    "tt_gated_scan_workspace_bytes": (ctypes.c_int, [_i64, _i64, _i32, ctypes.POINTER(_i64)]),
+    "tt_gated_scan_fwd": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i64, _i32, _i64, _i64, _i64, _i64,
+                                         _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "tt_gated_scan_bwd": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i64, _i32, _i64, _i64, _i64, _i64,
+                                         _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                         _vp]),
 }
 
 
@@ -256,6 +266,14 @@ def device() -> "torch.device":
 
 def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(t: "torch.Tensor"):
+    """Context with t's device current: launches, streams and workspaces are its own also when
+    the caller's current device is another one (nothing to enter when it is this one)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def padded_dim(d: int) -> int:

@@ -8,6 +8,8 @@ src/training/trainer.py:49-52,74-243).
   ItemHeadFn  ItemTower.forward after the text encoder (item_tower.py:194-209): concat with the
               brand/category embedding rows, projection, F.normalize; gradients for the
               projection, the embedding tables and (if required) the text embeddings.
+  LinearFn    nn.Linear in f32 (the recurrent buyer tower's gate), all three gradients.
+  NormalizeFn F.normalize(dim=1) of f32 rows.
 """
 from __future__ import annotations
 
@@ -132,3 +134,42 @@ class ItemHeadFn(torch.autograd.Function):
                     else:
                         dct = gt
         return dtext, None, None, dbt, dct, dW0, db0, dW3, db3, None, None
+
+
+class LinearFn(torch.autograd.Function):
+    """y = x W^T + b in f32 on tt_gemm_f32: x [M, K], W [N, K] (K a multiple of 32)."""
+
+    @staticmethod
+    def forward(ctx, x, W, b):
+        ctx.save_for_backward(x, W)
+        return GemmOps("f32", x.device).gemm(x, W, b)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, W = ctx.saved_tensors
+        ops = GemmOps("f32", x.device)
+        dy = dy.contiguous()
+        dx = ops.gemm(dy, ops.T(W, W.shape[0])) if ctx.needs_input_grad[0] else None
+        return dx, ops.dW(dy, x), ops.colsum(dy)
+
+
+class NormalizeFn(torch.autograd.Function):
+    """F.normalize(y, p=2, dim=1) of contiguous f32 rows."""
+
+    @staticmethod
+    def forward(ctx, y):
+        z = kernels.l2norm_rows(y, y.shape[1], _lib.TT_NORM_MAX_EPS, out=torch.empty_like(y))
+        ctx.save_for_backward(y, z)
+        return z
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dz):
+        y, z = ctx.saved_tensors
+        n, d = y.shape
+        dz = dz.contiguous()
+        dy = torch.empty_like(y)
+        check(lib().tt_l2norm_backward_f32(y.data_ptr(), d, z.data_ptr(), d, dz.data_ptr(), d, n,
+                                           d, dy.data_ptr(), d, stream_ptr()), "norm_bwd")
+        return dy

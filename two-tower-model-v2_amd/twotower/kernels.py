@@ -614,3 +614,98 @@ def attn_agg_l2(items, w, W1, b1, W2, b2, out=None, fused: bool = None):
                                       _ptr(W2), _ptr(b2), _ptr(out), out.stride(0), _ptr(ws),
                                       ws.numel(), stream_ptr()), "tt_attn_agg_l2_f32_ws")
     return out
+
+
+def _scan_rows(t, name):
+    """[B, S, D] with unit channel stride: (tensor, history stride, event stride)."""
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        t = t.contiguous()
+    return t, t.stride(0), t.stride(1)
+
+
+def _scan_args(x, gate, weights, h0):
+    require_device(x, "x")
+    require_device(gate, "gate")
+    if x.dtype not in _lib.DTYPES or gate.dtype != x.dtype:
+        raise TypeError(f"gated_scan: x and gate must both be float32 or bfloat16, got {x.dtype} "
+                        f"and {gate.dtype}")
+    if x.dim() != 3 or gate.shape != x.shape or x.shape[2] < 1:
+        raise ValueError(f"gated_scan: x and gate must be [B, S, D], got {tuple(x.shape)} and "
+                         f"{tuple(gate.shape)}")
+    b, s, d = x.shape
+    if weights is not None and tuple(weights.shape) != (b, s):
+        raise ValueError(f"gated_scan: weights must be [{b}, {s}], got {tuple(weights.shape)}")
+    if h0 is not None and tuple(h0.shape) != (b, d):
+        raise ValueError(f"gated_scan: h0 must be [{b}, {d}], got {tuple(h0.shape)}")
+    for t, name in ((gate, "gate"), (weights, "weights"), (h0, "h0")):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"gated_scan: {name} is on {t.device}, x on {x.device}")
+    if weights is not None:
+        weights = weights.detach().to(_f32)
+        if s > 1 and weights.stride(1) != 1:
+            weights = weights.contiguous()
+    if h0 is not None:
+        h0 = h0.detach().to(_f32).contiguous()
+    return weights, h0
+
+
+def _scan_workspace(b, s, d, device):
+    need = ctypes.c_int64(0)
+    check(lib().tt_gated_scan_workspace_bytes(b, s, d, ctypes.byref(need)),
+          "tt_gated_scan_workspace_bytes")
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+
+
+def gated_scan(x, gate, weights=None, h0=None, states: bool = True, save: bool = False):
+    """h_t = A_t h_{t-1} + (1 - A_t) x_t with A_t = sigmoid(gate_t) ** weights_t
+    (tt_gated_scan_fwd): x, gate [B, S, D] f32 or bf16, weights [B, S] (None: 1; a weight not above
+    0 is padding and leaves the state as it is), h0 [B, D] (None: 0) -> (h [B, S, D] in x's type
+    or None without ``states``, h_last [B, D] f32, the states gated_scan_backward needs or None
+    without ``save``)."""
+    weights, h0 = _scan_args(x, gate, weights, h0)
+    b, s, d = x.shape
+    with _lib.on_device(x):
+        x, xb, xs = _scan_rows(x, "x")
+        gate, gb, gs = _scan_rows(gate, "gate")
+        dev = x.device
+        h = torch.empty((b, s, d), dtype=x.dtype, device=dev) if states else None
+        last = torch.empty((b, d), dtype=_f32, device=dev)
+        ck = None
+        if save:
+            ck = torch.empty((b, -(-s // _lib.TT_SCAN_CKPT), d), dtype=_f32, device=dev)
+        ws = _scan_workspace(b, s, d, dev)
+        check(lib().tt_gated_scan_fwd(
+            _ptr(x), _ptr(gate), _lib.DTYPES[x.dtype], b, s, d, xb, xs, gb, gs, _ptr(weights),
+            weights.stride(0) if weights is not None else 0, _ptr(h0), _ptr(h), _ptr(last),
+            _ptr(ck), _ptr(ws), ws.numel() if ws is not None else 0, stream_ptr()),
+            "tt_gated_scan_fwd")
+    return h, last, ck
+
+
+def gated_scan_backward(x, gate, weights, saved, dh, dlast, need_h0: bool):
+    """Gradients (dx, dgate [B, S, D] in x's type, dh0 [B, D] f32 or None) of gated_scan for dh
+    [B, S, D] (or None) and dlast [B, D] (or None); ``saved`` from gated_scan(save=True)."""
+    weights, _ = _scan_args(x, gate, weights, None)
+    b, s, d = x.shape
+    if saved is None or tuple(saved.shape) != (b, -(-s // _lib.TT_SCAN_CKPT), d):
+        raise ValueError("gated_scan_backward: saved must come from gated_scan(save=True)")
+    if dh is not None and tuple(dh.shape) != (b, s, d):
+        raise ValueError(f"gated_scan_backward: dh must be [{b}, {s}, {d}]")
+    if dlast is not None and tuple(dlast.shape) != (b, d):
+        raise ValueError(f"gated_scan_backward: dlast must be [{b}, {d}]")
+    with _lib.on_device(x):
+        x, xb, xs = _scan_rows(x, "x")
+        gate, gb, gs = _scan_rows(gate, "gate")
+        dev = x.device
+        dh = dh.to(x.dtype).contiguous() if dh is not None else None
+        dlast = dlast.to(_f32).contiguous() if dlast is not None else None
+        dx = torch.empty((b, s, d), dtype=x.dtype, device=dev)
+        dgate = torch.empty((b, s, d), dtype=x.dtype, device=dev)
+        dh0 = torch.empty((b, d), dtype=_f32, device=dev) if need_h0 else None
+        ws = _scan_workspace(b, s, d, dev)
+        check(lib().tt_gated_scan_bwd(
+            _ptr(x), _ptr(gate), _lib.DTYPES[x.dtype], b, s, d, xb, xs, gb, gs, _ptr(weights),
+            weights.stride(0) if weights is not None else 0, _ptr(saved), _ptr(dh), _ptr(dlast),
+            _ptr(dx), _ptr(dgate), _ptr(dh0), _ptr(ws), ws.numel() if ws is not None else 0,
+            stream_ptr()), "tt_gated_scan_bwd")
+    return dx, dgate, dh0
