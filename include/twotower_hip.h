@@ -636,6 +636,47 @@ int tt_gated_scan_bwd(const void* x, const void* gate, int32_t dtype, int64_t B,
                       const float* dh_last, void* dx, void* dgate, float* dh0, void* workspace,
                       int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * AdamW (decoupled weight decay) over many tensors in one launch (tt_adamw.hip), moments in f32
+ * (state_bits 32) or in 8-bit codes with one f32 scale per 256 elements (state_bits 8); beside
+ * tt_adam_f32, which takes one flat f32 buffer without decay.
+ *   m = b1 m + (1-b1) g ; v = b2 v + (1-b2) g g
+ *   p = p (1 - lr wd) - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps)
+ * `tensors`: DEVICE table.  p and its gradient have one dtype (f32 or bf16, any alignment);
+ * exp_avg / exp_avg_sq: f32 [n rounded up to 4] (state_bits 32) or int8 / uint8 codes [n rounded up
+ * to 256] with scale_m / scale_v [ceil(n / 256)], 16-byte aligned.  An m code c stands for
+ * sign(c) s (c / 127)^2, a v code for s (c / 255)^4; an update codes each moment to the nearest.
+ * step (device): steps taken so far, advanced by the call, so a captured call may be replayed; blocks:
+ * ceil(n / chunk); ticket: scratch, zero before the first call.
+ * `items` (device): n_items pairs (tensor, chunk of it), all chunks of each tensor that takes
+ * part; tensors first .. first + n_grads - 1; grads: HOST array of their gradients' device
+ * addresses (NULL: no gradient, the tensor and its count stay as they are), n_grads <=
+ * TT_ADAMW_MAX_TENSORS.  Tensors must not overlap.  A gradient that is not finite makes its block
+ * of 256 moments (state_bits 8) not finite.
+ * tt_adamw_decode / tt_adamw_encode: 8-bit moments to and from f32 rows; tensor i's at offsets[i]
+ * (device array; a multiple of 4).
+ * --------------------------------------------------------------------------------- */
+#define TT_ADAMW_MAX_TENSORS 416
+typedef struct tt_adamw_tensor {
+  void* p;
+  void *exp_avg, *exp_avg_sq;
+  float *scale_m, *scale_v; /* state_bits 8 */
+  int64_t* step;
+  uint32_t* ticket;
+  int64_t n;
+  int32_t dtype, blocks;
+} tt_adamw_tensor;
+int tt_adamw_step(const tt_adamw_tensor* tensors, const int32_t* items, int64_t n_items,
+                  int32_t first, const void* const* grads, int32_t n_grads, int64_t chunk,
+                  int32_t state_bits, double lr, double beta1, double beta2, double eps,
+                  double weight_decay, void* stream);
+int tt_adamw_decode(const tt_adamw_tensor* tensors, const int32_t* items, int64_t n_items,
+                    int64_t chunk, const int64_t* offsets, float* exp_avg, float* exp_avg_sq,
+                    void* stream);
+int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_t n_items,
+                    int64_t chunk, const int64_t* offsets, const float* exp_avg,
+                    const float* exp_avg_sq, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

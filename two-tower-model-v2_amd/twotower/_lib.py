@@ -216,6 +216,11 @@ SIGNATURES = {
     "tt_gated_scan_bwd": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i64, _i32, _i64, _i64, _i64, _i64,
                                          _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
                                          _vp]),
+    "tt_adamw_step": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp, _i32, _i64, _i32,
+                                     ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                                     ctypes.c_double, ctypes.c_double, _vp]),
+    "tt_adamw_decode": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "tt_adamw_encode": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
 }
 
 

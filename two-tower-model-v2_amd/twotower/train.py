@@ -126,16 +126,26 @@ class TwoTowerTrainStep:
     ``graph=True`` captures forward + backward of each step shape in a HIP graph (torch's
     CUDAGraph over the same launches) after one eager warm-up call, and replays it: the ~35
     launches cost one graph launch of host time.  Inputs are copied into the graph's static
-    buffers (``input_buffers`` hands them out to write in place instead)."""
+    buffers (``input_buffers`` hands them out to write in place instead).
+
+    ``weight_decay`` > 0 or ``state_bits=8`` replace Adam by AdamW (twotower.optim: decoupled decay,
+    moments in 32 or 8 bits), still one launch over all parameters."""
 
     def __init__(self, item_tower, buyer_tower, temperature: float = 0.07, lr: float = 1e-4,
-                 betas=(0.9, 0.999), eps: float = 1e-8, prec: str = "f32", graph: bool = False):
+                 betas=(0.9, 0.999), eps: float = 1e-8, prec: str = "f32", graph: bool = False,
+                 weight_decay: float = 0.0, state_bits: int = 32):
         if buyer_tower.aggregation_method not in ("attention", "weighted_avg"):
             raise ValueError(f"Unknown aggregation method: {buyer_tower.aggregation_method}")
         self.attention = buyer_tower.aggregation_method == "attention"
         if prec not in ("f32", "bf16"):
             raise ValueError("prec must be 'f32' or 'bf16'")
         self.it, self.bt = item_tower, buyer_tower
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if not weight_decay >= 0.0:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        self.weight_decay, self.state_bits = weight_decay, state_bits
+        self.adamw = None  # MultiTensorAdamW over the parameters (weight_decay / 8-bit states)
         self.tau, self.lr, self.betas, self.eps, self.prec = temperature, lr, betas, eps, prec
         self.dev = _lib.device()
         self.ops = GemmOps(prec, self.dev)
@@ -176,6 +186,11 @@ class TwoTowerTrainStep:
         total = sum(v.numel() for v in objs.values())
         flat = torch.empty(total, dtype=torch.float32, device=self.dev)
         old_m, old_v = getattr(self, "m", None), getattr(self, "v", None)
+        multi = self.weight_decay > 0 or self.state_bits == 8
+        old_w = None
+        if self.adamw is not None:
+            old_w = {k: self.adamw.state_of(i, (p.numel(),))
+                     for i, (k, p) in enumerate(self.params.items())}
         fm = torch.zeros(total, dtype=torch.float32, device=self.dev)
         fv = torch.zeros(total, dtype=torch.float32, device=self.dev)
         self.flat_g = torch.zeros(total, dtype=torch.float32, device=self.dev)
@@ -196,6 +211,14 @@ class TwoTowerTrainStep:
             self._span[k] = (off, n)
             off += n
         self.flat_p, self.flat_m, self.flat_v = flat, fm, fv
+        if multi:
+            from .optim import MultiTensorAdamW
+
+            self.adamw = MultiTensorAdamW(list(self.params.values()), self.state_bits)
+            if old_w is not None:
+                self.adamw.load_state({i: old_w[k] for i, k in enumerate(self.params)
+                                       if k in old_w})
+            self.m, self.v, self.flat_m, self.flat_v = {}, {}, None, None
         self._objs = objs
         self._bufs = {}
         self._graphs = {}
@@ -532,6 +555,16 @@ class TwoTowerTrainStep:
                                   G["att2.w"].data_ptr(), G["att2.b"].data_ptr(), *emb, st),
               "bwd tail")
 
+    def _moments(self):
+        """Both moments by parameter name, f32 (decoded from 8 bits)."""
+        if self.adamw is None:
+            return self.m, self.v
+        out = []
+        for flat in self.adamw.moments():
+            out.append({k: flat[o:o + p.numel()].view(p.shape)
+                        for o, (k, p) in zip(self.adamw.offsets, self.params.items())})
+        return out
+
     # torch.optim.Adam state dict (the reference saves optimizer.state_dict(), trainer.py:330):
     # 'state' indexed by the position of the parameter in model.parameters(), 'param_groups'
     # with Adam's defaults.  Parameters the fused step does not train (the frozen text
@@ -539,12 +572,14 @@ class TwoTowerTrainStep:
     def optimizer_state_dict(self, model) -> Dict:
         pos = {p.data_ptr(): i for i, p in enumerate(model.parameters())}
         state = {}
+        m, v = self._moments()
         for k, p in self.params.items():
             if self.t > 0:
                 state[pos[p.data_ptr()]] = {"step": torch.tensor(float(self.t)),
-                                            "exp_avg": self.m[k].detach().cpu().clone(),
-                                            "exp_avg_sq": self.v[k].detach().cpu().clone()}
-        group = {"lr": self.lr, "betas": tuple(self.betas), "eps": self.eps, "weight_decay": 0,
+                                            "exp_avg": m[k].detach().cpu().clone(),
+                                            "exp_avg_sq": v[k].detach().cpu().clone()}
+        group = {"lr": self.lr, "betas": tuple(self.betas), "eps": self.eps,
+                 "weight_decay": self.weight_decay or 0,
                  "amsgrad": False, "maximize": False, "foreach": None, "capturable": False,
                  "differentiable": False, "fused": None, "decoupled_weight_decay": False,
                  "params": list(range(len(pos)))}
@@ -563,20 +598,24 @@ class TwoTowerTrainStep:
         st = sd["state"]
         steps = set()
         matched = 0
+        load = {}
         for k, p in self.params.items():
             i = pos[p.data_ptr()]
             e = st.get(i)
             if e is None:
                 continue
             ea, es = torch.as_tensor(e["exp_avg"]), torch.as_tensor(e["exp_avg_sq"])
-            if ea.numel() != self.m[k].numel() or es.numel() != self.v[k].numel():
+            if ea.numel() != p.numel() or es.numel() != p.numel():
                 raise ValueError(
                     f"optimizer state entry {i} holds {tuple(ea.shape)} moments, parameter {k} "
-                    f"needs {tuple(self.m[k].shape)}: the state dict indexes a different parameter "
+                    f"needs {tuple(p.shape)}: the state dict indexes a different parameter "
                     "list (e.g. a reference checkpoint, whose frozen text-encoder parameters come "
                     "first)")
-            self.m[k].copy_(ea.view_as(self.m[k]))
-            self.v[k].copy_(es.view_as(self.v[k]))
+            if self.adamw is None:
+                self.m[k].copy_(ea.view_as(self.m[k]))
+                self.v[k].copy_(es.view_as(self.v[k]))
+            else:
+                load[list(self.params).index(k)] = e
             steps.add(int(float(e["step"])))
             matched += 1
         if st and matched == 0:
@@ -585,6 +624,8 @@ class TwoTowerTrainStep:
         if len(steps) > 1:
             raise ValueError(f"inconsistent Adam step counts in the state dict: {sorted(steps)}")
         self.t = steps.pop() if steps else 0
+        if self.adamw is not None:
+            self.adamw.load_state(load)
         g = sd.get("param_groups", [{}])[0]
         self.lr = g.get("lr", self.lr)
         self.betas = tuple(g.get("betas", self.betas))
@@ -596,6 +637,10 @@ class TwoTowerTrainStep:
         self._check_layout()
         self.t += 1
         b1, b2 = self.betas
+        if self.adamw is not None:
+            self.adamw.step([grads[k].reshape(p.shape) for k, p in self.params.items()], self.lr,
+                            self.betas, self.eps, self.weight_decay)
+            return
         for k in self.params:
             if grads[k].data_ptr() != self.g[k].data_ptr():
                 self.g[k].copy_(grads[k].reshape(self.g[k].shape))
