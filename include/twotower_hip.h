@@ -677,6 +677,39 @@ int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_
                     int64_t chunk, const int64_t* offsets, const float* exp_avg,
                     const float* exp_avg_sq, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Log-probabilities over a catalog (tt_catalog.hip): for rows x [N, E] (ldx) and items w [V, E]
+ * (ldw), both of dtype (f32 or bf16), logits l = x.w / temperature + bias (bias [V] f32 or NULL;
+ * at or below -1e30, e.g. -inf: the item is taken out, whatever its vector holds).
+ *   log_prob[n] = l[n, ids[n]] - lse[n]   (ids [N]; an id outside [0, V): 0; NULL log_prob: not
+ *                 wanted; -inf if the item is taken out)
+ *   entropy[n]  = -sum_v p log p  (NULL: not wanted) ;  lse[n] = log sum_v exp l[n, v]
+ *   top_ids / top_log_prob [N, top]: the top (<= 32, <= V) largest logits by the product in 64
+ *                 bits, ties to the lower id (taken-out items last, with -inf)
+ * A row with every item taken out: lse -inf, entropy 0, log_prob -inf (0 without an id).
+ * _bwd: dx [N, E], dw [V, E] of dtype, contiguous (either may be NULL), for gradients g_log_prob and
+ * g_entropy [N] (either may be NULL), with the forward's lse and entropy.  A row whose gradients
+ * are 0 adds nothing, whatever its vector holds; taken-out items and empty rows get 0.
+ * E a multiple of 64; rows 16-byte aligned; N < 2^24, V < 2^30.  Sums in f32; the coefficients of
+ * the gradient products are in dtype.  The results do not depend on timing (no float atomics).
+ * --------------------------------------------------------------------------------- */
+int tt_catalog_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t E, int32_t dtype, int32_t top,
+                                        int64_t* bytes);
+int tt_catalog_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
+                        int64_t N, int64_t V, int32_t E, const int64_t* ids, const float* bias,
+                        float temperature, float* log_prob, float* entropy, float* lse,
+                        int32_t top, int64_t* top_ids, float* top_log_prob, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int tt_catalog_logprobs_bwd_workspace_bytes(int64_t N, int64_t V, int32_t E, int32_t dtype,
+                                            int32_t has_bias, int32_t want_dx, int32_t want_dw,
+                                            int64_t* bytes);
+int tt_catalog_logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
+                            int64_t N, int64_t V, int32_t E, const int64_t* ids,
+                            const float* bias, float temperature, const float* lse,
+                            const float* entropy, const float* g_log_prob,
+                            const float* g_entropy, void* dx, void* dw, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,929 @@
+// tt_catalog.hip -- log-probabilities of given items over a catalog, with the entropy and the top
+// alternatives of every row, and their gradient (gfx950).
+//
+//   l_nv = s x_n.w_v + bias_v         x [N, E], w [V, E] f32 or bf16;  s = 1 / temperature
+//   lse_n = log sum_v exp l_nv ;  p_nv = exp(l_nv - lse_n)
+//   log_prob_n = l_{n,id} - lse_n ;  entropy_n = lse_n - sum_v p_nv l_nv ;  top: the k largest l_nv
+//   backward (g, e: gradients of log_prob, entropy; H the entropy):
+//   c_nv = g_n ([v = id_n] - p_nv) - e_n p_nv (l_nv - lse_n + H_n) ;  dx = s C w ;  dw = s C^T x
+//
+// The N x V logits never exist in memory.  Everything is done in powers of two (z = l log2 e).
+//
+// k_logits<STAT>  128 items x 128 rows tiles on MFMA (bf16 16x16x32 or f32 16x16x4), a block
+//     walks its share of the catalog for its 128 rows.  The product is formed as w . x^T, so a lane
+//     holds 16 items of 4 rows: the running maximum m, L = sum 2^(z - m) and T = sum 2^(z - m) (z -
+//     m) of a row stay in the lane, with no exchange between lanes until the share's end.
+//     Entropy = ln 2 (log2 L - T / L): relative to the maximum, nothing cancels against lse.
+// k_combine       joins the shares; the given item's own logit in 64 bits.
+// top             the STAT pass also writes the maximum of every 16 items a lane saw (N V / 16
+//     floats).  The k largest logits lie in the k groups with the largest maxima; k + 8 groups are
+//     taken (32-bit maxima may swap near-equal ones), their items scored again in 64 bits, and
+//     ordered by that, ties by the lower id.
+// k_logits<COEF>  the same product again, its epilogue writing C (x's type) for a chunk of the catalog.
+// k_product       dx += C w (C rows, w as it lies) and dw = C^T x: operands whose rows run along the
+//     sum are read from LDS transposed (ds_read_b64_tr_b16; 4-byte reads in f32), so neither C nor
+//     w nor x is ever stored transposed.  Sums are split over blocks where the output alone gives too
+//     few (f32 partial sums, added in a fixed order: the result does not depend on timing).
+//
+// Items with a bias at or below -1e30 (-inf, the type's lowest) are taken out: probability 0 and
+// gradient 0 whatever their vectors hold.  Rows whose gradients are both 0 do not reach dw.
+#include "tt_common.hpp"
+
+namespace tt {
+
+typedef __bf16 ct_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 ct_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float ct_f32x2 __attribute__((ext_vector_type(2)));
+typedef short ct_s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ct_u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float CT_OUT = -1.0e30f;   // z of an item that is taken out
+constexpr float CT_NONE = -2.0e30f;  // maximum of nothing
+constexpr float CT_LOG2E = 1.4426950408889634f, CT_LN2 = 0.6931471805599453f;
+constexpr int CT_TILE = 128;            // tile edge (items, rows, columns)
+constexpr int CT_OP_B = CT_TILE * 128;  // one operand's stage: 128 rows x 128 B (or BK rows x 128 elements)
+constexpr int CT_TOP_MAX = 32, CT_TOP_EXTRA = 8;
+
+__device__ __forceinline__ void ct_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ct_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ct_dma(const void* g, char* l) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                   (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+}
+
+// ---- operand stages.  Row form ("K along the row"): 128 rows x 128 B, 16-B chunks XOR-swizzled by
+// (row >> 1) & 7.  Wave w of 4 loads pieces w, w + 4, ...: 8 rows each.
+template <typename T>
+struct RowStage {
+  int64_t off[4];
+  __device__ __forceinline__ void init(int64_t ld, int64_t row0, int64_t rows, int w, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = 8 * (w + 4 * j) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+      int64_t row = row0 + r;
+      row = row < rows ? row : rows - 1;  // past the end: loaded again, never used
+      off[j] = row * ld + c * (16 / (int)sizeof(T));
+    }
+  }
+  __device__ __forceinline__ void issue(const T* p, int64_t k0, char* lds, int w) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ct_dma(p + off[j] + k0, lds + 1024 * (w + 4 * j));
+  }
+};
+// fragments of 4 x 16 rows from row r0: f[s][i] = 16 B at chunk 4 s + g of row r0 + 16 i + rl
+__device__ __forceinline__ void row_frags(const char* lds, int r0, int lane, u32x4_t (&f)[2][4]) {
+  const int g = lane >> 4, rl = lane & 15, sw = (rl >> 1) & 7;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[s][i] = *(const u32x4_t*)(lds + (r0 + 16 * i + rl) * 128 + 16 * ((4 * s + g) ^ sw));
+}
+
+// Column form ("the sum runs down the rows"): BK rows x 128 elements, the operand as it lies.
+template <typename T>
+struct ColStage {
+  static constexpr int RPP = sizeof(T) == 2 ? 4 : 2;  // rows per 1-KB piece
+  int64_t off[4];
+  int row[4];
+  // cols: valid columns from c0 (a multiple of the chunk); past the end: loaded again, never used
+  __device__ __forceinline__ void init(int64_t c0, int64_t cols, int w, int lane) {
+    constexpr int EPC = 16 / (int)sizeof(T), CPR = 128 / EPC;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = RPP * (w + 4 * j) + lane / CPR, pc = lane % CPR;
+      const int sw = sizeof(T) == 2 ? ((r & 3) | ((r >> 1) & 4)) << 1 : ((r >> 2) & 3) << 2;
+      int64_t c = c0 + (int64_t)(pc ^ sw) * EPC;
+      c = c < cols ? c : cols - EPC;
+      row[j] = r;
+      off[j] = c;
+    }
+  }
+  __device__ __forceinline__ void issue(const T* p, int64_t ld, int64_t k0, int64_t rows, char* lds,
+                                        int w) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int64_t k = k0 + row[j];
+      k = k < rows ? k : rows - 1;  // past the end: the other operand is zero there
+      ct_dma(p + k * ld + off[j], lds + 1024 * (w + 4 * j));
+    }
+  }
+};
+// the same fragments as row_frags gives (16 B of the sum's index for column c0 + 16 i + rl)
+template <typename T>
+__device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32x4_t (&f)[2][4]) {
+  const int g = lane >> 4, rl = lane & 15;
+  if constexpr (sizeof(T) == 2) {
+    // a 16-lane group reads 4 rows x 16 columns: lane 4 q + c supplies row q, columns 4 c .. + 3 and
+    // receives column (its index)'s 4 rows
+    const int q = rl >> 2, c = rl & 3, sw = (q | ((g & 1) << 2)) << 1;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ct_u32x2 h[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = 32 * s + 8 * g + 4 * u + q;
+          const int chunk = (2 * (c0 / 16 + i) + (c >> 1)) ^ sw;
+          const char* p = lds + row * 256 + chunk * 16 + 8 * (c & 1);
+          h[u] = __builtin_bit_cast(ct_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                  (__attribute__((address_space(3))) ct_s16x4*)p));
+        }
+        f[s][i] = u32x4_t{h[0][0], h[0][1], h[1][0], h[1][1]};
+      }
+  } else {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int row = 16 * s + 4 * g + u;
+          const int chunk = (4 * (c0 / 16 + i) + (rl >> 2)) ^ (g << 2);
+          f[s][i][u] = *(const uint32_t*)(lds + row * 512 + chunk * 16 + 4 * (rl & 3));
+        }
+  }
+}
+
+// acc[i][j] += first[j] . second[i]: lane (g, rl) of block (i, j) holds first-index 16 j + 4 g + r,
+// second-index 16 i + rl
+template <typename T>
+__device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[2][4], const u32x4_t (&second)[2][4],
+                                        f32x4 (&acc)[4][4]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(ct_bf16x8, first[s][j]), __builtin_bit_cast(ct_bf16x8, second[s][i]),
+              acc[i][j], 0, 0, 0);
+        } else {
+          const f32x4 a = __builtin_bit_cast(f32x4, first[s][j]), b = __builtin_bit_cast(f32x4, second[s][i]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u], b[u], acc[i][j], 0, 0, 0);
+        }
+      }
+}
+
+__device__ __forceinline__ uint32_t ct_pack2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(ct_f32x2{a, b}, ct_bf16x2));
+}
+// 4 consecutive outputs
+template <typename T>
+__device__ __forceinline__ void ct_store4(T* p, const f32x4& v) {
+  if constexpr (sizeof(T) == 2) *(ct_u32x2*)p = ct_u32x2{ct_pack2(v[0], v[1]), ct_pack2(v[2], v[3])};
+  else *(f32x4*)p = v;
+}
+
+// (m, L, T) of two disjoint sets of items
+__device__ __forceinline__ void stat_join(float& m, float& L, float& T, float m2, float L2, float T2) {
+  const float M = fmaxf(m, m2);
+  const float a = __builtin_amdgcn_exp2f(m - M), b = __builtin_amdgcn_exp2f(m2 - M);
+  T = a * fmaf(m - M, L, T) + b * fmaf(m2 - M, L2, T2);
+  L = fmaf(a, L, b * L2);
+  m = M;
+}
+
+struct LogitArgs {
+  const void *x, *w;
+  int64_t ldx, ldw;
+  const float* bias;   // may be null
+  float s2;            // log2(e) / temperature
+  int N, V, E;
+  int n_tiles, splits, v_tiles;  // STAT: shares of the catalog; COEF: one tile a block
+  float4* part;        // STAT [splits, N] (m, L, T, -)
+  float* tmax;         // STAT: [N, 4 ceil(V / 64)] or null
+  const float4* rowc;  // COEF [N] (log2-domain lse, g, e, H)
+  const int64_t* ids;  // COEF
+  void* C;             // COEF [Npad, ldc]: items v_base .. of this chunk
+  int64_t ldc;
+  int v_base, Npad;
+};
+
+template <typename T, bool COEF, bool ENT>
+__global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
+  constexpr int BK = 128 / (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) char smem[4 * CT_OP_B];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wv = w >> 1, wn = w & 1, g = lane >> 4, rl = lane & 15;
+  // blocks of one share of the catalog next to each other (one XCD's L2)
+  const int lb = xcd_remap(blockIdx.x, gridDim.x);
+  const int sp = lb / a.n_tiles, tn = lb % a.n_tiles;
+  const int per = (a.v_tiles + a.splits - 1) / a.splits;
+  const int vt0 = sp * per, vt1 = vt0 + per < a.v_tiles ? vt0 + per : a.v_tiles;
+  const int n0 = tn * CT_TILE;
+  const T* x = (const T*)a.x;
+  const T* wt = (const T*)a.w;
+  const int nk = a.E / BK;
+
+  RowStage<T> sx, sw;
+  sx.init(a.ldx, n0, a.N, w, lane);
+  float m[4], L[4], TT[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = CT_NONE;
+    L[i] = TT[i] = 0.0f;
+  }
+  // loads run one stage ahead over (tile, k) as one sequence
+  int vt_i = vt0, k_i = 0, g_i = 0;
+  auto issue_next = [&]() __attribute__((always_inline)) {
+    if (vt_i >= vt1) return;
+    if (k_i == 0) sw.init(a.ldw, (int64_t)a.v_base + (int64_t)vt_i * CT_TILE, a.V, w, lane);
+    char* st = smem + (g_i & 1) * 2 * CT_OP_B;
+    sw.issue(wt, (int64_t)k_i * BK, st, w);
+    sx.issue(x, (int64_t)k_i * BK, st + CT_OP_B, w);
+    ++g_i;
+    if (++k_i == nk) {
+      k_i = 0;
+      ++vt_i;
+    }
+  };
+  issue_next();
+  int gs = 0;
+  for (int vt = vt0; vt < vt1; ++vt) {
+    const int v0 = a.v_base + vt * CT_TILE + 64 * wv;  // this wave's 64 items
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kt = 0; kt < nk; ++kt, ++gs) {
+      ct_wait_vm<0>();
+      ct_barrier();  // stage gs complete; every wave is done with the slot refilled next
+      issue_next();
+      const char* st = smem + (gs & 1) * 2 * CT_OP_B;
+      u32x4_t fw[2][4], fx[2][4];
+      row_frags(st, 64 * wv, lane, fw);
+      row_frags(st + CT_OP_B, 64 * wn, lane, fx);
+      ct_mfma<T>(fw, fx, acc);
+    }
+    const bool edge = v0 + 64 > a.V;
+    const bool sel = a.bias || edge;
+    f32x4 b2[4];
+    if (sel) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int v = v0 + 16 * j + 4 * g + r;
+          const float b = v < a.V ? (a.bias ? a.bias[v] : 0.0f) : -__builtin_huge_valf();
+          b2[j][r] = b > CT_OUT || b != b ? b * CT_LOG2E : CT_NONE;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + 64 * wn + 16 * i + rl;
+      f32x4 z[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float q = acc[i][j][r];
+          // (taken out: whatever the product is)
+          z[j][r] = sel ? (b2[j][r] == CT_NONE ? CT_OUT : fmaf(q, a.s2, b2[j][r])) : q * a.s2;
+        }
+      if constexpr (!COEF) {
+        float tm = CT_OUT;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          tm = fmaxf(fmaxf(fmaxf(z[j][0], z[j][1]), fmaxf(z[j][2], z[j][3])), tm);
+        if (a.tmax && n < a.N && v0 < a.V)
+          a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] = tm;
+        const float mn = fmaxf(m[i], tm), d = m[i] - mn;
+        const float sc = __builtin_amdgcn_exp2f(d);
+        if constexpr (ENT) TT[i] = sc * fmaf(d, L[i], TT[i]);
+        L[i] *= sc;
+        m[i] = mn;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float q = z[j][r] - mn;
+            const float e = __builtin_amdgcn_exp2f(q);
+            L[i] += e;
+            if constexpr (ENT) TT[i] = fmaf(e, q, TT[i]);
+          }
+      } else {
+        if (n < a.Npad) {
+          const bool in = n < a.N;
+          const float4 rc = in ? a.rowc[n] : float4{1.0e30f, 0.f, 0.f, 0.f};
+          const int64_t id = in ? a.ids ? a.ids[n] : -1 : -1;
+          const bool live = rc.x < 1.0e30f;
+          T* o = (T*)a.C + (int64_t)n * a.ldc + vt * CT_TILE + 64 * wv + 4 * g;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f32x4 c;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float lp = z[j][r] - rc.x;  // log2 p
+              const float p = __builtin_amdgcn_exp2f(lp);
+              const float k = ENT ? fmaf(rc.z, fmaf(lp, CT_LN2, rc.w), rc.y) : rc.y;
+              const bool hit = id == (int64_t)(v0 + 16 * j + 4 * g + r);
+              const float q = fmaf(-p, k, hit ? rc.y : 0.0f);
+              c[r] = live && !(z[j][r] == CT_OUT) ? q : 0.0f;
+            }
+            ct_store4<T>(o + 16 * j, c);
+          }
+        }
+      }
+    }
+  }
+  if constexpr (!COEF) {
+    ct_barrier();  // the last stage's reads are over: its memory takes the waves' statistics
+    float* red = (float*)smem;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int o = 16; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(m[i], o, 64), L2 = __shfl_xor(L[i], o, 64), T2 = __shfl_xor(TT[i], o, 64);
+        stat_join(m[i], L[i], TT[i], m2, L2, T2);
+      }
+      if (wv == 1 && g == 0) {
+        float* r = red + (64 * wn + 16 * i + rl) * 3;
+        r[0] = m[i];
+        r[1] = L[i];
+        r[2] = TT[i];
+      }
+    }
+    ct_barrier();
+    if (wv == 0 && g == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* r = red + (64 * wn + 16 * i + rl) * 3;
+        stat_join(m[i], L[i], TT[i], r[0], r[1], r[2]);
+        const int n = n0 + 64 * wn + 16 * i + rl;
+        if (n < a.N) a.part[(int64_t)sp * a.N + n] = float4{m[i], L[i], TT[i], 0.0f};
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float ct_elt(const T* p, int64_t i) {
+  if constexpr (sizeof(T) == 4) return p[i];
+  else return __uint_as_float((uint32_t)p[i] << 16);
+}
+template <typename T>
+__device__ __forceinline__ double wave_dot64(const T* x, const T* w, int E, int lane) {
+  double d = 0.0;
+  for (int e = lane; e < E; e += 64) d = fma((double)ct_elt(x, e), (double)ct_elt(w, e), d);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
+  return d;
+}
+
+// One wave per row: the shares' statistics joined, the given item's logit.
+template <typename T>
+__global__ __launch_bounds__(256) void k_combine(const float4* __restrict__ part, int splits, int N,
+                                                 int V, int E, const T* __restrict__ x, int64_t ldx,
+                                                 const T* __restrict__ w, int64_t ldw,
+                                                 const int64_t* __restrict__ ids,
+                                                 const float* __restrict__ bias, double s,
+                                                 float* __restrict__ logp, float* __restrict__ ent,
+                                                 float* __restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  float m = CT_NONE, L = 0.0f, TT = 0.0f;
+  for (int i = lane; i < splits; i += 64) {
+    const float4 p = part[(int64_t)i * N + n];
+    stat_join(m, L, TT, p.x, p.y, p.z);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float m2 = __shfl_xor(m, o, 64), L2 = __shfl_xor(L, o, 64), T2 = __shfl_xor(TT, o, 64);
+    stat_join(m, L, TT, m2, L2, T2);
+  }
+  const float inf = __builtin_huge_valf();
+  const bool empty = m <= CT_OUT && L == L;  // every item taken out (and no NaN)
+  const double l2 = log2((double)L);
+  const double ls = ((double)m + l2) * 0.6931471805599453;
+  if (logp) {
+    const int64_t id = ids[n];
+    float o = 0.0f;
+    if (id >= 0 && id < V) {
+      const float b = bias ? bias[id] : 0.0f;
+      const double l = s * wave_dot64(x + n * ldx, w + id * ldw, E, lane) + (double)b;
+      o = empty || b <= CT_OUT ? -inf : (float)(l - ls);
+    }
+    if (lane == 0) logp[n] = o;
+  }
+  if (lane == 0) {
+    if (ent) ent[n] = empty ? 0.0f : (float)((l2 - (double)TT / (double)L) * 0.6931471805599453);
+    lse[n] = empty ? -inf : (float)ls;
+  }
+}
+
+// ------------------------------------------------------------------- top alternatives
+// The keep largest of 64 x PER keys (+ the keep carried in `have`, one a lane), into lanes 0 .. keep
+// - 1 in descending order.  One maximum a round.
+template <int PER>
+__device__ __forceinline__ uint64_t wave_top(uint64_t (&key)[PER], uint64_t have, int keep, int lane) {
+  uint64_t out = 0;
+  for (int r = 0; r < keep; ++r) {
+    uint64_t best = have;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) best = key[i] > best ? key[i] : best;
+    uint64_t mx = best;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t t = shfl_xor_u64(mx, o);
+      mx = t > mx ? t : mx;
+    }
+    if (mx == 0) break;  // (keys are unique and above 0)
+    if (lane == r) out = mx;
+    if (have == mx) have = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] == mx) key[i] = 0;
+  }
+  return out;
+}
+
+// Groups of 16 items (tmax entries) of one row: the keep largest of every segment, key = (maximum,
+// ~group).  Block = (segment, row); its 4 waves take 1024 entries each at a time.
+__global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tmax, int64_t M, int seg_len,
+                                                    int nseg, int keep, uint64_t* __restrict__ out) {
+  __shared__ uint64_t red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t n = blockIdx.x / nseg;
+  const int sg = (int)(blockIdx.x % nseg);
+  const int64_t i0 = (int64_t)sg * seg_len, i1 = i0 + seg_len < M ? i0 + seg_len : M;
+  const float* row = tmax + n * M;
+  uint64_t have = 0;
+  for (int64_t b = i0 + w * 1024; b < i1; b += 4096) {
+    uint64_t key[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int64_t e = b + i * 64 + lane;
+      key[i] = e < i1 ? make_key(row[e], (uint32_t)e) : 0ull;
+    }
+    have = wave_top<16>(key, have, keep, lane);
+  }
+  red[w][lane] = have;
+  __syncthreads();
+  if (w == 0) {
+    uint64_t key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key[i] = red[i][lane];
+    const uint64_t r = wave_top<4>(key, 0ull, keep, lane);
+    if (lane < keep) out[(n * nseg + sg) * keep + lane] = r;
+  }
+}
+
+// One block per row: the keep largest groups of all segments, their items scored in 64 bits, the top
+// of them by (score, lower id).
+template <typename T>
+__global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ segs, int nseg, int keep,
+                                                   int top, const T* __restrict__ x, int64_t ldx,
+                                                   const T* __restrict__ w, int64_t ldw, int E, int V,
+                                                   const float* __restrict__ bias, double s,
+                                                   const float* __restrict__ lse,
+                                                   int64_t* __restrict__ ids_out, float* __restrict__ lp_out) {
+  constexpr int GMAX = CT_TOP_MAX + CT_TOP_EXTRA;
+  __shared__ uint64_t red[4][64];
+  __shared__ uint32_t grp[GMAX];
+  __shared__ int ngrp;
+  __shared__ double sc[GMAX * 16];
+  __shared__ int vid[GMAX * 16];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t n = blockIdx.x;
+  const int total = nseg * keep;
+  const uint64_t* src = segs + n * total;
+  uint64_t have = 0;
+  for (int b = wv * 256; b < total; b += 1024) {
+    uint64_t key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key[i] = b + i * 64 + lane < total ? src[b + i * 64 + lane] : 0ull;
+    have = wave_top<4>(key, have, keep, lane);
+  }
+  red[wv][lane] = have;
+  __syncthreads();
+  if (wv == 0) {
+    uint64_t key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key[i] = red[i][lane];
+    const uint64_t r = wave_top<4>(key, 0ull, keep, lane);
+    // groups that cannot hold one of the top: clearly below the top-th maximum (the margin is far
+    // above what 32-bit sums are off; see the ordering in 64 bits below)
+    const float kth = key_score(__shfl(r, top - 1 < keep ? top - 1 : keep - 1, 64));
+    const float best = key_score(__shfl(r, 0, 64));
+    const float margin = 0.0009765625f * (fabsf(kth) + fabsf(best) + 1.0f);
+    const bool use = lane < keep && r != 0 && !(key_score(r) < kth - margin);
+    const uint64_t bm = __ballot(use);
+    if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(r);
+    if (lane == 0) ngrp = __popcll(bm);
+  }
+  __syncthreads();
+  const int cand = ngrp * 16;
+  const T* xr = x + n * ldx;
+  // 16 lanes an item, 16 items of one group at a time
+  const int sub = tid >> 4, l16 = tid & 15;
+  for (int gi = 0; gi < ngrp; ++gi) {
+    const uint32_t q = grp[gi];
+    const int v = (int)(q >> 2) * 64 + 16 * (sub >> 2) + 4 * (int)(q & 3) + (sub & 3);
+    double d = 0.0;
+    if (v < V) {
+      const T* wr = w + (int64_t)v * ldw;
+      for (int e = l16; e < E; e += 16) d = fma((double)ct_elt(xr, e), (double)ct_elt(wr, e), d);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) d += __shfl_xor(d, o, 64);
+    if (l16 == 0) {
+      double l = -__builtin_huge_val();
+      if (v < V) {
+        const float b = bias ? bias[v] : 0.0f;
+        if (!(b <= CT_OUT)) l = s * d + (double)b;
+      }
+      sc[gi * 16 + sub] = l;
+      vid[gi * 16 + sub] = v < V ? v : 0x7fffffff;
+    }
+  }
+  __syncthreads();
+  const float ls = lse[n];
+  for (int c = tid; c < cand; c += 256) {
+    const double l = sc[c];
+    const int v = vid[c];
+    int rank = 0;  // NaN scores rank by id alone among themselves, below all others
+    for (int o = 0; o < cand; ++o) {
+      const double t = sc[o];
+      const bool gt = t > l || (l != l && t == t);
+      const bool eq = t == l || (t != t && l != l);
+      rank += gt || (eq && vid[o] < v) ? 1 : 0;
+    }
+    if (rank < top && v < V) {
+      ids_out[n * top + rank] = v;
+      lp_out[n * top + rank] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : (float)(l - (double)ls);
+    }
+  }
+}
+
+// ------------------------------------------------------------------- backward
+// Row constants, x with its dead rows (no gradient, or nothing to choose from) set to zero.
+template <typename T>
+__global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t ldx, int N, int E,
+                                              const float* __restrict__ lse, const float* __restrict__ ent,
+                                              const float* __restrict__ g, const float* __restrict__ e,
+                                              const int64_t* __restrict__ ids, int V,
+                                              float4* __restrict__ rowc, T* __restrict__ xo) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  const int64_t id = ids ? ids[n] : -1;
+  const float gn = g && id >= 0 && id < V ? g[n] : 0.0f, en = e ? e[n] : 0.0f;
+  const bool live = (gn != 0.0f || en != 0.0f) && !(lse[n] == -__builtin_huge_valf());
+  if (lane == 0)
+    rowc[n] = live ? float4{(float)((double)lse[n] * 1.4426950408889634), gn, en, ent ? ent[n] : 0.0f}
+                   : float4{1.0e30f, 0.f, 0.f, 0.f};
+  constexpr int PC = 16 / (int)sizeof(T);
+  for (int c = lane * PC; c < E; c += 64 * PC)
+    *(u32x4_t*)(xo + n * E + c) = live ? *(const u32x4_t*)(x + n * ldx + c) : u32x4_t{0, 0, 0, 0};
+}
+// w with the rows of items that are taken out set to zero (they may hold anything)
+template <typename T>
+__global__ __launch_bounds__(256) void k_items(const T* __restrict__ w, int64_t ldw, int V, int E,
+                                               const float* __restrict__ bias, T* __restrict__ wo) {
+  constexpr int PC = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 63;
+  for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < V; v += (int64_t)gridDim.x * 4) {
+    const bool out = bias[v] <= CT_OUT;
+    for (int c = lane * PC; c < E; c += 64 * PC)
+      *(u32x4_t*)(wo + v * E + c) = out ? u32x4_t{0, 0, 0, 0} : *(const u32x4_t*)(w + v * ldw + c);
+  }
+}
+
+// out[m][c] = scale sum_k A[m, k] B[k, c]; B [K rows, cols] as it lies; A rows [m][k] (ACOL false) or
+// as it lies [k][m] (ACOL).  K a multiple of BK (rows past a's or b's end are zero in A).  splits > 1
+// or acc: f32 partial sums part[split][M][cols] (acc: added to what is there), else out.
+struct ProductArgs {
+  const void *A, *B;
+  int64_t lda, ldb, a_rows, b_rows;
+  int M, cols, K, splits;
+  bool acc;
+  float scale;
+  void* out;
+  int64_t ldo;
+  float* part;
+};
+template <typename T, bool ACOL>
+__global__ __launch_bounds__(256, 2) void k_product(const ProductArgs a) {
+  constexpr int BK = 128 / (int)sizeof(T);
+  __shared__ __attribute__((aligned(16))) char smem[4 * CT_OP_B];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = w >> 1, wc = w & 1, g = lane >> 4, rl = lane & 15;
+  const int tc = (a.cols + CT_TILE - 1) / CT_TILE, tm = (a.M + CT_TILE - 1) / CT_TILE;
+  const int lb = xcd_remap(blockIdx.x, gridDim.x);
+  const int sp = lb / (tc * tm), t = lb % (tc * tm);
+  const int m0 = t / tc * CT_TILE, c0 = t % tc * CT_TILE;
+  const T* A = (const T*)a.A;
+  const T* B = (const T*)a.B;
+  const int nk = a.K / BK, per = (nk + a.splits - 1) / a.splits;
+  const int k0 = sp * per, k1 = k0 + per < nk ? k0 + per : nk;
+  RowStage<T> ra;
+  ColStage<T> ca, cb;
+  if constexpr (ACOL) ca.init(m0, a.lda, w, lane);  // (lda: whole tiles, all written)
+  else ra.init(a.lda, m0, a.a_rows, w, lane);
+  cb.init(c0, a.cols, w, lane);
+  auto issue = [&](int kt) __attribute__((always_inline)) {
+    char* st = smem + (kt & 1) * 2 * CT_OP_B;
+    if constexpr (ACOL) ca.issue(A, a.lda, (int64_t)kt * BK, a.a_rows, st, w);
+    else ra.issue(A, (int64_t)kt * BK, st, w);
+    cb.issue(B, a.ldb, (int64_t)kt * BK, a.b_rows, st + CT_OP_B, w);
+  };
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (k0 < k1) issue(k0);
+  for (int kt = k0; kt < k1; ++kt) {
+    ct_wait_vm<0>();
+    ct_barrier();
+    if (kt + 1 < k1) issue(kt + 1);
+    const char* st = smem + (kt & 1) * 2 * CT_OP_B;
+    u32x4_t fa[2][4], fb[2][4];
+    if constexpr (ACOL) col_frags<T>(st, 64 * wm, lane, fa);
+    else row_frags(st, 64 * wm, lane, fa);
+    col_frags<T>(st + CT_OP_B, 64 * wc, lane, fb);
+    ct_mfma<T>(fb, fa, acc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int mm = m0 + 64 * wm + 16 * i + rl;
+    if (mm >= a.M) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = c0 + 64 * wc + 16 * j + 4 * g;
+      if (c >= a.cols) continue;
+      if (a.part) {
+        f32x4* p = (f32x4*)(a.part + ((int64_t)sp * a.M + mm) * a.cols + c);
+        *p = a.acc ? *p + acc[i][j] : acc[i][j];
+      } else {
+        ct_store4<T>((T*)a.out + (int64_t)mm * a.ldo + c, acc[i][j] * a.scale);
+      }
+    }
+  }
+}
+// out = scale * (sum over the splits, in order)
+template <typename T>
+__global__ __launch_bounds__(256) void k_product_sum(const float* __restrict__ part, int splits, int64_t n4,
+                                                     float scale, T* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+    f32x4 s = ((const f32x4*)part)[i];
+    for (int k = 1; k < splits; ++k) s = s + ((const f32x4*)part)[(int64_t)k * n4 + i];
+    ct_store4<T>(out + 4 * i, s * scale);
+  }
+}
+
+// ------------------------------------------------------------------------------- host side
+static int64_t up(int64_t n, int64_t q) { return (n + q - 1) / q * q; }
+static int64_t cdiv(int64_t n, int64_t q) { return (n + q - 1) / q; }
+
+struct StatPlan {
+  int n_tiles, v_tiles, splits, keep, nseg, seg_len;
+  int64_t M, off_tmax, off_seg, bytes;
+};
+// Shares: about 512 blocks (two a CU).
+static StatPlan stat_plan(int64_t N, int64_t V, int top) {
+  StatPlan p{};
+  p.n_tiles = (int)cdiv(N, CT_TILE);
+  p.v_tiles = (int)cdiv(V, CT_TILE);
+  int64_t s = 512 / p.n_tiles;
+  s = s < 1 ? 1 : s > p.v_tiles ? p.v_tiles : s;
+  p.splits = (int)cdiv(p.v_tiles, cdiv(p.v_tiles, s));
+  p.bytes = up((int64_t)p.splits * N * 16, 256);
+  if (top > 0) {
+    p.keep = top + CT_TOP_EXTRA;
+    p.M = 4 * cdiv(V, 64);
+    // segments of 4096 groups, longer ones past 64 segments a row
+    p.seg_len = (int)(4096 * cdiv(p.M, 4096 * 64));
+    p.nseg = (int)cdiv(p.M, p.seg_len);
+    p.off_tmax = p.bytes;
+    p.off_seg = p.off_tmax + up(N * p.M * 4, 256);
+    p.bytes = p.off_seg + up(N * p.nseg * p.keep * 8, 256);
+  }
+  return p;
+}
+
+constexpr int64_t CT_C_BYTES = 256ll << 20;  // one chunk of C stays in the last-level cache
+struct BwdPlan {
+  int64_t Npad, Vc, n_chunks;
+  int sx, sw;
+  int64_t off_row, off_x, off_w, off_c, off_px, off_pw, bytes;
+};
+static int product_splits(int64_t M, int64_t cols, int64_t K, int BK) {
+  const int64_t tiles = cdiv(M, CT_TILE) * cdiv(cols, CT_TILE), nk = K / BK;
+  int64_t s = cdiv(512, tiles), most = nk / 4 > 1 ? nk / 4 : 1;
+  s = s < most ? s : most;
+  return (int)cdiv(nk, cdiv(nk, s));  // no empty split
+}
+static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, bool dx, bool dw) {
+  BwdPlan p{};
+  const int BK = (int)(128 / sz);
+  p.Npad = up(N, 64);
+  int64_t vc = CT_C_BYTES / (p.Npad * sz) / CT_TILE * CT_TILE;
+  vc = vc < CT_TILE ? CT_TILE : vc;
+  p.Vc = vc < up(V, CT_TILE) ? vc : up(V, CT_TILE);
+  p.n_chunks = cdiv(V, p.Vc);
+  int64_t o = up(N * 16, 256);
+  p.off_x = o;
+  o += up(N * E * sz, 256);
+  p.off_w = o;
+  if (bias) o += up(V * E * sz, 256);
+  p.off_c = o;
+  o += up(p.Npad * p.Vc * sz, 256);
+  p.sx = product_splits(N, E, p.Vc, BK);
+  p.sw = product_splits(p.Vc, E, p.Npad, BK);
+  p.off_px = o;
+  if (dx && (p.sx > 1 || p.n_chunks > 1)) o += up((int64_t)p.sx * N * E * 4, 256);
+  p.off_pw = o;
+  if (dw && p.sw > 1) o += up((int64_t)p.sw * p.Vc * E * 4, 256);
+  p.bytes = o;
+  return p;
+}
+
+static int ct_check(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype, int64_t N,
+                    int64_t V, int32_t E, float temperature, const char* fn) {
+  auto bad = [&](const char* m) { return fail(TT_ERR_INVALID, std::string(fn) + ": " + m); };
+  if (dtype != TT_DTYPE_F32 && dtype != TT_DTYPE_BF16) return bad("dtype must be f32 or bf16");
+  if (N < 0 || V < 1 || E < 64 || E % 64 != 0) return bad("need N >= 0, V >= 1, E a multiple of 64");
+  if (N >= (1ll << 24) || V >= (1ll << 30) || E > (1 << 20)) return bad("sizes out of range");
+  if (!(temperature > 0.0f)) return bad("temperature must be above 0");
+  if (N == 0) return TT_OK;
+  if (!x || !w) return bad("null pointer");
+  const int64_t sz = dtype == TT_DTYPE_F32 ? 4 : 2;
+  if (((uintptr_t)x | (uintptr_t)w) % 16 || (ldx * sz) % 16 || (ldw * sz) % 16 || ldx < E || ldw < E)
+    return bad("rows must be 16-byte aligned and at least E long");
+  return TT_OK;
+}
+
+template <typename T>
+static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int E,
+                        const int64_t* ids, const float* bias, float temperature, float* logp, float* ent,
+                        float* lse, int top, int64_t* top_ids, float* top_lp, char* ws, const StatPlan& p,
+                        hipStream_t st) {
+  const double s = 1.0 / (double)temperature;
+  LogitArgs a{};
+  a.x = x; a.w = w; a.ldx = ldx; a.ldw = ldw; a.bias = bias;
+  a.s2 = (float)(s * 1.4426950408889634);
+  a.N = (int)N; a.V = (int)V; a.E = E;
+  a.n_tiles = p.n_tiles; a.splits = p.splits; a.v_tiles = p.v_tiles;
+  a.part = (float4*)ws;
+  a.tmax = top ? (float*)(ws + p.off_tmax) : nullptr;
+  const dim3 grid((unsigned)(p.n_tiles * (int64_t)p.splits));
+  if (ent) hipLaunchKernelGGL((k_logits<T, false, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_logits<T, false, false>), grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_combine<T>, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, st, a.part, p.splits, (int)N,
+                     (int)V, E, (const T*)x, ldx, (const T*)w, ldw, ids, bias, s, logp, ent, lse);
+  if (top) {
+    uint64_t* seg = (uint64_t*)(ws + p.off_seg);
+    hipLaunchKernelGGL(k_top_groups, dim3((unsigned)(N * p.nseg)), dim3(256), 0, st, a.tmax, p.M, p.seg_len,
+                       p.nseg, p.keep, seg);
+    hipLaunchKernelGGL(k_top_items<T>, dim3((unsigned)N), dim3(256), 0, st, seg, p.nseg, p.keep, top,
+                       (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+  }
+  return check_launch("tt_catalog_logprobs");
+}
+
+template <typename T>
+static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int E,
+                        const int64_t* ids, const float* bias, float temperature, const float* lse,
+                        const float* ent, const float* g, const float* e, void* dx, void* dw, char* ws,
+                        const BwdPlan& p, hipStream_t st) {
+  const double s = 1.0 / (double)temperature;
+  float4* rowc = (float4*)ws;
+  T* xz = (T*)(ws + p.off_x);
+  hipLaunchKernelGGL(k_rows<T>, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, st, (const T*)x, ldx, (int)N, E, lse,
+                     ent, g, e, ids, (int)V, rowc, xz);
+  const T* wz = (const T*)w;
+  int64_t ldwz = ldw;
+  if (bias) {
+    const int64_t nb = cdiv(V, 4);
+    hipLaunchKernelGGL(k_items<T>, dim3((unsigned)(nb < 8192 ? nb : 8192)), dim3(256), 0, st, (const T*)w, ldw,
+                       (int)V, E, bias, (T*)(ws + p.off_w));
+    wz = (const T*)(ws + p.off_w);
+    ldwz = E;
+  }
+  T* C = (T*)(ws + p.off_c);
+  float* px = (float*)(ws + p.off_px);
+  const bool part_x = p.sx > 1 || p.n_chunks > 1;
+  for (int64_t c = 0; c < p.n_chunks; ++c) {
+    const int64_t vb = c * p.Vc, vn = V - vb < p.Vc ? V - vb : p.Vc;
+    LogitArgs a{};
+    a.x = xz; a.w = wz; a.ldx = E; a.ldw = ldwz; a.bias = bias;
+    a.s2 = (float)(s * 1.4426950408889634);
+    a.N = (int)N; a.V = (int)V; a.E = E;
+    a.n_tiles = (int)cdiv(N, CT_TILE);
+    a.v_tiles = a.splits = (int)cdiv(vn, CT_TILE);
+    a.rowc = rowc; a.ids = ids; a.C = C; a.ldc = p.Vc; a.v_base = (int)vb; a.Npad = (int)p.Npad;
+    const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits));
+    if (e) hipLaunchKernelGGL((k_logits<T, true, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_logits<T, true, false>), grid, dim3(256), 0, st, a);
+    const int64_t vk = up(vn, CT_TILE);
+    if (dx) {
+      ProductArgs q{};
+      q.A = C; q.lda = p.Vc; q.a_rows = p.Npad;
+      q.B = wz + vb * ldwz; q.ldb = ldwz; q.b_rows = V - vb;
+      q.M = (int)N; q.cols = E; q.K = (int)vk; q.splits = p.sx;
+      q.acc = c > 0; q.scale = (float)s; q.out = dx; q.ldo = E;
+      q.part = part_x ? px : nullptr;
+      hipLaunchKernelGGL((k_product<T, false>),
+                         dim3((unsigned)(cdiv(N, CT_TILE) * cdiv(E, CT_TILE) * p.sx)), dim3(256), 0, st, q);
+    }
+    if (dw) {
+      ProductArgs q{};
+      q.A = C; q.lda = p.Vc; q.a_rows = p.Npad;
+      q.B = xz; q.ldb = E; q.b_rows = N;
+      q.M = (int)vn; q.cols = E; q.K = (int)p.Npad; q.splits = p.sw;
+      q.scale = (float)s; q.out = (T*)dw + vb * E; q.ldo = E;
+      q.part = p.sw > 1 ? (float*)(ws + p.off_pw) : nullptr;
+      hipLaunchKernelGGL((k_product<T, true>),
+                         dim3((unsigned)(cdiv(vn, CT_TILE) * cdiv(E, CT_TILE) * p.sw)), dim3(256), 0, st, q);
+      if (q.part) {
+        const int64_t n4 = vn * E / 4, nb = cdiv(n4, 256);
+        hipLaunchKernelGGL(k_product_sum<T>, dim3((unsigned)(nb < 8192 ? nb : 8192)), dim3(256), 0, st,
+                           q.part, p.sw, n4, (float)s, (T*)q.out);
+      }
+    }
+  }
+  if (dx && part_x) {
+    const int64_t n4 = N * E / 4, nb = cdiv(n4, 256);
+    hipLaunchKernelGGL(k_product_sum<T>, dim3((unsigned)(nb < 8192 ? nb : 8192)), dim3(256), 0, st, px, p.sx, n4,
+                       (float)s, (T*)dx);
+  }
+  return check_launch("tt_catalog_logprobs_bwd");
+}
+
+}  // namespace tt
+
+using namespace tt;
+
+#define CT_SIZES_ONLY()                                                                            \
+  TT_REQUIRE(bytes, "null pointer");                                                               \
+  TT_REQUIRE(dtype == TT_DTYPE_F32 || dtype == TT_DTYPE_BF16, "dtype must be f32 or bf16");        \
+  TT_REQUIRE(N >= 0 && V >= 1 && E >= 64 && E % 64 == 0 && N < (1ll << 24) && V < (1ll << 30),     \
+             "sizes out of range")
+
+extern "C" int tt_catalog_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t E, int32_t dtype, int32_t top,
+                                                   int64_t* bytes) {
+  CT_SIZES_ONLY();
+  TT_REQUIRE(top >= 0 && top <= CT_TOP_MAX && top <= V, "need 0 <= top <= min(V, 32)");
+  *bytes = N > 0 ? stat_plan(N, V, top).bytes : 0;
+  return TT_OK;
+}
+
+extern "C" int tt_catalog_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
+                                   int64_t N, int64_t V, int32_t E, const int64_t* ids, const float* bias,
+                                   float temperature, float* log_prob, float* entropy, float* lse, int32_t top,
+                                   int64_t* top_ids, float* top_log_prob, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  if (int rc = ct_check(x, ldx, w, ldw, dtype, N, V, E, temperature, __func__)) return rc;
+  TT_REQUIRE(top >= 0 && top <= CT_TOP_MAX && top <= V, "need 0 <= top <= min(V, 32)");
+  if (N == 0) return TT_OK;
+  TT_REQUIRE(lse && (!log_prob || ids) && (top == 0 || (top_ids && top_log_prob)), "null pointer");
+  const StatPlan p = stat_plan(N, V, top);
+  TT_REQUIRE(N * (int64_t)p.nseg < (1ll << 24), "too many rows for this many items: pass fewer at a time");
+  if (!workspace || workspace_bytes < p.bytes)
+    return fail(TT_ERR_WORKSPACE, "tt_catalog_logprobs: workspace too small");
+  auto f = dtype == TT_DTYPE_F32 ? logprobs_fwd<float> : logprobs_fwd<uint16_t>;
+  return f(x, ldx, w, ldw, N, V, E, ids, bias, temperature, log_prob, entropy, lse, top, top_ids, top_log_prob,
+           (char*)workspace, p, (hipStream_t)stream);
+}
+
+extern "C" int tt_catalog_logprobs_bwd_workspace_bytes(int64_t N, int64_t V, int32_t E, int32_t dtype,
+                                                       int32_t has_bias, int32_t want_dx, int32_t want_dw,
+                                                       int64_t* bytes) {
+  CT_SIZES_ONLY();
+  *bytes = N > 0 ? bwd_plan(N, V, E, dtype == TT_DTYPE_F32 ? 4 : 2, has_bias != 0, want_dx != 0, want_dw != 0).bytes
+                 : 0;
+  return TT_OK;
+}
+
+extern "C" int tt_catalog_logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
+                                       int64_t N, int64_t V, int32_t E, const int64_t* ids, const float* bias,
+                                       float temperature, const float* lse, const float* entropy,
+                                       const float* g_log_prob, const float* g_entropy, void* dx, void* dw,
+                                       void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = ct_check(x, ldx, w, ldw, dtype, N, V, E, temperature, __func__)) return rc;
+  if (N == 0) {
+    TT_REQUIRE(!dw, "dw without rows: fill it with zeros");
+    return TT_OK;
+  }
+  TT_REQUIRE(lse && (!g_log_prob || ids) && (!g_entropy || entropy), "null pointer");
+  TT_REQUIRE(((uintptr_t)dx | (uintptr_t)dw) % 16 == 0, "dx and dw must be 16-byte aligned");
+  const BwdPlan p = bwd_plan(N, V, E, dtype == TT_DTYPE_F32 ? 4 : 2, bias != nullptr, dx != nullptr, dw != nullptr);
+  if (!workspace || workspace_bytes < p.bytes)
+    return fail(TT_ERR_WORKSPACE, "tt_catalog_logprobs_bwd: workspace too small");
+  auto f = dtype == TT_DTYPE_F32 ? logprobs_bwd<float> : logprobs_bwd<uint16_t>;
+  return f(x, ldx, w, ldw, N, V, E, ids, bias, temperature, lse, entropy, g_log_prob, g_entropy, dx, dw,
+           (char*)workspace, p, (hipStream_t)stream);
+}

@@ -221,6 +221,16 @@ SIGNATURES = {
                                      ctypes.c_double, ctypes.c_double, _vp]),
     "tt_adamw_decode": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
     "tt_adamw_encode": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "tt_catalog_logprobs_workspace_bytes": (ctypes.c_int, [_i64, _i64, _i32, _i32, _i32,
+                                                           ctypes.POINTER(_i64)]),
+    "tt_catalog_logprobs": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i32, _vp, _vp,
+                                           ctypes.c_float, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
+                                           _i64, _vp]),
+    "tt_catalog_logprobs_bwd_workspace_bytes": (ctypes.c_int, [_i64, _i64, _i32, _i32, _i32, _i32,
+                                                               _i32, ctypes.POINTER(_i64)]),
+    "tt_catalog_logprobs_bwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i32, _vp,
+                                               _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp,
+                                               _vp, _i64, _vp]),
 }
 
 

@@ -166,13 +166,15 @@ class Evaluator:
         self._cache[key] = out
         return out
 
-    def _batch(self, chunk, k) -> List[List[str]]:
-        histories = [inter for _, inter, _ in chunk]
+    def _encode(self, histories) -> np.ndarray:
         if hasattr(self.encoder, "encode_buyers"):
             emb = self.encoder.encode_buyers(histories, mode=self.mode)
         else:
             emb = np.stack([self.encoder.encode_buyer(h) for h in histories])
-        results = self.vector_db.retrieve_batch(np.asarray(emb, dtype=np.float32), k=k)
+        return np.asarray(emb, dtype=np.float32)
+
+    def _batch(self, chunk, k) -> List[List[str]]:
+        results = self.vector_db.retrieve_batch(self._encode([inter for _, inter, _ in chunk]), k=k)
         return [[pid for pid, _ in r] for r in results]
 
     # reference :372-512
@@ -261,6 +263,30 @@ class Evaluator:
                 seen.update(r)
         return {"coverage": compute_coverage(seen, set(all_product_ids)),
                 "unique_retrieved": len(seen), "total_products": len(all_product_ids)}
+
+    # an addition: the reference scores ranks only
+    def evaluate_likelihood(self, test_pairs, temperature: float = 0.07) -> Dict[str, float]:
+        """How probable the relevant items are under softmax(cosine / temperature) over the whole
+        catalog (VectorDatabase.log_probs): mean log-probability, its perplexity, and the mean
+        entropy of the buyers' distributions.  Relevant items that the catalog lacks do not
+        count."""
+        lp: List[float] = []
+        ent: List[float] = []
+        for b0 in range(0, len(test_pairs), self.batch_size):
+            chunk = test_pairs[b0: b0 + self.batch_size]
+            emb = self._encode([inter for _, inter, _ in chunk])
+            rows = [(i, p) for i, (_, _, rel) in enumerate(chunk) for p in sorted(rel)
+                    if p in self.vector_db.id_to_index]
+            if rows:
+                v, e, _ = self.vector_db.log_probs(emb[[i for i, _ in rows]],
+                                                   [p for _, p in rows], temperature)
+                lp.extend(v.tolist())
+                ent.extend({i: x for (i, _), x in zip(rows, e.tolist())}.values())
+        if not lp:
+            return {}
+        mean = float(np.mean(lp))
+        return {"log_prob_mean": mean, "perplexity": float(np.exp(-mean)),
+                "entropy_mean": float(np.mean(ent)), "items": len(lp)}
 
     # reference :641-700
     def evaluate_all(self, test_pairs, k_values: List[int] = [1, 5, 10, 20, 50],

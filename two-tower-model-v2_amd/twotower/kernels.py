@@ -709,3 +709,110 @@ def gated_scan_backward(x, gate, weights, saved, dh, dlast, need_h0: bool):
             _ptr(dx), _ptr(dgate), _ptr(dh0), _ptr(ws), ws.numel() if ws is not None else 0,
             stream_ptr()), "tt_gated_scan_bwd")
     return dx, dgate, dh0
+
+
+CATALOG_TOP_MAX = 32  # alternatives per row of catalog_logprobs
+
+
+def catalog_rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows as the catalog_logprobs kernels read them: length a multiple of 64 (zero columns are
+    added, which change no product), channels contiguous, rows 16-byte aligned.  No copy if they
+    already are."""
+    pad = (-t.shape[1]) % 64
+    if pad:
+        return torch.nn.functional.pad(t, (0, pad))
+    sz = t.element_size()
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1] or t.stride(0) * sz % 16 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _catalog_args(x, w, ids, bias):
+    require_device(x, "queries")
+    require_device(w, "items")
+    if x.dtype not in _lib.DTYPES or w.dtype != x.dtype:
+        raise TypeError("catalog_logprobs: queries and items must both be float32 or bfloat16, got "
+                        f"{x.dtype} and {w.dtype}")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.shape[1] < 1:
+        raise ValueError("catalog_logprobs: need queries [N, E] and items [V, E], got "
+                         f"{tuple(x.shape)} and {tuple(w.shape)}")
+    if w.shape[0] < 1:
+        raise ValueError("catalog_logprobs: no items")
+    if ids is not None and (tuple(ids.shape) != (x.shape[0],) or ids.dtype != torch.int64):
+        raise ValueError(f"catalog_logprobs: ids must be int64 [{x.shape[0]}], got {ids.dtype} "
+                         f"{tuple(ids.shape)}")
+    if bias is not None and tuple(bias.shape) != (w.shape[0],):
+        raise ValueError(f"catalog_logprobs: bias must be [{w.shape[0]}], got {tuple(bias.shape)}")
+    for t, name in ((w, "items"), (ids, "ids"), (bias, "bias")):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"catalog_logprobs: {name} on {t.device}, queries on {x.device}")
+
+
+def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entropy: bool = False,
+                     top: int = 0):
+    """tt_catalog_logprobs on catalog_rows' x [N, E] and w [V, E] -> (log_prob [N] f32 or None
+    without ids, entropy [N] f32 or None, lse [N] f32, top_ids [N, top] int64 and top_log_prob
+    [N, top] f32 or None)."""
+    _catalog_args(x, w, ids, bias)
+    n, e = x.shape
+    v = w.shape[0]
+    if not 0 <= top <= min(v, CATALOG_TOP_MAX):
+        raise ValueError(f"catalog_logprobs: need 0 <= top ({top}) <= min({v} items, "
+                         f"{CATALOG_TOP_MAX})")
+    if not temperature > 0:
+        raise ValueError(f"catalog_logprobs: temperature must be above 0, got {temperature}")
+    dt = _lib.DTYPES[x.dtype]
+    with _lib.on_device(x):
+        ids = ids.contiguous() if ids is not None else None
+        bias = bias.to(_f32).contiguous() if bias is not None else None
+        dev = x.device
+        lp = torch.empty(n, dtype=_f32, device=dev) if ids is not None else None
+        ent = torch.empty(n, dtype=_f32, device=dev) if entropy else None
+        lse = torch.empty(n, dtype=_f32, device=dev)
+        ti = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
+        tl = torch.empty((n, top), dtype=_f32, device=dev) if top else None
+        need = ctypes.c_int64(0)
+        check(lib().tt_catalog_logprobs_workspace_bytes(n, v, e, dt, top, ctypes.byref(need)),
+              "tt_catalog_logprobs_workspace_bytes")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        check(lib().tt_catalog_logprobs(
+            _ptr(x), x.stride(0), _ptr(w), w.stride(0), dt, n, v, e, _ptr(ids), _ptr(bias),
+            temperature, _ptr(lp), _ptr(ent), _ptr(lse), top, _ptr(ti), _ptr(tl), _ptr(ws),
+            ws.numel(), stream_ptr()), "tt_catalog_logprobs")
+    return lp, ent, lse, ti, tl
+
+
+def catalog_logprobs_backward(x, w, ids, bias, temperature, lse, ent, g, ge, need_x: bool,
+                              need_w: bool):
+    """(dx, dw) in x's type, contiguous (None where not needed), for gradients g of log_prob and ge
+    of the entropy ([N] f32, either may be None)."""
+    _catalog_args(x, w, ids, bias)
+    n, e = x.shape
+    v = w.shape[0]
+    for t, name in ((g, "g"), (ge, "ge"), (lse, "lse"), (ent, "entropy")):
+        if t is not None and (tuple(t.shape) != (n,) or t.dtype != _f32 or t.device != x.device):
+            raise ValueError(f"catalog_logprobs_backward: {name} must be float32 [{n}] on {x.device}")
+    if lse is None or (ge is not None and ent is None) or (g is not None and ids is None):
+        raise ValueError("catalog_logprobs_backward: lse, the entropy (for ge) and ids (for g) of "
+                         "the forward call are needed")
+    dt = _lib.DTYPES[x.dtype]
+    with _lib.on_device(x):
+        dev = x.device
+        if n == 0 or (g is None and ge is None):
+            return (torch.zeros((n, e), dtype=x.dtype, device=dev) if need_x else None,
+                    torch.zeros((v, e), dtype=x.dtype, device=dev) if need_w else None)
+        ids = ids.contiguous() if ids is not None else None
+        bias = bias.to(_f32).contiguous() if bias is not None else None
+        g, ge = (t.contiguous() if t is not None else None for t in (g, ge))
+        dx = torch.empty((n, e), dtype=x.dtype, device=dev) if need_x else None
+        dw = torch.empty((v, e), dtype=x.dtype, device=dev) if need_w else None
+        need = ctypes.c_int64(0)
+        check(lib().tt_catalog_logprobs_bwd_workspace_bytes(
+            n, v, e, dt, int(bias is not None), int(need_x), int(need_w), ctypes.byref(need)),
+            "tt_catalog_logprobs_bwd_workspace_bytes")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        check(lib().tt_catalog_logprobs_bwd(
+            _ptr(x), x.stride(0), _ptr(w), w.stride(0), dt, n, v, e, _ptr(ids), _ptr(bias),
+            temperature, _ptr(lse), _ptr(ent), _ptr(g), _ptr(ge), _ptr(dx), _ptr(dw), _ptr(ws),
+            ws.numel(), stream_ptr()), "tt_catalog_logprobs_bwd")
+    return dx, dw

@@ -6,15 +6,20 @@ negative_embeddings) -> scalar loss.  Forward and backward run in one HIP call
 reference's expanded [B, B, E] bmm (:55-61), and the gradients are two more GEMMs; autograd
 receives the precomputed input gradients.  ``prec="bf16"`` runs the GEMMs on bf16 MFMA
 (configs[4]'s "MFMA bf16" training step); the default "f32" matches the reference to ~1e-6.
+
+Beside it, for a softmax over a whole catalog instead of a batch (the reference has none):
+``catalog_log_probs`` (log-probabilities of given items, entropy, top alternatives; csrc/
+tt_catalog.hip, the logits are never stored) and ``CatalogSoftmaxLoss`` over it.
 """
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _lib, kernels
 from ._lib import check, lib, require_device, stream_ptr
 
 
@@ -71,3 +76,90 @@ class InfoNCELoss(nn.Module):
                 negative_embeddings: torch.Tensor) -> torch.Tensor:
         return _InfoNCEFn.apply(buyer_embeddings, positive_embeddings, negative_embeddings,
                                 self.temperature, self.prec)
+
+
+class LogProbs(NamedTuple):
+    """catalog_log_probs' result; what was not asked for is None."""
+    log_prob: Optional[torch.Tensor]  # [N] f32
+    entropy: Optional[torch.Tensor]  # [N] f32
+    top_ids: Optional[torch.Tensor]  # [N, top] int64
+    top_log_probs: Optional[torch.Tensor]  # [N, top] f32
+
+
+class _CatalogFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, ids, bias, temperature, entropy, top):
+        ctx.set_materialize_grads(False)
+        xr, wr = kernels.catalog_rows(x), kernels.catalog_rows(w)
+        lp, ent, lse, ti, tl = kernels.catalog_logprobs(xr, wr, ids, bias, temperature, entropy,
+                                                        top)
+        ctx.save_for_backward(xr, wr, ids, bias, lse, ent)
+        ctx.temperature, ctx.e = temperature, x.shape[1]
+        if top:
+            ctx.mark_non_differentiable(ti, tl)
+        return lp, ent, ti, tl
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, ge, _ti, _tl):
+        if ctx.needs_input_grad[3]:
+            raise NotImplementedError("gradients w.r.t. bias are not computed (it is a correction "
+                                      "of the sampling, not a parameter)")
+        x, w, ids, bias, lse, ent = ctx.saved_tensors
+        dx, dw = kernels.catalog_logprobs_backward(
+            x, w, ids, bias, ctx.temperature, lse, ent, g, ge, ctx.needs_input_grad[0],
+            ctx.needs_input_grad[1])
+        if x.shape[1] != ctx.e:
+            dx, dw = (t[:, :ctx.e] if t is not None else None for t in (dx, dw))
+        return dx, dw, None, None, None, None, None
+
+
+def catalog_log_probs(queries: torch.Tensor, items: torch.Tensor, ids: torch.Tensor = None,
+                      temperature: float = 0.07, bias: torch.Tensor = None, entropy: bool = False,
+                      top: int = 0) -> LogProbs:
+    """Under p(v | n) = softmax_v(queries_n . items_v / temperature + bias_v), for queries [N, E] and
+    items [V, E] (both f32 or both bf16, device):
+
+    log_prob  [N] log p(ids_n | n) for ids [N] int64; 0 for an id of -1 (a row without an item)
+    entropy   [N] (``entropy=True``)
+    top_ids, top_log_probs  [N, top]: the ``top`` (<= 32) most probable items, ordered by the
+              product in 64 bits, ties to the lower id
+
+    ``bias`` [V] f32: e.g. -log q of a sampled-softmax correction; -inf takes the item out (its
+    vector may hold anything).  A row with nothing left: log_prob -inf, entropy 0.  Differentiable in
+    queries and items (log_prob and entropy); the logits are never stored, so N x V is bounded by
+    time alone.  E is padded to a multiple of 64 (a copy) where it is not one."""
+    if torch.is_grad_enabled() and (queries.requires_grad or items.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
+        return LogProbs(*_CatalogFn.apply(queries, items, ids, bias, float(temperature), entropy,
+                                          top))
+    kernels._catalog_args(queries, items, ids, bias)
+    lp, ent, _, ti, tl = kernels.catalog_logprobs(
+        kernels.catalog_rows(queries.detach()), kernels.catalog_rows(items.detach()), ids, bias,
+        float(temperature), entropy, top)
+    return LogProbs(lp, ent, ti, tl)
+
+
+class CatalogSoftmaxLoss(nn.Module):
+    """Mean over the rows of -log p(id | buyer) over all items: InfoNCELoss's task with the whole
+    catalog (or any set of items) as the negatives.  Rows with id -1 do not count."""
+
+    def __init__(self, temperature: float = 0.07, entropy_weight: float = 0.0):
+        super().__init__()
+        if not temperature > 0:
+            raise ValueError(f"temperature must be above 0, got {temperature}")
+        self.temperature = temperature
+        self.entropy_weight = entropy_weight
+
+    def forward(self, buyer_embeddings: torch.Tensor, item_embeddings: torch.Tensor,
+                ids: torch.Tensor, bias: torch.Tensor = None) -> torch.Tensor:
+        """buyer_embeddings [N, E], item_embeddings [V, E], ids [N] -> scalar; entropy_weight > 0
+        also rewards the mean entropy (a penalty on overconfidence)."""
+        r = catalog_log_probs(buyer_embeddings, item_embeddings, ids, self.temperature, bias,
+                              entropy=self.entropy_weight != 0)
+        n = (ids >= 0).sum().clamp(min=1)
+        loss = -r.log_prob.sum() / n
+        if self.entropy_weight != 0:
+            loss = loss - self.entropy_weight * torch.where(
+                ids >= 0, r.entropy, torch.zeros_like(r.entropy)).sum() / n
+        return loss

@@ -700,6 +700,43 @@ class VectorDatabase:
             raise ValueError("Index not built. Call build_index() or load_index() first.")
         return self._to_results(*self._search_host(query_embeddings, k))
 
+    # -------------------------------------------------------------- additions
+    def log_probs(self, query_embeddings: np.ndarray, product_ids: Optional[List[str]] = None,
+                  temperature: float = 0.07, top: int = 0):
+        """Log-probabilities under softmax over the whole catalog of cosine / temperature (the
+        distribution InfoNCE trains towards): for queries [nq, d] and one product id each
+        (None: none) -> (log_prob [nq] float32, NaN for an id that is not in the catalog; entropy
+        [nq] float32; per query the ``top`` (<= 32) most probable products as (id, log_prob))."""
+        if self.index is None:
+            raise ValueError("Index not built. Call build_index() or load_index() first.")
+        q = np.asarray(query_embeddings)
+        q = q.reshape(1, -1) if q.ndim == 1 else q
+        if q.shape[1] != self.embedding_dim:
+            raise ValueError(f"Embedding dimension mismatch: expected {self.embedding_dim}, got "
+                             f"{q.shape[1]}")
+        if product_ids is not None and len(product_ids) != len(q):
+            raise ValueError(f"log_probs: {len(q)} queries, {len(product_ids)} product ids")
+        from .losses import catalog_log_probs
+
+        with _lib.on_device(self.index.xb):
+            dev = self.index.xb.device
+            rows = self.normalize_queries(
+                torch.from_numpy(np.ascontiguousarray(q, dtype=np.float32)).to(dev))
+            ids = None
+            if product_ids is not None:
+                ids = torch.tensor([self.id_to_index.get(p, -1) for p in product_ids],
+                                   dtype=torch.int64, device=dev)
+            r = catalog_log_probs(rows, self.index.xb[:self.index.ntotal], ids, temperature,
+                                  entropy=True, top=min(top, self.index.ntotal))
+            lp = None
+            if ids is not None:
+                lp = torch.where(ids >= 0, r.log_prob,
+                                 torch.full_like(r.log_prob, float("nan"))).cpu().numpy()
+            alt = [[] for _ in range(len(q))]
+            if top:
+                alt = self._to_results(r.top_log_probs.cpu().numpy(), r.top_ids.cpu().numpy())
+            return lp, r.entropy.cpu().numpy(), alt
+
     def get_embedding(self, product_id: str) -> Optional[np.ndarray]:
         """reference :211-231 (always None there: FAISS cannot reconstruct in that code)."""
         if self.index is None or self.id_to_index is None:
