@@ -423,64 +423,110 @@ __global__ __launch_bounds__(256) void k_combine(const float4* __restrict__ part
 }
 
 // ------------------------------------------------------------------- top alternatives
-// The keep largest of 64 x PER keys (+ the keep carried in `have`, one a lane), into lanes 0 .. keep
-// - 1 in descending order.  One maximum a round.
+// The keep largest keys (unique, above 0) of a wave's 64 x PER, written to out[0 .. count) in no
+// order; returns the count (uniform).  The keep-th largest high word is built bit by bit (32 rounds of
+// ballots: scalar work), ties at it by the same search over the low words.
 template <int PER>
-__device__ __forceinline__ uint64_t wave_top(uint64_t (&key)[PER], uint64_t have, int keep, int lane) {
-  uint64_t out = 0;
-  for (int r = 0; r < keep; ++r) {
-    uint64_t best = have;
+__device__ __forceinline__ int wave_select(const uint64_t (&key)[PER], int keep, uint64_t* out, int lane) {
+  int total = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) best = key[i] > best ? key[i] : best;
-    uint64_t mx = best;
+  for (int r = 0; r < PER; ++r) total += __popcll(__ballot(key[r] != 0ull));
+  uint32_t x = 0u, xl = 0u;  // taken: high > x, or high == x and low >= xl
+  if (total > keep) {
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = x | (1u << bit);
+      int c = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t t = shfl_xor_u64(mx, o);
-      mx = t > mx ? t : mx;
+      for (int r = 0; r < PER; ++r) c += __popcll(__ballot((uint32_t)(key[r] >> 32) >= cand));
+      if (c >= keep) x = cand;
     }
-    if (mx == 0) break;  // (keys are unique and above 0)
-    if (lane == r) out = mx;
-    if (have == mx) have = 0;
+    int gt = 0, eq = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] == mx) key[i] = 0;
+    for (int r = 0; r < PER; ++r) {
+      gt += __popcll(__ballot((uint32_t)(key[r] >> 32) > x));
+      eq += __popcll(__ballot((uint32_t)(key[r] >> 32) == x && key[r] != 0ull));
+    }
+    if (eq > keep - gt) {
+#pragma unroll 1
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t cand = xl | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+          c += __popcll(__ballot((uint32_t)(key[r] >> 32) == x && (uint32_t)key[r] >= cand));
+        if (c >= keep - gt) xl = cand;
+      }
+    }
   }
-  return out;
+  int base = 0;
+#pragma unroll
+  for (int r = 0; r < PER; ++r) {
+    const uint32_t h = (uint32_t)(key[r] >> 32);
+    const bool sel = key[r] != 0ull && (h > x || (h == x && (uint32_t)key[r] >= xl));
+    const uint64_t bm = __ballot(sel);
+    const int pos = base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(bm >> 32),
+                                                          __builtin_amdgcn_mbcnt_lo((uint32_t)bm, 0u));
+    if (sel && pos < keep) out[pos] = key[r];
+    base += __popcll(bm);
+  }
+  return base < keep ? base : keep;
 }
 
 // Groups of 16 items (tmax entries) of one row: the keep largest of every segment, key = (maximum,
-// ~group).  Block = (segment, row); its 4 waves take 1024 entries each at a time.
+// ~group).  Block = (segment, row): each of its 4 waves keeps the best of its 1024 entries at a
+// time, with those it has, wave 0 joins the four lists.  Unused places are 0.
 __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tmax, int64_t M, int seg_len,
                                                     int nseg, int keep, uint64_t* __restrict__ out) {
   __shared__ uint64_t red[4][64];
+  __shared__ uint64_t fin[64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t n = blockIdx.x / nseg;
   const int sg = (int)(blockIdx.x % nseg);
   const int64_t i0 = (int64_t)sg * seg_len, i1 = i0 + seg_len < M ? i0 + seg_len : M;
   const float* row = tmax + n * M;
-  uint64_t have = 0;
+  int have = 0;
   for (int64_t b = i0 + w * 1024; b < i1; b += 4096) {
-    uint64_t key[16];
+    uint64_t key[17];
+    key[16] = lane < have ? red[w][lane] : 0ull;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int64_t e = b + i * 64 + lane;
       key[i] = e < i1 ? make_key(row[e], (uint32_t)e) : 0ull;
     }
-    have = wave_top<16>(key, have, keep, lane);
+    wave_sync();
+    have = wave_select<17>(key, keep, red[w], lane);
+    wave_sync();
   }
-  red[w][lane] = have;
+  if (lane >= have) red[w][lane] = 0ull;
   __syncthreads();
   if (w == 0) {
     uint64_t key[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) key[i] = red[i][lane];
-    const uint64_t r = wave_top<4>(key, 0ull, keep, lane);
-    if (lane < keep) out[(n * nseg + sg) * keep + lane] = r;
+    const int c = wave_select<4>(key, keep, fin, lane);
+    wave_sync();
+    if (lane < keep) out[(n * nseg + sg) * keep + lane] = lane < c ? fin[lane] : 0ull;
   }
 }
 
-// One block per row: the keep largest groups of all segments, their items scored in 64 bits, the top
-// of them by (score, lower id).
+// 16 bytes of x and w -> sum of products in 64 bits
+template <typename T>
+__device__ __forceinline__ double dot16(const u32x4_t& a, const u32x4_t& b, double d) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      d = fma((double)__uint_as_float(a[i]), (double)__uint_as_float(b[i]), d);
+    } else {
+      d = fma((double)__uint_as_float(a[i] << 16), (double)__uint_as_float(b[i] << 16), d);
+      d = fma((double)__uint_as_float(a[i] & 0xffff0000u), (double)__uint_as_float(b[i] & 0xffff0000u), d);
+    }
+  }
+  return d;
+}
+
+// One block per row: the keep largest groups of all segments, their items scored in 64 bits (16 lanes
+// an item, 16-byte loads, four groups' items in flight), the top of them by (score, lower id).
 template <typename T>
 __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ segs, int nseg, int keep,
                                                    int top, const T* __restrict__ x, int64_t ldx,
@@ -489,77 +535,120 @@ __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ 
                                                    const float* __restrict__ lse,
                                                    int64_t* __restrict__ ids_out, float* __restrict__ lp_out) {
   constexpr int GMAX = CT_TOP_MAX + CT_TOP_EXTRA;
+  constexpr int PC = 16 / (int)sizeof(T);
   __shared__ uint64_t red[4][64];
-  __shared__ uint32_t grp[GMAX];
-  __shared__ int ngrp;
+  __shared__ uint64_t fin[64];
+  __shared__ uint32_t grp[64];
+  __shared__ int cnt[4];
+  __shared__ float s_floor;
   __shared__ double sc[GMAX * 16];
   __shared__ int vid[GMAX * 16];
+  __shared__ int nlist;
+  __shared__ short list[GMAX * 16];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t n = blockIdx.x;
   const int total = nseg * keep;
   const uint64_t* src = segs + n * total;
-  uint64_t have = 0;
+  int have = 0;
   for (int b = wv * 256; b < total; b += 1024) {
-    uint64_t key[4];
+    uint64_t key[5];
+    key[4] = lane < have ? red[wv][lane] : 0ull;
 #pragma unroll
     for (int i = 0; i < 4; ++i) key[i] = b + i * 64 + lane < total ? src[b + i * 64 + lane] : 0ull;
-    have = wave_top<4>(key, have, keep, lane);
+    wave_sync();
+    have = wave_select<5>(key, keep, red[wv], lane);
+    wave_sync();
   }
-  red[wv][lane] = have;
+  if (lane >= have) red[wv][lane] = 0ull;
+  if (tid == 0) nlist = 0;
   __syncthreads();
   if (wv == 0) {
     uint64_t key[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) key[i] = red[i][lane];
-    const uint64_t r = wave_top<4>(key, 0ull, keep, lane);
-    // groups that cannot hold one of the top: clearly below the top-th maximum (the margin is far
-    // above what 32-bit sums are off; see the ordering in 64 bits below)
-    const float kth = key_score(__shfl(r, top - 1 < keep ? top - 1 : keep - 1, 64));
-    const float best = key_score(__shfl(r, 0, 64));
-    const float margin = 0.0009765625f * (fabsf(kth) + fabsf(best) + 1.0f);
-    const bool use = lane < keep && r != 0 && !(key_score(r) < kth - margin);
+    const int c = wave_select<4>(key, keep, fin, lane);
+    wave_sync();
+    const uint64_t k1[1] = {lane < c ? fin[lane] : 0ull};
+    // the top-th largest maximum: the top-th largest logit is not below it, so a group or an item
+    // clearly below cannot be one of the top (the margin is far above what 32-bit sums are off)
+    const int t = wave_select<1>(k1, top, red[0], lane);
+    wave_sync();
+    float kth = __builtin_huge_valf(), best = -__builtin_huge_valf();
+    if (lane < t) kth = best = key_score(red[0][lane]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      kth = fminf(kth, __shfl_xor(kth, o, 64));
+      best = fmaxf(best, __shfl_xor(best, o, 64));
+    }
+    // (fewer than top groups, or taken-out items among the top: every item takes part)
+    const float floor = t < top || kth < 0.9f * CT_OUT ? -__builtin_huge_valf()
+                                : kth - 0.0009765625f * (fabsf(kth) + fabsf(best) + 1.0f);
+    const bool use = k1[0] != 0ull && !(key_score(k1[0]) < floor);
     const uint64_t bm = __ballot(use);
-    if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(r);
-    if (lane == 0) ngrp = __popcll(bm);
+    if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(k1[0]);
+    if (lane == 0) {
+      cnt[0] = __popcll(bm);
+      s_floor = floor;
+    }
   }
   __syncthreads();
-  const int cand = ngrp * 16;
+  const int ngrp = cnt[0];
+  const float floor = s_floor;
   const T* xr = x + n * ldx;
-  // 16 lanes an item, 16 items of one group at a time
   const int sub = tid >> 4, l16 = tid & 15;
-  for (int gi = 0; gi < ngrp; ++gi) {
-    const uint32_t q = grp[gi];
-    const int v = (int)(q >> 2) * 64 + 16 * (sub >> 2) + 4 * (int)(q & 3) + (sub & 3);
-    double d = 0.0;
-    if (v < V) {
-      const T* wr = w + (int64_t)v * ldw;
-      for (int e = l16; e < E; e += 16) d = fma((double)ct_elt(xr, e), (double)ct_elt(wr, e), d);
+  for (int g0 = 0; g0 < ngrp; g0 += 4) {
+    int v[4];
+    double d[4];
+    const T* wr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t q = grp[g0 + i < ngrp ? g0 + i : ngrp - 1];
+      v[i] = (int)(q >> 2) * 64 + 16 * (sub >> 2) + 4 * (int)(q & 3) + (sub & 3);
+      wr[i] = w + (int64_t)(v[i] < V ? v[i] : V - 1) * ldw;
+      d[i] = 0.0;
+    }
+    for (int e = l16 * PC; e < E; e += 16 * PC) {
+      const u32x4_t xv = *(const u32x4_t*)(xr + e);
+      u32x4_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = *(const u32x4_t*)(wr[i] + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = dot16<T>(xv, y[i], d[i]);
     }
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) d += __shfl_xor(d, o, 64);
-    if (l16 == 0) {
-      double l = -__builtin_huge_val();
-      if (v < V) {
-        const float b = bias ? bias[v] : 0.0f;
-        if (!(b <= CT_OUT)) l = s * d + (double)b;
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) d[i] += __shfl_xor(d[i], o, 64);
+      if (l16 == 0 && g0 + i < ngrp) {
+        double l = -__builtin_huge_val();
+        bool in = false;
+        if (v[i] < V) {
+          const float b = bias ? bias[v[i]] : 0.0f;
+          if (!(b <= CT_OUT)) l = s * d[i] + (double)b;
+          in = !(l * 1.4426950408889634 < (double)floor);  // (-inf, NaN: only where the floor lets them)
+        }
+        sc[(g0 + i) * 16 + sub] = l;
+        vid[(g0 + i) * 16 + sub] = v[i];
+        if (in) list[atomicAdd(&nlist, 1)] = (short)((g0 + i) * 16 + sub);
       }
-      sc[gi * 16 + sub] = l;
-      vid[gi * 16 + sub] = v < V ? v : 0x7fffffff;
     }
   }
   __syncthreads();
   const float ls = lse[n];
-  for (int c = tid; c < cand; c += 256) {
+  const int m = nlist;  // (in any order: ranks do not depend on it)
+  for (int i = tid; i < m; i += 256) {
+    const int c = list[i];
     const double l = sc[c];
     const int v = vid[c];
-    int rank = 0;  // NaN scores rank by id alone among themselves, below all others
-    for (int o = 0; o < cand; ++o) {
-      const double t = sc[o];
+    int rank = 0;  // NaN scores rank by id among themselves, below all others
+    for (int o = 0; o < m; ++o) {
+      const int q = list[o];
+      const double t = sc[q];
       const bool gt = t > l || (l != l && t == t);
       const bool eq = t == l || (t != t && l != l);
-      rank += gt || (eq && vid[o] < v) ? 1 : 0;
+      rank += gt || (eq && vid[q] < v) ? 1 : 0;
     }
-    if (rank < top && v < V) {
+    if (rank < top) {
       ids_out[n * top + rank] = v;
       lp_out[n * top + rank] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : (float)(l - (double)ls);
     }

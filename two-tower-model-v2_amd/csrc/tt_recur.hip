@@ -28,7 +28,7 @@ namespace tt {
 
 constexpr int RC_CK = 16;   // events between saved states
 constexpr int RC_U = 8;     // events whose rows are loaded together (forward)
-constexpr int RC_SEG = 16;  // segments of the chunk join
+constexpr int RC_SEG = 64, RC_JCH = 16;  // segments and channels of a block of the chunk join
 
 struct ScanArgs {
   const void *x, *gate;
@@ -178,16 +178,48 @@ __device__ __forceinline__ Gate gate_pow(float g, float w) {
   return o;
 }
 
+// The same for a whole weight of at most 64 (event weights are counts) by repeated squaring of the
+// pair (A, 1 - A): 1 - A B = (1 - A) + A (1 - B), sums of positive terms only, so both keep their
+// relative precision; some 10 operations instead of gate_pow's 50.
+__device__ __forceinline__ Gate gate_int(float g, int w) {
+  Gate b = gate_one(g);
+  const float sn = b.sn;
+  Gate o{1.0f, 0.0f, sn, true};
+  bool first = true;
+  for (int k = w;;) {
+    if (k & 1) {
+      if (first) {
+        o.a = b.a;
+        o.na = b.na;
+      } else {
+        o.na = fmaf(o.a, b.na, o.na);
+        o.a *= b.a;
+      }
+      first = false;
+    }
+    k >>= 1;
+    if (k == 0) break;
+    b.na = fmaf(b.a, b.na, b.na);
+    b.a *= b.a;
+  }
+  o.hi = o.na < 0.5f;
+  return o;
+}
+
 // unit = ((b * C) + c) * nw + wave-of-row; uniform over the wave
 struct Unit {
   int64_t b;
   int c, ch;  // chunk, first channel of this lane
+  bool ok;    // the row has this channel (else the lane reads channel 0 and writes nothing; it
+              // stays active, for the weights)
 };
 template <int VEC>
 __device__ __forceinline__ Unit unit_of(const ScanArgs& a, int64_t u, int lane) {
   Unit o;
   const int64_t bc = u / a.nw;
   o.ch = ((int)(u - bc * a.nw) * 64 + lane) * VEC;
+  o.ok = o.ch < a.D;
+  o.ch = o.ok ? o.ch : 0;
   o.b = bc / a.C;
   o.c = (int)(bc - o.b * a.C);
   return o;
@@ -204,6 +236,9 @@ __device__ __forceinline__ void with_gate(float w, const float (&g)[VEC], F&& f)
     if (w == 1.0f) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) f(i, gate_one(g[i]));
+    } else if (w <= 64.0f && truncf(w) == w) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f(i, gate_int(g[i], (int)w));
     } else {
       const float wc = fminf(w, 3.0e38f);  // an infinite weight: the state becomes x
 #pragma unroll
@@ -211,6 +246,17 @@ __device__ __forceinline__ void with_gate(float w, const float (&g)[VEC], F&& f)
     }
   }
 }
+// Weights are uniform over a wave (one history): 64 events' weights with one load, lane i's handed
+// out as a scalar, so that the choice of the gate's form is a scalar branch.
+struct Weights {
+  float v;
+  __device__ __forceinline__ void load(const float* wp, int64_t t, int64_t t1, int lane) {
+    v = t + lane < t1 ? wp[t + lane] : 0.0f;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), i));
+  }
+};
 
 // SUM: the chunk's (product of A, state from 0) only.  Else the chunk from its start state, with
 // h, h_last and the saved states as asked for.
@@ -225,7 +271,6 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
     if (uu >= nunits) break;
     const Unit un = unit_of<VEC>(a, uu, lane);
     if (SUM && un.c == a.C - 1) continue;  // the last chunk starts nothing
-    if (un.ch >= a.D) continue;
     const int64_t t0 = (int64_t)un.c * a.T, t1 = t0 + a.T < a.S ? t0 + a.T : a.S;
     const T* xp = (const T*)a.x + un.b * a.xsb + un.ch;
     const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
@@ -240,28 +285,29 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
                        : 0.0f;
     }
     P xn[RC_U], gn[RC_U];
-    float wn[RC_U];
+    Weights ws;
     auto load = [&](int64_t t) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         const int64_t tt = t + j < t1 ? t + j : t1 - 1;
         xn[j] = *(const P*)(xp + tt * a.xss);
         gn[j] = *(const P*)(gp + tt * a.gss);
-        if (WT) wn[j] = wp[tt];
       }
     };
     if (t0 < t1) load(t0);
     for (int64_t t = t0; t < t1; t += RC_U) {
       P xc[RC_U], gc[RC_U];
       float wc[RC_U];
+      const int wi = (int)(t - t0) & 63;
+      if (WT && wi == 0) ws.load(wp, t, t1, lane);
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         xc[j] = xn[j];
         gc[j] = gn[j];
-        wc[j] = WT ? wn[j] : 1.0f;
+        wc[j] = WT ? ws.get(wi + j) : 1.0f;
       }
       if (t + RC_U < t1) load(t + RC_U);
-      if (!SUM && a.ck && (t & (RC_CK - 1)) == 0) {
+      if (!SUM && a.ck && un.ok && (t & (RC_CK - 1)) == 0) {
         float* c = a.ck + (un.b * nck + t / RC_CK) * a.D + un.ch;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) c[i] = h[i];
@@ -276,10 +322,11 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
             h[i] = move(q, h[i], xv[i]);
             if (SUM) pa[i] = decay(q, pa[i]);
           });
-          if (!SUM && a.h) *(P*)((T*)a.h + (un.b * a.S + t + j) * a.D + un.ch) = pack<T, VEC>(h);
+          if (!SUM && a.h && un.ok) *(P*)((T*)a.h + (un.b * a.S + t + j) * a.D + un.ch) = pack<T, VEC>(h);
         }
       }
     }
+    if (!un.ok) continue;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       if (SUM) {
@@ -293,28 +340,29 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
 }
 
 // Joins the chunks of one history: carry[c] = the state before chunk c (REV: the gradient that
-// reaches the end of chunk c from the chunks after it).  64 channels x 16 segments of chunks per
-// block: a segment is composed to one (A, H), the segments before it give its start, a second
-// walk writes.  s <- A s + H over chunks c = 0.. (REV: C - 1 .. 1).
+// reaches the end of chunk c from the chunks after it).  16 channels x 64 segments of chunks per
+// block (few histories have many chunks: a thread's walk is short, its loads independent): a
+// segment is composed to one (A, H), the segments before it give its start by a scan in 6 steps,
+// a second walk writes.  s <- A s + H over chunks c = 0 .. (REV: C - 1 .. 1).
 template <bool REV>
-__global__ __launch_bounds__(64 * RC_SEG) void k_scan_join(const float* __restrict__ sumA,
-                                                           const float* __restrict__ sumH,
-                                                           const float* __restrict__ init,
-                                                           float* __restrict__ carry, int64_t B,
-                                                           int C, int D) {
-  __shared__ float sa[RC_SEG][64], sh[RC_SEG][64];
-  const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6;
-  const int nd = (D + 63) / 64;
+__global__ __launch_bounds__(RC_JCH * RC_SEG) void k_scan_join(const float* __restrict__ sumA,
+                                                               const float* __restrict__ sumH,
+                                                               const float* __restrict__ init,
+                                                               float* __restrict__ carry, int64_t B,
+                                                               int C, int D) {
+  __shared__ float sa[2][RC_SEG][RC_JCH], sh[2][RC_SEG][RC_JCH];
+  const int cl = threadIdx.x % RC_JCH, seg = threadIdx.x / RC_JCH;
+  const int nd = (D + RC_JCH - 1) / RC_JCH;
   const int per = (C + RC_SEG - 1) / RC_SEG;
   for (int64_t blk = blockIdx.x; blk < B * nd; blk += gridDim.x) {
     const int64_t b = blk / nd;
-    const int ch = (int)(blk - b * nd) * 64 + lane;
+    const int ch = (int)(blk - b * nd) * RC_JCH + cl;
     const bool ok = ch < D;
     const int i0 = seg * per < C ? seg * per : C, i1 = i0 + per < C ? i0 + per : C;
     auto at = [&](int i) { return (b * C + (REV ? C - 1 - i : i)) * D + (ok ? ch : 0); };
     float pa = 1.0f, ph = 0.0f;
     // (the last step's summary starts nothing and is not written: i runs to C - 2)
-#pragma unroll 8
+#pragma unroll 4
     for (int i = i0; i < i1; ++i) {
       if (i < C - 1) {
         const float A = sumA[at(i)], H = sumH[at(i)];
@@ -322,13 +370,25 @@ __global__ __launch_bounds__(64 * RC_SEG) void k_scan_join(const float* __restri
         pa *= A;
       }
     }
-    sa[seg][lane] = pa;
-    sh[seg][lane] = ph;
+    // composed over all segments up to this one
+    int k = 0;
+    sa[0][seg][cl] = pa;
+    sh[0][seg][cl] = ph;
     __syncthreads();
+#pragma unroll
+    for (int o = 1; o < RC_SEG; o <<= 1, k ^= 1) {
+      if (seg >= o) {
+        ph = fmaf(pa, sh[k][seg - o][cl], ph);
+        pa *= sa[k][seg - o][cl];
+      }
+      sa[k ^ 1][seg][cl] = pa;
+      sh[k ^ 1][seg][cl] = ph;
+      __syncthreads();
+    }
     float s = init && ok ? init[b * D + ch] : 0.0f;
-    for (int j = 0; j < seg; ++j) s = fmaf(sa[j][lane], s, sh[j][lane]);
+    if (seg > 0) s = fmaf(sa[k][seg - 1][cl], s, sh[k][seg - 1][cl]);
     if (ok) {
-#pragma unroll 8
+#pragma unroll 4
       for (int i = i0; i < i1; ++i) {
         carry[at(i)] = s;
         if (i < C - 1) s = fmaf(sumA[at(i)], s, sumH[at(i)]);
@@ -349,7 +409,7 @@ __global__ __launch_bounds__(256) void k_scan_bwd_sum(const ScanArgs a) {
     const int64_t uu = u0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (uu >= nunits) break;
     const Unit un = unit_of<VEC>(a, uu, lane);
-    if (un.c == 0 || un.ch >= a.D) continue;
+    if (un.c == 0) continue;
     const int64_t t0 = (int64_t)un.c * a.T, t1 = t0 + a.T < a.S ? t0 + a.T : a.S;
     const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
     const T* dp = a.dh ? (const T*)a.dh + un.b * a.S * a.D + un.ch : nullptr;
@@ -361,25 +421,26 @@ __global__ __launch_bounds__(256) void k_scan_bwd_sum(const ScanArgs a) {
       R[i] = 0.0f;
     }
     P gn[RC_U], dn[RC_U];
-    float wn[RC_U];
+    Weights ws;  // lane i: event t1 - 1 - 64 k - i
     auto load = [&](int64_t t) __attribute__((always_inline)) {  // events t, t - 1, ...
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         const int64_t tt = t - j > t0 ? t - j : t0;
         gn[j] = *(const P*)(gp + tt * a.gss);
         if (dp) dn[j] = *(const P*)(dp + tt * a.D);
-        if (WT) wn[j] = wp[tt];
       }
     };
     load(t1 - 1);
     for (int64_t t = t1 - 1; t >= t0; t -= RC_U) {
       P gc[RC_U], dc[RC_U];
       float wc[RC_U];
+      const int wi = (int)(t1 - 1 - t) & 63;
+      if (WT && wi == 0) ws.v = t - lane >= t0 ? wp[t - lane] : 0.0f;
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         gc[j] = gn[j];
         if (dp) dc[j] = dn[j];
-        wc[j] = WT ? wn[j] : 1.0f;
+        wc[j] = WT ? ws.get(wi + j) : 1.0f;
       }
       if (t - RC_U >= t0) load(t - RC_U);
 #pragma unroll
@@ -399,6 +460,7 @@ __global__ __launch_bounds__(256) void k_scan_bwd_sum(const ScanArgs a) {
         }
       }
     }
+    if (!un.ok) continue;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       a.sumA[(un.b * a.C + un.c) * a.D + un.ch + i] = pa[i];
@@ -417,7 +479,6 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const ScanArgs a) {
     const int64_t uu = u0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (uu >= nunits) break;
     const Unit un = unit_of<VEC>(a, uu, lane);
-    if (un.ch >= a.D) continue;
     const int64_t t0 = (int64_t)un.c * a.T, t1 = t0 + a.T < a.S ? t0 + a.T : a.S;
     const T* xp = (const T*)a.x + un.b * a.xsb + un.ch;
     const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
@@ -439,8 +500,11 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const ScanArgs a) {
         xr[j] = *(const P*)(xp + tt * a.xss);
         gr[j] = *(const P*)(gp + tt * a.gss);
         if (a.dh) dr[j] = *(const P*)((const T*)a.dh + ob + tt * a.D);
-        wr[j] = WT ? wp[tt] : 1.0f;
       }
+      Weights ws;
+      if (WT) ws.load(wp, s0, t1, lane);
+#pragma unroll
+      for (int j = 0; j < RC_CK; ++j) wr[j] = WT ? ws.get(j) : 1.0f;
       const float* c = a.ck + (un.b * nck + s0 / RC_CK) * a.D + un.ch;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) h[i] = c[i];
@@ -485,12 +549,14 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const ScanArgs a) {
             R[i] = __float_as_int(A[j][i]) < 0 ? fmaf(A[j][i], G[i], G[i]) : A[j][i] * G[i];
           }
           const int64_t o = ob + (s0 + j) * a.D;
-          *(P*)((T*)a.dx + o) = pack<T, VEC>(dxv);
-          *(P*)((T*)a.dgate + o) = pack<T, VEC>(dgv);
+          if (un.ok) {
+            *(P*)((T*)a.dx + o) = pack<T, VEC>(dxv);
+            *(P*)((T*)a.dgate + o) = pack<T, VEC>(dgv);
+          }
         }
       }
     }
-    if (a.dh0 && un.c == 0) {
+    if (a.dh0 && un.c == 0 && un.ok) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) a.dh0[un.b * a.D + un.ch + i] = R[i];
     }
@@ -580,7 +646,7 @@ static unsigned scan_grid(const ScanArgs& a) {
   return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
 }
 static unsigned join_grid(const ScanArgs& a) {
-  const int64_t blocks = a.B * ((a.D + 63) / 64);
+  const int64_t blocks = a.B * ((a.D + RC_JCH - 1) / RC_JCH);
   return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
 }
 
@@ -618,7 +684,7 @@ extern "C" int tt_gated_scan_fwd(const void* x, const void* gate, int32_t dtype,
   hipStream_t st = (hipStream_t)stream;
   if (p.C > 1) {
     scan_launch<KSum>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
-    hipLaunchKernelGGL(k_scan_join<false>, dim3(join_grid(a)), dim3(64 * RC_SEG), 0, st, a.sumA,
+    hipLaunchKernelGGL(k_scan_join<false>, dim3(join_grid(a)), dim3(RC_JCH * RC_SEG), 0, st, a.sumA,
                        a.sumH, a.h0, a.carry, B, a.C, D);
   }
   scan_launch<KFwd>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
@@ -645,7 +711,7 @@ extern "C" int tt_gated_scan_bwd(const void* x, const void* gate, int32_t dtype,
   hipStream_t st = (hipStream_t)stream;
   if (p.C > 1) {
     scan_launch<KBwdSum>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
-    hipLaunchKernelGGL(k_scan_join<true>, dim3(join_grid(a)), dim3(64 * RC_SEG), 0, st, a.sumA,
+    hipLaunchKernelGGL(k_scan_join<true>, dim3(join_grid(a)), dim3(RC_JCH * RC_SEG), 0, st, a.sumA,
                        a.sumH, a.dlast, a.carry, B, a.C, D);
   }
   scan_launch<KBwd>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
