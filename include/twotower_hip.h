@@ -624,7 +624,7 @@ int tt_adam_f32(float* p, const float* g, float* m, float* v, int64_t n, float l
  * --------------------------------------------------------------------------------- */
 #define TT_DTYPE_F32 0
 #define TT_DTYPE_BF16 1
-#define TT_SCAN_CKPT 16
+#define TT_SCAN_CKPT 8
 int tt_gated_scan_workspace_bytes(int64_t B, int64_t S, int32_t D, int64_t* bytes);
 int tt_gated_scan_fwd(const void* x, const void* gate, int32_t dtype, int64_t B, int64_t S,
                       int32_t D, int64_t x_sb, int64_t x_ss, int64_t g_sb, int64_t g_ss,

@@ -10,9 +10,9 @@
 // Backward, with R the gradient that reaches h_t from later events:
 //   G_t = dh_t + R ;  dx_t = (1 - A_t) G_t ;  dg_t = w_t A_t sigmoid(-g_t) (h_{t-1} - x_t) G_t
 //   R <- A_t G_t   (after event 0: the gradient of h0)
-// The state is needed in 32 bits there, so the forward pass saves it (f32) before every 16th
-// event, 1/16 of one f32 tensor, and the backward pass recomputes the 16 states between in
-// registers: cheaper to read than h itself (0.25 instead of 2 or 4 bytes an element) and the
+// The state is needed in 32 bits there, so the forward pass saves it (f32) before every 8th
+// event, 1/8 of one f32 tensor, and the backward pass recomputes the 8 states between in
+// registers: cheaper to read than h itself (0.5 instead of 2 or 4 bytes an element) and the
 // rounding of h to bf16 does not reach the gradients.
 //
 // Bound: HBM.  Forward 3 tensors (x, gate, h), backward 5 (x, gate, dh, dx, dgate).  A lane owns
@@ -26,7 +26,7 @@
 
 namespace tt {
 
-constexpr int RC_CK = 16;   // events between saved states
+constexpr int RC_CK = TT_SCAN_CKPT;  // events between saved states
 constexpr int RC_U = 8;     // events whose rows are loaded together (forward)
 constexpr int RC_SEG = 64, RC_JCH = 16;  // segments and channels of a block of the chunk join
 
@@ -110,6 +110,16 @@ __device__ __forceinline__ typename Pack<T, VEC>::type pack(const float (&v)[VEC
   return p;
 }
 
+// A chunk's product of A as one float: the product P itself, or minus 1 - P where that is below a
+// half (bit for bit a sign: P = 1 is -0).  1 - P is summed on its own: taken from a rounded P it
+// would be off by the roundings of all its factors, the same in every chunk of equal gates.
+__device__ __forceinline__ float enc_prod(float P, float n) { return n < 0.5f ? -n : P; }
+__device__ __forceinline__ void dec_prod(float e, float& P, float& n) {
+  const bool neg = (int)__float_as_uint(e) < 0;
+  P = neg ? 1.0f + e : e;
+  n = neg ? -e : 1.0f - e;
+}
+
 // exp(-|g|) to about 1 ulp: the product |g| log2(e) in two parts, the low one (< 2^-20) applied
 // to first order.
 __device__ __forceinline__ float exp_neg_abs(float g) {
@@ -119,30 +129,29 @@ __device__ __forceinline__ float exp_neg_abs(float g) {
   const float e = __builtin_amdgcn_exp2f(hi);
   return hi < -150.0f ? 0.0f : fmaf(e, lo * 0.693147181f, e);
 }
-// e = exp(-|g|), r = 1 / (1 + e): sigmoid(|g|) = r and sigmoid(-|g|) = e r, neither by a
-// difference, so 1 - A keeps its relative precision for long memories (A next to 1).
 struct Gate {
   float a, na;  // A, 1 - A
-  float sn;     // sigmoid(-g)
-  bool hi;      // A is nearer 1 than 0
 };
 // A s and A h + (1 - A) x.  Near 1 the part that leaves is computed from 1 - A: a rounded A would
 // be off 1 - (1 - A) by up to 2^-25, which a memory of 1 / (1 - A) events multiplies.
-__device__ __forceinline__ float decay(const Gate& q, float s) {
-  return q.hi ? fmaf(-q.na, s, s) : q.a * s;
+__device__ __forceinline__ float decay(float a, float na, float s) {
+  return na < 0.5f ? fmaf(-na, s, s) : a * s;
 }
-__device__ __forceinline__ float move(const Gate& q, float h, float x) {
-  return q.hi ? fmaf(q.na, x - h, h) : fmaf(q.a, h, q.na * x);
+__device__ __forceinline__ float move(float a, float na, float h, float x) {
+  return na < 0.5f ? fmaf(na, x - h, h) : fmaf(a, h, na * x);
 }
+// e = exp(-|g|), r = 1 / (1 + e): sigmoid(|g|) = r and sigmoid(-|g|) = e r, neither by a
+// difference, so 1 - A keeps its relative precision for long memories (A next to 1).  For bf16
+// gates the exponent is one product (2^-24 |g| off: far below the gate's own rounding; the
+// exponential is a fifth of the kernels' arithmetic, and that is what bounds them next to HBM).
+template <typename T>
 __device__ __forceinline__ Gate gate_one(float g) {
-  const float e = exp_neg_abs(g);
+  const float e = sizeof(T) == 4 ? exp_neg_abs(g) : __builtin_amdgcn_exp2f(-fabsf(g) * 1.44269504f);
   const float r = __builtin_amdgcn_rcpf(1.0f + e);
   const float er = e * r;
   Gate o;
-  o.hi = g >= 0.0f;
-  o.a = o.hi ? r : er;
-  o.na = o.hi ? er : r;
-  o.sn = o.na;
+  o.a = g >= 0.0f ? r : er;
+  o.na = g >= 0.0f ? er : r;
   return o;
 }
 // A = exp(-w softplus(-g)).  softplus(-g) = max(-g, 0) + log1p(e), log1p(e) = 2 atanh(e / (2 +
@@ -150,7 +159,6 @@ __device__ __forceinline__ Gate gate_one(float g) {
 // difference from 1 above (relative error < 2^-22 either way).
 __device__ __forceinline__ Gate gate_pow(float g, float w) {
   const float e = exp_neg_abs(g);
-  const float r = __builtin_amdgcn_rcpf(1.0f + e);
   const float z = e * __builtin_amdgcn_rcpf(2.0f + e), z2 = z * z;
   float s = fmaf(z2, 1.0f / 15.0f, 1.0f / 13.0f);
   s = fmaf(s, z2, 1.0f / 11.0f);
@@ -171,39 +179,49 @@ __device__ __forceinline__ Gate gate_pow(float g, float w) {
   const float nsmall = q * y;
   const float big = exp_neg_abs(y);
   Gate o;
-  o.hi = y < 0.35f;
-  o.a = o.hi ? 1.0f - nsmall : big;
-  o.na = o.hi ? nsmall : 1.0f - big;
-  o.sn = g >= 0.0f ? e * r : r;
+  o.a = y < 0.35f ? 1.0f - nsmall : big;
+  o.na = y < 0.35f ? nsmall : 1.0f - big;
   return o;
 }
 
-// The same for a whole weight of at most 64 (event weights are counts) by repeated squaring of the
-// pair (A, 1 - A): 1 - A B = (1 - A) + A (1 - B), sums of positive terms only, so both keep their
-// relative precision; some 10 operations instead of gate_pow's 50.
-__device__ __forceinline__ Gate gate_int(float g, int w) {
-  Gate b = gate_one(g);
-  const float sn = b.sn;
-  Gate o{1.0f, 0.0f, sn, true};
-  bool first = true;
-  for (int k = w;;) {
-    if (k & 1) {
-      if (first) {
-        o.a = b.a;
-        o.na = b.na;
-      } else {
-        o.na = fmaf(o.a, b.na, o.na);
-        o.a *= b.a;
-      }
-      first = false;
-    }
-    k >>= 1;
-    if (k == 0) break;
-    b.na = fmaf(b.a, b.na, b.na);
-    b.a *= b.a;
+// (A, 1 - A) of weight 1 -> of a whole weight w <= 64 (event weights are counts), by repeated
+// squaring of the pair: 1 - A B = (1 - A) + A (1 - B), sums of positive terms only, so both keep
+// their relative precision; some 10 operations a channel instead of gate_pow's 50.  w uniform.
+template <int VEC>
+__device__ __forceinline__ void gate_power(float (&a)[VEC], float (&na)[VEC], int w) {
+  float b[VEC], nb[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    b[i] = a[i];
+    nb[i] = na[i];
   }
-  o.hi = o.na < 0.5f;
-  return o;
+  while (!(w & 1)) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      nb[i] = fmaf(b[i], nb[i], nb[i]);
+      b[i] *= b[i];
+    }
+    w >>= 1;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    a[i] = b[i];
+    na[i] = nb[i];
+  }
+  while (w >>= 1) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      nb[i] = fmaf(b[i], nb[i], nb[i]);
+      b[i] *= b[i];
+    }
+    if (w & 1) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        na[i] = fmaf(a[i], nb[i], na[i]);
+        a[i] *= b[i];
+      }
+    }
+  }
 }
 
 // unit = ((b * C) + c) * nw + wave-of-row; uniform over the wave
@@ -225,38 +243,54 @@ __device__ __forceinline__ Unit unit_of(const ScanArgs& a, int64_t u, int lane) 
   return o;
 }
 
-// One event for VEC channels; w uniform.
-template <bool WT, int VEC, typename F>
-__device__ __forceinline__ void with_gate(float w, const float (&g)[VEC], F&& f) {
-  if constexpr (!WT) {
+// Weights are uniform over a wave (one history): 64 events' weights with one load, lane i's handed
+// out as a scalar, so that the choice of the gate's form is a scalar branch.
+__device__ __forceinline__ float lane_value(float v, int i) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), i));
+}
+// The gates of U events: weight 1 for all of them first, without a branch (their exponentials
+// overlap), then the other weights event by event.  KQ: also w A sigmoid(-g) (the backward's).
+template <typename T, int VEC, int U, bool WT, bool KQ>
+__device__ __forceinline__ void gates(const typename Pack<T, VEC>::type (&gp)[U], const float (&w)[U],
+                                      float (&a)[U][VEC], float (&na)[U][VEC], float (&kq)[KQ ? U : 1][VEC]) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f(i, gate_one(g[i]));
-  } else {
-    if (!(w > 0.0f)) return;
-    if (w == 1.0f) {
+  for (int j = 0; j < U; ++j) {
+    float g[VEC];
+    unpack<T, VEC>(gp[j], g);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f(i, gate_one(g[i]));
-    } else if (w <= 64.0f && truncf(w) == w) {
+    for (int i = 0; i < VEC; ++i) {
+      const Gate q = gate_one<T>(g[i]);
+      a[j][i] = q.a;
+      na[j][i] = q.na;
+      if (KQ) kq[j][i] = q.a * q.na;
+    }
+  }
+  if constexpr (WT) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f(i, gate_int(g[i], (int)w));
-    } else {
-      const float wc = fminf(w, 3.0e38f);  // an infinite weight: the state becomes x
+    for (int j = 0; j < U; ++j) {
+      if (w[j] == 1.0f || !(w[j] > 0.0f)) continue;
+      float sn[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f(i, gate_pow(g[i], wc));
+      for (int i = 0; i < VEC; ++i) sn[i] = na[j][i];
+      if (w[j] <= 64.0f && truncf(w[j]) == w[j]) {
+        gate_power<VEC>(a[j], na[j], (int)w[j]);
+      } else {
+        float g[VEC];
+        unpack<T, VEC>(gp[j], g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const Gate q = gate_pow(g[i], fminf(w[j], 3.0e38f));  // an infinite weight: h becomes x
+          a[j][i] = q.a;
+          na[j][i] = q.na;
+        }
+      }
+      if (KQ) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) kq[j][i] = w[j] * a[j][i] * sn[i];
+      }
     }
   }
 }
-// Weights are uniform over a wave (one history): 64 events' weights with one load, lane i's handed
-// out as a scalar, so that the choice of the gate's form is a scalar branch.
-struct Weights {
-  float v;
-  __device__ __forceinline__ void load(const float* wp, int64_t t, int64_t t1, int lane) {
-    v = t + lane < t1 ? wp[t + lane] : 0.0f;
-  }
-  __device__ __forceinline__ float get(int i) const {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), i));
-  }
-};
 
 // SUM: the chunk's (product of A, state from 0) only.  Else the chunk from its start state, with
 // h, h_last and the saved states as asked for.
@@ -275,17 +309,18 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
     const T* xp = (const T*)a.x + un.b * a.xsb + un.ch;
     const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
     const float* wp = WT ? a.w + un.b * a.wsb : nullptr;
-    float h[VEC], pa[VEC];
+    float h[VEC], pa[VEC], pn[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       pa[i] = 1.0f;
+      pn[i] = 0.0f;
       h[i] = SUM ? 0.0f
              : a.C > 1 ? a.carry[(un.b * a.C + un.c) * a.D + un.ch + i]
              : a.h0    ? a.h0[un.b * a.D + un.ch + i]
                        : 0.0f;
     }
     P xn[RC_U], gn[RC_U];
-    Weights ws;
+    float wl = 0.0f;
     auto load = [&](int64_t t) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
@@ -297,16 +332,17 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
     if (t0 < t1) load(t0);
     for (int64_t t = t0; t < t1; t += RC_U) {
       P xc[RC_U], gc[RC_U];
-      float wc[RC_U];
+      float wc[RC_U], A[RC_U][VEC], nA[RC_U][VEC], none[1][VEC];
       const int wi = (int)(t - t0) & 63;
-      if (WT && wi == 0) ws.load(wp, t, t1, lane);
+      if (WT && wi == 0) wl = t + lane < t1 ? wp[t + lane] : 0.0f;
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         xc[j] = xn[j];
         gc[j] = gn[j];
-        wc[j] = WT ? ws.get(wi + j) : 1.0f;
+        wc[j] = WT ? lane_value(wl, wi + j) : 1.0f;
       }
       if (t + RC_U < t1) load(t + RC_U);
+      gates<T, VEC, RC_U, WT, false>(gc, wc, A, nA, none);
       if (!SUM && a.ck && un.ok && (t & (RC_CK - 1)) == 0) {
         float* c = a.ck + (un.b * nck + t / RC_CK) * a.D + un.ch;
 #pragma unroll
@@ -315,13 +351,18 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         if (t + j < t1) {
-          float xv[VEC], gv[VEC];
-          unpack<T, VEC>(xc[j], xv);
-          unpack<T, VEC>(gc[j], gv);
-          with_gate<WT, VEC>(wc[j], gv, [&](int i, const Gate& q) __attribute__((always_inline)) {
-            h[i] = move(q, h[i], xv[i]);
-            if (SUM) pa[i] = decay(q, pa[i]);
-          });
+          if (!WT || wc[j] > 0.0f) {
+            float xv[VEC];
+            unpack<T, VEC>(xc[j], xv);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              h[i] = move(A[j][i], nA[j][i], h[i], xv[i]);
+              if (SUM) {
+                pn[i] = fmaf(pa[i], nA[j][i], pn[i]);
+                pa[i] = decay(A[j][i], nA[j][i], pa[i]);
+              }
+            }
+          }
           if (!SUM && a.h && un.ok) *(P*)((T*)a.h + (un.b * a.S + t + j) * a.D + un.ch) = pack<T, VEC>(h);
         }
       }
@@ -330,7 +371,7 @@ __global__ __launch_bounds__(256) void k_scan_fwd(const ScanArgs a) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       if (SUM) {
-        a.sumA[(un.b * a.C + un.c) * a.D + un.ch + i] = pa[i];
+        a.sumA[(un.b * a.C + un.c) * a.D + un.ch + i] = enc_prod(pa[i], pn[i]);
         a.sumH[(un.b * a.C + un.c) * a.D + un.ch + i] = h[i];
       } else if (un.c == a.C - 1) {
         a.h_last[un.b * a.D + un.ch + i] = h[i];
@@ -350,7 +391,7 @@ __global__ __launch_bounds__(RC_JCH * RC_SEG) void k_scan_join(const float* __re
                                                                const float* __restrict__ init,
                                                                float* __restrict__ carry, int64_t B,
                                                                int C, int D) {
-  __shared__ float sa[2][RC_SEG][RC_JCH], sh[2][RC_SEG][RC_JCH];
+  __shared__ float sa[2][RC_SEG][RC_JCH], sn[2][RC_SEG][RC_JCH], sh[2][RC_SEG][RC_JCH];
   const int cl = threadIdx.x % RC_JCH, seg = threadIdx.x / RC_JCH;
   const int nd = (D + RC_JCH - 1) / RC_JCH;
   const int per = (C + RC_SEG - 1) / RC_SEG;
@@ -360,38 +401,49 @@ __global__ __launch_bounds__(RC_JCH * RC_SEG) void k_scan_join(const float* __re
     const bool ok = ch < D;
     const int i0 = seg * per < C ? seg * per : C, i1 = i0 + per < C ? i0 + per : C;
     auto at = [&](int i) { return (b * C + (REV ? C - 1 - i : i)) * D + (ok ? ch : 0); };
-    float pa = 1.0f, ph = 0.0f;
+    // (P, n = 1 - P, H) of the segment's chunks, one after another
+    float pa = 1.0f, pn = 0.0f, ph = 0.0f;
     // (the last step's summary starts nothing and is not written: i runs to C - 2)
 #pragma unroll 4
     for (int i = i0; i < i1; ++i) {
       if (i < C - 1) {
-        const float A = sumA[at(i)], H = sumH[at(i)];
-        ph = fmaf(A, ph, H);
-        pa *= A;
+        float P, n;
+        dec_prod(sumA[at(i)], P, n);
+        ph = decay(P, n, ph) + sumH[at(i)];
+        pn = fmaf(pa, n, pn);
+        pa = decay(P, n, pa);
       }
     }
-    // composed over all segments up to this one
+    // ... and of all segments up to this one
     int k = 0;
     sa[0][seg][cl] = pa;
+    sn[0][seg][cl] = pn;
     sh[0][seg][cl] = ph;
     __syncthreads();
 #pragma unroll
     for (int o = 1; o < RC_SEG; o <<= 1, k ^= 1) {
       if (seg >= o) {
-        ph = fmaf(pa, sh[k][seg - o][cl], ph);
-        pa *= sa[k][seg - o][cl];
+        const float P = sa[k][seg - o][cl];
+        ph += decay(pa, pn, sh[k][seg - o][cl]);
+        pn = fmaf(pa, sn[k][seg - o][cl], pn);
+        pa *= P;
       }
       sa[k ^ 1][seg][cl] = pa;
+      sn[k ^ 1][seg][cl] = pn;
       sh[k ^ 1][seg][cl] = ph;
       __syncthreads();
     }
     float s = init && ok ? init[b * D + ch] : 0.0f;
-    if (seg > 0) s = fmaf(sa[k][seg - 1][cl], s, sh[k][seg - 1][cl]);
+    if (seg > 0) s = decay(sa[k][seg - 1][cl], sn[k][seg - 1][cl], s) + sh[k][seg - 1][cl];
     if (ok) {
 #pragma unroll 4
       for (int i = i0; i < i1; ++i) {
         carry[at(i)] = s;
-        if (i < C - 1) s = fmaf(sumA[at(i)], s, sumH[at(i)]);
+        if (i < C - 1) {
+          float P, n;
+          dec_prod(sumA[at(i)], P, n);
+          s = decay(P, n, s) + sumH[at(i)];
+        }
       }
     }
     __syncthreads();
@@ -400,7 +452,7 @@ __global__ __launch_bounds__(RC_JCH * RC_SEG) void k_scan_join(const float* __re
 
 // Reverse summary of a chunk: product of A, and the gradient that leaves its front when none
 // enters its end.
-template <typename T, int VEC, bool WT>
+template <typename T, int VEC, bool WT, bool DH>
 __global__ __launch_bounds__(256) void k_scan_bwd_sum(const ScanArgs a) {
   typedef typename Pack<T, VEC>::type P;
   const int lane = threadIdx.x & 63;
@@ -412,64 +464,69 @@ __global__ __launch_bounds__(256) void k_scan_bwd_sum(const ScanArgs a) {
     if (un.c == 0) continue;
     const int64_t t0 = (int64_t)un.c * a.T, t1 = t0 + a.T < a.S ? t0 + a.T : a.S;
     const T* gp = (const T*)a.gate + un.b * a.gsb + un.ch;
-    const T* dp = a.dh ? (const T*)a.dh + un.b * a.S * a.D + un.ch : nullptr;
+    const T* dp = (const T*)a.dh + un.b * a.S * a.D + un.ch;  // (DH)
     const float* wp = WT ? a.w + un.b * a.wsb : nullptr;
-    float R[VEC], pa[VEC];
+    float R[VEC], pa[VEC], pn[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       pa[i] = 1.0f;
+      pn[i] = 0.0f;
       R[i] = 0.0f;
     }
     P gn[RC_U], dn[RC_U];
-    Weights ws;  // lane i: event t1 - 1 - 64 k - i
+    float wl = 0.0f;  // lane i: event t1 - 1 - 64 k - i
     auto load = [&](int64_t t) __attribute__((always_inline)) {  // events t, t - 1, ...
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         const int64_t tt = t - j > t0 ? t - j : t0;
         gn[j] = *(const P*)(gp + tt * a.gss);
-        if (dp) dn[j] = *(const P*)(dp + tt * a.D);
+        if (DH) dn[j] = *(const P*)(dp + tt * a.D);
       }
     };
     load(t1 - 1);
     for (int64_t t = t1 - 1; t >= t0; t -= RC_U) {
       P gc[RC_U], dc[RC_U];
-      float wc[RC_U];
+      float wc[RC_U], A[RC_U][VEC], nA[RC_U][VEC], none[1][VEC];
       const int wi = (int)(t1 - 1 - t) & 63;
-      if (WT && wi == 0) ws.v = t - lane >= t0 ? wp[t - lane] : 0.0f;
+      if (WT && wi == 0) wl = t - lane >= t0 ? wp[t - lane] : 0.0f;
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         gc[j] = gn[j];
-        if (dp) dc[j] = dn[j];
-        wc[j] = WT ? ws.get(wi + j) : 1.0f;
+        if (DH) dc[j] = dn[j];
+        wc[j] = WT ? lane_value(wl, wi + j) : 1.0f;
       }
       if (t - RC_U >= t0) load(t - RC_U);
+      gates<T, VEC, RC_U, WT, false>(gc, wc, A, nA, none);
 #pragma unroll
       for (int j = 0; j < RC_U; ++j) {
         if (t - j >= t0) {
-          float gv[VEC], dv[VEC];
-          unpack<T, VEC>(gc[j], gv);
-          if (dp) {
+          if (DH) {
+            float dv[VEC];
             unpack<T, VEC>(dc[j], dv);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) R[i] += dv[i];
           }
-          with_gate<WT, VEC>(wc[j], gv, [&](int i, const Gate& q) __attribute__((always_inline)) {
-            R[i] = decay(q, R[i]);
-            pa[i] = decay(q, pa[i]);
-          });
+          if (!WT || wc[j] > 0.0f) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              R[i] = decay(A[j][i], nA[j][i], R[i]);
+              pn[i] = fmaf(pa[i], nA[j][i], pn[i]);
+              pa[i] = decay(A[j][i], nA[j][i], pa[i]);
+            }
+          }
         }
       }
     }
     if (!un.ok) continue;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      a.sumA[(un.b * a.C + un.c) * a.D + un.ch + i] = pa[i];
+      a.sumA[(un.b * a.C + un.c) * a.D + un.ch + i] = enc_prod(pa[i], pn[i]);
       a.sumH[(un.b * a.C + un.c) * a.D + un.ch + i] = R[i];
     }
   }
 }
 
-template <typename T, int VEC, bool WT>
+template <typename T, int VEC, bool WT, bool DH>
 __global__ __launch_bounds__(256) void k_scan_bwd(const ScanArgs a) {
   typedef typename Pack<T, VEC>::type P;
   const int lane = threadIdx.x & 63;
@@ -490,43 +547,50 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const ScanArgs a) {
       R[i] = a.C > 1 ? a.carry[(un.b * a.C + un.c) * a.D + un.ch + i]
              : a.dlast ? a.dlast[un.b * a.D + un.ch + i]
                        : 0.0f;
-    for (int64_t s0 = t1 > t0 ? (t1 - 1) / RC_CK * RC_CK : t0 - 1; s0 >= t0; s0 -= RC_CK) {
+    // RC_CK events at a time, the last first, the rows of the next ones loaded meanwhile
+    P xr[RC_CK], gr[RC_CK], dr[RC_CK];
+    float wl = 0.0f, cn[VEC];
+    auto load = [&](int64_t s0) __attribute__((always_inline)) {
       const int n = (int)(t1 - s0 < RC_CK ? t1 - s0 : RC_CK);
-      P xr[RC_CK], gr[RC_CK], dr[RC_CK];
-      float wr[RC_CK], h[VEC];
 #pragma unroll
       for (int j = 0; j < RC_CK; ++j) {
         const int64_t tt = s0 + (j < n ? j : n - 1);
         xr[j] = *(const P*)(xp + tt * a.xss);
         gr[j] = *(const P*)(gp + tt * a.gss);
-        if (a.dh) dr[j] = *(const P*)((const T*)a.dh + ob + tt * a.D);
+        if (DH) dr[j] = *(const P*)((const T*)a.dh + ob + tt * a.D);
       }
-      Weights ws;
-      if (WT) ws.load(wp, s0, t1, lane);
-#pragma unroll
-      for (int j = 0; j < RC_CK; ++j) wr[j] = WT ? ws.get(j) : 1.0f;
+      if (WT) wl = lane < n ? wp[s0 + lane] : 0.0f;
       const float* c = a.ck + (un.b * nck + s0 / RC_CK) * a.D + un.ch;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) h[i] = c[i];
-      // (A negative here: the decay is 1 - |A|, see decay())
-      float A[RC_CK][VEC], nA[RC_CK][VEC], q[RC_CK][VEC];
+      for (int i = 0; i < VEC; ++i) cn[i] = c[i];
+    };
+    int64_t s0 = t1 > t0 ? (t1 - 1) / RC_CK * RC_CK : t0 - 1;
+    if (s0 >= t0) load(s0);
+    for (; s0 >= t0; s0 -= RC_CK) {
+      const int n = (int)(t1 - s0 < RC_CK ? t1 - s0 : RC_CK);
+      P xc[RC_CK], gc[RC_CK], dc[RC_CK];
+      float wc[RC_CK], h[VEC], A[RC_CK][VEC], nA[RC_CK][VEC], q[RC_CK][VEC];
 #pragma unroll
       for (int j = 0; j < RC_CK; ++j) {
+        xc[j] = xr[j];
+        gc[j] = gr[j];
+        if (DH) dc[j] = dr[j];
+        wc[j] = WT ? lane_value(wl, j) : 1.0f;
+      }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {  // padding: the gradient passes by
-          A[j][i] = -0.0f;
-          nA[j][i] = q[j][i] = 0.0f;
-        }
-        if (j < n) {
-          float xv[VEC], gv[VEC];
-          unpack<T, VEC>(xr[j], xv);
-          unpack<T, VEC>(gr[j], gv);
-          with_gate<WT, VEC>(wr[j], gv, [&](int i, const Gate& o) __attribute__((always_inline)) {
-            A[j][i] = o.hi ? -o.na : o.a;
-            nA[j][i] = o.na;
-            q[j][i] = (h[i] - xv[i]) * (WT ? wr[j] * o.a : o.a) * o.sn;
-            h[i] = move(o, h[i], xv[i]);
-          });
+      for (int i = 0; i < VEC; ++i) h[i] = cn[i];
+      if (s0 - RC_CK >= t0) load(s0 - RC_CK);
+      gates<T, VEC, RC_CK, WT, true>(gc, wc, A, nA, q);
+#pragma unroll
+      for (int j = 0; j < RC_CK; ++j) {
+        if (!WT || wc[j] > 0.0f) {
+          float xv[VEC];
+          unpack<T, VEC>(xc[j], xv);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            q[j][i] *= h[i] - xv[i];
+            h[i] = move(A[j][i], nA[j][i], h[i], xv[i]);
+          }
         }
       }
 #pragma unroll
@@ -534,19 +598,23 @@ __global__ __launch_bounds__(256) void k_scan_bwd(const ScanArgs a) {
         if (j < n) {
           float G[VEC], dxv[VEC], dgv[VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) G[i] = R[i];
-          if (a.dh) {
-            float dv[VEC];
-            unpack<T, VEC>(dr[j], dv);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) G[i] += dv[i];
-          }
-          const bool live = !WT || wr[j] > 0.0f;
-#pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            dxv[i] = live ? nA[j][i] * G[i] : 0.0f;
-            dgv[i] = live ? q[j][i] * G[i] : 0.0f;
-            R[i] = __float_as_int(A[j][i]) < 0 ? fmaf(A[j][i], G[i], G[i]) : A[j][i] * G[i];
+            G[i] = R[i];
+            dxv[i] = dgv[i] = 0.0f;
+          }
+          if (DH) {
+            float dv[VEC];
+            unpack<T, VEC>(dc[j], dv);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) R[i] = G[i] = G[i] + dv[i];
+          }
+          if (!WT || wc[j] > 0.0f) {  // (else padding: the gradient passes by)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              dxv[i] = nA[j][i] * G[i];
+              dgv[i] = q[j][i] * G[i];
+              R[i] = decay(A[j][i], nA[j][i], G[i]);
+            }
           }
           const int64_t o = ob + (s0 + j) * a.D;
           if (un.ok) {
@@ -569,8 +637,8 @@ struct ScanPlan {
   int64_t T;
 };
 // VEC: two channels a lane where D, the strides and the addresses allow (4- or 8-byte loads),
-// else one.  Chunks: as many as give the card about 2048 waves, none shorter than 64 events; one
-// chunk when the histories alone give 1024.
+// else one.  Chunks: as many as give the card about 8192 waves (8 a SIMD), none shorter than 32
+// events; one chunk when the histories alone give 1024.
 static ScanPlan scan_plan(int64_t B, int64_t S, int D, bool vec_ok) {
   ScanPlan p;
   p.vec = vec_ok && D % 2 == 0 ? 2 : 1;
@@ -579,7 +647,7 @@ static ScanPlan scan_plan(int64_t B, int64_t S, int D, bool vec_ok) {
   p.T = S > 0 ? S : 1;
   const int64_t waves = B * p.nw;
   if (waves < 1024 && S >= 128) {
-    int64_t c = (2048 + waves - 1) / waves, cmax = (S + 63) / 64;
+    int64_t c = (8192 + waves - 1) / waves, cmax = (S + 31) / 32;
     c = c < cmax ? c : cmax;
     p.T = ((S + c - 1) / c + RC_CK - 1) / RC_CK * RC_CK;
     p.C = (int)((S + p.T - 1) / p.T);
@@ -597,27 +665,29 @@ static int64_t scan_ws(int64_t B, int64_t S, int D) {
   return need;
 }
 
-template <template <typename, int, bool> class K>
-static void scan_launch(int dtype, int vec, bool wt, unsigned grid, hipStream_t st,
-                        const ScanArgs& a) {
-#define RC_GO(T, V, W) hipLaunchKernelGGL((K<T, V, W>::fn), dim3(grid), dim3(256), 0, st, a)
-  if (dtype == TT_DTYPE_F32) {
-    if (vec == 2) { if (wt) RC_GO(float, 2, true); else RC_GO(float, 2, false); }
-    else { if (wt) RC_GO(float, 1, true); else RC_GO(float, 1, false); }
-  } else {
-    if (vec == 2) { if (wt) RC_GO(uint16_t, 2, true); else RC_GO(uint16_t, 2, false); }
-    else { if (wt) RC_GO(uint16_t, 1, true); else RC_GO(uint16_t, 1, false); }
-  }
-#undef RC_GO
+enum { RC_FWD, RC_FWD_SUM, RC_BWD, RC_BWD_SUM };
+template <int KIND, typename T, int V, bool W>
+static void scan_go(unsigned grid, hipStream_t st, const ScanArgs& a) {
+  void (*k)(const ScanArgs);
+  if constexpr (KIND == RC_FWD) k = k_scan_fwd<T, V, W, false>;
+  else if constexpr (KIND == RC_FWD_SUM) k = k_scan_fwd<T, V, W, true>;
+  else if constexpr (KIND == RC_BWD) k = a.dh ? k_scan_bwd<T, V, W, true> : k_scan_bwd<T, V, W, false>;
+  else k = a.dh ? k_scan_bwd_sum<T, V, W, true> : k_scan_bwd_sum<T, V, W, false>;
+  hipLaunchKernelGGL(k, dim3(grid), dim3(256), 0, st, a);
 }
-template <typename T, int V, bool W>
-struct KFwd { static constexpr auto fn = k_scan_fwd<T, V, W, false>; };
-template <typename T, int V, bool W>
-struct KSum { static constexpr auto fn = k_scan_fwd<T, V, W, true>; };
-template <typename T, int V, bool W>
-struct KBwd { static constexpr auto fn = k_scan_bwd<T, V, W>; };
-template <typename T, int V, bool W>
-struct KBwdSum { static constexpr auto fn = k_scan_bwd_sum<T, V, W>; };
+template <int KIND, typename T>
+static void scan_vec(int vec, unsigned grid, hipStream_t st, const ScanArgs& a) {
+  if (vec == 2) {
+    if (a.w) scan_go<KIND, T, 2, true>(grid, st, a); else scan_go<KIND, T, 2, false>(grid, st, a);
+  } else {
+    if (a.w) scan_go<KIND, T, 1, true>(grid, st, a); else scan_go<KIND, T, 1, false>(grid, st, a);
+  }
+}
+template <int KIND>
+static void scan_launch(int dtype, int vec, unsigned grid, hipStream_t st, const ScanArgs& a) {
+  if (dtype == TT_DTYPE_F32) scan_vec<KIND, float>(vec, grid, st, a);
+  else scan_vec<KIND, uint16_t>(vec, grid, st, a);
+}
 
 static bool addr_ok(const void* p, int64_t bytes) { return ((uintptr_t)p % bytes) == 0; }
 
@@ -683,11 +753,11 @@ extern "C" int tt_gated_scan_fwd(const void* x, const void* gate, int32_t dtype,
   if (int rc = scan_setup(a, dtype, p, workspace, workspace_bytes, {x, gate, h}, __func__)) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (p.C > 1) {
-    scan_launch<KSum>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+    scan_launch<RC_FWD_SUM>(dtype, p.vec, scan_grid(a), st, a);
     hipLaunchKernelGGL(k_scan_join<false>, dim3(join_grid(a)), dim3(RC_JCH * RC_SEG), 0, st, a.sumA,
                        a.sumH, a.h0, a.carry, B, a.C, D);
   }
-  scan_launch<KFwd>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+  scan_launch<RC_FWD>(dtype, p.vec, scan_grid(a), st, a);
   return check_launch("tt_gated_scan_fwd");
 }
 
@@ -710,10 +780,10 @@ extern "C" int tt_gated_scan_bwd(const void* x, const void* gate, int32_t dtype,
     return rc;
   hipStream_t st = (hipStream_t)stream;
   if (p.C > 1) {
-    scan_launch<KBwdSum>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+    scan_launch<RC_BWD_SUM>(dtype, p.vec, scan_grid(a), st, a);
     hipLaunchKernelGGL(k_scan_join<true>, dim3(join_grid(a)), dim3(RC_JCH * RC_SEG), 0, st, a.sumA,
                        a.sumH, a.dlast, a.carry, B, a.C, D);
   }
-  scan_launch<KBwd>(dtype, p.vec, w != nullptr, scan_grid(a), st, a);
+  scan_launch<RC_BWD>(dtype, p.vec, scan_grid(a), st, a);
   return check_launch("tt_gated_scan_bwd");
 }

@@ -38,7 +38,7 @@ TT_PREC_BF16 = 1
 TT_PREC_X3 = 2  # f32 operands, split-bf16 (hi + lo) MFMA products
 TT_ACT_NONE, TT_ACT_GELU, TT_ACT_RELU = 0, 1, 2
 TT_DTYPE_F32, TT_DTYPE_BF16 = 0, 1
-TT_SCAN_CKPT = 16  # events between the states tt_gated_scan_fwd saves for the backward pass
+TT_SCAN_CKPT = 8  # events between the states tt_gated_scan_fwd saves for the backward pass
 DTYPES = {torch.float32: TT_DTYPE_F32, torch.bfloat16: TT_DTYPE_BF16}
 
 
