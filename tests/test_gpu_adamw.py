@@ -206,6 +206,19 @@ def test_groups_scheduler_and_added_group():
         check_step(opt, params[i:i + 1], before[i:i + 1], 32, h)
 
 
+def test_step_hooks_and_closure():
+    from twotower.optim import AdamW
+
+    params = make(torch.float32, [(50,)])
+    opt = AdamW(params, **HP)
+    seen = []
+    opt.register_step_pre_hook(lambda o, a, k: seen.append(("pre", o is opt)))
+    opt.register_step_post_hook(lambda o, a, k: seen.append(("post", int(o.state[params[0]]["step"]))))
+    set_grads(params, 0)
+    assert opt.step(lambda: 7.0) == 7.0
+    assert seen == [("pre", True), ("post", 1)]
+
+
 def test_more_tensors_than_one_launch_takes():
     from twotower.optim import AdamW
 

@@ -86,7 +86,10 @@ def check_grad(got, want, size, T, dt):
 
 SHAPES = [(1, 1, 64), (1, 5, 64), (3, 64, 64), (5, 130, 128), (128, 128, 64), (129, 257, 192),
           (300, 1000, 384), (17, 70001, 64), (2, 20, 768), (64, 4099, 1024), (33, 333, 100),
-          (1000, 37, 64), (40, 500, 7)]
+          (1000, 37, 64), (40, 500, 7),
+          # more than 128 rows, E a multiple of 128: rows kept in registers
+          (129, 1, 128), (300, 31, 128), (200, 33, 256), (700, 1090, 384), (385, 64, 384),
+          (257, 999, 512), (130, 641, 640), (520, 2000, 768)]
 
 
 @pytest.mark.parametrize("N,V,E", SHAPES)

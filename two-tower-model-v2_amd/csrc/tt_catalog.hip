@@ -9,8 +9,8 @@
 //
 // The N x V logits never exist in memory.  Everything is done in powers of two (z = l log2 e).
 //
-// k_logits<STAT>  128 items x 128 rows tiles on MFMA (bf16 16x16x32 or f32 16x16x4), a block
-//     walks its share of the catalog for its 128 rows.  The product is formed as w . x^T, so a lane
+// k_logits<STAT>  128 items x 128 rows tiles (64 x 64 where that leaves CUs idle) on MFMA (bf16
+//     16x16x32 or f32 16x16x4), a block walks its share of the catalog for its 128 rows.  The product is formed as w . x^T, so a lane
 //     holds 16 items of 4 rows: the running maximum m, L = sum 2^(z - m) and T = sum 2^(z - m) (z -
 //     m) of a row stay in the lane, with no exchange between lanes until the share's end.
 //     Entropy = ln 2 (log2 L - T / L): relative to the maximum, nothing cancels against lse.
@@ -40,9 +40,8 @@ typedef uint32_t ct_u32x2 __attribute__((ext_vector_type(2)));
 constexpr float CT_OUT = -1.0e30f;   // z of an item that is taken out
 constexpr float CT_NONE = -2.0e30f;  // maximum of nothing
 constexpr float CT_LOG2E = 1.4426950408889634f, CT_LN2 = 0.6931471805599453f;
-constexpr int CT_TILE = 128;            // tile edge (items, rows, columns)
-constexpr int CT_OP_B = CT_TILE * 128;  // one operand's stage: 128 rows x 128 B (or BK rows x 128 elements)
-constexpr int CT_TOP_MAX = 32, CT_TOP_EXTRA = 8;
+constexpr int CT_TILE = 128;  // tile edge (items, rows, columns), or half of it
+constexpr int CT_TOP_MAX = 32, CT_TOP_EXTRA = 8, CT_TOP_NT = 512;
 
 __device__ __forceinline__ void ct_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <int N>
@@ -53,14 +52,15 @@ __device__ __forceinline__ void ct_dma(const void* g, char* l) {
                                    (__attribute__((address_space(3))) void*)l, 16, 0, 0);
 }
 
-// ---- operand stages.  Row form ("K along the row"): 128 rows x 128 B, 16-B chunks XOR-swizzled by
+// ---- operand stages, of 32 NB rows or columns (NB = 4: 128, or 2: 64; a wave's quarter of the tile
+// is 16 NB square).  Row form ("K along the row"): rows of 128 B, 16-B chunks XOR-swizzled by
 // (row >> 1) & 7.  Wave w of 4 loads pieces w, w + 4, ...: 8 rows each.
-template <typename T>
+template <typename T, int NB>
 struct RowStage {
-  int64_t off[4];
+  int64_t off[NB];
   __device__ __forceinline__ void init(int64_t ld, int64_t row0, int64_t rows, int w, int lane) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NB; ++j) {
       const int r = 8 * (w + 4 * j) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
       int64_t row = row0 + r;
       row = row < rows ? row : rows - 1;  // past the end: loaded again, never used
@@ -69,33 +69,39 @@ struct RowStage {
   }
   __device__ __forceinline__ void issue(const T* p, int64_t k0, char* lds, int w) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ct_dma(p + off[j] + k0, lds + 1024 * (w + 4 * j));
+    for (int j = 0; j < NB; ++j) ct_dma(p + off[j] + k0, lds + 1024 * (w + 4 * j));
   }
 };
-// fragments of 4 x 16 rows from row r0: f[s][i] = 16 B at chunk 4 s + g of row r0 + 16 i + rl
-__device__ __forceinline__ void row_frags(const char* lds, int r0, int lane, u32x4_t (&f)[2][4]) {
+// fragments of NB x 16 rows from row r0: f[s][i] = 16 B at chunk 4 s + g of row r0 + 16 i + rl
+template <int NB>
+__device__ __forceinline__ void row_frags(const char* lds, int r0, int lane, u32x4_t (&f)[2][NB]) {
   const int g = lane >> 4, rl = lane & 15, sw = (rl >> 1) & 7;
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NB; ++i)
       f[s][i] = *(const u32x4_t*)(lds + (r0 + 16 * i + rl) * 128 + 16 * ((4 * s + g) ^ sw));
 }
 
-// Column form ("the sum runs down the rows"): BK rows x 128 elements, the operand as it lies.
-template <typename T>
+// Column form ("the sum runs down the rows"): BK rows x 32 NB elements, the operand as it lies.
+template <typename T, int NB>
 struct ColStage {
-  static constexpr int RPP = sizeof(T) == 2 ? 4 : 2;  // rows per 1-KB piece
-  int64_t off[4];
-  int row[4];
+  static constexpr int EPC = 16 / (int)sizeof(T), CPR = 32 * NB / EPC;  // elements a chunk, chunks a row
+  static constexpr int RPP = 64 / CPR;                                  // rows per 1-KB piece
+  // swizzle of a row's chunks: the rows that one fragment read touches together lie in different
+  // banks (bf16: 8 rows of two chunks; f32: 4 rows of four)
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (sizeof(T) == 2) return NB == 4 ? ((r & 3) | ((r >> 1) & 4)) << 1 : (((r >> 1) & 1) | ((r >> 2) & 2)) << 1;
+    else return NB == 4 ? ((r >> 2) & 3) << 2 : ((r >> 2) & 3) << 2;
+  }
+  int64_t off[NB];
+  int row[NB];
   // cols: valid columns from c0 (a multiple of the chunk); past the end: loaded again, never used
   __device__ __forceinline__ void init(int64_t c0, int64_t cols, int w, int lane) {
-    constexpr int EPC = 16 / (int)sizeof(T), CPR = 128 / EPC;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NB; ++j) {
       const int r = RPP * (w + 4 * j) + lane / CPR, pc = lane % CPR;
-      const int sw = sizeof(T) == 2 ? ((r & 3) | ((r >> 1) & 4)) << 1 : ((r >> 2) & 3) << 2;
-      int64_t c = c0 + (int64_t)(pc ^ sw) * EPC;
+      int64_t c = c0 + (int64_t)(pc ^ swz(r)) * EPC;
       c = c < cols ? c : cols - EPC;
       row[j] = r;
       off[j] = c;
@@ -104,7 +110,7 @@ struct ColStage {
   __device__ __forceinline__ void issue(const T* p, int64_t ld, int64_t k0, int64_t rows, char* lds,
                                         int w) const {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NB; ++j) {
       int64_t k = k0 + row[j];
       k = k < rows ? k : rows - 1;  // past the end: the other operand is zero there
       ct_dma(p + k * ld + off[j], lds + 1024 * (w + 4 * j));
@@ -112,23 +118,24 @@ struct ColStage {
   }
 };
 // the same fragments as row_frags gives (16 B of the sum's index for column c0 + 16 i + rl)
-template <typename T>
-__device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32x4_t (&f)[2][4]) {
+template <typename T, int NB>
+__device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32x4_t (&f)[2][NB]) {
   const int g = lane >> 4, rl = lane & 15;
+  constexpr int ROW_B = 32 * NB * (int)sizeof(T);
   if constexpr (sizeof(T) == 2) {
     // a 16-lane group reads 4 rows x 16 columns: lane 4 q + c supplies row q, columns 4 c .. + 3 and
     // receives column (its index)'s 4 rows
-    const int q = rl >> 2, c = rl & 3, sw = (q | ((g & 1) << 2)) << 1;
+    const int q = rl >> 2, c = rl & 3;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NB; ++i) {
         ct_u32x2 h[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int row = 32 * s + 8 * g + 4 * u + q;
-          const int chunk = (2 * (c0 / 16 + i) + (c >> 1)) ^ sw;
-          const char* p = lds + row * 256 + chunk * 16 + 8 * (c & 1);
+          const int chunk = (2 * (c0 / 16 + i) + (c >> 1)) ^ ColStage<T, NB>::swz(row);
+          const char* p = lds + row * ROW_B + chunk * 16 + 8 * (c & 1);
           h[u] = __builtin_bit_cast(ct_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                   (__attribute__((address_space(3))) ct_s16x4*)p));
         }
@@ -138,27 +145,27 @@ __device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int row = 16 * s + 4 * g + u;
-          const int chunk = (4 * (c0 / 16 + i) + (rl >> 2)) ^ (g << 2);
-          f[s][i][u] = *(const uint32_t*)(lds + row * 512 + chunk * 16 + 4 * (rl & 3));
+          const int chunk = (4 * (c0 / 16 + i) + (rl >> 2)) ^ ColStage<T, NB>::swz(row);
+          f[s][i][u] = *(const uint32_t*)(lds + row * ROW_B + chunk * 16 + 4 * (rl & 3));
         }
   }
 }
 
 // acc[i][j] += first[j] . second[i]: lane (g, rl) of block (i, j) holds first-index 16 j + 4 g + r,
 // second-index 16 i + rl
-template <typename T>
-__device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[2][4], const u32x4_t (&second)[2][4],
-                                        f32x4 (&acc)[4][4]) {
+template <typename T, int NB>
+__device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[2][NB], const u32x4_t (&second)[2][NB],
+                                        f32x4 (&acc)[NB][NB]) {
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < NB; ++j) {
         if constexpr (sizeof(T) == 2) {
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
               __builtin_bit_cast(ct_bf16x8, first[s][j]), __builtin_bit_cast(ct_bf16x8, second[s][i]),
@@ -204,13 +211,14 @@ struct LogitArgs {
   const int64_t* ids;  // COEF
   void* C;             // COEF [Npad, ldc]: items v_base .. of this chunk
   int64_t ldc;
-  int v_base, Npad;
+  int v_base, v_count, Npad;  // v_count: items from v_base on (k_ring)
 };
 
-template <typename T, bool COEF, bool ENT>
-__global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
-  constexpr int BK = 128 / (int)sizeof(T);
-  __shared__ __attribute__((aligned(16))) char smem[4 * CT_OP_B];
+template <typename T, bool COEF, bool ENT, int NB>
+__global__ __launch_bounds__(256, NB == 4 ? 2 : 3) void k_logits(const LogitArgs a) {
+  constexpr int BK = 128 / (int)sizeof(T), TILE = 32 * NB, WT = 16 * NB, OP_B = TILE * 128;
+  __shared__ __attribute__((aligned(16))) char smem[4 * OP_B];
+  __shared__ float half[NB == 2 && !COEF ? TILE : 1][4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wv = w >> 1, wn = w & 1, g = lane >> 4, rl = lane & 15;
@@ -219,16 +227,16 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
   const int sp = lb / a.n_tiles, tn = lb % a.n_tiles;
   const int per = (a.v_tiles + a.splits - 1) / a.splits;
   const int vt0 = sp * per, vt1 = vt0 + per < a.v_tiles ? vt0 + per : a.v_tiles;
-  const int n0 = tn * CT_TILE;
+  const int n0 = tn * TILE;
   const T* x = (const T*)a.x;
   const T* wt = (const T*)a.w;
   const int nk = a.E / BK;
 
-  RowStage<T> sx, sw;
+  RowStage<T, NB> sx, sw;
   sx.init(a.ldx, n0, a.N, w, lane);
-  float m[4], L[4], TT[4];
+  float m[NB], L[NB], TT[NB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < NB; ++i) {
     m[i] = CT_NONE;
     L[i] = TT[i] = 0.0f;
   }
@@ -236,10 +244,10 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
   int vt_i = vt0, k_i = 0, g_i = 0;
   auto issue_next = [&]() __attribute__((always_inline)) {
     if (vt_i >= vt1) return;
-    if (k_i == 0) sw.init(a.ldw, (int64_t)a.v_base + (int64_t)vt_i * CT_TILE, a.V, w, lane);
-    char* st = smem + (g_i & 1) * 2 * CT_OP_B;
+    if (k_i == 0) sw.init(a.ldw, (int64_t)a.v_base + (int64_t)vt_i * TILE, a.V, w, lane);
+    char* st = smem + (g_i & 1) * 2 * OP_B;
     sw.issue(wt, (int64_t)k_i * BK, st, w);
-    sx.issue(x, (int64_t)k_i * BK, st + CT_OP_B, w);
+    sx.issue(x, (int64_t)k_i * BK, st + OP_B, w);
     ++g_i;
     if (++k_i == nk) {
       k_i = 0;
@@ -249,28 +257,29 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
   issue_next();
   int gs = 0;
   for (int vt = vt0; vt < vt1; ++vt) {
-    const int v0 = a.v_base + vt * CT_TILE + 64 * wv;  // this wave's 64 items
-    f32x4 acc[4][4];
+    const int v0 = a.v_base + vt * TILE + WT * wv;  // this wave's items
+    f32x4 acc[NB][NB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int kt = 0; kt < nk; ++kt, ++gs) {
       ct_wait_vm<0>();
       ct_barrier();  // stage gs complete; every wave is done with the slot refilled next
       issue_next();
-      const char* st = smem + (gs & 1) * 2 * CT_OP_B;
-      u32x4_t fw[2][4], fx[2][4];
-      row_frags(st, 64 * wv, lane, fw);
-      row_frags(st + CT_OP_B, 64 * wn, lane, fx);
-      ct_mfma<T>(fw, fx, acc);
+      const char* st = smem + (gs & 1) * 2 * OP_B;
+      u32x4_t fw[2][NB], fx[2][NB];
+      row_frags<NB>(st, WT * wv, lane, fw);
+      row_frags<NB>(st + OP_B, WT * wn, lane, fx);
+      ct_mfma<T, NB>(fw, fx, acc);
     }
-    const bool edge = v0 + 64 > a.V;
+    float tmx[NB];
+    const bool edge = v0 + WT > a.V;
     const bool sel = a.bias || edge;
-    f32x4 b2[4];
+    f32x4 b2[NB];
     if (sel) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int v = v0 + 16 * j + 4 * g + r;
@@ -279,11 +288,11 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = n0 + 64 * wn + 16 * i + rl;
-      f32x4 z[4];
+    for (int i = 0; i < NB; ++i) {
+      const int n = n0 + WT * wn + 16 * i + rl;
+      f32x4 z[NB];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float q = acc[i][j][r];
@@ -293,17 +302,23 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
       if constexpr (!COEF) {
         float tm = CT_OUT;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NB; ++j)
           tm = fmaxf(fmaxf(fmaxf(z[j][0], z[j][1]), fmaxf(z[j][2], z[j][3])), tm);
-        if (a.tmax && n < a.N && v0 < a.V)
-          a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] = tm;
+        if (a.tmax) {
+          if constexpr (NB == 4) {
+            if (n < a.N && v0 < a.V) a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] = tm;
+          } else {  // (the tile's 64 items lie in two waves)
+            if (wv == 1) half[WT * wn + 16 * i + rl][g] = tm;
+            tmx[i] = tm;
+          }
+        }
         const float mn = fmaxf(m[i], tm), d = m[i] - mn;
         const float sc = __builtin_amdgcn_exp2f(d);
         if constexpr (ENT) TT[i] = sc * fmaf(d, L[i], TT[i]);
         L[i] *= sc;
         m[i] = mn;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float q = z[j][r] - mn;
@@ -317,9 +332,9 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
           const float4 rc = in ? a.rowc[n] : float4{1.0e30f, 0.f, 0.f, 0.f};
           const int64_t id = in ? a.ids ? a.ids[n] : -1 : -1;
           const bool live = rc.x < 1.0e30f;
-          T* o = (T*)a.C + (int64_t)n * a.ldc + vt * CT_TILE + 64 * wv + 4 * g;
+          T* o = (T*)a.C + (int64_t)n * a.ldc + vt * TILE + WT * wv + 4 * g;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < NB; ++j) {
             f32x4 c;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -335,19 +350,32 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
         }
       }
     }
+    if constexpr (!COEF && NB == 2) {
+      if (a.tmax) {
+        ct_barrier();
+        if (wv == 0) {
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const int n = n0 + WT * wn + 16 * i + rl;
+            if (n < a.N) a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] =
+                             fmaxf(tmx[i], half[WT * wn + 16 * i + rl][g]);
+          }
+        }
+      }
+    }
   }
   if constexpr (!COEF) {
     ct_barrier();  // the last stage's reads are over: its memory takes the waves' statistics
     float* red = (float*)smem;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < NB; ++i) {
 #pragma unroll
       for (int o = 16; o < 64; o <<= 1) {
         const float m2 = __shfl_xor(m[i], o, 64), L2 = __shfl_xor(L[i], o, 64), T2 = __shfl_xor(TT[i], o, 64);
         stat_join(m[i], L[i], TT[i], m2, L2, T2);
       }
       if (wv == 1 && g == 0) {
-        float* r = red + (64 * wn + 16 * i + rl) * 3;
+        float* r = red + (WT * wn + 16 * i + rl) * 3;
         r[0] = m[i];
         r[1] = L[i];
         r[2] = TT[i];
@@ -356,12 +384,257 @@ __global__ __launch_bounds__(256, 2) void k_logits(const LogitArgs a) {
     ct_barrier();
     if (wv == 0 && g == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* r = red + (64 * wn + 16 * i + rl) * 3;
+      for (int i = 0; i < NB; ++i) {
+        const float* r = red + (WT * wn + 16 * i + rl) * 3;
         stat_join(m[i], L[i], TT[i], r[0], r[1], r[2]);
-        const int n = n0 + 64 * wn + 16 * i + rl;
+        const int n = n0 + WT * wn + 16 * i + rl;
         if (n < a.N) a.part[(int64_t)sp * a.N + n] = float4{m[i], L[i], TT[i], 0.0f};
       }
+    }
+  }
+}
+
+// ---- bf16, E a multiple of 128 up to 384, more than 128 rows: k_ring.  The rows' vectors stay in
+// registers (QB blocks of 16 rows a wave, 8 waves: 128 QB rows a block), the catalog streams through
+// LDS in tiles of 32 items, SLOTS - 1 tiles ahead, one barrier a tile.  An item fragment read from
+// LDS feeds QB MFMAs (the 128 x 128 tile kernel reads a fragment of either side for every two: LDS
+// there is as busy as the matrix pipes), and the previous tile's exponentials run between this
+// tile's MFMAs.  The maximum is only moved when a tile exceeds it by 2^16, so the common tile
+// costs one fma, one exponential and two adds a logit.
+constexpr int CR_NT = 512;
+template <int KS>
+struct RingCfg {
+  static constexpr int QB = KS <= 8 ? 4 : 3;
+  static constexpr int TB = KS * 2048;             // bytes of a tile: 32 rows x KS x 64
+  static constexpr int SLOTS = 4;
+  static constexpr int PW = KS / 4;                // 1-KB pieces a wave loads of a tile
+  static constexpr int ROWS = 128 * QB;
+};
+
+template <int KS, bool COEF, bool ENT, bool BIAS>
+__global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
+  using C = RingCfg<KS>;
+  constexpr int QB = C::QB, TB = C::TB, SLOTS = C::SLOTS, PW = C::PW;
+  constexpr int OPS = PW + (BIAS ? 1 : 0);  // DMA instructions a wave issues per tile
+  __shared__ __attribute__((aligned(16))) char smem[SLOTS * TB];
+  __shared__ __attribute__((aligned(16))) float sbias[SLOTS + 1][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, rl = lane & 15;
+  const int lb = xcd_remap(blockIdx.x, gridDim.x);
+  const int sp = lb / a.n_tiles, tn = lb % a.n_tiles;
+  // shares in pairs of tiles (64 items: the groups of 16 that the top alternatives use)
+  const int per = (a.v_tiles + a.splits - 1) / a.splits;
+  const int v_end = a.v_base + a.v_count;
+  const int t0 = 2 * sp * per;
+  // (COEF: whole pairs, so that the products' 64-item steps find every coefficient written)
+  const int nt = COEF ? 2 * ((a.v_count + 63) / 64) : (a.v_count + 31) / 32;
+  const int t1 = t0 + 2 * per < nt ? t0 + 2 * per : nt;
+  const int nb = tn * C::ROWS + w * 16 * QB;  // this wave's first row
+  const uint16_t* x = (const uint16_t*)a.x;
+  const uint16_t* wt = (const uint16_t*)a.w;
+
+  // tile bytes [1024 p, +1024) = 64 chunks of 16 B in row order; row r's chunk c lies at c ^ (r & 15)
+  int64_t off[PW];
+  int row[PW];
+#pragma unroll
+  for (int j = 0; j < PW; ++j) {
+    const int c = (w + 8 * j) * 64 + lane;
+    row[j] = c / (4 * KS);
+    off[j] = ((c % (4 * KS)) ^ (row[j] & 15)) * 8;
+  }
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    char* st = smem + (t % SLOTS) * TB;
+    const int v0 = a.v_base + 32 * t;
+#pragma unroll
+    for (int j = 0; j < PW; ++j) {
+      int v = v0 + row[j];
+      v = v < v_end ? v : v_end - 1;  // past the end: loaded again, never used
+      ct_dma(wt + (int64_t)v * a.ldw + off[j], st + 1024 * (w + 8 * j));
+    }
+    if constexpr (BIAS) {
+      int v = v0 + lane;
+      v = v < v_end ? v : v_end - 1;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.bias + v),
+                                       (__attribute__((address_space(3))) void*)sbias[t % (SLOTS + 1)], 4, 0, 0);
+    }
+  };
+  if (t0 >= t1) return;
+
+  u32x4_t xf[KS][QB];
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    int n = nb + 16 * q + rl;
+    n = n < a.N ? n : a.N - 1;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) xf[k][q] = *(const u32x4_t*)(x + (int64_t)n * a.ldx + 32 * k + 8 * g);
+  }
+  float m[QB], L[QB], TT[QB], tm[QB];
+  float4 rc[QB];
+  int id[QB];
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    m[q] = CT_NONE;
+    L[q] = TT[q] = 0.0f;
+    tm[q] = CT_OUT;
+    const int n = nb + 16 * q + rl;
+    if constexpr (COEF) {
+      rc[q] = n < a.N ? a.rowc[n] : float4{1.0e30f, 0.f, 0.f, 0.f};
+      const int64_t i = n < a.N && a.ids ? a.ids[n] : -1;
+      id[q] = i >= 0 && i < a.V ? (int)i : -1;
+    }
+  }
+  // the loads above are complete before the first counted wait: the DMA sequence starts clean
+  ct_wait_vm<0>();
+#pragma unroll
+  for (int p = 0; p < SLOTS - 1; ++p)
+    if (t0 + p < t1) issue(t0 + p);
+
+  uint32_t fo[4];  // fragment offsets in a tile: chunk (4 k + g) ^ rl, k = 0 .. 3 (+ 256 B every 4)
+#pragma unroll
+  for (int k = 0; k < 4; ++k) fo[k] = (uint32_t)(rl * KS * 64 + 16 * ((4 * k + g) ^ rl));
+
+  // logits of the previous tile's block (q, rows 16 rb + 4 g ..)
+  auto bias4 = [&](int t, int rb) __attribute__((always_inline)) {
+    f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (BIAS) {
+      const f32x4 raw = *(const f32x4*)(sbias[t % (SLOTS + 1)] + 16 * rb + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) b[r] = raw[r] > CT_OUT || raw[r] != raw[r] ? raw[r] * CT_LOG2E : CT_NONE;
+    }
+    return b;
+  };
+  // z: in place of the products; edge: items past the end are taken out
+  auto to_z = [&](f32x4 (&acc)[QB][2], int t, bool edge) __attribute__((always_inline)) {
+    if (!BIAS && !edge) return;  // (scaled where used)
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      const f32x4 b = bias4(t, rb);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool out = (BIAS && b[r] == CT_NONE) || (edge && a.v_base + 32 * t + 16 * rb + 4 * g + r >= v_end);
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+          const float z = fmaf(acc[q][rb][r], a.s2, b[r]);
+          acc[q][rb][r] = out ? CT_OUT : z;
+        }
+      }
+    }
+  };
+  // the tile's maximum per row; the running maximum moved where it has to be
+  auto head = [&](f32x4 (&acc)[QB][2], int t, float s2) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+      const f32x4 &u = acc[q][0], &v = acc[q][1];
+      const float mx = fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))) * s2;
+      const float zm = fmaxf(mx, CT_OUT);
+      if (a.tmax) {
+        tm[q] = (t & 1) ? fmaxf(tm[q], zm) : zm;
+        const int n = nb + 16 * q + rl;
+        if (((t & 1) || t + 1 >= nt) && n < a.N)
+          a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (t >> 1) * 4 + g] = tm[q];
+      }
+      if (__any(zm > m[q] + 16.0f)) {
+        const float mn = fmaxf(m[q], zm), d = m[q] - mn, sc = __builtin_amdgcn_exp2f(d);
+        if constexpr (ENT) TT[q] = sc * fmaf(d, L[q], TT[q]);
+        L[q] *= sc;
+        m[q] = mn;
+      }
+    }
+  };
+  auto body = [&](const f32x4& v, int q, int rb, int t, float s2, bool zform) __attribute__((always_inline)) {
+    if constexpr (!COEF) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float d = fmaf(v[r], s2, -m[q]);
+        const float e = __builtin_amdgcn_exp2f(d);
+        L[q] += e;
+        if constexpr (ENT) TT[q] = fmaf(e, d, TT[q]);
+      }
+    } else {
+      const int n = nb + 16 * q + rl, vi = a.v_base + 32 * t + 16 * rb + 4 * g;
+      const bool live = rc[q].x < 1.0e30f;
+      f32x4 c;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float lp = fmaf(v[r], s2, -rc[q].x);
+        const float p = __builtin_amdgcn_exp2f(lp);
+        const float k = ENT ? fmaf(rc[q].z, fmaf(lp, CT_LN2, rc[q].w), rc[q].y) : rc[q].y;
+        const float o = fmaf(-p, k, id[q] == vi + r ? rc[q].y : 0.0f);
+        c[r] = live && !(zform && v[r] == CT_OUT) ? o : 0.0f;
+      }
+      if (n < a.Npad) ct_store4<uint16_t>((uint16_t*)a.C + (int64_t)n * a.ldc + 32 * t + 16 * rb + 4 * g, c);
+    }
+  };
+
+  f32x4 A[QB][2], B[QB][2];
+  // tile t into cur, with the previous tile's epilogue between its steps
+  auto tile = [&](int t, f32x4 (&cur)[QB][2], f32x4 (&prev)[QB][2], bool has_prev) __attribute__((always_inline)) {
+    if (t + SLOTS - 1 <= t1) ct_wait_vm<(SLOTS - 2) * OPS>();
+    else ct_wait_vm<0>();
+    ct_barrier();  // tile t is complete; every wave is done with the slot refilled next
+    if (t + SLOTS - 1 < t1) issue(t + SLOTS - 1);
+    const char* st = smem + (t % SLOTS) * TB;
+    const bool edge = COEF && has_prev && a.v_base + 32 * t > v_end;  // (the previous tile's)
+    float s2 = a.s2;
+    if (has_prev) {
+      to_z(prev, t - 1, edge);
+      if (BIAS || edge) s2 = 1.0f;
+      if constexpr (!COEF) head(prev, t - 1, s2);
+    }
+#pragma unroll
+    for (int q = 0; q < QB; ++q)
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) cur[q][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      u32x4_t f[2];
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+        f[rb] = *(const u32x4_t*)(st + fo[k & 3] + (k >> 2) * 256 + rb * 16 * KS * 64);
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+          cur[q][rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ct_bf16x8, f[rb]),
+                                                               __builtin_bit_cast(ct_bf16x8, xf[k][q]), cur[q][rb], 0, 0, 0);
+      if (has_prev) {  // the 2 QB blocks of the epilogue spread over the KS steps
+#pragma unroll
+        for (int e = 0; e < 2 * QB; ++e)
+          if (e * KS / (2 * QB) == k) body(prev[e >> 1][e & 1], e >> 1, e & 1, t - 1, s2, BIAS || edge);
+      }
+    }
+  };
+  tile(t0, A, B, false);
+  int t = t0 + 1;
+  for (; t + 1 < t1; t += 2) {
+    tile(t, B, A, true);
+    tile(t + 1, A, B, true);
+  }
+  auto finish = [&](f32x4 (&acc)[QB][2]) __attribute__((always_inline)) {  // the last tile's epilogue
+    const bool edge = a.v_base + 32 * t1 > v_end;
+    to_z(acc, t1 - 1, edge);
+    const float s2 = BIAS || edge ? 1.0f : a.s2;
+    if constexpr (!COEF) head(acc, t1 - 1, s2);
+#pragma unroll
+    for (int e = 0; e < 2 * QB; ++e) body(acc[e >> 1][e & 1], e >> 1, e & 1, t1 - 1, s2, BIAS || edge);
+  };
+  if (t < t1) {
+    tile(t, B, A, true);
+    finish(B);
+  } else {
+    finish(A);
+  }
+  if constexpr (!COEF) {  // a row's four lanes
+#pragma unroll
+    for (int q = 0; q < QB; ++q) {
+#pragma unroll
+      for (int o = 16; o < 64; o <<= 1) {
+        const float m2 = __shfl_xor(m[q], o, 64), L2 = __shfl_xor(L[q], o, 64), T2 = __shfl_xor(TT[q], o, 64);
+        stat_join(m[q], L[q], TT[q], m2, L2, T2);
+      }
+      const int n = nb + 16 * q + rl;
+      if (g == 0 && n < a.N) a.part[(int64_t)sp * a.N + n] = float4{m[q], L[q], TT[q], 0.0f};
     }
   }
 }
@@ -380,18 +653,28 @@ __device__ __forceinline__ double wave_dot64(const T* x, const T* w, int E, int 
   return d;
 }
 
+struct CombineArgs {
+  const float4* part;
+  int splits, N, V, E;
+  const void *x, *w;
+  int64_t ldx, ldw;
+  const int64_t* ids;
+  const float* bias;
+  double s;
+  float *logp, *ent, *lse;
+};
 // One wave per row: the shares' statistics joined, the given item's logit.
 template <typename T>
-__global__ __launch_bounds__(256) void k_combine(const float4* __restrict__ part, int splits, int N,
-                                                 int V, int E, const T* __restrict__ x, int64_t ldx,
-                                                 const T* __restrict__ w, int64_t ldw,
-                                                 const int64_t* __restrict__ ids,
-                                                 const float* __restrict__ bias, double s,
-                                                 float* __restrict__ logp, float* __restrict__ ent,
-                                                 float* __restrict__ lse) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= N) return;
+__device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int lane) {
+  const T* x = (const T*)a.x;
+  const T* w = (const T*)a.w;
+  const float4* part = a.part;
+  const int splits = a.splits, N = a.N, V = a.V, E = a.E;
+  const int64_t ldx = a.ldx, ldw = a.ldw;
+  const int64_t* ids = a.ids;
+  const float* bias = a.bias;
+  const double s = a.s;
+  float *logp = a.logp, *ent = a.ent, *lse = a.lse;
   float m = CT_NONE, L = 0.0f, TT = 0.0f;
   for (int i = lane; i < splits; i += 64) {
     const float4 p = part[(int64_t)i * N + n];
@@ -420,6 +703,11 @@ __global__ __launch_bounds__(256) void k_combine(const float4* __restrict__ part
     if (ent) ent[n] = empty ? 0.0f : (float)((l2 - (double)TT / (double)L) * 0.6931471805599453);
     lse[n] = empty ? -inf : (float)ls;
   }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_combine(const CombineArgs a) {
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n < a.N) combine_row<T>(a, n, threadIdx.x & 63);
 }
 
 // ------------------------------------------------------------------- top alternatives
@@ -474,13 +762,21 @@ __device__ __forceinline__ int wave_select(const uint64_t (&key)[PER], int keep,
 }
 
 // Groups of 16 items (tmax entries) of one row: the keep largest of every segment, key = (maximum,
-// ~group).  Block = (segment, row): each of its 4 waves keeps the best of its 1024 entries at a
+// ~group).  The launch's last blocks join the statistics (k_combine's work, which nothing here waits
+// for: one launch less).  Block = (segment, row): each of its 4 waves keeps the best of its 1024 entries at a
 // time, with those it has, wave 0 joins the four lists.  Unused places are 0.
+template <typename T>
 __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tmax, int64_t M, int seg_len,
-                                                    int nseg, int keep, uint64_t* __restrict__ out) {
+                                                    int nseg, int keep, uint64_t* __restrict__ out,
+                                                    unsigned n_seg_blocks, const CombineArgs ca) {
   __shared__ uint64_t red[4][64];
   __shared__ uint64_t fin[64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (blockIdx.x >= n_seg_blocks) {
+    const int64_t r = (int64_t)(blockIdx.x - n_seg_blocks) * 4 + w;
+    if (r < ca.N) combine_row<T>(ca, r, lane);
+    return;
+  }
   const int64_t n = blockIdx.x / nseg;
   const int sg = (int)(blockIdx.x % nseg);
   const int64_t i0 = (int64_t)sg * seg_len, i1 = i0 + seg_len < M ? i0 + seg_len : M;
@@ -495,7 +791,35 @@ __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tm
       key[i] = e < i1 ? make_key(row[e], (uint32_t)e) : 0ull;
     }
     wave_sync();
-    have = wave_select<17>(key, keep, red[w], lane);
+    // a bound first: of the lanes' largest keys the keep-th largest (high words), which at least keep
+    // keys reach; few others do, so the exact choice is then among one key a lane
+    uint64_t lm = key[0];
+#pragma unroll
+    for (int i = 1; i < 17; ++i) lm = key[i] > lm ? key[i] : lm;
+    uint32_t bound = 0u;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = bound | (1u << bit);
+      if (__popcll(__ballot((uint32_t)(lm >> 32) >= cand)) >= keep) bound = cand;
+    }
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < 17; ++i) {
+      const bool in = key[i] != 0ull && (uint32_t)(key[i] >> 32) >= bound;
+      const uint64_t bm = __ballot(in);
+      const int pos = c + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(bm >> 32),
+                                                         __builtin_amdgcn_mbcnt_lo((uint32_t)bm, 0u));
+      if (in && pos < 64) red[w][pos] = key[i];
+      c += __popcll(bm);
+    }
+    wave_sync();
+    if (c <= 64) {
+      const uint64_t k1[1] = {lane < c ? red[w][lane] : 0ull};
+      wave_sync();
+      have = wave_select<1>(k1, keep, red[w], lane);
+    } else {  // (many equal maxima)
+      have = wave_select<17>(key, keep, red[w], lane);
+    }
     wave_sync();
   }
   if (lane >= have) red[w][lane] = 0ull;
@@ -526,9 +850,9 @@ __device__ __forceinline__ double dot16(const u32x4_t& a, const u32x4_t& b, doub
 }
 
 // One block per row: the keep largest groups of all segments, their items scored in 64 bits (16 lanes
-// an item, 16-byte loads, four groups' items in flight), the top of them by (score, lower id).
+// an item, 16-byte loads, 128 items in flight), the top of them by (score, lower id).
 template <typename T>
-__global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ segs, int nseg, int keep,
+__global__ __launch_bounds__(CT_TOP_NT) void k_top_items(const uint64_t* __restrict__ segs, int nseg, int keep,
                                                    int top, const T* __restrict__ x, int64_t ldx,
                                                    const T* __restrict__ w, int64_t ldw, int E, int V,
                                                    const float* __restrict__ bias, double s,
@@ -536,7 +860,8 @@ __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ 
                                                    int64_t* __restrict__ ids_out, float* __restrict__ lp_out) {
   constexpr int GMAX = CT_TOP_MAX + CT_TOP_EXTRA;
   constexpr int PC = 16 / (int)sizeof(T);
-  __shared__ uint64_t red[4][64];
+  constexpr int NW = CT_TOP_NT / 64, NG = CT_TOP_NT / 16;
+  __shared__ uint64_t red[NW][64];
   __shared__ uint64_t fin[64];
   __shared__ uint32_t grp[64];
   __shared__ int cnt[4];
@@ -550,7 +875,7 @@ __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ 
   const int total = nseg * keep;
   const uint64_t* src = segs + n * total;
   int have = 0;
-  for (int b = wv * 256; b < total; b += 1024) {
+  for (int b = wv * 256; b < total; b += NW * 256) {
     uint64_t key[5];
     key[4] = lane < have ? red[wv][lane] : 0ull;
 #pragma unroll
@@ -563,10 +888,10 @@ __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ 
   if (tid == 0) nlist = 0;
   __syncthreads();
   if (wv == 0) {
-    uint64_t key[4];
+    uint64_t key[NW];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) key[i] = red[i][lane];
-    const int c = wave_select<4>(key, keep, fin, lane);
+    for (int i = 0; i < NW; ++i) key[i] = red[i][lane];
+    const int c = wave_select<NW>(key, keep, fin, lane);
     wave_sync();
     const uint64_t k1[1] = {lane < c ? fin[lane] : 0ull};
     // the top-th largest maximum: the top-th largest logit is not below it, so a group or an item
@@ -595,18 +920,20 @@ __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ 
   const int ngrp = cnt[0];
   const float floor = s_floor;
   const T* xr = x + n * ldx;
-  const int sub = tid >> 4, l16 = tid & 15;
-  for (int g0 = 0; g0 < ngrp; g0 += 4) {
+  const int sub = tid >> 4, l16 = tid & 15, cand = ngrp * 16;
+  for (int i0 = sub; i0 < cand; i0 += 4 * NG) {
     int v[4];
     double d[4];
     const T* wr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t q = grp[g0 + i < ngrp ? g0 + i : ngrp - 1];
-      v[i] = (int)(q >> 2) * 64 + 16 * (sub >> 2) + 4 * (int)(q & 3) + (sub & 3);
+      const int c = i0 + i * NG < cand ? i0 + i * NG : i0, it = c & 15;
+      const uint32_t q = grp[c >> 4];
+      v[i] = (int)(q >> 2) * 64 + 16 * (it >> 2) + 4 * (int)(q & 3) + (it & 3);
       wr[i] = w + (int64_t)(v[i] < V ? v[i] : V - 1) * ldw;
       d[i] = 0.0;
     }
+#pragma unroll 2
     for (int e = l16 * PC; e < E; e += 16 * PC) {
       const u32x4_t xv = *(const u32x4_t*)(xr + e);
       u32x4_t y[4];
@@ -619,7 +946,8 @@ __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ 
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) d[i] += __shfl_xor(d[i], o, 64);
-      if (l16 == 0 && g0 + i < ngrp) {
+      const int c = i0 + i * NG;
+      if (l16 == 0 && c < cand) {
         double l = -__builtin_huge_val();
         bool in = false;
         if (v[i] < V) {
@@ -627,16 +955,16 @@ __global__ __launch_bounds__(256) void k_top_items(const uint64_t* __restrict__ 
           if (!(b <= CT_OUT)) l = s * d[i] + (double)b;
           in = !(l * 1.4426950408889634 < (double)floor);  // (-inf, NaN: only where the floor lets them)
         }
-        sc[(g0 + i) * 16 + sub] = l;
-        vid[(g0 + i) * 16 + sub] = v[i];
-        if (in) list[atomicAdd(&nlist, 1)] = (short)((g0 + i) * 16 + sub);
+        sc[c] = l;
+        vid[c] = v[i];
+        if (in) list[atomicAdd(&nlist, 1)] = (short)c;
       }
     }
   }
   __syncthreads();
   const float ls = lse[n];
   const int m = nlist;  // (in any order: ranks do not depend on it)
-  for (int i = tid; i < m; i += 256) {
+  for (int i = tid; i < m; i += CT_TOP_NT) {
     const int c = list[i];
     const double l = sc[c];
     const int v = vid[c];
@@ -702,56 +1030,56 @@ struct ProductArgs {
   int64_t ldo;
   float* part;
 };
-template <typename T, bool ACOL>
-__global__ __launch_bounds__(256, 2) void k_product(const ProductArgs a) {
-  constexpr int BK = 128 / (int)sizeof(T);
-  __shared__ __attribute__((aligned(16))) char smem[4 * CT_OP_B];
+template <typename T, bool ACOL, int NB>
+__global__ __launch_bounds__(256, NB == 4 ? 2 : 3) void k_product(const ProductArgs a) {
+  constexpr int BK = 128 / (int)sizeof(T), TILE = 32 * NB, WT = 16 * NB, OP_B = TILE * 128;
+  __shared__ __attribute__((aligned(16))) char smem[4 * OP_B];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w >> 1, wc = w & 1, g = lane >> 4, rl = lane & 15;
-  const int tc = (a.cols + CT_TILE - 1) / CT_TILE, tm = (a.M + CT_TILE - 1) / CT_TILE;
+  const int tc = (a.cols + TILE - 1) / TILE, tm = (a.M + TILE - 1) / TILE;
   const int lb = xcd_remap(blockIdx.x, gridDim.x);
   const int sp = lb / (tc * tm), t = lb % (tc * tm);
-  const int m0 = t / tc * CT_TILE, c0 = t % tc * CT_TILE;
+  const int m0 = t / tc * TILE, c0 = t % tc * TILE;
   const T* A = (const T*)a.A;
   const T* B = (const T*)a.B;
   const int nk = a.K / BK, per = (nk + a.splits - 1) / a.splits;
   const int k0 = sp * per, k1 = k0 + per < nk ? k0 + per : nk;
-  RowStage<T> ra;
-  ColStage<T> ca, cb;
+  RowStage<T, NB> ra;
+  ColStage<T, NB> ca, cb;
   if constexpr (ACOL) ca.init(m0, a.lda, w, lane);  // (lda: whole tiles, all written)
   else ra.init(a.lda, m0, a.a_rows, w, lane);
   cb.init(c0, a.cols, w, lane);
   auto issue = [&](int kt) __attribute__((always_inline)) {
-    char* st = smem + (kt & 1) * 2 * CT_OP_B;
+    char* st = smem + (kt & 1) * 2 * OP_B;
     if constexpr (ACOL) ca.issue(A, a.lda, (int64_t)kt * BK, a.a_rows, st, w);
     else ra.issue(A, (int64_t)kt * BK, st, w);
-    cb.issue(B, a.ldb, (int64_t)kt * BK, a.b_rows, st + CT_OP_B, w);
+    cb.issue(B, a.ldb, (int64_t)kt * BK, a.b_rows, st + OP_B, w);
   };
-  f32x4 acc[4][4];
+  f32x4 acc[NB][NB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (k0 < k1) issue(k0);
   for (int kt = k0; kt < k1; ++kt) {
     ct_wait_vm<0>();
     ct_barrier();
     if (kt + 1 < k1) issue(kt + 1);
-    const char* st = smem + (kt & 1) * 2 * CT_OP_B;
-    u32x4_t fa[2][4], fb[2][4];
-    if constexpr (ACOL) col_frags<T>(st, 64 * wm, lane, fa);
-    else row_frags(st, 64 * wm, lane, fa);
-    col_frags<T>(st + CT_OP_B, 64 * wc, lane, fb);
-    ct_mfma<T>(fb, fa, acc);
+    const char* st = smem + (kt & 1) * 2 * OP_B;
+    u32x4_t fa[2][NB], fb[2][NB];
+    if constexpr (ACOL) col_frags<T, NB>(st, WT * wm, lane, fa);
+    else row_frags<NB>(st, WT * wm, lane, fa);
+    col_frags<T, NB>(st + OP_B, WT * wc, lane, fb);
+    ct_mfma<T, NB>(fb, fa, acc);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int mm = m0 + 64 * wm + 16 * i + rl;
+  for (int i = 0; i < NB; ++i) {
+    const int mm = m0 + WT * wm + 16 * i + rl;
     if (mm >= a.M) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = c0 + 64 * wc + 16 * j + 4 * g;
+    for (int j = 0; j < NB; ++j) {
+      const int c = c0 + WT * wc + 16 * j + 4 * g;
       if (c >= a.cols) continue;
       if (a.part) {
         f32x4* p = (f32x4*)(a.part + ((int64_t)sp * a.M + mm) * a.cols + c);
@@ -777,18 +1105,61 @@ __global__ __launch_bounds__(256) void k_product_sum(const float* __restrict__ p
 static int64_t up(int64_t n, int64_t q) { return (n + q - 1) / q * q; }
 static int64_t cdiv(int64_t n, int64_t q) { return (n + q - 1) / q; }
 
+// k_ring takes these
+static bool ring_ok(int64_t N, int E, int64_t sz) { return sz == 2 && N > 128 && E % 128 == 0 && E <= 384; }
+static int ring_rows(int E) { return 128 * (E <= 256 ? 4 : 3); }
+template <int KS, bool COEF>
+static void ring_go(const LogitArgs& a, bool ent, hipStream_t st) {
+  const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits));
+  static_assert(RingCfg<KS>::ROWS == 128 * RingCfg<KS>::QB, "");
+  if (a.bias) {
+    if (ent) hipLaunchKernelGGL((k_ring<KS, COEF, true, true>), grid, dim3(CR_NT), 0, st, a);
+    else hipLaunchKernelGGL((k_ring<KS, COEF, false, true>), grid, dim3(CR_NT), 0, st, a);
+  } else {
+    if (ent) hipLaunchKernelGGL((k_ring<KS, COEF, true, false>), grid, dim3(CR_NT), 0, st, a);
+    else hipLaunchKernelGGL((k_ring<KS, COEF, false, false>), grid, dim3(CR_NT), 0, st, a);
+  }
+}
+template <bool COEF>
+static void ring_launch(const LogitArgs& a, bool ent, hipStream_t st) {
+  switch (a.E / 32) {
+    case 4: return ring_go<4, COEF>(a, ent, st);
+    case 8: return ring_go<8, COEF>(a, ent, st);
+    default: return ring_go<12, COEF>(a, ent, st);
+  }
+}
+// rows a block takes, and shares of `pairs` (64 items each) for about one block a CU
+static void ring_shape(int64_t N, int64_t V, int E, int& n_tiles, int& pairs, int& splits) {
+  n_tiles = (int)cdiv(N, ring_rows(E));
+  pairs = (int)cdiv(V, 64);
+  int64_t s = 256 / n_tiles;
+  s = s < 1 ? 1 : s > pairs ? pairs : s;
+  splits = (int)cdiv(pairs, cdiv(pairs, s));
+}
+
+// Tile edge of k_logits: 128, or 64 where 128 would give the 256 CUs less than a block each (512 x
+// 2560 x 768 f32: 57 us with 80 blocks of 128, @F32SMALL@ us with 320 of 64).
+static int logits_edge(int64_t N, int64_t V) { return cdiv(N, 128) * cdiv(V, 128) < 256 ? 64 : 128; }
+
 struct StatPlan {
-  int n_tiles, v_tiles, splits, keep, nseg, seg_len;
+  bool ring;
+  int edge, n_tiles, v_tiles, splits, keep, nseg, seg_len;
   int64_t M, off_tmax, off_seg, bytes;
 };
-// Shares: about 512 blocks (two a CU).
-static StatPlan stat_plan(int64_t N, int64_t V, int top) {
+// Shares: about 512 blocks (two a CU; three of the small tiles).
+static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
   StatPlan p{};
-  p.n_tiles = (int)cdiv(N, CT_TILE);
-  p.v_tiles = (int)cdiv(V, CT_TILE);
-  int64_t s = 512 / p.n_tiles;
-  s = s < 1 ? 1 : s > p.v_tiles ? p.v_tiles : s;
-  p.splits = (int)cdiv(p.v_tiles, cdiv(p.v_tiles, s));
+  p.ring = ring_ok(N, E, sz);
+  if (p.ring) {
+    ring_shape(N, V, E, p.n_tiles, p.v_tiles, p.splits);
+  } else {
+    p.edge = logits_edge(N, V);
+    p.n_tiles = (int)cdiv(N, p.edge);
+    p.v_tiles = (int)cdiv(V, p.edge);
+    int64_t s = (p.edge == 64 ? 768 : 512) / p.n_tiles;
+    s = s < 1 ? 1 : s > p.v_tiles ? p.v_tiles : s;
+    p.splits = (int)cdiv(p.v_tiles, cdiv(p.v_tiles, s));
+  }
   p.bytes = up((int64_t)p.splits * N * 16, 256);
   if (top > 0) {
     p.keep = top + CT_TOP_EXTRA;
@@ -806,14 +1177,26 @@ static StatPlan stat_plan(int64_t N, int64_t V, int top) {
 constexpr int64_t CT_C_BYTES = 256ll << 20;  // one chunk of C stays in the last-level cache
 struct BwdPlan {
   int64_t Npad, Vc, n_chunks;
-  int sx, sw;
+  int sx, sw, ex, ew;  // splits and tile edges of the two products
   int64_t off_row, off_x, off_w, off_c, off_px, off_pw, bytes;
 };
-static int product_splits(int64_t M, int64_t cols, int64_t K, int BK) {
-  const int64_t tiles = cdiv(M, CT_TILE) * cdiv(cols, CT_TILE), nk = K / BK;
-  int64_t s = cdiv(512, tiles), most = nk / 4 > 1 ? nk / 4 : 1;
-  s = s < most ? s : most;
-  return (int)cdiv(nk, cdiv(nk, s));  // no empty split
+// Tile edge and splits of a product of K / BK steps: the least of (rounds of the card's block slots)
+// x (steps a block walks, and 6 more for its start and end), with a step's worth a 0.75 M floats of
+// partial sums; the small tile where the large one leaves CUs idle.
+static void product_shape(int64_t M, int64_t cols, int64_t K, int BK, int& edge, int& splits) {
+  edge = cdiv(M, 128) * cdiv(cols, 128) < 256 ? 64 : 128;
+  const int64_t tiles = cdiv(M, edge) * cdiv(cols, edge), nk = K / BK, slots = edge == 64 ? 768 : 512;
+  double best = 0;
+  splits = 1;
+  for (int64_t s = 1; s <= 16 && (s == 1 || s * 4 <= nk); ++s) {
+    const double c = (double)cdiv(tiles * s, slots) * (double)(cdiv(nk, s) + 6) +
+                     (s > 1 ? 1.3e-6 * (double)(s * M * cols) : 0.0);
+    if (s == 1 || c < best) {
+      best = c;
+      splits = (int)s;
+    }
+  }
+  splits = (int)cdiv(nk, cdiv(nk, splits));  // no empty split
 }
 static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, bool dx, bool dw) {
   BwdPlan p{};
@@ -830,14 +1213,31 @@ static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, 
   if (bias) o += up(V * E * sz, 256);
   p.off_c = o;
   o += up(p.Npad * p.Vc * sz, 256);
-  p.sx = product_splits(N, E, p.Vc, BK);
-  p.sw = product_splits(p.Vc, E, p.Npad, BK);
+  product_shape(N, E, p.Vc, BK, p.ex, p.sx);
+  product_shape(p.Vc, E, p.Npad, BK, p.ew, p.sw);
   p.off_px = o;
   if (dx && (p.sx > 1 || p.n_chunks > 1)) o += up((int64_t)p.sx * N * E * 4, 256);
   p.off_pw = o;
   if (dw && p.sw > 1) o += up((int64_t)p.sw * p.Vc * E * 4, 256);
   p.bytes = o;
   return p;
+}
+template <typename T, bool ACOL>
+static void product_launch(const ProductArgs& q, int edge, hipStream_t st) {
+  const dim3 grid((unsigned)(cdiv(q.M, edge) * cdiv(q.cols, edge) * q.splits));
+  if (edge == 64) hipLaunchKernelGGL((k_product<T, ACOL, 2>), grid, dim3(256), 0, st, q);
+  else hipLaunchKernelGGL((k_product<T, ACOL, 4>), grid, dim3(256), 0, st, q);
+}
+template <typename T, bool COEF>
+static void logits_launch(const LogitArgs& a, int edge, bool ent, hipStream_t st) {
+  const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits));
+  if (edge == 64) {
+    if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, 2>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_logits<T, COEF, false, 2>), grid, dim3(256), 0, st, a);
+  } else {
+    if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_logits<T, COEF, false, 4>), grid, dim3(256), 0, st, a);
+  }
 }
 
 static int ct_check(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype, int64_t N,
@@ -868,17 +1268,20 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   a.n_tiles = p.n_tiles; a.splits = p.splits; a.v_tiles = p.v_tiles;
   a.part = (float4*)ws;
   a.tmax = top ? (float*)(ws + p.off_tmax) : nullptr;
-  const dim3 grid((unsigned)(p.n_tiles * (int64_t)p.splits));
-  if (ent) hipLaunchKernelGGL((k_logits<T, false, true>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_logits<T, false, false>), grid, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(k_combine<T>, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, st, a.part, p.splits, (int)N,
-                     (int)V, E, (const T*)x, ldx, (const T*)w, ldw, ids, bias, s, logp, ent, lse);
+  a.v_count = (int)V;
+  if (p.ring) ring_launch<false>(a, ent != nullptr, st);
+  else logits_launch<T, false>(a, p.edge, ent != nullptr, st);
+  const CombineArgs ca{a.part, p.splits, (int)N, (int)V, E, x, w, ldx, ldw, ids, bias, s, logp, ent, lse};
+  const unsigned cb = (unsigned)cdiv(N, 4);
   if (top) {
     uint64_t* seg = (uint64_t*)(ws + p.off_seg);
-    hipLaunchKernelGGL(k_top_groups, dim3((unsigned)(N * p.nseg)), dim3(256), 0, st, a.tmax, p.M, p.seg_len,
-                       p.nseg, p.keep, seg);
-    hipLaunchKernelGGL(k_top_items<T>, dim3((unsigned)N), dim3(256), 0, st, seg, p.nseg, p.keep, top,
+    const unsigned sb = (unsigned)(N * p.nseg);
+    hipLaunchKernelGGL(k_top_groups<T>, dim3(sb + cb), dim3(256), 0, st, a.tmax, p.M, p.seg_len, p.nseg,
+                       p.keep, seg, sb, ca);
+    hipLaunchKernelGGL(k_top_items<T>, dim3((unsigned)N), dim3(CT_TOP_NT), 0, st, seg, p.nseg, p.keep, top,
                        (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+  } else {
+    hipLaunchKernelGGL(k_combine<T>, dim3(cb), dim3(256), 0, st, ca);
   }
   return check_launch("tt_catalog_logprobs");
 }
@@ -911,13 +1314,18 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     a.x = xz; a.w = wz; a.ldx = E; a.ldw = ldwz; a.bias = bias;
     a.s2 = (float)(s * 1.4426950408889634);
     a.N = (int)N; a.V = (int)V; a.E = E;
-    a.n_tiles = (int)cdiv(N, CT_TILE);
-    a.v_tiles = a.splits = (int)cdiv(vn, CT_TILE);
     a.rowc = rowc; a.ids = ids; a.C = C; a.ldc = p.Vc; a.v_base = (int)vb; a.Npad = (int)p.Npad;
-    const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits));
-    if (e) hipLaunchKernelGGL((k_logits<T, true, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_logits<T, true, false>), grid, dim3(256), 0, st, a);
-    const int64_t vk = up(vn, CT_TILE);
+    a.v_count = (int)vn;
+    if (ring_ok(N, E, sizeof(T))) {
+      ring_shape(N, vn, E, a.n_tiles, a.v_tiles, a.splits);
+      ring_launch<true>(a, e != nullptr, st);
+    } else {
+      const int edge = logits_edge(N, vn);
+      a.n_tiles = (int)cdiv(N, edge);
+      a.v_tiles = a.splits = (int)cdiv(vn, edge);
+      logits_launch<T, true>(a, edge, e != nullptr, st);
+    }
+    const int64_t vk = up(vn, 64);
     if (dx) {
       ProductArgs q{};
       q.A = C; q.lda = p.Vc; q.a_rows = p.Npad;
@@ -925,8 +1333,7 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       q.M = (int)N; q.cols = E; q.K = (int)vk; q.splits = p.sx;
       q.acc = c > 0; q.scale = (float)s; q.out = dx; q.ldo = E;
       q.part = part_x ? px : nullptr;
-      hipLaunchKernelGGL((k_product<T, false>),
-                         dim3((unsigned)(cdiv(N, CT_TILE) * cdiv(E, CT_TILE) * p.sx)), dim3(256), 0, st, q);
+      product_launch<T, false>(q, p.ex, st);
     }
     if (dw) {
       ProductArgs q{};
@@ -935,8 +1342,7 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       q.M = (int)vn; q.cols = E; q.K = (int)p.Npad; q.splits = p.sw;
       q.scale = (float)s; q.out = (T*)dw + vb * E; q.ldo = E;
       q.part = p.sw > 1 ? (float*)(ws + p.off_pw) : nullptr;
-      hipLaunchKernelGGL((k_product<T, true>),
-                         dim3((unsigned)(cdiv(vn, CT_TILE) * cdiv(E, CT_TILE) * p.sw)), dim3(256), 0, st, q);
+      product_launch<T, true>(q, p.ew, st);
       if (q.part) {
         const int64_t n4 = vn * E / 4, nb = cdiv(n4, 256);
         hipLaunchKernelGGL(k_product_sum<T>, dim3((unsigned)(nb < 8192 ? nb : 8192)), dim3(256), 0, st,
@@ -966,7 +1372,7 @@ extern "C" int tt_catalog_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t
                                                    int64_t* bytes) {
   CT_SIZES_ONLY();
   TT_REQUIRE(top >= 0 && top <= CT_TOP_MAX && top <= V, "need 0 <= top <= min(V, 32)");
-  *bytes = N > 0 ? stat_plan(N, V, top).bytes : 0;
+  *bytes = N > 0 ? stat_plan(N, V, E, dtype == TT_DTYPE_F32 ? 4 : 2, top).bytes : 0;
   return TT_OK;
 }
 
@@ -979,7 +1385,7 @@ extern "C" int tt_catalog_logprobs(const void* x, int64_t ldx, const void* w, in
   TT_REQUIRE(top >= 0 && top <= CT_TOP_MAX && top <= V, "need 0 <= top <= min(V, 32)");
   if (N == 0) return TT_OK;
   TT_REQUIRE(lse && (!log_prob || ids) && (top == 0 || (top_ids && top_log_prob)), "null pointer");
-  const StatPlan p = stat_plan(N, V, top);
+  const StatPlan p = stat_plan(N, V, E, dtype == TT_DTYPE_F32 ? 4 : 2, top);
   TT_REQUIRE(N * (int64_t)p.nseg < (1ll << 24), "too many rows for this many items: pass fewer at a time");
   if (!workspace || workspace_bytes < p.bytes)
     return fail(TT_ERR_WORKSPACE, "tt_catalog_logprobs: workspace too small");

@@ -7,6 +7,7 @@ Python exception instead of reaching a kernel with inconsistent sizes.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -616,44 +617,77 @@ def attn_agg_l2(items, w, W1, b1, W2, b2, out=None, fused: bool = None):
     return out
 
 
-def _scan_rows(t, name):
+
+def _addr(t):
+    """Device address for the C call (None: NULL)."""
+    return t.data_ptr() if t is not None else None
+
+
+def _as(t, dtype):
+    """t as dtype, contiguous, without autograd history; itself when it already is."""
+    if t.dtype is dtype and not t.requires_grad and t.is_contiguous():
+        return t
+    return t.detach().to(dtype).contiguous()
+
+
+def _same_device(x, others, what):
+    idx = x.get_device()
+    for t, name in others:
+        if t is not None and t.get_device() != idx:
+            raise ValueError(f"{what}: {name} is on {t.device}, {x.device} is expected")
+
+
+def _scan_rows(t):
     """[B, S, D] with unit channel stride: (tensor, history stride, event stride)."""
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    st = t.stride()
+    if st[2] != 1 and t.shape[2] > 1:
         t = t.contiguous()
-    return t, t.stride(0), t.stride(1)
+        st = t.stride()
+    return t, st[0], st[1]
 
 
 def _scan_args(x, gate, weights, h0):
-    require_device(x, "x")
-    require_device(gate, "gate")
-    if x.dtype not in _lib.DTYPES or gate.dtype != x.dtype:
+    dt = _lib.DTYPES.get(x.dtype)
+    if not x.is_cuda or not gate.is_cuda:
+        require_device(x, "x")
+        require_device(gate, "gate")
+    if dt is None or gate.dtype is not x.dtype:
         raise TypeError(f"gated_scan: x and gate must both be float32 or bfloat16, got {x.dtype} "
                         f"and {gate.dtype}")
-    if x.dim() != 3 or gate.shape != x.shape or x.shape[2] < 1:
+    shape = x.shape
+    if len(shape) != 3 or gate.shape != shape or shape[2] < 1:
         raise ValueError(f"gated_scan: x and gate must be [B, S, D], got {tuple(x.shape)} and "
                          f"{tuple(gate.shape)}")
-    b, s, d = x.shape
-    if weights is not None and tuple(weights.shape) != (b, s):
+    b, s, d = shape
+    if weights is not None and weights.shape != (b, s):
         raise ValueError(f"gated_scan: weights must be [{b}, {s}], got {tuple(weights.shape)}")
-    if h0 is not None and tuple(h0.shape) != (b, d):
+    if h0 is not None and h0.shape != (b, d):
         raise ValueError(f"gated_scan: h0 must be [{b}, {d}], got {tuple(h0.shape)}")
-    for t, name in ((gate, "gate"), (weights, "weights"), (h0, "h0")):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"gated_scan: {name} is on {t.device}, x on {x.device}")
+    _same_device(x, ((gate, "gate"), (weights, "weights"), (h0, "h0")), "gated_scan")
+    ws = 0
     if weights is not None:
-        weights = weights.detach().to(_f32)
+        if weights.dtype is not _f32 or weights.requires_grad:
+            weights = weights.detach().to(_f32)
         if s > 1 and weights.stride(1) != 1:
             weights = weights.contiguous()
-    if h0 is not None:
-        h0 = h0.detach().to(_f32).contiguous()
-    return weights, h0
+        ws = weights.stride(0)
+    return dt, b, s, d, weights, ws, _as(h0, _f32) if h0 is not None else None
 
 
-def _scan_workspace(b, s, d, device):
+SCAN_SPLIT_MIN = 128  # histories shorter than this are never split: no workspace
+
+
+@functools.lru_cache(maxsize=1024)
+def _scan_workspace_bytes(b, s, d):
     need = ctypes.c_int64(0)
     check(lib().tt_gated_scan_workspace_bytes(b, s, d, ctypes.byref(need)),
           "tt_gated_scan_workspace_bytes")
-    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    return need.value
+
+
+def _scan_workspace(b, s, d, device):
+    n = _scan_workspace_bytes(b, s, d) if s >= SCAN_SPLIT_MIN and b else 0
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def gated_scan(x, gate, weights=None, h0=None, states: bool = True, save: bool = False):
@@ -662,11 +696,10 @@ def gated_scan(x, gate, weights=None, h0=None, states: bool = True, save: bool =
     0 is padding and leaves the state as it is), h0 [B, D] (None: 0) -> (h [B, S, D] in x's type
     or None without ``states``, h_last [B, D] f32, the states gated_scan_backward needs or None
     without ``save``)."""
-    weights, h0 = _scan_args(x, gate, weights, h0)
-    b, s, d = x.shape
+    dt, b, s, d, weights, wsb, h0 = _scan_args(x, gate, weights, h0)
     with _lib.on_device(x):
-        x, xb, xs = _scan_rows(x, "x")
-        gate, gb, gs = _scan_rows(gate, "gate")
+        x, xb, xs = _scan_rows(x)
+        gate, gb, gs = _scan_rows(gate)
         dev = x.device
         h = torch.empty((b, s, d), dtype=x.dtype, device=dev) if states else None
         last = torch.empty((b, d), dtype=_f32, device=dev)
@@ -675,39 +708,38 @@ def gated_scan(x, gate, weights=None, h0=None, states: bool = True, save: bool =
             ck = torch.empty((b, -(-s // _lib.TT_SCAN_CKPT), d), dtype=_f32, device=dev)
         ws = _scan_workspace(b, s, d, dev)
         check(lib().tt_gated_scan_fwd(
-            _ptr(x), _ptr(gate), _lib.DTYPES[x.dtype], b, s, d, xb, xs, gb, gs, _ptr(weights),
-            weights.stride(0) if weights is not None else 0, _ptr(h0), _ptr(h), _ptr(last),
-            _ptr(ck), _ptr(ws), ws.numel() if ws is not None else 0, stream_ptr()),
-            "tt_gated_scan_fwd")
+            x.data_ptr(), gate.data_ptr(), dt, b, s, d, xb, xs, gb, gs, _addr(weights), wsb,
+            _addr(h0), _addr(h), last.data_ptr(), _addr(ck), _addr(ws),
+            ws.numel() if ws is not None else 0, stream_ptr()), "tt_gated_scan_fwd")
     return h, last, ck
 
 
 def gated_scan_backward(x, gate, weights, saved, dh, dlast, need_h0: bool):
     """Gradients (dx, dgate [B, S, D] in x's type, dh0 [B, D] f32 or None) of gated_scan for dh
     [B, S, D] (or None) and dlast [B, D] (or None); ``saved`` from gated_scan(save=True)."""
-    weights, _ = _scan_args(x, gate, weights, None)
-    b, s, d = x.shape
-    if saved is None or tuple(saved.shape) != (b, -(-s // _lib.TT_SCAN_CKPT), d):
+    dt, b, s, d, weights, wsb, _ = _scan_args(x, gate, weights, None)
+    if saved is None or saved.shape != (b, -(-s // _lib.TT_SCAN_CKPT), d):
         raise ValueError("gated_scan_backward: saved must come from gated_scan(save=True)")
-    if dh is not None and tuple(dh.shape) != (b, s, d):
+    if dh is not None and dh.shape != (b, s, d):
         raise ValueError(f"gated_scan_backward: dh must be [{b}, {s}, {d}]")
-    if dlast is not None and tuple(dlast.shape) != (b, d):
+    if dlast is not None and dlast.shape != (b, d):
         raise ValueError(f"gated_scan_backward: dlast must be [{b}, {d}]")
+    _same_device(x, ((saved, "saved"), (dh, "dh"), (dlast, "dlast")), "gated_scan_backward")
     with _lib.on_device(x):
-        x, xb, xs = _scan_rows(x, "x")
-        gate, gb, gs = _scan_rows(gate, "gate")
+        x, xb, xs = _scan_rows(x)
+        gate, gb, gs = _scan_rows(gate)
         dev = x.device
-        dh = dh.to(x.dtype).contiguous() if dh is not None else None
-        dlast = dlast.to(_f32).contiguous() if dlast is not None else None
+        dh = _as(dh, x.dtype) if dh is not None else None
+        dlast = _as(dlast, _f32) if dlast is not None else None
         dx = torch.empty((b, s, d), dtype=x.dtype, device=dev)
         dgate = torch.empty((b, s, d), dtype=x.dtype, device=dev)
         dh0 = torch.empty((b, d), dtype=_f32, device=dev) if need_h0 else None
         ws = _scan_workspace(b, s, d, dev)
         check(lib().tt_gated_scan_bwd(
-            _ptr(x), _ptr(gate), _lib.DTYPES[x.dtype], b, s, d, xb, xs, gb, gs, _ptr(weights),
-            weights.stride(0) if weights is not None else 0, _ptr(saved), _ptr(dh), _ptr(dlast),
-            _ptr(dx), _ptr(dgate), _ptr(dh0), _ptr(ws), ws.numel() if ws is not None else 0,
-            stream_ptr()), "tt_gated_scan_bwd")
+            x.data_ptr(), gate.data_ptr(), dt, b, s, d, xb, xs, gb, gs, _addr(weights), wsb,
+            saved.data_ptr(), _addr(dh), _addr(dlast), dx.data_ptr(), dgate.data_ptr(),
+            _addr(dh0), _addr(ws), ws.numel() if ws is not None else 0, stream_ptr()),
+            "tt_gated_scan_bwd")
     return dx, dgate, dh0
 
 
@@ -721,16 +753,20 @@ def catalog_rows(t: torch.Tensor) -> torch.Tensor:
     pad = (-t.shape[1]) % 64
     if pad:
         return torch.nn.functional.pad(t, (0, pad))
-    sz = t.element_size()
-    if t.stride(1) != 1 or t.stride(0) < t.shape[1] or t.stride(0) * sz % 16 or t.data_ptr() % 16:
+    st = t.stride()
+    if (st[1] != 1 or st[0] < t.shape[1] or st[0] * t.element_size() % 16
+            or t.data_ptr() % 16):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _catalog_args(x, w, ids, bias):
-    require_device(x, "queries")
-    require_device(w, "items")
-    if x.dtype not in _lib.DTYPES or w.dtype != x.dtype:
+def catalog_check(x, w, ids, bias) -> int:
+    """Validates queries, items, ids and bias of the catalog log-probabilities; the dtype code."""
+    if not x.is_cuda or not w.is_cuda:
+        require_device(x, "queries")
+        require_device(w, "items")
+    dt = _lib.DTYPES.get(x.dtype)
+    if dt is None or w.dtype is not x.dtype:
         raise TypeError("catalog_logprobs: queries and items must both be float32 or bfloat16, got "
                         f"{x.dtype} and {w.dtype}")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.shape[1] < 1:
@@ -738,14 +774,30 @@ def _catalog_args(x, w, ids, bias):
                          f"{tuple(x.shape)} and {tuple(w.shape)}")
     if w.shape[0] < 1:
         raise ValueError("catalog_logprobs: no items")
-    if ids is not None and (tuple(ids.shape) != (x.shape[0],) or ids.dtype != torch.int64):
+    if ids is not None and (ids.shape != (x.shape[0],) or ids.dtype is not torch.int64):
         raise ValueError(f"catalog_logprobs: ids must be int64 [{x.shape[0]}], got {ids.dtype} "
                          f"{tuple(ids.shape)}")
-    if bias is not None and tuple(bias.shape) != (w.shape[0],):
+    if bias is not None and bias.shape != (w.shape[0],):
         raise ValueError(f"catalog_logprobs: bias must be [{w.shape[0]}], got {tuple(bias.shape)}")
-    for t, name in ((w, "items"), (ids, "ids"), (bias, "bias")):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"catalog_logprobs: {name} on {t.device}, queries on {x.device}")
+    _same_device(x, ((w, "items"), (ids, "ids"), (bias, "bias")), "catalog_logprobs")
+    return dt
+
+
+@functools.lru_cache(maxsize=1024)
+def _catalog_ws_bytes(n, v, e, dt, top):
+    need = ctypes.c_int64(0)
+    check(lib().tt_catalog_logprobs_workspace_bytes(n, v, e, dt, top, ctypes.byref(need)),
+          "tt_catalog_logprobs_workspace_bytes")
+    return need.value
+
+
+@functools.lru_cache(maxsize=1024)
+def _catalog_bwd_ws_bytes(n, v, e, dt, bias, need_x, need_w):
+    need = ctypes.c_int64(0)
+    check(lib().tt_catalog_logprobs_bwd_workspace_bytes(n, v, e, dt, bias, need_x, need_w,
+                                                        ctypes.byref(need)),
+          "tt_catalog_logprobs_bwd_workspace_bytes")
+    return need.value
 
 
 def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entropy: bool = False,
@@ -753,7 +805,7 @@ def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entro
     """tt_catalog_logprobs on catalog_rows' x [N, E] and w [V, E] -> (log_prob [N] f32 or None
     without ids, entropy [N] f32 or None, lse [N] f32, top_ids [N, top] int64 and top_log_prob
     [N, top] f32 or None)."""
-    _catalog_args(x, w, ids, bias)
+    dt = catalog_check(x, w, ids, bias)
     n, e = x.shape
     v = w.shape[0]
     if not 0 <= top <= min(v, CATALOG_TOP_MAX):
@@ -761,24 +813,20 @@ def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entro
                          f"{CATALOG_TOP_MAX})")
     if not temperature > 0:
         raise ValueError(f"catalog_logprobs: temperature must be above 0, got {temperature}")
-    dt = _lib.DTYPES[x.dtype]
     with _lib.on_device(x):
         ids = ids.contiguous() if ids is not None else None
-        bias = bias.to(_f32).contiguous() if bias is not None else None
+        bias = _as(bias, _f32) if bias is not None else None
         dev = x.device
-        lp = torch.empty(n, dtype=_f32, device=dev) if ids is not None else None
-        ent = torch.empty(n, dtype=_f32, device=dev) if entropy else None
-        lse = torch.empty(n, dtype=_f32, device=dev)
+        # one allocation for the f32 results of a row
+        out = torch.empty((3, n), dtype=_f32, device=dev)
+        lp, ent, lse = out[0] if ids is not None else None, out[1] if entropy else None, out[2]
         ti = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
         tl = torch.empty((n, top), dtype=_f32, device=dev) if top else None
-        need = ctypes.c_int64(0)
-        check(lib().tt_catalog_logprobs_workspace_bytes(n, v, e, dt, top, ctypes.byref(need)),
-              "tt_catalog_logprobs_workspace_bytes")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        ws = torch.empty(_catalog_ws_bytes(n, v, e, dt, top), dtype=torch.uint8, device=dev)
         check(lib().tt_catalog_logprobs(
-            _ptr(x), x.stride(0), _ptr(w), w.stride(0), dt, n, v, e, _ptr(ids), _ptr(bias),
-            temperature, _ptr(lp), _ptr(ent), _ptr(lse), top, _ptr(ti), _ptr(tl), _ptr(ws),
-            ws.numel(), stream_ptr()), "tt_catalog_logprobs")
+            x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), dt, n, v, e, _addr(ids),
+            _addr(bias), temperature, _addr(lp), _addr(ent), lse.data_ptr(), top, _addr(ti),
+            _addr(tl), ws.data_ptr(), ws.numel(), stream_ptr()), "tt_catalog_logprobs")
     return lp, ent, lse, ti, tl
 
 
@@ -786,33 +834,31 @@ def catalog_logprobs_backward(x, w, ids, bias, temperature, lse, ent, g, ge, nee
                               need_w: bool):
     """(dx, dw) in x's type, contiguous (None where not needed), for gradients g of log_prob and ge
     of the entropy ([N] f32, either may be None)."""
-    _catalog_args(x, w, ids, bias)
+    dt = catalog_check(x, w, ids, bias)
     n, e = x.shape
     v = w.shape[0]
     for t, name in ((g, "g"), (ge, "ge"), (lse, "lse"), (ent, "entropy")):
-        if t is not None and (tuple(t.shape) != (n,) or t.dtype != _f32 or t.device != x.device):
-            raise ValueError(f"catalog_logprobs_backward: {name} must be float32 [{n}] on {x.device}")
+        if t is not None and (t.shape != (n,) or t.dtype is not _f32):
+            raise ValueError(f"catalog_logprobs_backward: {name} must be float32 [{n}]")
+    _same_device(x, ((g, "g"), (ge, "ge"), (lse, "lse"), (ent, "entropy")),
+                 "catalog_logprobs_backward")
     if lse is None or (ge is not None and ent is None) or (g is not None and ids is None):
         raise ValueError("catalog_logprobs_backward: lse, the entropy (for ge) and ids (for g) of "
                          "the forward call are needed")
-    dt = _lib.DTYPES[x.dtype]
     with _lib.on_device(x):
         dev = x.device
         if n == 0 or (g is None and ge is None):
             return (torch.zeros((n, e), dtype=x.dtype, device=dev) if need_x else None,
                     torch.zeros((v, e), dtype=x.dtype, device=dev) if need_w else None)
         ids = ids.contiguous() if ids is not None else None
-        bias = bias.to(_f32).contiguous() if bias is not None else None
-        g, ge = (t.contiguous() if t is not None else None for t in (g, ge))
+        bias = _as(bias, _f32) if bias is not None else None
+        g, ge, lse, ent = (t.contiguous() if t is not None else None for t in (g, ge, lse, ent))
         dx = torch.empty((n, e), dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty((v, e), dtype=x.dtype, device=dev) if need_w else None
-        need = ctypes.c_int64(0)
-        check(lib().tt_catalog_logprobs_bwd_workspace_bytes(
-            n, v, e, dt, int(bias is not None), int(need_x), int(need_w), ctypes.byref(need)),
-            "tt_catalog_logprobs_bwd_workspace_bytes")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        ws = torch.empty(_catalog_bwd_ws_bytes(n, v, e, dt, int(bias is not None), int(need_x),
+                                               int(need_w)), dtype=torch.uint8, device=dev)
         check(lib().tt_catalog_logprobs_bwd(
-            _ptr(x), x.stride(0), _ptr(w), w.stride(0), dt, n, v, e, _ptr(ids), _ptr(bias),
-            temperature, _ptr(lse), _ptr(ent), _ptr(g), _ptr(ge), _ptr(dx), _ptr(dw), _ptr(ws),
-            ws.numel(), stream_ptr()), "tt_catalog_logprobs_bwd")
+            x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), dt, n, v, e, _addr(ids),
+            _addr(bias), temperature, lse.data_ptr(), _addr(ent), _addr(g), _addr(ge), _addr(dx),
+            _addr(dw), ws.data_ptr(), ws.numel(), stream_ptr()), "tt_catalog_logprobs_bwd")
     return dx, dw

@@ -90,6 +90,7 @@ class _CatalogFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, ids, bias, temperature, entropy, top):
         ctx.set_materialize_grads(False)
+        kernels.catalog_check(x, w, ids, bias)
         xr, wr = kernels.catalog_rows(x), kernels.catalog_rows(w)
         lp, ent, lse, ti, tl = kernels.catalog_logprobs(xr, wr, ids, bias, temperature, entropy,
                                                         top)
@@ -133,10 +134,10 @@ def catalog_log_probs(queries: torch.Tensor, items: torch.Tensor, ids: torch.Ten
                                     or (bias is not None and bias.requires_grad)):
         return LogProbs(*_CatalogFn.apply(queries, items, ids, bias, float(temperature), entropy,
                                           top))
-    kernels._catalog_args(queries, items, ids, bias)
+    kernels.catalog_check(queries, items, ids, bias)
     lp, ent, _, ti, tl = kernels.catalog_logprobs(
-        kernels.catalog_rows(queries.detach()), kernels.catalog_rows(items.detach()), ids, bias,
-        float(temperature), entropy, top)
+        kernels.catalog_rows(queries), kernels.catalog_rows(items), ids, bias, float(temperature),
+        entropy, top)
     return LogProbs(lp, ent, ti, tl)
 
 

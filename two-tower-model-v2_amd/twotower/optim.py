@@ -8,10 +8,13 @@ captured in a HIP graph advances on every replay (with the learning rate of the 
 from __future__ import annotations
 
 import ctypes
+from itertools import chain
 from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 import torch
+from torch.optim.optimizer import _global_optimizer_post_hooks as _post_hooks
+from torch.optim.optimizer import _global_optimizer_pre_hooks as _pre_hooks
 
 from . import _lib
 from ._lib import check, lib, require_device, stream_ptr
@@ -40,6 +43,7 @@ class MultiTensorAdamW:
         for i, t in enumerate(tensors):
             self._check(t, f"parameter {i}")
         self.device = dev = tensors[0].device
+        self._dev_index = tensors[0].get_device()
         if any(t.device != dev for t in tensors):
             raise ValueError("the parameters of one table must be on one device")
         at = np.concatenate([[0], np.cumsum([_round_up(n, 64) for n in self.sizes])])
@@ -126,32 +130,32 @@ class MultiTensorAdamW:
              weight_decay: float, first: int = 0) -> None:
         """One step of tensors first .. first + len(grads) - 1 (the others stay); a gradient None
         leaves its tensor and its step count as they are."""
+        sizes, dtypes, dev = self.sizes, self.dtypes, self._dev_index
         with _lib.on_device(self._tab):
             keep = []
             ptrs = []
             for i, g in enumerate(grads, first):
-                if g is None or self.sizes[i] == 0:
+                if g is None or sizes[i] == 0:
                     ptrs.append(None)
                     continue
-                if (g.dtype is not self.dtypes[i] or g.device != self.device
-                        or g.numel() != self.sizes[i] or g.layout is not torch.strided):
+                if (g.layout is not torch.strided or g.dtype is not dtypes[i]
+                        or g.numel() != sizes[i] or g.get_device() != dev):
                     raise ValueError(f"AdamW: the gradient of parameter {i} must be a dense "
-                                     f"{self.dtypes[i]} tensor of {self.sizes[i]} elements on "
+                                     f"{dtypes[i]} tensor of {sizes[i]} elements on "
                                      f"{self.device}, got {g.dtype} {tuple(g.shape)} "
                                      f"({g.layout}) on {g.device}")
                 if not g.is_contiguous():
-                    g = g.contiguous()
+                    g = g.detach().contiguous()
                     keep.append(g)
                 ptrs.append(g.data_ptr())
             st = stream_ptr()
             for a in range(0, len(ptrs), MAX_TENSORS):
                 part = ptrs[a:a + MAX_TENSORS]
                 i0, i1 = self._item0[first + a], self._item0[first + a + len(part)]
-                arr = (ctypes.c_void_p * len(part))(*part)
                 check(lib().tt_adamw_step(
                     self._tab.data_ptr(), self._items.data_ptr() + 8 * i0, i1 - i0, first + a,
-                    arr, len(part), self.chunk, self.bits, lr, betas[0], betas[1], eps,
-                    weight_decay, st), "tt_adamw_step")
+                    (ctypes.c_void_p * len(part))(*part), len(part), self.chunk, self.bits, lr,
+                    betas[0], betas[1], eps, weight_decay, st), "tt_adamw_step")
 
     def moments(self, out=None):
         """(exp_avg, exp_avg_sq) of all tensors as f32 buffers, tensor i's at offsets[i]: the state
@@ -321,8 +325,29 @@ class AdamW(torch.optim.Optimizer):
                 for j, p in enumerate(ps):
                     self.state[p] = t.state_of(first + j, p.shape)
 
-    @torch.no_grad()
     def step(self, closure=None):
+        """One step of every parameter that has a gradient."""
+        if (_pre_hooks or _post_hooks or self._optimizer_step_pre_hooks
+                or self._optimizer_step_post_hooks):
+            return self._hooked_step(closure)
+        return self._step(closure)
+
+    # torch wraps every optimizer's step in a profiler range (some 5 us of host time, as much as the
+    # whole launch of a small set); marked as wrapped, step runs the registered hooks itself
+    step.hooked = True
+
+    def _hooked_step(self, closure):
+        args, kwargs = (self, closure), {}
+        for hook in chain(_pre_hooks.values(), self._optimizer_step_pre_hooks.values()):
+            new = hook(self, args, kwargs)
+            if new is not None:
+                args, kwargs = new
+        out = self._step(*args[1:], **kwargs)
+        for hook in chain(self._optimizer_step_post_hooks.values(), _post_hooks.values()):
+            hook(self, args, kwargs)
+        return out
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -330,13 +355,9 @@ class AdamW(torch.optim.Optimizer):
         if not self._tables:
             self._build()
         for t, spans in self._tables:
-            ptrs, moved = t.ptrs, False
-            for _, first, ps in spans:
-                for j, p in enumerate(ps):
-                    if p.data_ptr() != ptrs[first + j] or p.dtype is not t.dtypes[first + j]:
-                        moved = True
-            if moved:  # a parameter's storage was replaced
-                t.bind([p.detach() for _, _, ps in spans for p in ps])
+            ptrs = [p.data_ptr() for _, _, ps in spans for p in ps]
+            if ptrs != t.ptrs or [p.dtype for _, _, ps in spans for p in ps] != t.dtypes:
+                t.bind([p.detach() for _, _, ps in spans for p in ps])  # a storage was replaced
             for gi, first, ps in spans:
                 g = self.param_groups[gi]
                 t.step([p.grad for p in ps], g["lr"], g["betas"], g["eps"], g["weight_decay"],
