@@ -139,6 +139,15 @@ def test_forward_and_gradients_vs_f64(N, V, E, dt, bias):
         check_grad(dw, ref["dw"], ref["dw_size"], T, dt)
 
 
+@pytest.mark.parametrize("N,V,E", [
+    (300, 33000, 64), (700, 22001, 192), (2049, 8200, 512),  # 256 x 256 tiles, the last ones cut
+    (1281, 20100, 64),                                       # dw: some tiles whole, the rest split
+    (4100, 66000, 64)])                                      # and in three chunks
+@pytest.mark.parametrize("bias", [False, True])
+def test_large_tiles(N, V, E, bias):
+    test_forward_and_gradients_vs_f64(N, V, E, torch.bfloat16, bias)
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 def test_catalog_in_chunks(dt):
     """More logits than one chunk of coefficients holds (256 MB): partial sums across chunks."""

@@ -9,10 +9,11 @@
 //
 // The N x V logits never exist in memory.  Everything is done in powers of two (z = l log2 e).
 //
-// k_logits<STAT>  128 items x 128 rows tiles (64 x 64 where that leaves CUs idle) on MFMA (bf16
-//     16x16x32 or f32 16x16x4), a block walks its share of the catalog for its 128 rows.  The product is formed as w . x^T, so a lane
-//     holds 16 items of 4 rows: the running maximum m, L = sum 2^(z - m) and T = sum 2^(z - m) (z -
-//     m) of a row stay in the lane, with no exchange between lanes until the share's end.
+// k_logits<STAT>  tiles of 128 items x 128 rows (64 x 64 where that leaves CUs idle, 256 x 256 where
+//     those fill them) on MFMA (bf16 16x16x32 or f32 16x16x4); a block walks its share of the catalog
+//     for its rows.  The product is formed as w . x^T, so a lane holds a few items of 4 rows: the
+//     running maximum m, L = sum 2^(z - m) and T = sum 2^(z - m) (z - m) of a row stay in the lane,
+//     with no exchange between lanes until the share's end.
 //     Entropy = ln 2 (log2 L - T / L): relative to the maximum, nothing cancels against lse.
 // k_combine       joins the shares; the given item's own logit in 64 bits.
 // top             the STAT pass also writes the maximum of every 16 items a lane saw (N V / 16
@@ -22,8 +23,9 @@
 // k_logits<COEF>  the same product again, its epilogue writing C (x's type) for a chunk of the catalog.
 // k_product       dx += C w (C rows, w as it lies) and dw = C^T x: operands whose rows run along the
 //     sum are read from LDS transposed (ds_read_b64_tr_b16; 4-byte reads in f32), so neither C nor
-//     w nor x is ever stored transposed.  Sums are split over blocks where the output alone gives too
-//     few (f32 partial sums, added in a fixed order: the result does not depend on timing).
+//     w nor x is ever stored transposed.  What the output's tiles leave of the last round of blocks is
+//     filled by splitting their sums (f32 partial sums, added in a fixed order: the result does not
+//     depend on timing).
 //
 // Items with a bias at or below -1e30 (-inf, the type's lowest) are taken out: probability 0 and
 // gradient 0 whatever their vectors hold.  Rows whose gradients are both 0 do not reach dw.
@@ -41,7 +43,7 @@ constexpr float CT_OUT = -1.0e30f;   // z of an item that is taken out
 constexpr float CT_NONE = -2.0e30f;  // maximum of nothing
 constexpr float CT_LOG2E = 1.4426950408889634f, CT_LN2 = 0.6931471805599453f;
 constexpr int CT_TILE = 128;  // tile edge (items, rows, columns), or half of it
-constexpr int CT_TOP_MAX = 32, CT_TOP_EXTRA = 8, CT_TOP_NT = 512;
+constexpr int CT_TOP_MAX = 32, CT_TOP_EXTRA = 8;
 
 __device__ __forceinline__ void ct_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 template <int N>
@@ -54,14 +56,15 @@ __device__ __forceinline__ void ct_dma(const void* g, char* l) {
 
 // ---- operand stages, of 32 NB rows or columns (NB = 4: 128, or 2: 64; a wave's quarter of the tile
 // is 16 NB square).  Row form ("K along the row"): rows of 128 B, 16-B chunks XOR-swizzled by
-// (row >> 1) & 7.  Wave w of 4 loads pieces w, w + 4, ...: 8 rows each.
-template <typename T, int NB>
+// (row >> 1) & 7.  Wave w of NWV loads pieces w, w + NWV, ...: 8 rows each.
+template <typename T, int NB, int NWV = 4>
 struct RowStage {
-  int64_t off[NB];
+  static constexpr int PW = 4 * NB / NWV;  // 1-KB pieces a wave loads
+  int64_t off[PW];
   __device__ __forceinline__ void init(int64_t ld, int64_t row0, int64_t rows, int w, int lane) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int r = 8 * (w + 4 * j) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+    for (int j = 0; j < PW; ++j) {
+      const int r = 8 * (w + NWV * j) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
       int64_t row = row0 + r;
       row = row < rows ? row : rows - 1;  // past the end: loaded again, never used
       off[j] = row * ld + c * (16 / (int)sizeof(T));
@@ -69,7 +72,7 @@ struct RowStage {
   }
   __device__ __forceinline__ void issue(const T* p, int64_t k0, char* lds, int w) const {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) ct_dma(p + off[j] + k0, lds + 1024 * (w + 4 * j));
+    for (int j = 0; j < PW; ++j) ct_dma(p + off[j] + k0, lds + 1024 * (w + NWV * j));
   }
 };
 // fragments of NB x 16 rows from row r0: f[s][i] = 16 B at chunk 4 s + g of row r0 + 16 i + rl
@@ -84,23 +87,24 @@ __device__ __forceinline__ void row_frags(const char* lds, int r0, int lane, u32
 }
 
 // Column form ("the sum runs down the rows"): BK rows x 32 NB elements, the operand as it lies.
-template <typename T, int NB>
+template <typename T, int NB, int NWV = 4>
 struct ColStage {
+  static constexpr int PW = 4 * NB / NWV;
   static constexpr int EPC = 16 / (int)sizeof(T), CPR = 32 * NB / EPC;  // elements a chunk, chunks a row
   static constexpr int RPP = 64 / CPR;                                  // rows per 1-KB piece
   // swizzle of a row's chunks: the rows that one fragment read touches together lie in different
   // banks (bf16: 8 rows of two chunks; f32: 4 rows of four)
   static __device__ __forceinline__ int swz(int r) {
-    if constexpr (sizeof(T) == 2) return NB == 4 ? ((r & 3) | ((r >> 1) & 4)) << 1 : (((r >> 1) & 1) | ((r >> 2) & 2)) << 1;
-    else return NB == 4 ? ((r >> 2) & 3) << 2 : ((r >> 2) & 3) << 2;
+    if constexpr (sizeof(T) == 2) return NB >= 4 ? ((r & 3) | ((r >> 1) & 4)) << 1 : (((r >> 1) & 1) | ((r >> 2) & 2)) << 1;
+    else return ((r >> 2) & 3) << 2;
   }
-  int64_t off[NB];
-  int row[NB];
+  int64_t off[PW];
+  int row[PW];
   // cols: valid columns from c0 (a multiple of the chunk); past the end: loaded again, never used
   __device__ __forceinline__ void init(int64_t c0, int64_t cols, int w, int lane) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int r = RPP * (w + 4 * j) + lane / CPR, pc = lane % CPR;
+    for (int j = 0; j < PW; ++j) {
+      const int r = RPP * (w + NWV * j) + lane / CPR, pc = lane % CPR;
       int64_t c = c0 + (int64_t)(pc ^ swz(r)) * EPC;
       c = c < cols ? c : cols - EPC;
       row[j] = r;
@@ -110,16 +114,16 @@ struct ColStage {
   __device__ __forceinline__ void issue(const T* p, int64_t ld, int64_t k0, int64_t rows, char* lds,
                                         int w) const {
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
+    for (int j = 0; j < PW; ++j) {
       int64_t k = k0 + row[j];
       k = k < rows ? k : rows - 1;  // past the end: the other operand is zero there
-      ct_dma(p + k * ld + off[j], lds + 1024 * (w + 4 * j));
+      ct_dma(p + k * ld + off[j], lds + 1024 * (w + NWV * j));
     }
   }
 };
 // the same fragments as row_frags gives (16 B of the sum's index for column c0 + 16 i + rl)
-template <typename T, int NB>
-__device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32x4_t (&f)[2][NB]) {
+template <typename T, int NB, int NF = NB>
+__device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32x4_t (&f)[2][NF]) {
   const int g = lane >> 4, rl = lane & 15;
   constexpr int ROW_B = 32 * NB * (int)sizeof(T);
   if constexpr (sizeof(T) == 2) {
@@ -129,7 +133,7 @@ __device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
+      for (int i = 0; i < NF; ++i) {
         ct_u32x2 h[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -145,7 +149,7 @@ __device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+      for (int i = 0; i < NF; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int row = 16 * s + 4 * g + u;
@@ -157,15 +161,15 @@ __device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32
 
 // acc[i][j] += first[j] . second[i]: lane (g, rl) of block (i, j) holds first-index 16 j + 4 g + r,
 // second-index 16 i + rl
-template <typename T, int NB>
-__device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[2][NB], const u32x4_t (&second)[2][NB],
-                                        f32x4 (&acc)[NB][NB]) {
+template <typename T, int NJ, int NI = NJ>
+__device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[2][NJ], const u32x4_t (&second)[2][NI],
+                                        f32x4 (&acc)[NI][NJ]) {
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int j = 0; j < NB; ++j) {
+      for (int j = 0; j < NJ; ++j) {
         if constexpr (sizeof(T) == 2) {
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
               __builtin_bit_cast(ct_bf16x8, first[s][j]), __builtin_bit_cast(ct_bf16x8, second[s][i]),
@@ -204,7 +208,7 @@ struct LogitArgs {
   const float* bias;   // may be null
   float s2;            // log2(e) / temperature
   int N, V, E;
-  int n_tiles, splits, v_tiles;  // STAT: shares of the catalog; COEF: one tile a block
+  int n_tiles, splits, v_tiles;  // tiles of rows, shares of the catalog, tiles of items
   float4* part;        // STAT [splits, N] (m, L, T, -)
   float* tmax;         // STAT: [N, 4 ceil(V / 64)] or null
   const float4* rowc;  // COEF [N] (log2-domain lse, g, e, H)
@@ -214,40 +218,60 @@ struct LogitArgs {
   int v_base, v_count, Npad;  // v_count: items from v_base on (k_ring)
 };
 
+// A tile of 32 NB rows x 32 NB items: 4 waves of 16 NB x 16 NB, or (NB = 8, bf16) 8 waves of 64 rows x
+// 128 items, where a matrix instruction takes 3/8 of a fragment from LDS (NB = 4: 1/2, which keeps LDS
+// as busy as the matrix pipes).
+template <int NB>
+struct Tile {
+  static constexpr int EDGE = 32 * NB, NWV = NB == 8 ? 8 : 4, NT = 64 * NWV;
+  static constexpr int ROW_WV = NB == 8 ? 4 : 2;       // waves along the rows; 2 along the items (columns)
+  static constexpr int FI = NB == 8 ? 4 : NB, FJ = NB;  // 16-blocks of a wave: rows, items
+  static constexpr int OP_B = EDGE * 128, PER_EU = NB == 2 ? 3 : 2;
+};
+
 template <typename T, bool COEF, bool ENT, int NB>
-__global__ __launch_bounds__(256, NB == 4 ? 2 : 3) void k_logits(const LogitArgs a) {
-  constexpr int BK = 128 / (int)sizeof(T), TILE = 32 * NB, WT = 16 * NB, OP_B = TILE * 128;
-  __shared__ __attribute__((aligned(16))) char smem[4 * OP_B];
-  __shared__ float half[NB == 2 && !COEF ? TILE : 1][4];
+__global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const LogitArgs a) {
+  using TL = Tile<NB>;
+  constexpr int BK = 128 / (int)sizeof(T), FI = TL::FI, FJ = TL::FJ, HJ = FJ < 4 ? FJ : 4;
+  __shared__ __attribute__((aligned(16))) char smem[4 * TL::OP_B];
+  __shared__ float half[NB == 2 && !COEF ? TL::EDGE : 1][4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wv = w >> 1, wn = w & 1, g = lane >> 4, rl = lane & 15;
+  const int wn = w % TL::ROW_WV, wv = w / TL::ROW_WV, g = lane >> 4, rl = lane & 15;
   // blocks of one share of the catalog next to each other (one XCD's L2)
   const int lb = xcd_remap(blockIdx.x, gridDim.x);
   const int sp = lb / a.n_tiles, tn = lb % a.n_tiles;
   const int per = (a.v_tiles + a.splits - 1) / a.splits;
   const int vt0 = sp * per, vt1 = vt0 + per < a.v_tiles ? vt0 + per : a.v_tiles;
-  const int n0 = tn * TILE;
+  const int nw = 16 * FI * wn, n0 = tn * TL::EDGE + nw, v_end = a.v_base + a.v_count;
   const T* x = (const T*)a.x;
   const T* wt = (const T*)a.w;
   const int nk = a.E / BK;
 
-  RowStage<T, NB> sx, sw;
-  sx.init(a.ldx, n0, a.N, w, lane);
-  float m[NB], L[NB], TT[NB];
+  RowStage<T, NB, TL::NWV> sx, sw;
+  sx.init(a.ldx, (int64_t)tn * TL::EDGE, a.N, w, lane);
+  float m[FI], L[FI], TT[FI];
+  float4 rc[FI];
+  int id[FI];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
+  for (int i = 0; i < FI; ++i) {
     m[i] = CT_NONE;
     L[i] = TT[i] = 0.0f;
+    if constexpr (COEF) {
+      const int n = n0 + 16 * i + rl;
+      rc[i] = n < a.N ? a.rowc[n] : float4{1.0e30f, 0.f, 0.f, 0.f};
+      const int64_t q = n < a.N && a.ids ? a.ids[n] : -1;
+      id[i] = q >= 0 && q < a.V ? (int)q : -1;
+    }
   }
   // loads run one stage ahead over (tile, k) as one sequence
   int vt_i = vt0, k_i = 0, g_i = 0;
   auto issue_next = [&]() __attribute__((always_inline)) {
     if (vt_i >= vt1) return;
-    if (k_i == 0) sw.init(a.ldw, (int64_t)a.v_base + (int64_t)vt_i * TILE, a.V, w, lane);
-    char* st = smem + (g_i & 1) * 2 * OP_B;
+    if (k_i == 0) sw.init(a.ldw, (int64_t)a.v_base + (int64_t)vt_i * TL::EDGE, v_end, w, lane);
+    char* st = smem + (g_i & 1) * 2 * TL::OP_B;
     sw.issue(wt, (int64_t)k_i * BK, st, w);
-    sx.issue(x, (int64_t)k_i * BK, st + OP_B, w);
+    sx.issue(x, (int64_t)k_i * BK, st + TL::OP_B, w);
     ++g_i;
     if (++k_i == nk) {
       k_i = 0;
@@ -257,108 +281,125 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : 3) void k_logits(const LogitArgs
   issue_next();
   int gs = 0;
   for (int vt = vt0; vt < vt1; ++vt) {
-    const int v0 = a.v_base + vt * TILE + WT * wv;  // this wave's items
-    f32x4 acc[NB][NB];
+    f32x4 acc[FI][FJ];
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < FI; ++i)
 #pragma unroll
-      for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int kt = 0; kt < nk; ++kt, ++gs) {
       ct_wait_vm<0>();
       ct_barrier();  // stage gs complete; every wave is done with the slot refilled next
       issue_next();
-      const char* st = smem + (gs & 1) * 2 * OP_B;
-      u32x4_t fw[2][NB], fx[2][NB];
-      row_frags<NB>(st, WT * wv, lane, fw);
-      row_frags<NB>(st + OP_B, WT * wn, lane, fx);
-      ct_mfma<T, NB>(fw, fx, acc);
+      const char* st = smem + (gs & 1) * 2 * TL::OP_B;
+      u32x4_t fw[2][FJ], fx[2][FI];
+      row_frags<FJ>(st, 16 * FJ * wv, lane, fw);
+      row_frags<FI>(st + TL::OP_B, nw, lane, fx);
+      ct_mfma<T, FJ, FI>(fw, fx, acc);
     }
-    float tmx[NB];
-    const bool edge = v0 + WT > a.V;
-    const bool sel = a.bias || edge;
-    f32x4 b2[NB];
-    if (sel) {
+    // up to 64 of the wave's items at a time
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+    for (int h = 0; h < FJ / HJ; ++h) {
+      const int c0 = vt * TL::EDGE + 16 * FJ * wv + 64 * h, v0 = a.v_base + c0;
+      const bool edge = v0 + 16 * HJ > v_end;
+      const bool sel = a.bias || edge;
+      f32x4 b2[HJ];
+      if (sel) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int v = v0 + 16 * j + 4 * g + r;
-          const float b = v < a.V ? (a.bias ? a.bias[v] : 0.0f) : -__builtin_huge_valf();
-          b2[j][r] = b > CT_OUT || b != b ? b * CT_LOG2E : CT_NONE;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int n = n0 + WT * wn + 16 * i + rl;
-      f32x4 z[NB];
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float q = acc[i][j][r];
-          // (taken out: whatever the product is)
-          z[j][r] = sel ? (b2[j][r] == CT_NONE ? CT_OUT : fmaf(q, a.s2, b2[j][r])) : q * a.s2;
-        }
-      if constexpr (!COEF) {
-        float tm = CT_OUT;
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-          tm = fmaxf(fmaxf(fmaxf(z[j][0], z[j][1]), fmaxf(z[j][2], z[j][3])), tm);
-        if (a.tmax) {
-          if constexpr (NB == 4) {
-            if (n < a.N && v0 < a.V) a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] = tm;
-          } else {  // (the tile's 64 items lie in two waves)
-            if (wv == 1) half[WT * wn + 16 * i + rl][g] = tm;
-            tmx[i] = tm;
-          }
-        }
-        const float mn = fmaxf(m[i], tm), d = m[i] - mn;
-        const float sc = __builtin_amdgcn_exp2f(d);
-        if constexpr (ENT) TT[i] = sc * fmaf(d, L[i], TT[i]);
-        L[i] *= sc;
-        m[i] = mn;
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < HJ; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float q = z[j][r] - mn;
-            const float e = __builtin_amdgcn_exp2f(q);
-            L[i] += e;
-            if constexpr (ENT) TT[i] = fmaf(e, q, TT[i]);
+            const int v = v0 + 16 * j + 4 * g + r;
+            const float b = v < v_end ? (a.bias ? a.bias[v] : 0.0f) : -__builtin_huge_valf();
+            b2[j][r] = b > CT_OUT || b != b ? b * CT_LOG2E : CT_NONE;
           }
-      } else {
-        if (n < a.Npad) {
-          const bool in = n < a.N;
-          const float4 rc = in ? a.rowc[n] : float4{1.0e30f, 0.f, 0.f, 0.f};
-          const int64_t id = in ? a.ids ? a.ids[n] : -1 : -1;
-          const bool live = rc.x < 1.0e30f;
-          T* o = (T*)a.C + (int64_t)n * a.ldc + vt * TILE + WT * wv + 4 * g;
+      }
+      const float s2 = sel ? 1.0f : a.s2;
+      float tmx[FI];
 #pragma unroll
-          for (int j = 0; j < NB; ++j) {
-            f32x4 c;
+      for (int i = 0; i < FI; ++i) {
+        const int n = n0 + 16 * i + rl;
+        f32x4* z = acc[i] + HJ * h;
+        if (sel) {
+#pragma unroll
+          for (int j = 0; j < HJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)  // (taken out: whatever the product is)
+              z[j][r] = b2[j][r] == CT_NONE ? CT_OUT : fmaf(z[j][r], a.s2, b2[j][r]);
+        }
+        if constexpr (!COEF) {
+          float mx = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3]));
+#pragma unroll
+          for (int j = 1; j < HJ; ++j)
+            mx = fmaxf(fmaxf(fmaxf(z[j][0], z[j][1]), fmaxf(z[j][2], z[j][3])), mx);
+          const float tm = fmaxf(mx * s2, CT_OUT);
+          if (a.tmax) {
+            if constexpr (NB >= 4) {
+              if (n < a.N && v0 < v_end)
+                a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] = tm;
+            } else {  // (the tile's 64 items lie in two waves)
+              if (wv == 1) half[nw + 16 * i + rl][g] = tm;
+              tmx[i] = tm;
+            }
+          }
+          // the maximum is moved only where a logit exceeds it by 2^16
+          if (__any(tm > m[i] + 16.0f)) {
+            const float mn = fmaxf(m[i], tm), d = m[i] - mn, sc = __builtin_amdgcn_exp2f(d);
+            if constexpr (ENT) TT[i] = sc * fmaf(d, L[i], TT[i]);
+            L[i] *= sc;
+            m[i] = mn;
+          }
+#pragma unroll
+          for (int j = 0; j < HJ; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float lp = z[j][r] - rc.x;  // log2 p
-              const float p = __builtin_amdgcn_exp2f(lp);
-              const float k = ENT ? fmaf(rc.z, fmaf(lp, CT_LN2, rc.w), rc.y) : rc.y;
-              const bool hit = id == (int64_t)(v0 + 16 * j + 4 * g + r);
-              const float q = fmaf(-p, k, hit ? rc.y : 0.0f);
-              c[r] = live && !(z[j][r] == CT_OUT) ? q : 0.0f;
+              const float d = fmaf(z[j][r], s2, -m[i]);
+              const float e = __builtin_amdgcn_exp2f(d);
+              L[i] += e;
+              if constexpr (ENT) TT[i] = fmaf(e, d, TT[i]);
             }
-            ct_store4<T>(o + 16 * j, c);
+        } else {
+          const bool live = rc[i].x < 1.0e30f;
+          const bool store = n < a.Npad && c0 < a.ldc;
+          T* o = (T*)a.C + (int64_t)n * a.ldc + c0;
+          f32x4 c[HJ];
+#pragma unroll
+          for (int j = 0; j < HJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float lp = fmaf(z[j][r], s2, -rc[i].x);  // log2 p
+              const float p = __builtin_amdgcn_exp2f(lp);
+              const float k = ENT ? fmaf(rc[i].z, fmaf(lp, CT_LN2, rc[i].w), rc[i].y) : rc[i].y;
+              const float q = fmaf(-p, k, id[i] == v0 + 16 * j + 4 * g + r ? rc[i].y : 0.0f);
+              c[j][r] = live && !(sel && z[j][r] == CT_OUT) ? q : 0.0f;
+            }
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < HJ; ++j)
+              if (store) *(f32x4*)(o + 16 * j + 4 * g) = c[j];
+          } else {
+            // v_permlane16_swap pairs two 16-item blocks: 8 consecutive items a lane, 16-byte stores
+#pragma unroll
+            for (int j = 0; j < HJ; j += 2) {
+              const auto s0 = __builtin_amdgcn_permlane16_swap(ct_pack2(c[j][0], c[j][1]),
+                                                               ct_pack2(c[j + 1][0], c[j + 1][1]), false, false);
+              const auto s1 = __builtin_amdgcn_permlane16_swap(ct_pack2(c[j][2], c[j][3]),
+                                                               ct_pack2(c[j + 1][2], c[j + 1][3]), false, false);
+              if (store)
+                *(u32x4_t*)(o + 16 * j + 16 * (g & 1) + 8 * (g >> 1)) = u32x4_t{s0[0], s1[0], s0[1], s1[1]};
+            }
           }
         }
       }
-    }
-    if constexpr (!COEF && NB == 2) {
-      if (a.tmax) {
-        ct_barrier();
-        if (wv == 0) {
+      if constexpr (!COEF && NB == 2) {
+        if (a.tmax) {
+          ct_barrier();
+          if (wv == 0) {
 #pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            const int n = n0 + WT * wn + 16 * i + rl;
-            if (n < a.N) a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] =
-                             fmaxf(tmx[i], half[WT * wn + 16 * i + rl][g]);
+            for (int i = 0; i < FI; ++i) {
+              const int n = n0 + 16 * i + rl;
+              if (n < a.N) a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] =
+                               fmaxf(tmx[i], half[nw + 16 * i + rl][g]);
+            }
           }
         }
       }
@@ -368,14 +409,14 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : 3) void k_logits(const LogitArgs
     ct_barrier();  // the last stage's reads are over: its memory takes the waves' statistics
     float* red = (float*)smem;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
+    for (int i = 0; i < FI; ++i) {
 #pragma unroll
       for (int o = 16; o < 64; o <<= 1) {
         const float m2 = __shfl_xor(m[i], o, 64), L2 = __shfl_xor(L[i], o, 64), T2 = __shfl_xor(TT[i], o, 64);
         stat_join(m[i], L[i], TT[i], m2, L2, T2);
       }
       if (wv == 1 && g == 0) {
-        float* r = red + (WT * wn + 16 * i + rl) * 3;
+        float* r = red + (nw + 16 * i + rl) * 3;
         r[0] = m[i];
         r[1] = L[i];
         r[2] = TT[i];
@@ -384,10 +425,10 @@ __global__ __launch_bounds__(256, NB == 4 ? 2 : 3) void k_logits(const LogitArgs
     ct_barrier();
     if (wv == 0 && g == 0) {
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const float* r = red + (WT * wn + 16 * i + rl) * 3;
+      for (int i = 0; i < FI; ++i) {
+        const float* r = red + (nw + 16 * i + rl) * 3;
         stat_join(m[i], L[i], TT[i], r[0], r[1], r[2]);
-        const int n = n0 + WT * wn + 16 * i + rl;
+        const int n = n0 + 16 * i + rl;
         if (n < a.N) a.part[(int64_t)sp * a.N + n] = float4{m[i], L[i], TT[i], 0.0f};
       }
     }
@@ -851,8 +892,8 @@ __device__ __forceinline__ double dot16(const u32x4_t& a, const u32x4_t& b, doub
 
 // One block per row: the keep largest groups of all segments, their items scored in 64 bits (16 lanes
 // an item, 16-byte loads, 128 items in flight), the top of them by (score, lower id).
-template <typename T>
-__global__ __launch_bounds__(CT_TOP_NT) void k_top_items(const uint64_t* __restrict__ segs, int nseg, int keep,
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ segs, int nseg, int keep,
                                                    int top, const T* __restrict__ x, int64_t ldx,
                                                    const T* __restrict__ w, int64_t ldw, int E, int V,
                                                    const float* __restrict__ bias, double s,
@@ -860,7 +901,7 @@ __global__ __launch_bounds__(CT_TOP_NT) void k_top_items(const uint64_t* __restr
                                                    int64_t* __restrict__ ids_out, float* __restrict__ lp_out) {
   constexpr int GMAX = CT_TOP_MAX + CT_TOP_EXTRA;
   constexpr int PC = 16 / (int)sizeof(T);
-  constexpr int NW = CT_TOP_NT / 64, NG = CT_TOP_NT / 16;
+  constexpr int NW = NT / 64, NG = NT / 16;
   __shared__ uint64_t red[NW][64];
   __shared__ uint64_t fin[64];
   __shared__ uint32_t grp[64];
@@ -964,7 +1005,7 @@ __global__ __launch_bounds__(CT_TOP_NT) void k_top_items(const uint64_t* __restr
   __syncthreads();
   const float ls = lse[n];
   const int m = nlist;  // (in any order: ranks do not depend on it)
-  for (int i = tid; i < m; i += CT_TOP_NT) {
+  for (int i = tid; i < m; i += NT) {
     const int c = list[i];
     const double l = sc[c];
     const int v = vid[c];
@@ -1023,82 +1064,100 @@ __global__ __launch_bounds__(256) void k_items(const T* __restrict__ w, int64_t 
 struct ProductArgs {
   const void *A, *B;
   int64_t lda, ldb, a_rows, b_rows;
-  int M, cols, K, splits;
-  bool acc;
+  int M, cols, K;
+  int whole, splits;  // tiles from `whole` on have their sums split over that many blocks
+  bool all, acc;      // all: also the whole tiles go to part; acc: part is added to
   float scale;
   void* out;
   int64_t ldo;
-  float* part;
+  float* part;        // [block from the first that writes here, tile edge^2]
 };
 template <typename T, bool ACOL, int NB>
-__global__ __launch_bounds__(256, NB == 4 ? 2 : 3) void k_product(const ProductArgs a) {
-  constexpr int BK = 128 / (int)sizeof(T), TILE = 32 * NB, WT = 16 * NB, OP_B = TILE * 128;
-  __shared__ __attribute__((aligned(16))) char smem[4 * OP_B];
+__global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(const ProductArgs a) {
+  using TL = Tile<NB>;
+  constexpr int BK = 128 / (int)sizeof(T), FI = TL::FI, FJ = TL::FJ, EDGE = TL::EDGE;
+  __shared__ __attribute__((aligned(16))) char smem[4 * TL::OP_B];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = w >> 1, wc = w & 1, g = lane >> 4, rl = lane & 15;
-  const int tc = (a.cols + TILE - 1) / TILE, tm = (a.M + TILE - 1) / TILE;
-  const int lb = xcd_remap(blockIdx.x, gridDim.x);
-  const int sp = lb / (tc * tm), t = lb % (tc * tm);
-  const int m0 = t / tc * TILE, c0 = t % tc * TILE;
+  const int wm = w % TL::ROW_WV, wc = w / TL::ROW_WV, g = lane >> 4, rl = lane & 15;
+  const int tc = (a.cols + EDGE - 1) / EDGE, tiles = tc * ((a.M + EDGE - 1) / EDGE);
+  const int nk = a.K / BK;
+  int t, k0 = 0, k1 = nk, slot = -1;
+  if ((int)blockIdx.x < a.whole) {
+    t = xcd_remap(blockIdx.x, a.whole);
+    if (a.all) slot = t;
+  } else {
+    const int u = xcd_remap(blockIdx.x - a.whole, gridDim.x - a.whole), r = tiles - a.whole;
+    const int per = (nk + a.splits - 1) / a.splits;
+    t = a.whole + u % r;
+    k0 = u / r * per;
+    k1 = k0 + per < nk ? k0 + per : nk;
+    slot = u + (a.all ? a.whole : 0);
+  }
+  const int m0 = t / tc * EDGE, c0 = t % tc * EDGE;
   const T* A = (const T*)a.A;
   const T* B = (const T*)a.B;
-  const int nk = a.K / BK, per = (nk + a.splits - 1) / a.splits;
-  const int k0 = sp * per, k1 = k0 + per < nk ? k0 + per : nk;
-  RowStage<T, NB> ra;
-  ColStage<T, NB> ca, cb;
+  RowStage<T, NB, TL::NWV> ra;
+  ColStage<T, NB, TL::NWV> ca, cb;
   if constexpr (ACOL) ca.init(m0, a.lda, w, lane);  // (lda: whole tiles, all written)
   else ra.init(a.lda, m0, a.a_rows, w, lane);
   cb.init(c0, a.cols, w, lane);
   auto issue = [&](int kt) __attribute__((always_inline)) {
-    char* st = smem + (kt & 1) * 2 * OP_B;
+    char* st = smem + (kt & 1) * 2 * TL::OP_B;
     if constexpr (ACOL) ca.issue(A, a.lda, (int64_t)kt * BK, a.a_rows, st, w);
     else ra.issue(A, (int64_t)kt * BK, st, w);
-    cb.issue(B, a.ldb, (int64_t)kt * BK, a.b_rows, st + OP_B, w);
+    cb.issue(B, a.ldb, (int64_t)kt * BK, a.b_rows, st + TL::OP_B, w);
   };
-  f32x4 acc[NB][NB];
+  f32x4 acc[FI][FJ];
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int i = 0; i < FI; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (k0 < k1) issue(k0);
   for (int kt = k0; kt < k1; ++kt) {
     ct_wait_vm<0>();
     ct_barrier();
     if (kt + 1 < k1) issue(kt + 1);
-    const char* st = smem + (kt & 1) * 2 * OP_B;
-    u32x4_t fa[2][NB], fb[2][NB];
-    if constexpr (ACOL) col_frags<T, NB>(st, WT * wm, lane, fa);
-    else row_frags<NB>(st, WT * wm, lane, fa);
-    col_frags<T, NB>(st + OP_B, WT * wc, lane, fb);
-    ct_mfma<T, NB>(fb, fa, acc);
+    const char* st = smem + (kt & 1) * 2 * TL::OP_B;
+    u32x4_t fa[2][FI], fb[2][FJ];
+    if constexpr (ACOL) col_frags<T, NB, FI>(st, 16 * FI * wm, lane, fa);
+    else row_frags<FI>(st, 16 * FI * wm, lane, fa);
+    col_frags<T, NB, FJ>(st + TL::OP_B, 16 * FJ * wc, lane, fb);
+    ct_mfma<T, FJ, FI>(fb, fa, acc);
   }
+  float* part = slot >= 0 ? a.part + (int64_t)slot * (EDGE * EDGE) : nullptr;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int mm = m0 + WT * wm + 16 * i + rl;
-    if (mm >= a.M) continue;
+  for (int i = 0; i < FI; ++i) {
+    const int mr = 16 * FI * wm + 16 * i + rl;
+    if (m0 + mr >= a.M) continue;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int c = c0 + WT * wc + 16 * j + 4 * g;
-      if (c >= a.cols) continue;
-      if (a.part) {
-        f32x4* p = (f32x4*)(a.part + ((int64_t)sp * a.M + mm) * a.cols + c);
+    for (int j = 0; j < FJ; ++j) {
+      const int cr = 16 * FJ * wc + 16 * j + 4 * g;
+      if (c0 + cr >= a.cols) continue;
+      if (part) {
+        f32x4* p = (f32x4*)(part + mr * EDGE + cr);
         *p = a.acc ? *p + acc[i][j] : acc[i][j];
       } else {
-        ct_store4<T>((T*)a.out + (int64_t)mm * a.ldo + c, acc[i][j] * a.scale);
+        ct_store4<T>((T*)a.out + (int64_t)(m0 + mr) * a.ldo + c0 + cr, acc[i][j] * a.scale);
       }
     }
   }
 }
-// out = scale * (sum over the splits, in order)
+// out = scale * (sum over a tile's blocks, in order); edge^2 / 1024 blocks for each tile in part
 template <typename T>
-__global__ __launch_bounds__(256) void k_product_sum(const float* __restrict__ part, int splits, int64_t n4,
-                                                     float scale, T* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
-    f32x4 s = ((const f32x4*)part)[i];
-    for (int k = 1; k < splits; ++k) s = s + ((const f32x4*)part)[(int64_t)k * n4 + i];
-    ct_store4<T>(out + 4 * i, s * scale);
-  }
+__global__ __launch_bounds__(256) void k_product_sum(const ProductArgs a, int edge) {
+  const int tc = (a.cols + edge - 1) / edge, tiles = tc * ((a.M + edge - 1) / edge);
+  const int bt = edge * edge / 1024, i = blockIdx.x / bt;
+  const int t = i + (a.all ? 0 : a.whole), r = tiles - a.whole;
+  const int e = (blockIdx.x % bt * 256 + threadIdx.x) * 4;
+  const int mm = t / tc * edge + e / edge, c = t % tc * edge + e % edge;
+  if (mm >= a.M || c >= a.cols) return;
+  const int64_t sq = edge * edge;
+  const float* p = a.part + (int64_t)i * sq + e;
+  f32x4 s = *(const f32x4*)p;
+  if (t >= a.whole)
+    for (int k = 1; k < a.splits; ++k) s = s + *(const f32x4*)(p + k * r * sq);
+  ct_store4<T>((T*)a.out + (int64_t)mm * a.ldo + c, s * a.scale);
 }
 
 // ------------------------------------------------------------------------------- host side
@@ -1106,7 +1165,7 @@ static int64_t up(int64_t n, int64_t q) { return (n + q - 1) / q * q; }
 static int64_t cdiv(int64_t n, int64_t q) { return (n + q - 1) / q; }
 
 // k_ring takes these
-static bool ring_ok(int64_t N, int E, int64_t sz) { return sz == 2 && N > 128 && E % 128 == 0 && E <= 384; }
+static bool ring_ok(int64_t N, int E, int64_t sz) { return sz == 2 && N > 128 && E % 128 == 0 && E <= 384 && !getenv("NORING"); }
 static int ring_rows(int E) { return 128 * (E <= 256 ? 4 : 3); }
 template <int KS, bool COEF>
 static void ring_go(const LogitArgs& a, bool ent, hipStream_t st) {
@@ -1137,9 +1196,21 @@ static void ring_shape(int64_t N, int64_t V, int E, int& n_tiles, int& pairs, in
   splits = (int)cdiv(pairs, cdiv(pairs, s));
 }
 
-// Tile edge of k_logits: 128, or 64 where 128 would give the 256 CUs less than a block each (512 x
-// 2560 x 768 f32: 57 us with 80 blocks of 128, @F32SMALL@ us with 320 of 64).
-static int logits_edge(int64_t N, int64_t V) { return cdiv(N, 128) * cdiv(V, 128) < 256 ? 64 : 128; }
+// Tile edge of the logits' kernels: 128; 64 where 128 would give the 256 CUs less than a block each
+// (512 x 2560 x 768 f32: 57 us with 80 blocks of 128, 32 us with 320 of 64); 256 in bf16 where that
+// gives each CU one (4096 x 65537 x 768: 559 us with 128, 465 with 256).
+static int logits_edge(int64_t N, int64_t V, int64_t sz) {
+  if (sz == 2 && N > 128 && cdiv(N, 256) * cdiv(V, 256) >= 256) return 256;
+  return cdiv(N, 128) * cdiv(V, 128) < 256 ? 64 : 128;
+}
+// shares of the catalog: as many as there are block slots for
+static void logits_shape(int64_t N, int64_t V, int edge, int& n_tiles, int& v_tiles, int& splits) {
+  n_tiles = (int)cdiv(N, edge);
+  v_tiles = (int)cdiv(V, edge);
+  int64_t s = (edge == 64 ? 768 : edge == 128 ? 512 : 256) / n_tiles;
+  s = s < 1 ? 1 : s > v_tiles ? v_tiles : s;
+  splits = (int)cdiv(v_tiles, cdiv(v_tiles, s));
+}
 
 struct StatPlan {
   bool ring;
@@ -1153,12 +1224,8 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
   if (p.ring) {
     ring_shape(N, V, E, p.n_tiles, p.v_tiles, p.splits);
   } else {
-    p.edge = logits_edge(N, V);
-    p.n_tiles = (int)cdiv(N, p.edge);
-    p.v_tiles = (int)cdiv(V, p.edge);
-    int64_t s = (p.edge == 64 ? 768 : 512) / p.n_tiles;
-    s = s < 1 ? 1 : s > p.v_tiles ? p.v_tiles : s;
-    p.splits = (int)cdiv(p.v_tiles, cdiv(p.v_tiles, s));
+    p.edge = logits_edge(N, V, sz);
+    logits_shape(N, V, p.edge, p.n_tiles, p.v_tiles, p.splits);
   }
   p.bytes = up((int64_t)p.splits * N * 16, 256);
   if (top > 0) {
@@ -1176,35 +1243,56 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
 
 constexpr int64_t CT_C_BYTES = 256ll << 20;  // one chunk of C stays in the last-level cache
 struct BwdPlan {
-  int64_t Npad, Vc, n_chunks;
-  int sx, sw, ex, ew;  // splits and tile edges of the two products
-  int64_t off_row, off_x, off_w, off_c, off_px, off_pw, bytes;
+  int64_t Npad, Vc, n_chunks, off_x, off_w, off_c, off_px, off_pw, bytes;
 };
-// Tile edge and splits of a product of K / BK steps: the least of (rounds of the card's block slots)
-// x (steps a block walks, and 6 more for its start and end), with a step's worth a 0.75 M floats of
-// partial sums; the small tile where the large one leaves CUs idle.
-static void product_shape(int64_t M, int64_t cols, int64_t K, int BK, int& edge, int& splits) {
-  edge = cdiv(M, 128) * cdiv(cols, 128) < 256 ? 64 : 128;
-  const int64_t tiles = cdiv(M, edge) * cdiv(cols, edge), nk = K / BK, slots = edge == 64 ? 768 : 512;
+
+// A product's tiles: their edge, how many are summed by one block each, and over how many blocks the
+// sums of the others are split.
+struct ProductPlan {
+  int edge, whole, splits;
+  int64_t part;  // floats of partial sums (all: of whole tiles too)
+};
+// The cards' slots are filled with whole tiles first; what is left over, or all where that is less than
+// a round, is split.  Chosen: the least of (steps of 128 bytes that a slot walks, and 6 more a block for
+// its start and end) x (a step's time), and 1 us per M floats of partial sums.  Step times, us, with all
+// slots busy (bf16, measured on 4096 x 21888 x 768 and 2048 x 20096 x 384): 64 0.6, 128 1.1, 256 2.0
+// (1.07 PFLOP/s).
+static ProductPlan product_plan(int64_t M, int64_t cols, int64_t K, int64_t sz, bool all) {
+  static const int edges[3] = {64, 128, 256}, slots[3] = {768, 512, 256};
+  static const double step[3] = {0.6, 1.1, 2.0};
+  const int64_t nk = K / (128 / sz);
+  ProductPlan b{};
   double best = 0;
-  splits = 1;
-  for (int64_t s = 1; s <= 16 && (s == 1 || s * 4 <= nk); ++s) {
-    const double c = (double)cdiv(tiles * s, slots) * (double)(cdiv(nk, s) + 6) +
-                     (s > 1 ? 1.3e-6 * (double)(s * M * cols) : 0.0);
-    if (s == 1 || c < best) {
-      best = c;
-      splits = (int)s;
+  for (int i = 0; i < (sz == 2 ? 3 : 2); ++i) {
+    const int64_t tiles = cdiv(M, edges[i]) * cdiv(cols, edges[i]), sq = edges[i] * edges[i];
+    const int64_t full = tiles / slots[i], rest = tiles % slots[i];
+    for (int64_t s = 1; s <= 64 && (s == 1 || s * 4 <= nk); ++s) {
+      if (s > 1 && (rest == 0 || rest * s > 4 * slots[i])) break;
+      const int64_t ks = cdiv(nk, s), sr = cdiv(nk, ks);  // no empty split
+      const bool split = sr > 1;
+      const int64_t part = sq * ((split ? rest * sr : all ? rest : 0) + (all ? full * slots[i] : 0));
+      const double c = step[i] * (double)(full * (nk + 6) + cdiv(rest * sr, slots[i]) * (ks + 6)) +
+                       1.0e-6 * (double)part + (split && !all ? 4.0 : 0.0);
+      if (b.edge == 0 || c < best) {
+        best = c;
+        b = ProductPlan{edges[i], (int)(split ? full * slots[i] : tiles), (int)sr, part};
+      }
     }
   }
-  splits = (int)cdiv(nk, cdiv(nk, splits));  // no empty split
+  return b;
+}
+static ProductPlan plan_dx(int64_t N, int64_t E, int64_t sz, const BwdPlan& p) {
+  return product_plan(N, E, p.Vc, sz, p.n_chunks > 1);
+}
+static ProductPlan plan_dw(int64_t vn, int64_t E, int64_t sz, const BwdPlan& p) {
+  return product_plan(vn, E, p.Npad, sz, false);
 }
 static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, bool dx, bool dw) {
   BwdPlan p{};
-  const int BK = (int)(128 / sz);
   p.Npad = up(N, 64);
   int64_t vc = CT_C_BYTES / (p.Npad * sz) / CT_TILE * CT_TILE;
   vc = vc < CT_TILE ? CT_TILE : vc;
-  p.Vc = vc < up(V, CT_TILE) ? vc : up(V, CT_TILE);
+  p.Vc = up(cdiv(V, cdiv(V, vc)), CT_TILE);  // chunks of like size
   p.n_chunks = cdiv(V, p.Vc);
   int64_t o = up(N * 16, 256);
   p.off_x = o;
@@ -1213,24 +1301,48 @@ static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, 
   if (bias) o += up(V * E * sz, 256);
   p.off_c = o;
   o += up(p.Npad * p.Vc * sz, 256);
-  product_shape(N, E, p.Vc, BK, p.ex, p.sx);
-  product_shape(p.Vc, E, p.Npad, BK, p.ew, p.sw);
   p.off_px = o;
-  if (dx && (p.sx > 1 || p.n_chunks > 1)) o += up((int64_t)p.sx * N * E * 4, 256);
+  if (dx) o += plan_dx(N, E, sz, p).part * 4;
   p.off_pw = o;
-  if (dw && p.sw > 1) o += up((int64_t)p.sw * p.Vc * E * 4, 256);
+  if (dw) {
+    const int64_t a = plan_dw(p.Vc, E, sz, p).part, b = plan_dw(V - (p.n_chunks - 1) * p.Vc, E, sz, p).part;
+    o += (a > b ? a : b) * 4;
+  }
   p.bytes = o;
   return p;
 }
 template <typename T, bool ACOL>
-static void product_launch(const ProductArgs& q, int edge, hipStream_t st) {
-  const dim3 grid((unsigned)(cdiv(q.M, edge) * cdiv(q.cols, edge) * q.splits));
-  if (edge == 64) hipLaunchKernelGGL((k_product<T, ACOL, 2>), grid, dim3(256), 0, st, q);
+static void product_launch(ProductArgs& q, const ProductPlan& p, hipStream_t st) {
+  q.whole = p.whole;
+  q.splits = p.splits;
+  const int64_t tiles = cdiv(q.M, p.edge) * cdiv(q.cols, p.edge);
+  const dim3 grid((unsigned)(p.whole + (tiles - p.whole) * p.splits));
+  if constexpr (sizeof(T) == 2) {
+    if (p.edge == 256) {
+      hipLaunchKernelGGL((k_product<T, ACOL, 8>), grid, dim3(512), 0, st, q);
+      return;
+    }
+  }
+  if (p.edge == 64) hipLaunchKernelGGL((k_product<T, ACOL, 2>), grid, dim3(256), 0, st, q);
   else hipLaunchKernelGGL((k_product<T, ACOL, 4>), grid, dim3(256), 0, st, q);
+}
+template <typename T>
+static void product_sum(const ProductArgs& q, const ProductPlan& p, hipStream_t st) {
+  const int64_t tiles = cdiv(q.M, p.edge) * cdiv(q.cols, p.edge) - (q.all ? 0 : p.whole);
+  if (tiles == 0) return;
+  const dim3 grid((unsigned)(p.edge * p.edge / 1024 * tiles));
+  hipLaunchKernelGGL(k_product_sum<T>, grid, dim3(256), 0, st, q, p.edge);
 }
 template <typename T, bool COEF>
 static void logits_launch(const LogitArgs& a, int edge, bool ent, hipStream_t st) {
   const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits));
+  if constexpr (sizeof(T) == 2) {
+    if (edge == 256) {
+      if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, 8>), grid, dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((k_logits<T, COEF, false, 8>), grid, dim3(512), 0, st, a);
+      return;
+    }
+  }
   if (edge == 64) {
     if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, 2>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_logits<T, COEF, false, 2>), grid, dim3(256), 0, st, a);
@@ -1278,8 +1390,12 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     const unsigned sb = (unsigned)(N * p.nseg);
     hipLaunchKernelGGL(k_top_groups<T>, dim3(sb + cb), dim3(256), 0, st, a.tmax, p.M, p.seg_len, p.nseg,
                        p.keep, seg, sb, ca);
-    hipLaunchKernelGGL(k_top_items<T>, dim3((unsigned)N), dim3(CT_TOP_NT), 0, st, seg, p.nseg, p.keep, top,
-                       (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+    if (N <= 512)  // a block of 512 a row while rows are few: one buyer 26 -> 21 us, 2049 rows 65 -> 90 us
+      hipLaunchKernelGGL((k_top_items<T, 512>), dim3((unsigned)N), dim3(512), 0, st, seg, p.nseg, p.keep, top,
+                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+    else
+      hipLaunchKernelGGL((k_top_items<T, 256>), dim3((unsigned)N), dim3(256), 0, st, seg, p.nseg, p.keep, top,
+                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
   } else {
     hipLaunchKernelGGL(k_combine<T>, dim3(cb), dim3(256), 0, st, ca);
   }
@@ -1307,7 +1423,8 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   }
   T* C = (T*)(ws + p.off_c);
   float* px = (float*)(ws + p.off_px);
-  const bool part_x = p.sx > 1 || p.n_chunks > 1;
+  const ProductPlan px_plan = plan_dx(N, E, sizeof(T), p);
+  ProductArgs qx{};
   for (int64_t c = 0; c < p.n_chunks; ++c) {
     const int64_t vb = c * p.Vc, vn = V - vb < p.Vc ? V - vb : p.Vc;
     LogitArgs a{};
@@ -1320,41 +1437,33 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       ring_shape(N, vn, E, a.n_tiles, a.v_tiles, a.splits);
       ring_launch<true>(a, e != nullptr, st);
     } else {
-      const int edge = logits_edge(N, vn);
-      a.n_tiles = (int)cdiv(N, edge);
-      a.v_tiles = a.splits = (int)cdiv(vn, edge);
+      const int edge = logits_edge(N, vn, sizeof(T));
+      logits_shape(N, vn, edge, a.n_tiles, a.v_tiles, a.splits);
       logits_launch<T, true>(a, edge, e != nullptr, st);
     }
     const int64_t vk = up(vn, 64);
     if (dx) {
-      ProductArgs q{};
-      q.A = C; q.lda = p.Vc; q.a_rows = p.Npad;
-      q.B = wz + vb * ldwz; q.ldb = ldwz; q.b_rows = V - vb;
-      q.M = (int)N; q.cols = E; q.K = (int)vk; q.splits = p.sx;
-      q.acc = c > 0; q.scale = (float)s; q.out = dx; q.ldo = E;
-      q.part = part_x ? px : nullptr;
-      product_launch<T, false>(q, p.ex, st);
+      qx.A = C; qx.lda = p.Vc; qx.a_rows = p.Npad;
+      qx.B = wz + vb * ldwz; qx.ldb = ldwz; qx.b_rows = V - vb;
+      qx.M = (int)N; qx.cols = E; qx.K = (int)vk;
+      qx.all = p.n_chunks > 1; qx.acc = c > 0;
+      qx.scale = (float)s; qx.out = dx; qx.ldo = E;
+      qx.part = px;
+      product_launch<T, false>(qx, px_plan, st);
     }
     if (dw) {
       ProductArgs q{};
       q.A = C; q.lda = p.Vc; q.a_rows = p.Npad;
       q.B = xz; q.ldb = E; q.b_rows = N;
-      q.M = (int)vn; q.cols = E; q.K = (int)p.Npad; q.splits = p.sw;
+      q.M = (int)vn; q.cols = E; q.K = (int)p.Npad;
       q.scale = (float)s; q.out = (T*)dw + vb * E; q.ldo = E;
-      q.part = p.sw > 1 ? (float*)(ws + p.off_pw) : nullptr;
-      product_launch<T, true>(q, p.ew, st);
-      if (q.part) {
-        const int64_t n4 = vn * E / 4, nb = cdiv(n4, 256);
-        hipLaunchKernelGGL(k_product_sum<T>, dim3((unsigned)(nb < 8192 ? nb : 8192)), dim3(256), 0, st,
-                           q.part, p.sw, n4, (float)s, (T*)q.out);
-      }
+      q.part = (float*)(ws + p.off_pw);
+      const ProductPlan pw = plan_dw(vn, E, sizeof(T), p);
+      product_launch<T, true>(q, pw, st);
+      product_sum<T>(q, pw, st);
     }
   }
-  if (dx && part_x) {
-    const int64_t n4 = N * E / 4, nb = cdiv(n4, 256);
-    hipLaunchKernelGGL(k_product_sum<T>, dim3((unsigned)(nb < 8192 ? nb : 8192)), dim3(256), 0, st, px, p.sx, n4,
-                       (float)s, (T*)dx);
-  }
+  if (dx) product_sum<T>(qx, px_plan, st);
   return check_launch("tt_catalog_logprobs_bwd");
 }
 
