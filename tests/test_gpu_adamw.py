@@ -321,6 +321,32 @@ def test_captured_step_advances_on_replay(bits):
                 assert torch.equal(v, b.state[q][key])
 
 
+def test_what_a_captured_step_forbids():
+    """A replay would go on with the tables and gradients of the capture."""
+    from twotower.optim import AdamW
+
+    p, q = (torch.nn.Parameter(torch.ones(300, device="cuda")) for _ in range(2))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], **HP)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.add_param_group({"params": [q]})
+    assert len(opt.param_groups) == 1
+    old = p.data
+    p.grad = None
+    p.data = p.data.bfloat16()
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    p.data = old
+    before = p.detach().clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (p != before).all()
+
+
 def test_replaced_storage_is_followed():
     from twotower.optim import AdamW
 

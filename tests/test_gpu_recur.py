@@ -341,3 +341,17 @@ def test_buyer_tower_recurrent():
     assert not host.is_cuda and torch.equal(host, got.detach().cpu())
     other = BuyerTower(E, "recurrent")
     other.load_state_dict({k: v.cpu() for k, v in tower.state_dict().items()})
+
+
+def test_tower_states_of_other_types_and_no_buyers():
+    from twotower import BuyerTower
+
+    torch.manual_seed(0)
+    tower = BuyerTower(64, "recurrent").cuda()
+    st = torch.randn(3, 64, device="cuda").bfloat16()
+    assert torch.equal(tower.embed_state(st), tower.embed_state(st.float()))
+    x, w = torch.randn(3, 2, 64, device="cuda"), torch.ones(3, 2, device="cuda")
+    assert torch.equal(tower.recurrent_state(x, w, st), tower.recurrent_state(x, w, st.float()))
+    assert tower(x[:0], w[:0]).shape == (0, 64)
+    assert torch.equal(tower.recurrent_state(x[:, :0], w[:, :0], st), st.float())
+    assert not tower(x[:, :0], w[:, :0]).any()

@@ -111,3 +111,14 @@ def test_trained_tower_reaches_the_serving_paths():
     for bad in ((q[:, :10], None), (q, ["p1"])):
         with pytest.raises(ValueError):
             db.log_probs(*bad)
+
+
+def test_log_probs_without_queries():
+    from twotower import VectorDatabase
+
+    db = VectorDatabase(64)
+    db.build_index(np.eye(5, 64, dtype=np.float32), [f"p{i}" for i in range(5)])
+    lp, ent, alt = db.log_probs(np.zeros((0, 64), np.float32), [], top=3)
+    assert lp.shape == ent.shape == (0,) and alt == []
+    lp, ent, alt = db.log_probs(np.eye(2, 64, dtype=np.float64), ["p0", "p1"], top=9)
+    assert len(alt[0]) == 5 and abs(alt[1][0][1] - lp[1]) < 1e-5

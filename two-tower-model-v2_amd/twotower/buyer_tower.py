@@ -110,7 +110,8 @@ class BuyerTower(nn.Module):
         from .autograd_ops import NormalizeFn
 
         home = state.device
-        return NormalizeFn.apply(self._on_device(state).contiguous()).to(home)
+        state = self._on_device(state).to(torch.float32).contiguous()
+        return (NormalizeFn.apply(state) if state.shape[0] else state).to(home)
 
     def recurrent_aggregation(self, item_embeddings: torch.Tensor,
                               weights: torch.Tensor) -> torch.Tensor:

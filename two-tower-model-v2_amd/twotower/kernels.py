@@ -811,15 +811,15 @@ def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entro
     if not 0 <= top <= min(v, CATALOG_TOP_MAX):
         raise ValueError(f"catalog_logprobs: need 0 <= top ({top}) <= min({v} items, "
                          f"{CATALOG_TOP_MAX})")
-    if not temperature > 0:
+    if not temperature >= 1e-30:  # (its reciprocal is taken in f32)
         raise ValueError(f"catalog_logprobs: temperature must be above 0, got {temperature}")
     with _lib.on_device(x):
         ids = ids.contiguous() if ids is not None else None
         bias = _as(bias, _f32) if bias is not None else None
         dev = x.device
-        # one allocation for the f32 results of a row
-        out = torch.empty((3, n), dtype=_f32, device=dev)
-        lp, ent, lse = out[0] if ids is not None else None, out[1] if entropy else None, out[2]
+        lp = torch.empty(n, dtype=_f32, device=dev) if ids is not None else None
+        ent = torch.empty(n, dtype=_f32, device=dev) if entropy else None
+        lse = torch.empty(n, dtype=_f32, device=dev)
         ti = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
         tl = torch.empty((n, top), dtype=_f32, device=dev) if top else None
         ws = torch.empty(_catalog_ws_bytes(n, v, e, dt, top), dtype=torch.uint8, device=dev)

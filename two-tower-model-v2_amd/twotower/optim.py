@@ -257,7 +257,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
         self.state_bits = state_bits
         self._tables: List = []  # (MultiTensorAdamW, [(group index, first, params)])
-        self._retired: List = []
+        self._captured = False  # a HIP graph holds a step with these tables
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, group) -> None:
@@ -265,11 +265,14 @@ class AdamW(torch.optim.Optimizer):
         g = self.param_groups[-1]
         try:
             self._check_group(g)
+            if getattr(self, "_captured", False):
+                raise RuntimeError("AdamW: a step of this optimizer was captured in a HIP graph, "
+                                   "whose replays would go on with the moments of before: add "
+                                   "parameter groups first")
         except Exception:
             self.param_groups.pop()
             raise
         if getattr(self, "_tables", None):  # keep the moments, lay the tables out anew
-            self._retired.extend(self._tables)  # (a captured step still points there)
             self._tables = []
             self._build()
 
@@ -295,7 +298,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._tables, self._retired = [], []  # built for the copy's own parameters when needed
+        self._tables, self._captured = [], False  # built for the copy's own parameters when needed
 
     def _build(self) -> None:
         """Tables for the present groups, with the moments that self.state holds."""
@@ -354,9 +357,15 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if not self._tables:
             self._build()
+        if not self._captured and torch.cuda.is_current_stream_capturing():
+            self._captured = True
         for t, spans in self._tables:
             ptrs = [p.data_ptr() for _, _, ps in spans for p in ps]
-            if ptrs != t.ptrs or [p.dtype for _, _, ps in spans for p in ps] != t.dtypes:
+            dtypes = [p.dtype for _, _, ps in spans for p in ps]
+            if ptrs != t.ptrs or dtypes != t.dtypes:
+                if self._captured and dtypes != t.dtypes:
+                    raise RuntimeError("AdamW: a parameter changed its type after a step was "
+                                       "captured in a HIP graph, which reads gradients of the old")
                 t.bind([p.detach() for _, _, ps in spans for p in ps])  # a storage was replaced
             for gi, first, ps in spans:
                 g = self.param_groups[gi]

@@ -716,18 +716,22 @@ class VectorDatabase:
                              f"{q.shape[1]}")
         if product_ids is not None and len(product_ids) != len(q):
             raise ValueError(f"log_probs: {len(q)} queries, {len(product_ids)} product ids")
+        if len(q) == 0:
+            none = np.zeros(0, np.float32)
+            return none if product_ids is not None else None, none, []
         from .losses import catalog_log_probs
 
-        with _lib.on_device(self.index.xb):
-            dev = self.index.xb.device
+        with self.index._lock:  # one state of the catalog
+            xb, n = self.index.xb, self.index.ntotal
+        with _lib.on_device(xb):
+            dev = xb.device
             rows = self.normalize_queries(
                 torch.from_numpy(np.ascontiguousarray(q, dtype=np.float32)).to(dev))
             ids = None
             if product_ids is not None:
                 ids = torch.tensor([self.id_to_index.get(p, -1) for p in product_ids],
                                    dtype=torch.int64, device=dev)
-            r = catalog_log_probs(rows, self.index.xb[:self.index.ntotal], ids, temperature,
-                                  entropy=True, top=min(top, self.index.ntotal))
+            r = catalog_log_probs(rows, xb[:n], ids, temperature, entropy=True, top=min(top, n))
             lp = None
             if ids is not None:
                 lp = torch.where(ids >= 0, r.log_prob,
