@@ -394,6 +394,32 @@ def test_offsets_past_32_bits():
     assert ((dw[-70:].double() - want).abs() <= size * 3 * BF16_HALF).all()
 
 
+def test_results_changed_in_place_before_the_backward_pass():
+    from twotower.losses import catalog_log_probs
+
+    x, w, ids, _ = make(9, 200, 64, torch.float32)
+    grads = []
+    for change in (False, True):
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        r = catalog_log_probs(xl, wl, ids)
+        lp = r.log_prob
+        lp = lp.mul_(2.0) if change else lp * 2.0
+        lp.sum().backward()
+        grads.append((xl.grad, wl.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_one_tensor_as_queries_and_items():
+    from twotower.losses import catalog_log_probs
+
+    x, _, _, _ = make(70, 5, 64, torch.float32, drop=False)
+    ids = torch.arange(70, device="cuda").roll(1)
+    a, b, c = (x.clone().requires_grad_() for _ in range(3))
+    catalog_log_probs(a, a, ids).log_prob.sum().backward()
+    catalog_log_probs(b, c, ids).log_prob.sum().backward()
+    assert torch.equal(a.grad, b.grad + c.grad)
+
+
 def test_refusals_on_the_device():
     from twotower.losses import CatalogSoftmaxLoss, catalog_log_probs
 
@@ -406,6 +432,7 @@ def test_refusals_on_the_device():
                           ((x, w[:5]), dict(top=6), ValueError),
                           ((x, w), dict(top=-1), ValueError),
                           ((x, w), dict(temperature=0.0), ValueError),
+                          ((x, w), dict(temperature=1e-39), ValueError),
                           ((x, w), dict(temperature=float("nan")), ValueError),
                           ((x, w), dict(bias=b.cpu()), ValueError)):
         with pytest.raises(exc):

@@ -685,10 +685,27 @@ __device__ __forceinline__ float ct_elt(const T* p, int64_t i) {
   if constexpr (sizeof(T) == 4) return p[i];
   else return __uint_as_float((uint32_t)p[i] << 16);
 }
+// 16 bytes of x and w -> sum of products in 64 bits
+template <typename T>
+__device__ __forceinline__ double dot16(const u32x4_t& a, const u32x4_t& b, double d) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      d = fma((double)__uint_as_float(a[i]), (double)__uint_as_float(b[i]), d);
+    } else {
+      d = fma((double)__uint_as_float(a[i] << 16), (double)__uint_as_float(b[i] << 16), d);
+      d = fma((double)__uint_as_float(a[i] & 0xffff0000u), (double)__uint_as_float(b[i] & 0xffff0000u), d);
+    }
+  }
+  return d;
+}
+
+// x . w in 64 bits (E a multiple of 64, rows 16-byte aligned)
 template <typename T>
 __device__ __forceinline__ double wave_dot64(const T* x, const T* w, int E, int lane) {
+  constexpr int PC = 16 / (int)sizeof(T);
   double d = 0.0;
-  for (int e = lane; e < E; e += 64) d = fma((double)ct_elt(x, e), (double)ct_elt(w, e), d);
+  for (int e = lane * PC; e < E; e += 64 * PC) d = dot16<T>(*(const u32x4_t*)(x + e), *(const u32x4_t*)(w + e), d);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o, 64);
   return d;
@@ -717,9 +734,17 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   const double s = a.s;
   float *logp = a.logp, *ent = a.ent, *lse = a.lse;
   float m = CT_NONE, L = 0.0f, TT = 0.0f;
-  for (int i = lane; i < splits; i += 64) {
-    const float4 p = part[(int64_t)i * N + n];
-    stat_join(m, L, TT, p.x, p.y, p.z);
+  const int64_t id = logp ? ids[n] : -1;
+  const bool has = id >= 0 && id < V;
+  const float b = has && bias ? bias[id] : 0.0f;
+  const double dot = has ? wave_dot64(x + n * ldx, w + id * ldw, E, lane) : 0.0;
+  for (int i0 = lane; i0 < splits; i0 += 256) {  // 4 loads on their way
+    float4 p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      p[i] = i0 + 64 * i < splits ? part[(int64_t)(i0 + 64 * i) * N + n] : float4{CT_NONE, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) stat_join(m, L, TT, p[i].x, p[i].y, p[i].z);
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -731,13 +756,8 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   const double l2 = log2((double)L);
   const double ls = ((double)m + l2) * 0.6931471805599453;
   if (logp) {
-    const int64_t id = ids[n];
-    float o = 0.0f;
-    if (id >= 0 && id < V) {
-      const float b = bias ? bias[id] : 0.0f;
-      const double l = s * wave_dot64(x + n * ldx, w + id * ldw, E, lane) + (double)b;
-      o = empty || b <= CT_OUT ? -inf : (float)(l - ls);
-    }
+    const double l = s * dot + (double)b;
+    const float o = !has ? 0.0f : empty || b <= CT_OUT ? -inf : (float)(l - ls);
     if (lane == 0) logp[n] = o;
   }
   if (lane == 0) {
@@ -770,7 +790,7 @@ __device__ __forceinline__ int wave_select(const uint64_t (&key)[PER], int keep,
       for (int r = 0; r < PER; ++r) c += __popcll(__ballot((uint32_t)(key[r] >> 32) >= cand));
       if (c >= keep) x = cand;
     }
-    int gt = 0, eq = 0;
+  int gt = 0, eq = 0;
 #pragma unroll
     for (int r = 0; r < PER; ++r) {
       gt += __popcll(__ballot((uint32_t)(key[r] >> 32) > x));
@@ -802,16 +822,30 @@ __device__ __forceinline__ int wave_select(const uint64_t (&key)[PER], int keep,
   return base < keep ? base : keep;
 }
 
+// how many of n keys in LDS are above `mine` (n even; every lane reads the same two at a time)
+__device__ __forceinline__ int key_rank(const uint64_t* keys, int n, uint64_t mine) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  int r = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; i += 2) {
+    const u64x2 k = *(const u64x2*)(keys + i);
+    r += (k[0] > mine ? 1 : 0) + (k[1] > mine ? 1 : 0);
+  }
+  return r;
+}
+
 // Groups of 16 items (tmax entries) of one row: the keep largest of every segment, key = (maximum,
 // ~group).  The launch's last blocks join the statistics (k_combine's work, which nothing here waits
 // for: one launch less).  Block = (segment, row): each of its 4 waves keeps the best of its 1024 entries at a
-// time, with those it has, wave 0 joins the four lists.  Unused places are 0.
+// time, with those it has; of the four lists every key's rank is counted.  Unused places are 0.
 template <typename T>
 __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tmax, int64_t M, int seg_len,
                                                     int nseg, int keep, uint64_t* __restrict__ out,
                                                     unsigned n_seg_blocks, const CombineArgs ca) {
   __shared__ uint64_t red[4][64];
+  __shared__ __attribute__((aligned(16))) uint64_t all[258];
   __shared__ uint64_t fin[64];
+  __shared__ int cnt[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if (blockIdx.x >= n_seg_blocks) {
     const int64_t r = (int64_t)(blockIdx.x - n_seg_blocks) * 4 + w;
@@ -832,16 +866,26 @@ __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tm
       key[i] = e < i1 ? make_key(row[e], (uint32_t)e) : 0ull;
     }
     wave_sync();
-    // a bound first: of the lanes' largest keys the keep-th largest (high words), which at least keep
-    // keys reach; few others do, so the exact choice is then among one key a lane
-    uint64_t lm = key[0];
+    // a bound first: of the largest keys of the lanes' halves the keep-th largest (the upper 20 bits:
+    // 2^-11 of it), which at least keep keys reach; few others do
+    uint64_t l0 = key[0], l1 = key[8];
 #pragma unroll
-    for (int i = 1; i < 17; ++i) lm = key[i] > lm ? key[i] : lm;
+    for (int i = 1; i < 8; ++i) {
+      l0 = key[i] > l0 ? key[i] : l0;
+      l1 = key[8 + i] > l1 ? key[8 + i] : l1;
+    }
+    l1 = key[16] > l1 ? key[16] : l1;
+    const uint32_t h0 = (uint32_t)(l0 >> 32), h1 = (uint32_t)(l1 >> 32);
     uint32_t bound = 0u;
 #pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t cand = bound | (1u << bit);
-      if (__popcll(__ballot((uint32_t)(lm >> 32) >= cand)) >= keep) bound = cand;
+    for (int bit = 30; bit >= 12; bit -= 2) {
+      int k = 0;
+#pragma unroll
+      for (uint32_t q = 1; q < 4; ++q) {
+        const uint32_t cand = bound | (q << bit);
+        k += __popcll(__ballot(h0 >= cand)) + __popcll(__ballot(h1 >= cand)) >= keep;
+      }
+      bound |= (uint32_t)k << bit;
     }
     int c = 0;
 #pragma unroll
@@ -855,39 +899,31 @@ __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tm
     }
     wave_sync();
     if (c <= 64) {
-      const uint64_t k1[1] = {lane < c ? red[w][lane] : 0ull};
-      wave_sync();
-      have = wave_select<1>(k1, keep, red[w], lane);
+      have = c;  // (some more than keep: sorted out at the end)
     } else {  // (many equal maxima)
       have = wave_select<17>(key, keep, red[w], lane);
     }
     wave_sync();
   }
-  if (lane >= have) red[w][lane] = 0ull;
+  if (lane == 0) cnt[w] = have;
+  if (threadIdx.x < 64) fin[threadIdx.x] = 0ull;
   __syncthreads();
-  if (w == 0) {
-    uint64_t key[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) key[i] = red[i][lane];
-    const int c = wave_select<4>(key, keep, fin, lane);
-    wave_sync();
-    if (lane < keep) out[(n * nseg + sg) * keep + lane] = lane < c ? fin[lane] : 0ull;
-  }
-}
-
-// 16 bytes of x and w -> sum of products in 64 bits
-template <typename T>
-__device__ __forceinline__ double dot16(const u32x4_t& a, const u32x4_t& b, double d) {
+  int base = 0, nk = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      d = fma((double)__uint_as_float(a[i]), (double)__uint_as_float(b[i]), d);
-    } else {
-      d = fma((double)__uint_as_float(a[i] << 16), (double)__uint_as_float(b[i] << 16), d);
-      d = fma((double)__uint_as_float(a[i] & 0xffff0000u), (double)__uint_as_float(b[i] & 0xffff0000u), d);
-    }
+    base += i < w ? cnt[i] : 0;
+    nk += cnt[i];
   }
-  return d;
+  if (lane < have) all[base + lane] = red[w][lane];
+  if (threadIdx.x == 0) all[nk] = 0ull;
+  __syncthreads();
+  if ((int)threadIdx.x < nk) {
+    const uint64_t mine = all[threadIdx.x];
+    const int r = key_rank(all, (nk + 1) & ~1, mine);
+    if (r < keep) fin[r] = mine;
+  }
+  __syncthreads();
+  if (w == 0 && lane < keep) out[(n * nseg + sg) * keep + lane] = fin[lane];
 }
 
 // One block per row: the keep largest groups of all segments, their items scored in 64 bits (16 lanes
@@ -902,7 +938,7 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
   constexpr int GMAX = CT_TOP_MAX + CT_TOP_EXTRA;
   constexpr int PC = 16 / (int)sizeof(T);
   constexpr int NW = NT / 64, NG = NT / 16;
-  __shared__ uint64_t red[NW][64];
+  __shared__ __attribute__((aligned(16))) uint64_t red[NW][64];
   __shared__ uint64_t fin[64];
   __shared__ uint32_t grp[64];
   __shared__ int cnt[4];
@@ -915,43 +951,46 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
   const int64_t n = blockIdx.x;
   const int total = nseg * keep;
   const uint64_t* src = segs + n * total;
-  int have = 0;
-  for (int b = wv * 256; b < total; b += NW * 256) {
-    uint64_t key[5];
-    key[4] = lane < have ? red[wv][lane] : 0ull;
+  if (total <= NT) {
+    red[wv][lane] = tid < total ? src[tid] : 0ull;
+  } else {
+    int have = 0;
+    for (int b = wv * 256; b < total; b += NW * 256) {
+      uint64_t key[5];
+      key[4] = lane < have ? red[wv][lane] : 0ull;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) key[i] = b + i * 64 + lane < total ? src[b + i * 64 + lane] : 0ull;
-    wave_sync();
-    have = wave_select<5>(key, keep, red[wv], lane);
-    wave_sync();
+      for (int i = 0; i < 4; ++i) key[i] = b + i * 64 + lane < total ? src[b + i * 64 + lane] : 0ull;
+      wave_sync();
+      have = wave_select<5>(key, keep, red[wv], lane);
+      wave_sync();
+    }
+    if (lane >= have) red[wv][lane] = 0ull;
   }
-  if (lane >= have) red[wv][lane] = 0ull;
+  if (tid < 64) fin[tid] = 0ull;
   if (tid == 0) nlist = 0;
   __syncthreads();
+  {
+    const int used = total <= NT ? (total + 1) & ~1 : NT;
+    if (wv * 64 < used) {
+      const uint64_t mine = red[wv][lane];
+      const int r = key_rank(&red[0][0], used, mine);
+      if (mine != 0ull && r < keep) fin[r] = mine;
+    }
+  }
+  __syncthreads();
   if (wv == 0) {
-    uint64_t key[NW];
-#pragma unroll
-    for (int i = 0; i < NW; ++i) key[i] = red[i][lane];
-    const int c = wave_select<NW>(key, keep, fin, lane);
-    wave_sync();
-    const uint64_t k1[1] = {lane < c ? fin[lane] : 0ull};
+    const uint64_t k1 = lane < keep ? fin[lane] : 0ull;
     // the top-th largest maximum: the top-th largest logit is not below it, so a group or an item
     // clearly below cannot be one of the top (the margin is far above what 32-bit sums are off)
-    const int t = wave_select<1>(k1, top, red[0], lane);
-    wave_sync();
-    float kth = __builtin_huge_valf(), best = -__builtin_huge_valf();
-    if (lane < t) kth = best = key_score(red[0][lane]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      kth = fminf(kth, __shfl_xor(kth, o, 64));
-      best = fmaxf(best, __shfl_xor(best, o, 64));
-    }
+    const uint64_t last = fin[top - 1];
+    const int t = last != 0ull ? top : 0;
+    const float kth = key_score(last), best = key_score(fin[0]);
     // (fewer than top groups, or taken-out items among the top: every item takes part)
     const float floor = t < top || kth < 0.9f * CT_OUT ? -__builtin_huge_valf()
                                 : kth - 0.0009765625f * (fabsf(kth) + fabsf(best) + 1.0f);
-    const bool use = k1[0] != 0ull && !(key_score(k1[0]) < floor);
+    const bool use = k1 != 0ull && !(key_score(k1) < floor);
     const uint64_t bm = __ballot(use);
-    if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(k1[0]);
+    if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(k1);
     if (lane == 0) {
       cnt[0] = __popcll(bm);
       s_floor = floor;
@@ -1358,7 +1397,7 @@ static int ct_check(const void* x, int64_t ldx, const void* w, int64_t ldw, int3
   if (dtype != TT_DTYPE_F32 && dtype != TT_DTYPE_BF16) return bad("dtype must be f32 or bf16");
   if (N < 0 || V < 1 || E < 64 || E % 64 != 0) return bad("need N >= 0, V >= 1, E a multiple of 64");
   if (N >= (1ll << 24) || V >= (1ll << 30) || E > (1 << 20)) return bad("sizes out of range");
-  if (!(temperature > 0.0f)) return bad("temperature must be above 0");
+  if (!(temperature >= 1.0e-30f)) return bad("temperature must be above 0 (at least 1e-30)");
   if (N == 0) return TT_OK;
   if (!x || !w) return bad("null pointer");
   const int64_t sz = dtype == TT_DTYPE_F32 ? 4 : 2;
@@ -1390,7 +1429,12 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     const unsigned sb = (unsigned)(N * p.nseg);
     hipLaunchKernelGGL(k_top_groups<T>, dim3(sb + cb), dim3(256), 0, st, a.tmax, p.M, p.seg_len, p.nseg,
                        p.keep, seg, sb, ca);
-    if (N <= 512)  // a block of 512 a row while rows are few: one buyer 26 -> 21 us, 2049 rows 65 -> 90 us
+    // more threads a row while rows are few: 33 rows 24 us with 1024 (31 with 512); 2049 rows 53 us with
+    // 256 (90 with 512)
+    if (N <= 128)
+      hipLaunchKernelGGL((k_top_items<T, 1024>), dim3((unsigned)N), dim3(1024), 0, st, seg, p.nseg, p.keep, top,
+                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+    else if (N <= 512)
       hipLaunchKernelGGL((k_top_items<T, 512>), dim3((unsigned)N), dim3(512), 0, st, seg, p.nseg, p.keep, top,
                          (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
     else
