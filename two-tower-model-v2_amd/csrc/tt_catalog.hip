@@ -75,15 +75,15 @@ struct RowStage {
     for (int j = 0; j < PW; ++j) ct_dma(p + off[j] + k0, lds + 1024 * (w + NWV * j));
   }
 };
-// fragments of NB x 16 rows from row r0: f[s][i] = 16 B at chunk 4 s + g of row r0 + 16 i + rl
-template <int NB>
-__device__ __forceinline__ void row_frags(const char* lds, int r0, int lane, u32x4_t (&f)[2][NB]) {
+// fragments of NB x 16 rows from row r0: f[s][i] = 16 B at chunk 4 (s0 + s) + g of row r0 + 16 i + rl
+template <int NB, int NS>
+__device__ __forceinline__ void row_frags(const char* lds, int r0, int lane, u32x4_t (&f)[NS][NB], int s0 = 0) {
   const int g = lane >> 4, rl = lane & 15, sw = (rl >> 1) & 7;
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-      f[s][i] = *(const u32x4_t*)(lds + (r0 + 16 * i + rl) * 128 + 16 * ((4 * s + g) ^ sw));
+      f[s][i] = *(const u32x4_t*)(lds + (r0 + 16 * i + rl) * 128 + 16 * ((4 * (s0 + s) + g) ^ sw));
 }
 
 // Column form ("the sum runs down the rows"): BK rows x 32 NB elements, the operand as it lies.
@@ -122,8 +122,8 @@ struct ColStage {
   }
 };
 // the same fragments as row_frags gives (16 B of the sum's index for column c0 + 16 i + rl)
-template <typename T, int NB, int NF = NB>
-__device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32x4_t (&f)[2][NF]) {
+template <typename T, int NB, int NF, int NS>
+__device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32x4_t (&f)[NS][NF], int s0 = 0) {
   const int g = lane >> 4, rl = lane & 15;
   constexpr int ROW_B = 32 * NB * (int)sizeof(T);
   if constexpr (sizeof(T) == 2) {
@@ -131,13 +131,13 @@ __device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32
     // receives column (its index)'s 4 rows
     const int q = rl >> 2, c = rl & 3;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int i = 0; i < NF; ++i) {
         ct_u32x2 h[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int row = 32 * s + 8 * g + 4 * u + q;
+          const int row = 32 * (s0 + s) + 8 * g + 4 * u + q;
           const int chunk = (2 * (c0 / 16 + i) + (c >> 1)) ^ ColStage<T, NB>::swz(row);
           const char* p = lds + row * ROW_B + chunk * 16 + 8 * (c & 1);
           h[u] = __builtin_bit_cast(ct_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -147,12 +147,12 @@ __device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32
       }
   } else {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int i = 0; i < NF; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int row = 16 * s + 4 * g + u;
+          const int row = 16 * (s0 + s) + 4 * g + u;
           const int chunk = (4 * (c0 / 16 + i) + (rl >> 2)) ^ ColStage<T, NB>::swz(row);
           f[s][i][u] = *(const uint32_t*)(lds + row * ROW_B + chunk * 16 + 4 * (rl & 3));
         }
@@ -161,11 +161,11 @@ __device__ __forceinline__ void col_frags(const char* lds, int c0, int lane, u32
 
 // acc[i][j] += first[j] . second[i]: lane (g, rl) of block (i, j) holds first-index 16 j + 4 g + r,
 // second-index 16 i + rl
-template <typename T, int NJ, int NI = NJ>
-__device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[2][NJ], const u32x4_t (&second)[2][NI],
+template <typename T, int NJ, int NI, int NS>
+__device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[NS][NJ], const u32x4_t (&second)[NS][NI],
                                         f32x4 (&acc)[NI][NJ]) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -228,6 +228,11 @@ struct Tile {
   static constexpr int FI = NB == 8 ? 4 : NB, FJ = NB;  // 16-blocks of a wave: rows, items
   static constexpr int OP_B = EDGE * 128, PER_EU = NB == 2 ? 3 : 2;
 };
+__device__ __forceinline__ void ct_turn() {  // a barrier that no matrix instruction moves across
+  __builtin_amdgcn_sched_barrier(0);
+  ct_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 template <typename T, bool COEF, bool ENT, int NB>
 __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const LogitArgs a) {
@@ -292,9 +297,9 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       issue_next();
       const char* st = smem + (gs & 1) * 2 * TL::OP_B;
       u32x4_t fw[2][FJ], fx[2][FI];
-      row_frags<FJ>(st, 16 * FJ * wv, lane, fw);
-      row_frags<FI>(st + TL::OP_B, nw, lane, fx);
-      ct_mfma<T, FJ, FI>(fw, fx, acc);
+      row_frags(st, 16 * FJ * wv, lane, fw);
+      row_frags(st + TL::OP_B, nw, lane, fx);
+      ct_mfma<T>(fw, fx, acc);
     }
     // up to 64 of the wave's items at a time
 #pragma unroll
@@ -1115,6 +1120,10 @@ template <typename T, bool ACOL, int NB>
 __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(const ProductArgs a) {
   using TL = Tile<NB>;
   constexpr int BK = 128 / (int)sizeof(T), FI = TL::FI, FJ = TL::FJ, EDGE = TL::EDGE;
+  // 8 waves, two on a SIMD: one of them reads fragments while the other multiplies, half a stage at a
+  // time, a turn apart all along (4096 x 21888 x 768: dx 176 -> 150 us, dw 172 -> 146.  k_logits, whose
+  // tiles end in long vector work that both should do at once, lost by it: 465 -> 524)
+  constexpr bool TURNS = NB == 8;
   __shared__ __attribute__((aligned(16))) char smem[4 * TL::OP_B];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1152,17 +1161,48 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(cons
   for (int i = 0; i < FI; ++i)
 #pragma unroll
     for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto frags = [&](const char* st, auto& fa, auto& fb, int s) __attribute__((always_inline)) {
+    if constexpr (ACOL) col_frags<T, NB>(st, 16 * FI * wm, lane, fa, s);
+    else row_frags(st, 16 * FI * wm, lane, fa, s);
+    col_frags<T, NB>(st + TL::OP_B, 16 * FJ * wc, lane, fb, s);
+  };
+  const int late = TURNS ? w >> 2 : 0;
   if (k0 < k1) issue(k0);
-  for (int kt = k0; kt < k1; ++kt) {
+  if constexpr (TURNS) {
     ct_wait_vm<0>();
-    ct_barrier();
-    if (kt + 1 < k1) issue(kt + 1);
+    ct_turn();
+    if (late) {
+      if (k0 + 1 < k1) issue(k0 + 1);
+      ct_turn();
+    }
+  }
+  for (int kt = k0; kt < k1; ++kt) {
     const char* st = smem + (kt & 1) * 2 * TL::OP_B;
-    u32x4_t fa[2][FI], fb[2][FJ];
-    if constexpr (ACOL) col_frags<T, NB, FI>(st, 16 * FI * wm, lane, fa);
-    else row_frags<FI>(st, 16 * FI * wm, lane, fa);
-    col_frags<T, NB, FJ>(st + TL::OP_B, 16 * FJ * wc, lane, fb);
-    ct_mfma<T, FJ, FI>(fb, fa, acc);
+    if constexpr (TURNS) {
+      // (the slot's last reads ended with the last turn)
+      if (!late && kt + 1 < k1) issue(kt + 1);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4_t fa[1][FI], fb[1][FJ];
+        frags(st, fa, fb, s);
+        if (s == 1 && late) ct_wait_vm<0>();
+        ct_turn();
+        if (s == 1 && late && kt + 2 < k1) issue(kt + 2);
+        ct_mfma<T>(fb, fa, acc);
+        if (s == 1 && !late) ct_wait_vm<0>();
+        ct_turn();
+      }
+    } else {
+      ct_wait_vm<0>();
+      ct_barrier();
+      if (kt + 1 < k1) issue(kt + 1);
+      u32x4_t fa[2][FI], fb[2][FJ];
+      frags(st, fa, fb, 0);
+      ct_mfma<T>(fb, fa, acc);
+    }
+  }
+  if constexpr (TURNS) {
+    if (!late) ct_turn();
   }
   float* part = slot >= 0 ? a.part + (int64_t)slot * (EDGE * EDGE) : nullptr;
 #pragma unroll
@@ -1294,11 +1334,11 @@ struct ProductPlan {
 // The cards' slots are filled with whole tiles first; what is left over, or all where that is less than
 // a round, is split.  Chosen: the least of (steps of 128 bytes that a slot walks, and 6 more a block for
 // its start and end) x (a step's time), and 1 us per M floats of partial sums.  Step times, us, with all
-// slots busy (bf16, measured on 4096 x 21888 x 768 and 2048 x 20096 x 384): 64 0.6, 128 1.1, 256 2.0
-// (1.07 PFLOP/s).
+// slots busy (bf16, measured on 4096 x 21888 x 768 and 2048 x 20096 x 384): 64 0.6, 128 1.1, 256 1.75
+// (1.25 PFLOP/s).
 static ProductPlan product_plan(int64_t M, int64_t cols, int64_t K, int64_t sz, bool all) {
   static const int edges[3] = {64, 128, 256}, slots[3] = {768, 512, 256};
-  static const double step[3] = {0.6, 1.1, 2.0};
+  static const double step[3] = {0.6, 1.1, 1.75};
   const int64_t nk = K / (128 / sz);
   ProductPlan b{};
   double best = 0;
