@@ -87,7 +87,6 @@ def check_grad(got, want, size, T, dt):
 SHAPES = [(1, 1, 64), (1, 5, 64), (3, 64, 64), (5, 130, 128), (128, 128, 64), (129, 257, 192),
           (300, 1000, 384), (17, 70001, 64), (2, 20, 768), (64, 4099, 1024), (33, 333, 100),
           (1000, 37, 64), (40, 500, 7),
-          # more than 128 rows, E a multiple of 128: rows kept in registers
           (129, 1, 128), (300, 31, 128), (200, 33, 256), (700, 1090, 384), (385, 64, 384),
           (257, 999, 512), (130, 641, 640), (520, 2000, 768)]
 
@@ -142,7 +141,8 @@ def test_forward_and_gradients_vs_f64(N, V, E, dt, bias):
 @pytest.mark.parametrize("N,V,E", [
     (300, 33000, 64), (700, 22001, 192), (2049, 8200, 512),  # 256 x 256 tiles, the last ones cut
     (1281, 20100, 64),                                       # dw: some tiles whole, the rest split
-    (4100, 66000, 64)])                                      # and in three chunks
+    (4100, 66000, 64),                                       # and in three chunks
+    (769, 50021, 384), (1152, 29200, 384)])                  # rows kept in registers
 @pytest.mark.parametrize("bias", [False, True])
 def test_large_tiles(N, V, E, bias):
     test_forward_and_gradients_vs_f64(N, V, E, torch.bfloat16, bias)

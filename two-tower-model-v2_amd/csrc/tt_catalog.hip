@@ -219,8 +219,8 @@ struct LogitArgs {
 };
 
 // A tile of 32 NB rows x 32 NB items: 4 waves of 16 NB x 16 NB, or (NB = 8, bf16) 8 waves of 64 rows x
-// 128 items, where a matrix instruction takes 3/8 of a fragment from LDS (NB = 4: 1/2, which keeps LDS
-// as busy as the matrix pipes).
+// 128 items: half the loads per product, and 3/8 of a fragment read from LDS per matrix instruction
+// (NB = 4: 1/2).
 template <int NB>
 struct Tile {
   static constexpr int EDGE = 32 * NB, NWV = NB == 8 ? 8 : 4, NT = 64 * NWV;
@@ -440,17 +440,15 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
   }
 }
 
-// ---- bf16, E a multiple of 128 up to 384, more than 128 rows: k_ring.  The rows' vectors stay in
-// registers (QB blocks of 16 rows a wave, 8 waves: 128 QB rows a block), the catalog streams through
-// LDS in tiles of 32 items, SLOTS - 1 tiles ahead, one barrier a tile.  An item fragment read from
-// LDS feeds QB MFMAs (the 128 x 128 tile kernel reads a fragment of either side for every two: LDS
-// there is as busy as the matrix pipes), and the previous tile's exponentials run between this
-// tile's MFMAs.  The maximum is only moved when a tile exceeds it by 2^16, so the common tile
-// costs one fma, one exponential and two adds a logit.
+// ---- bf16, E = 384, many rows: k_ring.  The rows' vectors stay in registers (3 blocks of 16 rows a
+// wave, 8 waves: 384 rows a block; no longer E leaves room for that, and at a shorter one k_logits
+// re-reads less), the catalog streams through LDS in tiles of 32 items, SLOTS - 1 tiles ahead, one
+// barrier a tile, and the previous tile's exponentials run between this tile's MFMAs.  Bound by the
+// two together: 2049 x 100003 with entropy and alternatives 214 us (0.74 PFLOP/s).
 constexpr int CR_NT = 512;
 template <int KS>
 struct RingCfg {
-  static constexpr int QB = KS <= 8 ? 4 : 3;
+  static constexpr int QB = 3;
   static constexpr int TB = KS * 2048;             // bytes of a tile: 32 rows x KS x 64
   static constexpr int SLOTS = 4;
   static constexpr int PW = KS / 4;                // 1-KB pieces a wave loads of a tile
@@ -1243,13 +1241,18 @@ __global__ __launch_bounds__(256) void k_product_sum(const ProductArgs a, int ed
 static int64_t up(int64_t n, int64_t q) { return (n + q - 1) / q * q; }
 static int64_t cdiv(int64_t n, int64_t q) { return (n + q - 1) / q; }
 
-// k_ring takes these
-static bool ring_ok(int64_t N, int E, int64_t sz) { return sz == 2 && N > 128 && E % 128 == 0 && E <= 384 && !getenv("NORING"); }
-static int ring_rows(int E) { return 128 * (E <= 256 ? 4 : 3); }
-template <int KS, bool COEF>
-static void ring_go(const LogitArgs& a, bool ent, hipStream_t st) {
+// k_ring against k_logits' 256 x 256 tiles, us: 4096 x 30000 102 : 113 (coefficients 118 : 136), 1024 x
+// 100000 93 : 98 (111 : 122), 2049 x 100003 with entropy 214 : 248; not where blocks of 384 rows leave
+// more empty, nor in small problems (200 x 3000 13 : 6).  E = 256: 47 : 46, E = 128: 99 : 107 (108 : 97).
+constexpr int CR_E = 384, CR_ROWS = 384;
+static bool ring_ok(int64_t N, int64_t V, int E, int64_t sz) {
+  return sz == 2 && E == CR_E && 100 * up(N, CR_ROWS) <= 115 * up(N, 256) && N * V >= (1ll << 25);
+}
+template <bool COEF>
+static void ring_launch(const LogitArgs& a, bool ent, hipStream_t st) {
+  constexpr int KS = CR_E / 32;
+  static_assert(RingCfg<KS>::ROWS == CR_ROWS, "");
   const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits));
-  static_assert(RingCfg<KS>::ROWS == 128 * RingCfg<KS>::QB, "");
   if (a.bias) {
     if (ent) hipLaunchKernelGGL((k_ring<KS, COEF, true, true>), grid, dim3(CR_NT), 0, st, a);
     else hipLaunchKernelGGL((k_ring<KS, COEF, false, true>), grid, dim3(CR_NT), 0, st, a);
@@ -1258,17 +1261,9 @@ static void ring_go(const LogitArgs& a, bool ent, hipStream_t st) {
     else hipLaunchKernelGGL((k_ring<KS, COEF, false, false>), grid, dim3(CR_NT), 0, st, a);
   }
 }
-template <bool COEF>
-static void ring_launch(const LogitArgs& a, bool ent, hipStream_t st) {
-  switch (a.E / 32) {
-    case 4: return ring_go<4, COEF>(a, ent, st);
-    case 8: return ring_go<8, COEF>(a, ent, st);
-    default: return ring_go<12, COEF>(a, ent, st);
-  }
-}
-// rows a block takes, and shares of `pairs` (64 items each) for about one block a CU
-static void ring_shape(int64_t N, int64_t V, int E, int& n_tiles, int& pairs, int& splits) {
-  n_tiles = (int)cdiv(N, ring_rows(E));
+// shares of `pairs` (64 items each) for about one block a CU
+static void ring_shape(int64_t N, int64_t V, int& n_tiles, int& pairs, int& splits) {
+  n_tiles = (int)cdiv(N, CR_ROWS);
   pairs = (int)cdiv(V, 64);
   int64_t s = 256 / n_tiles;
   s = s < 1 ? 1 : s > pairs ? pairs : s;
@@ -1299,9 +1294,9 @@ struct StatPlan {
 // Shares: about 512 blocks (two a CU; three of the small tiles).
 static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
   StatPlan p{};
-  p.ring = ring_ok(N, E, sz);
+  p.ring = ring_ok(N, V, E, sz);
   if (p.ring) {
-    ring_shape(N, V, E, p.n_tiles, p.v_tiles, p.splits);
+    ring_shape(N, V, p.n_tiles, p.v_tiles, p.splits);
   } else {
     p.edge = logits_edge(N, V, sz);
     logits_shape(N, V, p.edge, p.n_tiles, p.v_tiles, p.splits);
@@ -1517,8 +1512,8 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     a.N = (int)N; a.V = (int)V; a.E = E;
     a.rowc = rowc; a.ids = ids; a.C = C; a.ldc = p.Vc; a.v_base = (int)vb; a.Npad = (int)p.Npad;
     a.v_count = (int)vn;
-    if (ring_ok(N, E, sizeof(T))) {
-      ring_shape(N, vn, E, a.n_tiles, a.v_tiles, a.splits);
+    if (ring_ok(N, vn, E, sizeof(T))) {
+      ring_shape(N, vn, a.n_tiles, a.v_tiles, a.splits);
       ring_launch<true>(a, e != nullptr, st);
     } else {
       const int edge = logits_edge(N, vn, sizeof(T));
