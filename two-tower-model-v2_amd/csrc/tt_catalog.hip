@@ -27,6 +27,10 @@
 //     filled by splitting their sums (f32 partial sums, added in a fixed order: the result does not
 //     depend on timing).
 //
+// Bound: small N by reading w (1 x 1M x 384 bf16: 143 - 160 us, 4.8 - 5.4 TB/s), large N by the matrix
+// pipes with the loads that feed them (4096 x 65537 x 768 bf16: statistics 470 us, 0.88 PFLOP/s;
+// coefficients 195 us and the products 152, 150 us per 21888 items, 0.71, 0.91, 0.92 PFLOP/s).
+//
 // Items with a bias at or below -1e30 (-inf, the type's lowest) are taken out: probability 0 and
 // gradient 0 whatever their vectors hold.  Rows whose gradients are both 0 do not reach dw.
 #include "tt_common.hpp"

@@ -22,6 +22,12 @@
 // first launch reduces every chunk to (product of A, state reached from 0), a second joins the
 // chunks, the third runs the chunks from their true start states.  The split pass reads x and
 // gate twice (from the 256 MB last-level cache where they fit).
+//
+// Measured: 512 histories x 100 events x 768 f32, one chunk: forward without h 91 us, backward 106
+// us (4.7 TB/s over both).  8 x 16384 x 768 bf16 with weights, split: sums 118 us, join 8, main pass
+// 130 (4.6 TB/s); backward 117, 8, 205 (4.9 TB/s).  The summing passes are bound by the gates'
+// arithmetic (exponential, reciprocal, powers of the weights), at 3.4 TB/s: walking them the other
+// way in time, so that they end on what the main pass starts with, changed nothing.
 #include "tt_common.hpp"
 
 namespace tt {
