@@ -138,6 +138,28 @@ def test_forward_and_gradients_vs_f64(N, V, E, dt, bias):
         check_grad(dw, ref["dw"], ref["dw_size"], T, dt)
 
 
+@pytest.mark.parametrize("N,V,E", [(33, 4000, 64), (500, 2500, 128), (200, 4001, 192)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_without_alternatives_vs_f64(N, V, E, bias):
+    from twotower.losses import catalog_log_probs
+
+    x, w, ids, b = make(N, V, E, torch.float32, bias=bias)
+    gen = torch.Generator().manual_seed(13)
+    g, ge = torch.randn(N, generator=gen).cuda(), torch.randn(N, generator=gen).cuda()
+    ref = reference(x, w, ids, b, 0.07, g, ge)
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    r = catalog_log_probs(xl, wl, ids, 0.07, b, entropy=True)
+    ok = torch.isfinite(ref["log_prob"])
+    assert torch.equal(torch.isfinite(r.log_prob), ok)
+    err = (r.log_prob.detach().double() - ref["log_prob"]).abs()[ok]
+    assert (err <= ref["T"] + U * ref["log_prob"].abs()[ok]).all()
+    err = (r.entropy.detach().double() - ref["entropy"]).abs()
+    assert (err <= 2 * ref["T"] * (1 + ref["range"])).all()
+    torch.autograd.backward([r.log_prob, r.entropy], [g, ge])
+    check_grad(xl.grad, ref["dx"], ref["dx_size"], ref["T"], torch.float32)
+    check_grad(wl.grad, ref["dw"], ref["dw_size"], ref["T"], torch.float32)
+
+
 @pytest.mark.parametrize("N,V,E", [
     (300, 33000, 64), (700, 22001, 192), (2049, 8200, 512),  # 256 x 256 tiles, the last ones cut
     (1281, 20100, 64),                                       # dw: some tiles whole, the rest split
@@ -418,6 +440,23 @@ def test_one_tensor_as_queries_and_items():
     catalog_log_probs(a, a, ids).log_prob.sum().backward()
     catalog_log_probs(b, c, ids).log_prob.sum().backward()
     assert torch.equal(a.grad, b.grad + c.grad)
+
+
+def test_ids_outside_the_catalog_are_rows_without_an_item():
+    from twotower.losses import CatalogSoftmaxLoss, catalog_log_probs
+
+    x, w, ids, _ = make(12, 50, 64, torch.float32, drop=False)
+    grads = []
+    for none in (-1, 50, 2 ** 62, -2 ** 62):
+        i = ids.clone()
+        i[3], i[7] = none, none
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = CatalogSoftmaxLoss(0.1, 0.2)(xl, wl, i)
+        loss.backward()
+        assert (catalog_log_probs(x, w, i).log_prob[[3, 7]] == 0).all()
+        grads.append((loss.detach(), xl.grad, wl.grad))
+    for g in grads[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(g, grads[0]))
 
 
 def test_refusals_on_the_device():

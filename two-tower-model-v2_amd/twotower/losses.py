@@ -121,7 +121,8 @@ def catalog_log_probs(queries: torch.Tensor, items: torch.Tensor, ids: torch.Ten
     """Under p(v | n) = softmax_v(queries_n . items_v / temperature + bias_v), for queries [N, E] and
     items [V, E] (both f32 or both bf16, device):
 
-    log_prob  [N] log p(ids_n | n) for ids [N] int64; 0 for an id of -1 (a row without an item)
+    log_prob  [N] log p(ids_n | n) for ids [N] int64; 0 for an id of -1 (a row without an item; so
+              is any id outside 0 .. V - 1)
     entropy   [N] (``entropy=True``)
     top_ids, top_log_probs  [N, top]: the ``top`` (<= 32) most probable items, ordered by the
               product in 64 bits, ties to the lower id
@@ -143,7 +144,8 @@ def catalog_log_probs(queries: torch.Tensor, items: torch.Tensor, ids: torch.Ten
 
 class CatalogSoftmaxLoss(nn.Module):
     """Mean over the rows of -log p(id | buyer) over all items: InfoNCELoss's task with the whole
-    catalog (or any set of items) as the negatives.  Rows with id -1 do not count."""
+    catalog (or any set of items) as the negatives.  Rows with id -1 (or any outside the catalog) do
+    not count."""
 
     def __init__(self, temperature: float = 0.07, entropy_weight: float = 0.0):
         super().__init__()
@@ -158,9 +160,10 @@ class CatalogSoftmaxLoss(nn.Module):
         also rewards the mean entropy (a penalty on overconfidence)."""
         r = catalog_log_probs(buyer_embeddings, item_embeddings, ids, self.temperature, bias,
                               entropy=self.entropy_weight != 0)
-        n = (ids >= 0).sum().clamp(min=1)
+        has = (ids >= 0) & (ids < item_embeddings.shape[0])
+        n = has.sum().clamp(min=1)
         loss = -r.log_prob.sum() / n
         if self.entropy_weight != 0:
             loss = loss - self.entropy_weight * torch.where(
-                ids >= 0, r.entropy, torch.zeros_like(r.entropy)).sum() / n
+                has, r.entropy, torch.zeros_like(r.entropy)).sum() / n
         return loss
