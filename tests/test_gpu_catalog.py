@@ -138,6 +138,31 @@ def test_forward_and_gradients_vs_f64(N, V, E, dt, bias):
         check_grad(dw, ref["dw"], ref["dw_size"], T, dt)
 
 
+@pytest.mark.parametrize("dt,N,V,E", [
+    (torch.float32, 5, 200, 768), (torch.float32, 200, 1003, 64), (torch.bfloat16, 5, 205, 768),
+    (torch.bfloat16, 130, 1000, 192), (torch.bfloat16, 700, 22001, 64),
+    (torch.bfloat16, 769, 50021, 384)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_log_prob_of_likely_items_keeps_its_precision(dt, N, V, E, bias):
+    """log p = -log(1 + r), r the other items' share: its own logit's error does not enter (it is the
+    same on both sides), the others' only with their share, which leaves the roundings of the sums.
+    Of r = p_other / p: off by T r, and the sum by its roundings (V / 8 + 64 at most)."""
+    from twotower.losses import catalog_log_probs
+
+    gen = torch.Generator().manual_seed(N + V)
+    w = torch.nn.functional.normalize(torch.randn(V, E, generator=gen), dim=1)
+    ids = torch.cat([torch.tensor([V - 1, 0]), torch.randint(0, V, (N - 2,), generator=gen)])
+    x = torch.nn.functional.normalize(w[ids] + 0.6 * torch.randn(N, E, generator=gen) / E ** 0.5, dim=1)
+    x, w, ids = x.to(dt).cuda(), w.to(dt).cuda(), ids.cuda()
+    b = torch.randn(V, generator=gen).cuda() if bias else None
+    ref = reference(x, w, ids, b, 0.05)
+    r = catalog_log_probs(x, w, ids, 0.05, b, entropy=True)
+    p = torch.exp(ref["log_prob"])
+    tol = 2 * ref["T"] * (1 - p) / p + U * (min(V / 8, 4096) + 64)
+    err = (r.log_prob.double() - ref["log_prob"]).abs()
+    assert (p > 0.9).any() and (err <= tol).all(), (err / tol).max().item()
+
+
 @pytest.mark.parametrize("N,V,E", [(33, 4000, 64), (500, 2500, 128), (200, 4001, 192)])
 @pytest.mark.parametrize("bias", [False, True])
 def test_without_alternatives_vs_f64(N, V, E, bias):

@@ -15,12 +15,15 @@
 //     running maximum m, L = sum 2^(z - m) and T = sum 2^(z - m) (z - m) of a row stay in the lane,
 //     with no exchange between lanes until the share's end.
 //     Entropy = ln 2 (log2 L - T / L): relative to the maximum, nothing cancels against lse.
-// k_combine       joins the shares; the given item's own logit in 64 bits.
+// k_combine       joins the shares; the given item's own logit in 64 bits, also in the joined sums.
 // top             the STAT pass also writes the maximum of every 16 items a lane saw (N V / 16
 //     floats).  The k largest logits lie in the k groups with the largest maxima; k + 8 groups are
 //     taken (32-bit maxima may swap near-equal ones), their items scored again in 64 bits, and
 //     ordered by that, ties by the lower id.
-// k_logits<COEF>  the same product again, its epilogue writing C (x's type) for a chunk of the catalog.
+// k_logits<COEF>  the same product again, its epilogue writing C for a chunk of the catalog, in x's type:
+//     the products take it as an operand of their matrix instructions.  In bf16 a coefficient is off by
+//     up to 2^-8 of itself, which few rows do not average out (dw of 7 rows 2.8e-3 off, where the
+//     rounding of dw alone makes 1.7e-3; of 4096 rows 2.0e-3).
 // k_product       dx += C w (C rows, w as it lies) and dw = C^T x: operands whose rows run along the
 //     sum are read from LDS transposed (ds_read_b64_tr_b16; 4-byte reads in f32), so neither C nor
 //     w nor x is ever stored transposed.  What the output's tiles leave of the last round of blocks is
@@ -187,6 +190,29 @@ __device__ __forceinline__ void ct_mfma(const u32x4_t (&first)[NS][NJ], const u3
       }
 }
 
+// The same for one stage.  In f32 a stage's products are summed on their own and added as a whole: one
+// chain over all of a row's products would be off by some sqrt(E / 3) roundings of the sum (16 at E =
+// 768), this way by 3 (23 x 536 x 448: gradients 9.6e-7 -> 3.3e-7 off, 512 x 2560 x 768: 1 us a launch).
+// The bf16 instructions sum 32 products at a time already.
+template <typename T, int NJ, int NI, int NS>
+__device__ __forceinline__ void ct_stage(const u32x4_t (&first)[NS][NJ], const u32x4_t (&second)[NS][NI],
+                                         f32x4 (&acc)[NI][NJ]) {
+  if constexpr (sizeof(T) == 2) {
+    ct_mfma<T>(first, second, acc);
+  } else {
+    f32x4 part[NI][NJ];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) part[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    ct_mfma<T>(first, second, part);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = acc[i][j] + part[i][j];
+  }
+}
+
 __device__ __forceinline__ uint32_t ct_pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(ct_f32x2{a, b}, ct_bf16x2));
 }
@@ -303,7 +329,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       u32x4_t fw[2][FJ], fx[2][FI];
       row_frags(st, 16 * FJ * wv, lane, fw);
       row_frags(st + TL::OP_B, nw, lane, fx);
-      ct_mfma<T>(fw, fx, acc);
+      ct_stage<T>(fw, fx, acc);
     }
     // up to 64 of the wave's items at a time
 #pragma unroll
@@ -350,8 +376,8 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
               tmx[i] = tm;
             }
           }
-          // the maximum is moved only where a logit exceeds it by 2^16
-          if (__any(tm > m[i] + 16.0f)) {
+          // the maximum is moved only where a logit exceeds it twofold
+          if (__any(tm > m[i] + 1.0f)) {
             const float mn = fmaxf(m[i], tm), d = m[i] - mn, sc = __builtin_amdgcn_exp2f(d);
             if constexpr (ENT) TT[i] = sc * fmaf(d, L[i], TT[i]);
             L[i] *= sc;
@@ -582,7 +608,7 @@ __global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
         if (((t & 1) || t + 1 >= nt) && n < a.N)
           a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (t >> 1) * 4 + g] = tm[q];
       }
-      if (__any(zm > m[q] + 16.0f)) {
+      if (__any(zm > m[q] + 1.0f)) {
         const float mn = fmaxf(m[q], zm), d = m[q] - mn, sc = __builtin_amdgcn_exp2f(d);
         if constexpr (ENT) TT[q] = sc * fmaf(d, L[q], TT[q]);
         L[q] *= sc;
@@ -718,6 +744,40 @@ __device__ __forceinline__ double wave_dot64(const T* x, const T* w, int E, int 
   return d;
 }
 
+// x . w as k_logits and k_ring form it, to the bit: the same instructions in the same order (every
+// row and column of the block is the same)
+template <typename T>
+__device__ __forceinline__ float mfma_dot(const T* x, const T* w, int E, int lane) {
+  const int g = lane >> 4;
+  f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
+  constexpr int BK = 128 / (int)sizeof(T), PC = 16 / (int)sizeof(T);
+  for (int k0 = 0; k0 < E; k0 += 4 * BK) {  // 4 stages' loads on their way
+    u32x4_t fw[4][2][1], fx[4][2][1];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int k = (k0 + q * BK < E ? k0 + q * BK : k0) + PC * (4 * s + g);
+        fw[q][s][0] = *(const u32x4_t*)(w + k);
+        fx[q][s][0] = *(const u32x4_t*)(x + k);
+      }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (k0 + q * BK < E) ct_stage<T>(fw[q], fx[q], acc);
+  }
+  return acc[0][0][0];
+}
+// What the statistics' sums change by when one item's logit z (as they have it) is put right: dz =
+// exact - z, in powers of two, d = z - m.  log p of an item that has nearly all the probability is a
+// difference of two logits that both hold its own: they have to be the same one (4 x 50 x 768, p next to
+// 1: log p 2.9e-5 -> 1.1e-6 of itself off; 3 - 7 us of latency a call).
+__device__ __forceinline__ void put_right(double dz, double d, double& L, double& TT) {
+  if (!(fabs(dz) < 0.125) || !(d > -1000.0)) return;  // (not finite, or without weight)
+  const double e = exp2(d), q = e * expm1(dz * 0.6931471805599453);
+  TT += q * (d + dz) + e * dz;
+  L += q;
+}
+
 struct CombineArgs {
   const float4* part;
   int splits, N, V, E;
@@ -726,6 +786,8 @@ struct CombineArgs {
   const int64_t* ids;
   const float* bias;
   double s;
+  float s2;   // log2(e) s, as the statistics' kernel has it
+  int group;  // items of a wave there: a group that ends past V has its logits rounded on their own
   float *logp, *ent, *lse;
 };
 // One wave per row: the shares' statistics joined, the given item's logit.
@@ -745,6 +807,7 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   const bool has = id >= 0 && id < V;
   const float b = has && bias ? bias[id] : 0.0f;
   const double dot = has ? wave_dot64(x + n * ldx, w + id * ldw, E, lane) : 0.0;
+  const float dot32 = has ? mfma_dot(x + n * ldx, w + id * ldw, E, lane) : 0.0f;
   for (int i0 = lane; i0 < splits; i0 += 256) {  // 4 loads on their way
     float4 p[4];
 #pragma unroll
@@ -760,15 +823,21 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   }
   const float inf = __builtin_huge_valf();
   const bool empty = m <= CT_OUT && L == L;  // every item taken out (and no NaN)
-  const double l2 = log2((double)L);
-  const double ls = ((double)m + l2) * 0.6931471805599453;
+  const double ls = ((double)m + log2((double)L)) * 0.6931471805599453;
+  const double l = s * dot + (double)b;
+  double L2 = (double)L, T2 = (double)TT;
+  if (has && !(b <= CT_OUT)) {
+    const bool own = bias || ((int)id / a.group + 1) * a.group > V;
+    const double z = own ? (double)fmaf(dot32, a.s2, b * CT_LOG2E) : (double)dot32 * (double)a.s2;
+    put_right(l * 1.4426950408889634 - z, z - (double)m, L2, T2);
+  }
+  const double l2 = log2(L2);
   if (logp) {
-    const double l = s * dot + (double)b;
-    const float o = !has ? 0.0f : empty || b <= CT_OUT ? -inf : (float)(l - ls);
+    const float o = !has ? 0.0f : empty || b <= CT_OUT ? -inf : (float)(l - ((double)m + l2) * 0.6931471805599453);
     if (lane == 0) logp[n] = o;
   }
   if (lane == 0) {
-    if (ent) ent[n] = empty ? 0.0f : (float)((l2 - (double)TT / (double)L) * 0.6931471805599453);
+    if (ent) ent[n] = empty ? 0.0f : (float)((l2 - T2 / L2) * 0.6931471805599453);
     lse[n] = empty ? -inf : (float)ls;
   }
 }
@@ -1200,7 +1269,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(cons
       if (kt + 1 < k1) issue(kt + 1);
       u32x4_t fa[2][FI], fb[2][FJ];
       frags(st, fa, fb, 0);
-      ct_mfma<T>(fb, fa, acc);
+      ct_stage<T>(fb, fa, acc);
     }
   }
   if constexpr (TURNS) {
@@ -1461,7 +1530,8 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   a.v_count = (int)V;
   if (p.ring) ring_launch<false>(a, ent != nullptr, st);
   else logits_launch<T, false>(a, p.edge, ent != nullptr, st);
-  const CombineArgs ca{a.part, p.splits, (int)N, (int)V, E, x, w, ldx, ldw, ids, bias, s, logp, ent, lse};
+  const CombineArgs ca{a.part, p.splits, (int)N, (int)V, E, x, w, ldx, ldw, ids, bias, s, a.s2,
+                       p.ring || p.edge == 64 ? 32 : 64, logp, ent, lse};
   const unsigned cb = (unsigned)cdiv(N, 4);
   if (top) {
     uint64_t* seg = (uint64_t*)(ws + p.off_seg);
