@@ -163,6 +163,28 @@ def test_log_prob_of_likely_items_keeps_its_precision(dt, N, V, E, bias):
     assert (p > 0.9).any() and (err <= tol).all(), (err / tol).max().item()
 
 
+@pytest.mark.parametrize("N,V,E", [(1, 70, 64), (7, 141, 192), (33, 3001, 64), (64, 500, 128),
+                                   (50, 20000, 64), (40, 9, 100)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_few_bf16_rows_have_exact_gradients(N, V, E, bias):
+    """Up to 64 rows the coefficients are held in two bf16 parts (2^-16 of them at most is lost): only
+    the result is rounded, by half a step."""
+    from twotower.losses import catalog_log_probs
+
+    x, w, ids, b = make(N, V, E, torch.bfloat16, bias=bias, seed=3)
+    gen = torch.Generator().manual_seed(17)
+    g, ge = torch.randn(N, generator=gen).cuda(), torch.randn(N, generator=gen).cuda()
+    ref = reference(x, w, ids, b, 0.07, g, ge)
+    xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+    r = catalog_log_probs(xl, wl, ids, 0.07, b, entropy=True)
+    torch.autograd.backward([r.log_prob, r.entropy], [g, ge])
+    for got, key in ((xl.grad, "dx"), (wl.grad, "dw")):
+        tol = ref[key + "_size"] * (4 * ref["T"] + 4096 * U + 2.0 ** -16) + BF16_HALF * ref[key].abs()
+        # (the rounded value is itself off by the first part: its half step too)
+        tol = tol * (1 + BF16_HALF) + 1e-30
+        assert ((got.double() - ref[key]).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("N,V,E", [(33, 4000, 64), (500, 2500, 128), (200, 4001, 192)])
 @pytest.mark.parametrize("bias", [False, True])
 def test_without_alternatives_vs_f64(N, V, E, bias):

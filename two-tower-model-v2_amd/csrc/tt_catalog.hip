@@ -21,9 +21,10 @@
 //     taken (32-bit maxima may swap near-equal ones), their items scored again in 64 bits, and
 //     ordered by that, ties by the lower id.
 // k_logits<COEF>  the same product again, its epilogue writing C for a chunk of the catalog, in x's type:
-//     the products take it as an operand of their matrix instructions.  In bf16 a coefficient is off by
-//     up to 2^-8 of itself, which few rows do not average out (dw of 7 rows 2.8e-3 off, where the
-//     rounding of dw alone makes 1.7e-3; of 4096 rows 2.0e-3).
+//     the products take it as an operand of their matrix instructions.  In bf16 a coefficient is then off
+//     by up to 2^-8 of itself, which makes 2.0e-3 of the gradients of 4096 rows (their own rounding
+//     1.7e-3); up to 64 rows, where one coefficient may be all of a sum (2.8e-3 at 7 rows), it is kept in
+//     two parts.
 // k_product       dx += C w (C rows, w as it lies) and dw = C^T x: operands whose rows run along the
 //     sum are read from LDS transposed (ds_read_b64_tr_b16; 4-byte reads in f32), so neither C nor
 //     w nor x is ever stored transposed.  What the output's tiles leave of the last round of blocks is
@@ -245,7 +246,8 @@ struct LogitArgs {
   const int64_t* ids;  // COEF
   void* C;             // COEF [Npad, ldc]: items v_base .. of this chunk
   int64_t ldc;
-  int v_base, v_count, Npad;  // v_count: items from v_base on (k_ring)
+  int v_base, v_count, Npad;  // v_count: items from v_base on
+  bool two;            // COEF in bf16: row n + N of C takes what the rounding of row n leaves
 };
 
 // A tile of 32 NB rows x 32 NB items: 4 waves of 16 NB x 16 NB, or (NB = 8, bf16) 8 waves of 64 rows x
@@ -394,7 +396,8 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
             }
         } else {
           const bool live = rc[i].x < 1.0e30f;
-          const bool store = n < a.Npad && c0 < a.ldc;
+          const bool two = NB <= 4 && sizeof(T) == 2 && a.two;
+          const bool store = n < (two ? a.N : a.Npad) && c0 < a.ldc;
           T* o = (T*)a.C + (int64_t)n * a.ldc + c0;
           f32x4 c[HJ];
 #pragma unroll
@@ -413,14 +416,25 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
               if (store) *(f32x4*)(o + 16 * j + 4 * g) = c[j];
           } else {
             // v_permlane16_swap pairs two 16-item blocks: 8 consecutive items a lane, 16-byte stores
+            auto put = [&](T* row, bool in) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < HJ; j += 2) {
-              const auto s0 = __builtin_amdgcn_permlane16_swap(ct_pack2(c[j][0], c[j][1]),
-                                                               ct_pack2(c[j + 1][0], c[j + 1][1]), false, false);
-              const auto s1 = __builtin_amdgcn_permlane16_swap(ct_pack2(c[j][2], c[j][3]),
-                                                               ct_pack2(c[j + 1][2], c[j + 1][3]), false, false);
-              if (store)
-                *(u32x4_t*)(o + 16 * j + 16 * (g & 1) + 8 * (g >> 1)) = u32x4_t{s0[0], s1[0], s0[1], s1[1]};
+              for (int j = 0; j < HJ; j += 2) {
+                const auto s0 = __builtin_amdgcn_permlane16_swap(ct_pack2(c[j][0], c[j][1]),
+                                                                 ct_pack2(c[j + 1][0], c[j + 1][1]), false, false);
+                const auto s1 = __builtin_amdgcn_permlane16_swap(ct_pack2(c[j][2], c[j][3]),
+                                                                 ct_pack2(c[j + 1][2], c[j + 1][3]), false, false);
+                if (in)
+                  *(u32x4_t*)(row + 16 * j + 16 * (g & 1) + 8 * (g >> 1)) = u32x4_t{s0[0], s1[0], s0[1], s1[1]};
+              }
+            };
+            put(o, store);
+            if (two) {  // (rows from N on are 0: they fill C up to Npad)
+#pragma unroll
+              for (int j = 0; j < HJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  c[j][r] -= __uint_as_float(ct_pack2(c[j][r], 0.0f) << 16);
+              put(o + (int64_t)a.N * a.ldc, n + a.N < a.Npad && c0 < a.ldc);
             }
           }
         }
@@ -1140,13 +1154,14 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
 }
 
 // ------------------------------------------------------------------- backward
-// Row constants, x with its dead rows (no gradient, or nothing to choose from) set to zero.
+// Row constants, x with its dead rows (no gradient, or nothing to choose from) set to zero (two: once
+// more, for the second rows of C).
 template <typename T>
 __global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t ldx, int N, int E,
                                               const float* __restrict__ lse, const float* __restrict__ ent,
                                               const float* __restrict__ g, const float* __restrict__ e,
                                               const int64_t* __restrict__ ids, int V,
-                                              float4* __restrict__ rowc, T* __restrict__ xo) {
+                                              float4* __restrict__ rowc, T* __restrict__ xo, bool two) {
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= N) return;
@@ -1158,7 +1173,11 @@ __global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t l
                    : float4{1.0e30f, 0.f, 0.f, 0.f};
   constexpr int PC = 16 / (int)sizeof(T);
   for (int c = lane * PC; c < E; c += 64 * PC)
-    *(u32x4_t*)(xo + n * E + c) = live ? *(const u32x4_t*)(x + n * ldx + c) : u32x4_t{0, 0, 0, 0};
+  {
+    const u32x4_t v = live ? *(const u32x4_t*)(x + n * ldx + c) : u32x4_t{0, 0, 0, 0};
+    *(u32x4_t*)(xo + n * E + c) = v;
+    if (two) *(u32x4_t*)(xo + (n + N) * E + c) = v;
+  }
 }
 // w with the rows of items that are taken out set to zero (they may hold anything)
 template <typename T>
@@ -1391,6 +1410,7 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
 constexpr int64_t CT_C_BYTES = 256ll << 20;  // one chunk of C stays in the last-level cache
 struct BwdPlan {
   int64_t Npad, Vc, n_chunks, off_x, off_w, off_c, off_px, off_pw, bytes;
+  bool two;  // C in two bf16 rows a row
 };
 
 // A product's tiles: their edge, how many are summed by one block each, and over how many blocks the
@@ -1429,21 +1449,24 @@ static ProductPlan product_plan(int64_t M, int64_t cols, int64_t K, int64_t sz, 
   return b;
 }
 static ProductPlan plan_dx(int64_t N, int64_t E, int64_t sz, const BwdPlan& p) {
-  return product_plan(N, E, p.Vc, sz, p.n_chunks > 1);
+  return product_plan(N, E, p.Vc, sz, p.n_chunks > 1 || p.two);
 }
 static ProductPlan plan_dw(int64_t vn, int64_t E, int64_t sz, const BwdPlan& p) {
   return product_plan(vn, E, p.Npad, sz, false);
 }
 static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, bool dx, bool dw) {
   BwdPlan p{};
-  p.Npad = up(N, 64);
+  // few bf16 rows: coefficients in two parts, 16 bits of them (one part's rounding, 2^-8, would be as
+  // large as the result's own; the calls are bound by reading w and by their launches)
+  p.two = sz == 2 && N <= 64;
+  p.Npad = up(p.two ? 2 * N : N, 64);
   int64_t vc = CT_C_BYTES / (p.Npad * sz) / CT_TILE * CT_TILE;
   vc = vc < CT_TILE ? CT_TILE : vc;
   p.Vc = up(cdiv(V, cdiv(V, vc)), CT_TILE);  // chunks of like size
   p.n_chunks = cdiv(V, p.Vc);
   int64_t o = up(N * 16, 256);
   p.off_x = o;
-  o += up(N * E * sz, 256);
+  o += up((p.two ? 2 * N : N) * E * sz, 256);
   p.off_w = o;
   if (bias) o += up(V * E * sz, 256);
   p.off_c = o;
@@ -1564,7 +1587,7 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   float4* rowc = (float4*)ws;
   T* xz = (T*)(ws + p.off_x);
   hipLaunchKernelGGL(k_rows<T>, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, st, (const T*)x, ldx, (int)N, E, lse,
-                     ent, g, e, ids, (int)V, rowc, xz);
+                     ent, g, e, ids, (int)V, rowc, xz, p.two);
   const T* wz = (const T*)w;
   int64_t ldwz = ldw;
   if (bias) {
@@ -1586,12 +1609,13 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     a.N = (int)N; a.V = (int)V; a.E = E;
     a.rowc = rowc; a.ids = ids; a.C = C; a.ldc = p.Vc; a.v_base = (int)vb; a.Npad = (int)p.Npad;
     a.v_count = (int)vn;
+    a.two = p.two;
     if (ring_ok(N, vn, E, sizeof(T))) {
       ring_shape(N, vn, a.n_tiles, a.v_tiles, a.splits);
       ring_launch<true>(a, e != nullptr, st);
     } else {
       const int edge = logits_edge(N, vn, sizeof(T));
-      logits_shape(N, vn, edge, a.n_tiles, a.v_tiles, a.splits);
+      logits_shape(p.two ? p.Npad - N : N, vn, edge, a.n_tiles, a.v_tiles, a.splits);
       logits_launch<T, true>(a, edge, e != nullptr, st);
     }
     const int64_t vk = up(vn, 64);
@@ -1599,15 +1623,20 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       qx.A = C; qx.lda = p.Vc; qx.a_rows = p.Npad;
       qx.B = wz + vb * ldwz; qx.ldb = ldwz; qx.b_rows = V - vb;
       qx.M = (int)N; qx.cols = E; qx.K = (int)vk;
-      qx.all = p.n_chunks > 1; qx.acc = c > 0;
+      qx.all = p.n_chunks > 1 || p.two; qx.acc = c > 0;
       qx.scale = (float)s; qx.out = dx; qx.ldo = E;
       qx.part = px;
       product_launch<T, false>(qx, px_plan, st);
+      if (p.two) {
+        qx.A = C + N * p.Vc; qx.a_rows = p.Npad - N;
+        qx.acc = true;
+        product_launch<T, false>(qx, px_plan, st);
+      }
     }
     if (dw) {
       ProductArgs q{};
       q.A = C; q.lda = p.Vc; q.a_rows = p.Npad;
-      q.B = xz; q.ldb = E; q.b_rows = N;
+      q.B = xz; q.ldb = E; q.b_rows = p.two ? 2 * N : N;
       q.M = (int)vn; q.cols = E; q.K = (int)p.Npad;
       q.scale = (float)s; q.out = (T*)dw + vb * E; q.ldo = E;
       q.part = (float*)(ws + p.off_pw);
