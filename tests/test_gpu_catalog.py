@@ -164,7 +164,8 @@ def test_log_prob_of_likely_items_keeps_its_precision(dt, N, V, E, bias):
 
 
 @pytest.mark.parametrize("N,V,E", [(1, 70, 64), (7, 141, 192), (33, 3001, 64), (64, 500, 128),
-                                   (50, 20000, 64), (40, 9, 100)])
+                                   (50, 20000, 64), (40, 9, 100),
+                                   (3, 2100001, 64)])  # (the catalog in two chunks)
 @pytest.mark.parametrize("bias", [False, True])
 def test_few_bf16_rows_have_exact_gradients(N, V, E, bias):
     """Up to 64 rows the coefficients are held in two bf16 parts (2^-16 of them at most is lost): only
