@@ -1031,7 +1031,7 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
   __shared__ __attribute__((aligned(16))) uint64_t red[NW][64];
   __shared__ uint64_t fin[64];
   __shared__ uint32_t grp[64];
-  __shared__ int cnt[4];
+  __shared__ int s_groups;
   __shared__ float s_floor;
   __shared__ double sc[GMAX * 16];
   __shared__ int vid[GMAX * 16];
@@ -1082,12 +1082,12 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
     const uint64_t bm = __ballot(use);
     if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(k1);
     if (lane == 0) {
-      cnt[0] = __popcll(bm);
+      s_groups = __popcll(bm);
       s_floor = floor;
     }
   }
   __syncthreads();
-  const int ngrp = cnt[0];
+  const int ngrp = s_groups;
   const float floor = s_floor;
   const T* xr = x + n * ldx;
   const int sub = tid >> 4, l16 = tid & 15, cand = ngrp * 16;
@@ -1408,11 +1408,6 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
 }
 
 constexpr int64_t CT_C_BYTES = 256ll << 20;  // one chunk of C stays in the last-level cache
-struct BwdPlan {
-  int64_t Npad, Vc, n_chunks, off_x, off_w, off_c, off_px, off_pw, bytes;
-  bool two;  // C in two bf16 rows a row
-};
-
 // A product's tiles: their edge, how many are summed by one block each, and over how many blocks the
 // sums of the others are split.
 struct ProductPlan {
@@ -1448,12 +1443,11 @@ static ProductPlan product_plan(int64_t M, int64_t cols, int64_t K, int64_t sz, 
   }
   return b;
 }
-static ProductPlan plan_dx(int64_t N, int64_t E, int64_t sz, const BwdPlan& p) {
-  return product_plan(N, E, p.Vc, sz, p.n_chunks > 1 || p.two);
-}
-static ProductPlan plan_dw(int64_t vn, int64_t E, int64_t sz, const BwdPlan& p) {
-  return product_plan(vn, E, p.Npad, sz, false);
-}
+struct BwdPlan {
+  int64_t Npad, Vc, n_chunks, off_x, off_w, off_c, off_px, off_pw, bytes;
+  bool two;  // C in two bf16 rows a row
+  ProductPlan px, pw, pw_last;  // dx; dw of a chunk, of the last chunk
+};
 static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, bool dx, bool dw) {
   BwdPlan p{};
   // few bf16 rows: coefficients in two parts, 16 bits of them (one part's rounding, 2^-8, would be as
@@ -1472,11 +1466,16 @@ static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, 
   p.off_c = o;
   o += up(p.Npad * p.Vc * sz, 256);
   p.off_px = o;
-  if (dx) o += plan_dx(N, E, sz, p).part * 4;
+  if (dx) {
+    p.px = product_plan(N, E, p.Vc, sz, p.n_chunks > 1 || p.two);
+    o += p.px.part * 4;
+  }
   p.off_pw = o;
   if (dw) {
-    const int64_t a = plan_dw(p.Vc, E, sz, p).part, b = plan_dw(V - (p.n_chunks - 1) * p.Vc, E, sz, p).part;
-    o += (a > b ? a : b) * 4;
+    const int64_t last = V - (p.n_chunks - 1) * p.Vc;
+    p.pw_last = product_plan(last, E, p.Npad, sz, false);
+    p.pw = p.n_chunks > 1 ? product_plan(p.Vc, E, p.Npad, sz, false) : p.pw_last;
+    o += (p.pw.part > p.pw_last.part ? p.pw.part : p.pw_last.part) * 4;
   }
   p.bytes = o;
   return p;
@@ -1599,7 +1598,6 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   }
   T* C = (T*)(ws + p.off_c);
   float* px = (float*)(ws + p.off_px);
-  const ProductPlan px_plan = plan_dx(N, E, sizeof(T), p);
   ProductArgs qx{};
   for (int64_t c = 0; c < p.n_chunks; ++c) {
     const int64_t vb = c * p.Vc, vn = V - vb < p.Vc ? V - vb : p.Vc;
@@ -1626,11 +1624,11 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       qx.all = p.n_chunks > 1 || p.two; qx.acc = c > 0;
       qx.scale = (float)s; qx.out = dx; qx.ldo = E;
       qx.part = px;
-      product_launch<T, false>(qx, px_plan, st);
+      product_launch<T, false>(qx, p.px, st);
       if (p.two) {
         qx.A = C + N * p.Vc; qx.a_rows = p.Npad - N;
         qx.acc = true;
-        product_launch<T, false>(qx, px_plan, st);
+        product_launch<T, false>(qx, p.px, st);
       }
     }
     if (dw) {
@@ -1640,12 +1638,12 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       q.M = (int)vn; q.cols = E; q.K = (int)p.Npad;
       q.scale = (float)s; q.out = (T*)dw + vb * E; q.ldo = E;
       q.part = (float*)(ws + p.off_pw);
-      const ProductPlan pw = plan_dw(vn, E, sizeof(T), p);
+      const ProductPlan& pw = c + 1 < p.n_chunks ? p.pw : p.pw_last;
       product_launch<T, true>(q, pw, st);
       product_sum<T>(q, pw, st);
     }
   }
-  if (dx) product_sum<T>(qx, px_plan, st);
+  if (dx) product_sum<T>(qx, p.px, st);
   return check_launch("tt_catalog_logprobs_bwd");
 }
 

@@ -801,11 +801,11 @@ def _catalog_bwd_ws_bytes(n, v, e, dt, bias, need_x, need_w):
 
 
 def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entropy: bool = False,
-                     top: int = 0):
+                     top: int = 0, checked: int = None):
     """tt_catalog_logprobs on catalog_rows' x [N, E] and w [V, E] -> (log_prob [N] f32 or None
     without ids, entropy [N] f32 or None, lse [N] f32, top_ids [N, top] int64 and top_log_prob
-    [N, top] f32 or None)."""
-    dt = catalog_check(x, w, ids, bias)
+    [N, top] f32 or None).  ``checked``: what catalog_check said of these arguments."""
+    dt = catalog_check(x, w, ids, bias) if checked is None else checked
     n, e = x.shape
     v = w.shape[0]
     if not 0 <= top <= min(v, CATALOG_TOP_MAX):
@@ -831,10 +831,10 @@ def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entro
 
 
 def catalog_logprobs_backward(x, w, ids, bias, temperature, lse, ent, g, ge, need_x: bool,
-                              need_w: bool):
+                              need_w: bool, checked: int = None):
     """(dx, dw) in x's type, contiguous (None where not needed), for gradients g of log_prob and ge
-    of the entropy ([N] f32, either may be None)."""
-    dt = catalog_check(x, w, ids, bias)
+    of the entropy ([N] f32, either may be None).  ``checked``: see catalog_logprobs."""
+    dt = catalog_check(x, w, ids, bias) if checked is None else checked
     n, e = x.shape
     v = w.shape[0]
     for t, name in ((g, "g"), (ge, "ge"), (lse, "lse"), (ent, "entropy")):

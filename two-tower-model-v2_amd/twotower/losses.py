@@ -90,10 +90,10 @@ class _CatalogFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, ids, bias, temperature, entropy, top):
         ctx.set_materialize_grads(False)
-        kernels.catalog_check(x, w, ids, bias)
+        dt = ctx.dt = kernels.catalog_check(x, w, ids, bias)
         xr, wr = kernels.catalog_rows(x), kernels.catalog_rows(w)
         lp, ent, lse, ti, tl = kernels.catalog_logprobs(xr, wr, ids, bias, temperature, entropy,
-                                                        top)
+                                                        top, dt)
         ctx.save_for_backward(xr, wr, ids, bias, lse, ent)
         ctx.temperature, ctx.e = temperature, x.shape[1]
         if top:
@@ -109,7 +109,7 @@ class _CatalogFn(torch.autograd.Function):
         x, w, ids, bias, lse, ent = ctx.saved_tensors
         dx, dw = kernels.catalog_logprobs_backward(
             x, w, ids, bias, ctx.temperature, lse, ent, g, ge, ctx.needs_input_grad[0],
-            ctx.needs_input_grad[1])
+            ctx.needs_input_grad[1], ctx.dt)
         if x.shape[1] != ctx.e:
             dx, dw = (t[:, :ctx.e] if t is not None else None for t in (dx, dw))
         return dx, dw, None, None, None, None, None
@@ -135,10 +135,10 @@ def catalog_log_probs(queries: torch.Tensor, items: torch.Tensor, ids: torch.Ten
                                     or (bias is not None and bias.requires_grad)):
         return LogProbs(*_CatalogFn.apply(queries, items, ids, bias, float(temperature), entropy,
                                           top))
-    kernels.catalog_check(queries, items, ids, bias)
+    dt = kernels.catalog_check(queries, items, ids, bias)
     lp, ent, _, ti, tl = kernels.catalog_logprobs(
         kernels.catalog_rows(queries), kernels.catalog_rows(items), ids, bias, float(temperature),
-        entropy, top)
+        entropy, top, dt)
     return LogProbs(lp, ent, ti, tl)
 
 
