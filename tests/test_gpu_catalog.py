@@ -163,6 +163,20 @@ def test_log_prob_of_likely_items_keeps_its_precision(dt, N, V, E, bias):
     assert (p > 0.9).any() and (err <= tol).all(), (err / tol).max().item()
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_certain_rows_stay_at_0(dt):
+    """One item has all the probability (the others' is below any float): log p and entropy are 0 and
+    never past it."""
+    from twotower.losses import catalog_log_probs
+
+    x, w, ids, _ = make(300, 700, 192, dt, drop=False)
+    r = catalog_log_probs(w[ids], w, ids, 0.002, entropy=True, top=3)
+    T = U * ((192 + 4) * 500 * 1.01 + 700 / 8 + 64)
+    assert (r.log_prob <= 0).all() and (r.top_log_probs <= 0).all() and (r.entropy >= 0).all()
+    assert (r.log_prob >= -U * 152).all() and (r.entropy <= U * 152).all()
+    assert (r.top_log_probs[:, 0] >= -T).all() and torch.equal(r.top_ids[:, 0], ids)
+
+
 @pytest.mark.parametrize("N,V,E", [(1, 70, 64), (7, 141, 192), (33, 3001, 64), (64, 500, 128),
                                    (50, 20000, 64), (40, 9, 100),
                                    (3, 2100001, 64)])  # (the catalog in two chunks)

@@ -792,6 +792,9 @@ __device__ __forceinline__ void put_right(double dz, double d, double& L, double
   L += q;
 }
 
+// log p is at most 0: what rounding puts above is 0 (a NaN stays)
+__device__ __forceinline__ float at_most_0(float v) { return v > 0.0f ? 0.0f : v; }
+
 struct CombineArgs {
   const float4* part;
   int splits, N, V, E;
@@ -847,11 +850,13 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   }
   const double l2 = log2(L2);
   if (logp) {
-    const float o = !has ? 0.0f : empty || b <= CT_OUT ? -inf : (float)(l - ((double)m + l2) * 0.6931471805599453);
+    const float o = !has ? 0.0f : empty || b <= CT_OUT ? -inf
+                    : at_most_0((float)(l - ((double)m + l2) * 0.6931471805599453));
     if (lane == 0) logp[n] = o;
   }
   if (lane == 0) {
-    if (ent) ent[n] = empty ? 0.0f : (float)((l2 - T2 / L2) * 0.6931471805599453);
+    const float h = (float)((l2 - T2 / L2) * 0.6931471805599453);
+    if (ent) ent[n] = empty || h < 0.0f ? 0.0f : h;
     lse[n] = empty ? -inf : (float)ls;
   }
 }
@@ -1148,7 +1153,7 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
     }
     if (rank < top) {
       ids_out[n * top + rank] = v;
-      lp_out[n * top + rank] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : (float)(l - (double)ls);
+      lp_out[n * top + rank] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : at_most_0((float)(l - (double)ls));
     }
   }
 }
