@@ -19,7 +19,8 @@
 // top             the STAT pass also writes the maximum of every 16 items a lane saw (N V / 16
 //     floats).  The k largest logits lie in the k groups with the largest maxima; k + 8 groups are
 //     taken (32-bit maxima may swap near-equal ones), their items scored again in 64 bits, and
-//     ordered by that, ties by the lower id.
+//     ordered by that, ties by the lower id.  What 32-bit logits are off by at most is known: see
+//     logit_error; the STAT pass also takes the largest item norm that this needs.
 // k_logits<COEF>  the same product again, its epilogue writing C for a chunk of the catalog, in x's type:
 //     the products take it as an operand of their matrix instructions.  In bf16 a coefficient is then off
 //     by up to 2^-8 of itself, which makes 2.0e-3 of the gradients of 4096 rows (their own rounding
@@ -224,6 +225,21 @@ __device__ __forceinline__ void ct_store4(T* p, const f32x4& v) {
   else *(f32x4*)p = v;
 }
 
+// d + the sum of the squares of 16 bytes of a vector
+template <typename T>
+__device__ __forceinline__ float sumsq16(const u32x4_t& v, float d) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      d = fmaf(__uint_as_float(v[i]), __uint_as_float(v[i]), d);
+    } else {
+      const ct_bf16x2 b = __builtin_bit_cast(ct_bf16x2, v[i]);
+      d = __builtin_amdgcn_fdot2_f32_bf16(b, b, d, false);
+    }
+  }
+  return d;
+}
+
 // (m, L, T) of two disjoint sets of items
 __device__ __forceinline__ void stat_join(float& m, float& L, float& T, float m2, float L2, float T2) {
   const float M = fmaxf(m, m2);
@@ -242,6 +258,7 @@ struct LogitArgs {
   int n_tiles, splits, v_tiles;  // tiles of rows, shares of the catalog, tiles of items
   float4* part;        // STAT [splits, N] (m, L, T, -)
   float* tmax;         // STAT: [N, 4 ceil(V / 64)] or null
+  float* wsq;          // STAT with tmax: [blocks] what no |w_v|^2 that the block looked at exceeds
   const float4* rowc;  // COEF [N] (log2-domain lse, g, e, H)
   const int64_t* ids;  // COEF
   void* C;             // COEF [Npad, ldc]: items v_base .. of this chunk
@@ -290,6 +307,10 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
   float m[FI], L[FI], TT[FI];
   float4 rc[FI];
   int id[FI];
+  // the items' norms (with tmax): a tile's by the block of the row tile that its number falls to; every
+  // lane sums the squares of what it loaded itself (8 lanes a row)
+  constexpr int PW = decltype(sw)::PW;
+  float sq[PW], wmx = 0.0f;
 #pragma unroll
   for (int i = 0; i < FI; ++i) {
     m[i] = CT_NONE;
@@ -323,15 +344,37 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
     for (int i = 0; i < FI; ++i)
 #pragma unroll
       for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const bool nrm = !COEF && a.tmax && vt % a.n_tiles == tn;
+#pragma unroll
+    for (int j = 0; j < PW; ++j) sq[j] = 0.0f;
     for (int kt = 0; kt < nk; ++kt, ++gs) {
       ct_wait_vm<0>();
       ct_barrier();  // stage gs complete; every wave is done with the slot refilled next
       issue_next();
       const char* st = smem + (gs & 1) * 2 * TL::OP_B;
+      if constexpr (!COEF) {
+        if (nrm) {
+#pragma unroll
+          for (int j = 0; j < PW; ++j)
+            sq[j] = sumsq16<T>(*(const u32x4_t*)(st + 1024 * (w + TL::NWV * j) + 16 * lane), sq[j]);
+        }
+      }
       u32x4_t fw[2][FJ], fx[2][FI];
       row_frags(st, 16 * FJ * wv, lane, fw);
       row_frags(st + TL::OP_B, nw, lane, fx);
       ct_stage<T>(fw, fx, acc);
+    }
+    if constexpr (!COEF) {
+      if (nrm) {
+#pragma unroll
+        for (int j = 0; j < PW; ++j) {
+          float t = sq[j];
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) t += __shfl_xor(t, o, 64);
+          const int v = a.v_base + vt * TL::EDGE + 8 * (w + TL::NWV * j) + (lane >> 3);
+          if (v < v_end && !(a.bias && a.bias[v] <= CT_OUT)) wmx = fmaxf(wmx, t);  // (a NaN: left out)
+        }
+      }
     }
     // up to 64 of the wave's items at a time
 #pragma unroll
@@ -471,7 +514,17 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
         r[2] = TT[i];
       }
     }
+    if (a.tmax) {
+      const float t = __uint_as_float(wave_max_u32(__float_as_uint(wmx)));
+      if (lane == 0) red[TL::EDGE * 3 + w] = t;
+    }
     ct_barrier();
+    if (a.tmax && tid == 0) {
+      float t = red[TL::EDGE * 3];
+#pragma unroll
+      for (int i = 1; i < TL::NWV; ++i) t = fmaxf(t, red[TL::EDGE * 3 + i]);
+      a.wsq[blockIdx.x] = t;
+    }
     if (wv == 0 && g == 0) {
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
@@ -506,6 +559,11 @@ __global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
   constexpr int OPS = PW + (BIAS ? 1 : 0);  // DMA instructions a wave issues per tile
   __shared__ __attribute__((aligned(16))) char smem[SLOTS * TB];
   __shared__ __attribute__((aligned(16))) float sbias[SLOTS + 1][64];
+  // the items' norms (with tmax; a tile's by the block of the row tile that its number falls to): every
+  // lane the squares of the 16 bytes of a row that it loaded, the largest over all tiles for each place
+  // in the row, and the sum of these at the end.  No norm exceeds it (of like vectors it is some 2 times
+  // the squares), and no register is held for it, of which there are none to spare.
+  __shared__ uint32_t place[4 * KS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, rl = lane & 15;
@@ -523,8 +581,7 @@ __global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
   const uint16_t* wt = (const uint16_t*)a.w;
 
   // tile bytes [1024 p, +1024) = 64 chunks of 16 B in row order; row r's chunk c lies at c ^ (r & 15)
-  int64_t off[PW];
-  int row[PW];
+  int off[PW], row[PW];
 #pragma unroll
   for (int j = 0; j < PW; ++j) {
     const int c = (w + 8 * j) * 64 + lane;
@@ -547,7 +604,13 @@ __global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
                                        (__attribute__((address_space(3))) void*)sbias[t % (SLOTS + 1)], 4, 0, 0);
     }
   };
-  if (t0 >= t1) return;
+  if constexpr (!COEF) {
+    if (tid < 4 * KS) place[tid] = 0u;  // (used after a tile's barrier)
+  }
+  if (t0 >= t1) {  // (no share is empty)
+    if (!COEF && a.tmax && tid == 0) a.wsq[blockIdx.x] = 0.0f;
+    return;
+  }
 
   u32x4_t xf[KS][QB];
 #pragma unroll
@@ -663,6 +726,19 @@ __global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
     ct_barrier();  // tile t is complete; every wave is done with the slot refilled next
     if (t + SLOTS - 1 < t1) issue(t + SLOTS - 1);
     const char* st = smem + (t % SLOTS) * TB;
+    if constexpr (!COEF) {
+      if (a.tmax && t % a.n_tiles == tn) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+        for (int j = 0; j < PW; ++j) {
+          const float q = sumsq16<uint16_t>(*(const u32x4_t*)(st + 1024 * (w + 8 * j) + 16 * lane), 0.0f);
+          const int c = (w + 8 * j) * 64 + lane, r = c / (4 * KS);
+          if (a.v_base + 32 * t + r < v_end && !(BIAS && sbias[t % (SLOTS + 1)][r] <= CT_OUT))
+            atomicMax(&place[(c % (4 * KS)) ^ (r & 15)], __float_as_uint(fmaxf(q, 0.0f)));  // (a NaN: left out)
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
     const bool edge = COEF && has_prev && a.v_base + 32 * t > v_end;  // (the previous tile's)
     float s2 = a.s2;
     if (has_prev) {
@@ -713,7 +789,16 @@ __global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
   } else {
     finish(A);
   }
-  if constexpr (!COEF) {  // a row's four lanes
+  if constexpr (!COEF) {
+    if (a.tmax) {
+      ct_barrier();
+      if (tid == 0) {
+        float t = 0.0f;
+        for (int i = 0; i < 4 * KS; ++i) t += __uint_as_float(place[i]);
+        a.wsq[blockIdx.x] = t;
+      }
+    }
+    // a row's four lanes
 #pragma unroll
     for (int q = 0; q < QB; ++q) {
 #pragma unroll
@@ -795,6 +880,17 @@ __device__ __forceinline__ void put_right(double dz, double d, double& L, double
 // log p is at most 0: what rounding puts above is 0 (a NaN stays)
 __device__ __forceinline__ float at_most_0(float v) { return v > 0.0f ? 0.0f : v; }
 
+// What a row's 32-bit logits (in powers of two) are off by at most, 4 u |z| besides: every one of the
+// E products and sums (and the few operations after them) rounds or cuts off at most 2^-23 of sum |x_e
+// w_e| <= |x| |w|, whatever the order; elements, products and sums below the least normal number may
+// count as 0.  xsq, wsq: squares in f32, off by less than 1 in 100; those that the squaring loses are
+// of elements below 2^-63.
+__device__ __forceinline__ float logit_error(float s2, int E, float xsq, float wsq) {
+  const float r = sqrtf((float)E), tiny = 1.2e-19f * r;
+  const float X = 1.01f * sqrtf(xsq) + tiny, W = 1.01f * sqrtf(wsq) + tiny;
+  return s2 * (X * W) * ((float)(E + 24) * 1.2e-7f) + s2 * (1.2e-38f * (float)E) * (2.0f + X + W);
+}
+
 struct CombineArgs {
   const float4* part;
   int splits, N, V, E;
@@ -806,6 +902,9 @@ struct CombineArgs {
   float s2;   // log2(e) s, as the statistics' kernel has it
   int group;  // items of a wave there: a group that ends past V has its logits rounded on their own
   float *logp, *ent, *lse;
+  const float* wsq;  // with alternatives: [n_wsq] of the statistics' blocks
+  int n_wsq;
+  float* err;        // [N] logit_error
 };
 // One wave per row: the shares' statistics joined, the given item's logit.
 template <typename T>
@@ -837,6 +936,18 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   for (int o = 1; o < 64; o <<= 1) {
     const float m2 = __shfl_xor(m, o, 64), L2 = __shfl_xor(L, o, 64), T2 = __shfl_xor(TT, o, 64);
     stat_join(m, L, TT, m2, L2, T2);
+  }
+  if (a.err) {
+    float xsq = 0.0f, wsq = 0.0f;
+    constexpr int PC = 16 / (int)sizeof(T);
+    for (int e = lane * PC; e < E; e += 64 * PC) xsq = sumsq16<T>(*(const u32x4_t*)(x + n * ldx + e), xsq);
+    for (int i = lane; i < a.n_wsq; i += 64) wsq = fmaxf(wsq, a.wsq[i]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      xsq += __shfl_xor(xsq, o, 64);
+      wsq = fmaxf(wsq, __shfl_xor(wsq, o, 64));
+    }
+    if (lane == 0) a.err[n] = logit_error(a.s2, E, xsq, wsq);
   }
   const float inf = __builtin_huge_valf();
   const bool empty = m <= CT_OUT && L == L;  // every item taken out (and no NaN)
@@ -1028,7 +1139,7 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
                                                    int top, const T* __restrict__ x, int64_t ldx,
                                                    const T* __restrict__ w, int64_t ldw, int E, int V,
                                                    const float* __restrict__ bias, double s,
-                                                   const float* __restrict__ lse,
+                                                   const float* __restrict__ lse, const float* __restrict__ err,
                                                    int64_t* __restrict__ ids_out, float* __restrict__ lp_out) {
   constexpr int GMAX = CT_TOP_MAX + CT_TOP_EXTRA;
   constexpr int PC = 16 / (int)sizeof(T);
@@ -1062,7 +1173,6 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
     if (lane >= have) red[wv][lane] = 0ull;
   }
   if (tid < 64) fin[tid] = 0ull;
-  if (tid == 0) nlist = 0;
   __syncthreads();
   {
     const int used = total <= NT ? (total + 1) & ~1 : NT;
@@ -1073,70 +1183,79 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
     }
   }
   __syncthreads();
-  if (wv == 0) {
-    const uint64_t k1 = lane < keep ? fin[lane] : 0ull;
-    // the top-th largest maximum: the top-th largest logit is not below it, so a group or an item
-    // clearly below cannot be one of the top (the margin is far above what 32-bit sums are off)
-    const uint64_t last = fin[top - 1];
-    const int t = last != 0ull ? top : 0;
-    const float kth = key_score(last), best = key_score(fin[0]);
-    // (fewer than top groups, or taken-out items among the top: every item takes part)
-    const float floor = t < top || kth < 0.9f * CT_OUT ? -__builtin_huge_valf()
-                                : kth - 0.0009765625f * (fabsf(kth) + fabsf(best) + 1.0f);
-    const bool use = k1 != 0ull && !(key_score(k1) < floor);
-    const uint64_t bm = __ballot(use);
-    if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(k1);
-    if (lane == 0) {
-      s_groups = __popcll(bm);
-      s_floor = floor;
-    }
-  }
-  __syncthreads();
-  const int ngrp = s_groups;
-  const float floor = s_floor;
+  const float e0 = err[n];
   const T* xr = x + n * ldx;
-  const int sub = tid >> 4, l16 = tid & 15, cand = ngrp * 16;
-  for (int i0 = sub; i0 < cand; i0 += 4 * NG) {
-    int v[4];
-    double d[4];
-    const T* wr[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = i0 + i * NG < cand ? i0 + i * NG : i0, it = c & 15;
-      const uint32_t q = grp[c >> 4];
-      v[i] = (int)(q >> 2) * 64 + 16 * (it >> 2) + 4 * (int)(q & 3) + (it & 3);
-      wr[i] = w + (int64_t)(v[i] < V ? v[i] : V - 1) * ldw;
-      d[i] = 0.0;
-    }
-#pragma unroll 2
-    for (int e = l16 * PC; e < E; e += 16 * PC) {
-      const u32x4_t xv = *(const u32x4_t*)(xr + e);
-      u32x4_t y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = *(const u32x4_t*)(wr[i] + e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = dot16<T>(xv, y[i], d[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) d[i] += __shfl_xor(d[i], o, 64);
-      const int c = i0 + i * NG;
-      if (l16 == 0 && c < cand) {
-        double l = -__builtin_huge_val();
-        bool in = false;
-        if (v[i] < V) {
-          const float b = bias ? bias[v[i]] : 0.0f;
-          if (!(b <= CT_OUT)) l = s * d[i] + (double)b;
-          in = !(l * 1.4426950408889634 < (double)floor);  // (-inf, NaN: only where the floor lets them)
-        }
-        sc[c] = l;
-        vid[c] = v[i];
-        if (in) list[atomicAdd(&nlist, 1)] = (short)c;
+  const int sub = tid >> 4, l16 = tid & 15;
+  for (bool all = false;; all = true) {
+    if (wv == 0) {
+      const uint64_t k1 = lane < keep ? fin[lane] : 0ull;
+      // the top-th largest maximum: top groups hold an item each that is not below it in 32 bits, so the
+      // top-th largest exact logit is not below it by more than a 32-bit logit is off.  A group whose
+      // maximum is clearly below that holds none of the top, nor is one of the top below it in 64 bits.
+      const uint64_t last = fin[top - 1];
+      const float kth = key_score(last);
+      float fl = kth - (2.01f * e0 + 2.0e-6f * fabsf(kth));
+      // (fewer than top groups, taken-out items among the top, values past 32 bits or not numbers, or
+      // fewer than top items found: every item of the groups kept takes part)
+      if (all || last == 0ull || kth < 0.9f * CT_OUT || !(fabsf(fl) < 3.0e38f)) fl = -__builtin_huge_valf();
+      const bool use = k1 != 0ull && !(key_score(k1) < fl);
+      const uint64_t bm = __ballot(use);
+      if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(k1);
+      if (lane == 0) {
+        s_groups = __popcll(bm);
+        s_floor = fl;
+        nlist = 0;
       }
     }
+    __syncthreads();
+    const int cand = s_groups * 16;
+    const float floor = s_floor;
+    for (int i0 = sub; i0 < cand; i0 += 4 * NG) {
+      int v[4];
+      double d[4];
+      const T* wr[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = i0 + i * NG < cand ? i0 + i * NG : i0, it = c & 15;
+        const uint32_t q = grp[c >> 4];
+        v[i] = (int)(q >> 2) * 64 + 16 * (it >> 2) + 4 * (int)(q & 3) + (it & 3);
+        wr[i] = w + (int64_t)(v[i] < V ? v[i] : V - 1) * ldw;
+        d[i] = 0.0;
+      }
+#pragma unroll 2
+      for (int e = l16 * PC; e < E; e += 16 * PC) {
+        const u32x4_t xv = *(const u32x4_t*)(xr + e);
+        u32x4_t y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = *(const u32x4_t*)(wr[i] + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = dot16<T>(xv, y[i], d[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) d[i] += __shfl_xor(d[i], o, 64);
+        const int c = i0 + i * NG;
+        if (l16 == 0 && c < cand) {
+          double l = -__builtin_huge_val();
+          bool in = false;
+          if (v[i] < V) {
+            const float b = bias ? bias[v[i]] : 0.0f;
+            if (!(b <= CT_OUT)) l = s * d[i] + (double)b;
+            in = !(l * 1.4426950408889634 < (double)floor);  // (-inf, NaN: only where the floor lets them)
+          }
+          sc[c] = l;
+          vid[c] = v[i];
+          if (in) list[atomicAdd(&nlist, 1)] = (short)c;
+        }
+      }
+    }
+    __syncthreads();
+    // (a second round only where sums in 32 bits went past their range: all the groups kept hold at
+    // least top items)
+    if (all || nlist >= top) break;
+    __syncthreads();
   }
-  __syncthreads();
   const float ls = lse[n];
   const int m = nlist;  // (in any order: ranks do not depend on it)
   for (int i = tid; i < m; i += NT) {
@@ -1386,7 +1505,7 @@ static void logits_shape(int64_t N, int64_t V, int edge, int& n_tiles, int& v_ti
 struct StatPlan {
   bool ring;
   int edge, n_tiles, v_tiles, splits, keep, nseg, seg_len;
-  int64_t M, off_tmax, off_seg, bytes;
+  int64_t M, off_tmax, off_seg, off_wsq, off_err, bytes;
 };
 // Shares: about 512 blocks (two a CU; three of the small tiles).
 static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
@@ -1407,7 +1526,9 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
     p.nseg = (int)cdiv(p.M, p.seg_len);
     p.off_tmax = p.bytes;
     p.off_seg = p.off_tmax + up(N * p.M * 4, 256);
-    p.bytes = p.off_seg + up(N * p.nseg * p.keep * 8, 256);
+    p.off_wsq = p.off_seg + up(N * p.nseg * p.keep * 8, 256);
+    p.off_err = p.off_wsq + up((int64_t)p.n_tiles * p.splits * 4, 256);
+    p.bytes = p.off_err + up(N * 4, 256);
   }
   return p;
 }
@@ -1554,11 +1675,13 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   a.n_tiles = p.n_tiles; a.splits = p.splits; a.v_tiles = p.v_tiles;
   a.part = (float4*)ws;
   a.tmax = top ? (float*)(ws + p.off_tmax) : nullptr;
+  a.wsq = top ? (float*)(ws + p.off_wsq) : nullptr;
   a.v_count = (int)V;
   if (p.ring) ring_launch<false>(a, ent != nullptr, st);
   else logits_launch<T, false>(a, p.edge, ent != nullptr, st);
   const CombineArgs ca{a.part, p.splits, (int)N, (int)V, E, x, w, ldx, ldw, ids, bias, s, a.s2,
-                       p.ring || p.edge == 64 ? 32 : 64, logp, ent, lse};
+                       p.ring || p.edge == 64 ? 32 : 64, logp, ent, lse, a.wsq, p.n_tiles * p.splits,
+                       top ? (float*)(ws + p.off_err) : nullptr};
   const unsigned cb = (unsigned)cdiv(N, 4);
   if (top) {
     uint64_t* seg = (uint64_t*)(ws + p.off_seg);
@@ -1569,13 +1692,13 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     // 256 (90 with 512)
     if (N <= 128)
       hipLaunchKernelGGL((k_top_items<T, 1024>), dim3((unsigned)N), dim3(1024), 0, st, seg, p.nseg, p.keep, top,
-                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, ca.err, top_ids, top_lp);
     else if (N <= 512)
       hipLaunchKernelGGL((k_top_items<T, 512>), dim3((unsigned)N), dim3(512), 0, st, seg, p.nseg, p.keep, top,
-                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, ca.err, top_ids, top_lp);
     else
       hipLaunchKernelGGL((k_top_items<T, 256>), dim3((unsigned)N), dim3(256), 0, st, seg, p.nseg, p.keep, top,
-                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, top_ids, top_lp);
+                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, ca.err, top_ids, top_lp);
   } else {
     hipLaunchKernelGGL(k_combine<T>, dim3(cb), dim3(256), 0, st, ca);
   }
