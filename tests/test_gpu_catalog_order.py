@@ -1,5 +1,6 @@
 """The top alternatives of the catalog log-probabilities (csrc/tt_catalog.hip) where 32-bit logits
-cannot order them: products that cancel.  The order is that of the product in 64 bits, ties to the lower id; every place is written."""
+cannot order them: products that cancel, crowds of items closer than a 32-bit sum resolves.  The
+order is that of the product in 64 bits, ties to the lower id; every place is written."""
 import pytest
 import torch
 
@@ -41,7 +42,7 @@ def check(x, w, temp, top, b=None):
 
 
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [1, 2, 40])
+@pytest.mark.parametrize("V", [1, 2, 40, 700, 5000])
 def test_products_that_cancel(dt, V):
     """x = (c, c, 0, ...), w_v = (r_v, -r_v, 0, ...): every exact logit is 0, the 32-bit ones are what
     the products' rounding leaves."""
@@ -55,7 +56,7 @@ def test_products_that_cancel(dt, V):
 
 
 @pytest.mark.parametrize("norm", [1.0, 100.0, 1000.0])
-@pytest.mark.parametrize("V", [1, 2, 40])
+@pytest.mark.parametrize("V", [1, 2, 40, 300])
 def test_items_orthogonal_to_the_query(norm, V):
     """Items orthogonal to the query but for their own rounding, at norms of 1 to 1000."""
     gen = torch.Generator().manual_seed(int(norm) + V)
@@ -65,3 +66,69 @@ def test_items_orthogonal_to_the_query(norm, V):
             w = torch.randn(V, E, generator=gen).double()
             w = torch.nn.functional.normalize(w - (w @ x.t()) * x, dim=1)
             check((norm * x).float().cuda(), (norm * w).float().cuda(), 0.07, min(V, 10))
+
+
+def crowd(N, V, E, members, dt, seed):
+    """A catalog with ``members`` items (at random places) around each of 3 vectors, their elements a
+    few last bits apart, and queries near one of the three."""
+    gen = torch.Generator().manual_seed(seed)
+    w = torch.nn.functional.normalize(torch.randn(V, E, generator=gen), dim=1)
+    centre = torch.nn.functional.normalize(torch.randn(3, E, generator=gen), dim=1)
+    at = torch.randperm(V, generator=gen)[:3 * members]
+    ulp = torch.finfo(dt).eps
+    near = centre.repeat_interleave(members, 0)
+    hit = torch.rand(near.shape, generator=gen) < (0.5 if dt == torch.float32 else 2.0 / E)
+    w[at] = near * (1 + ulp * torch.randint(-2, 3, near.shape, generator=gen) * hit)
+    x = torch.nn.functional.normalize(
+        centre[torch.randint(0, 3, (N,), generator=gen)]
+        + 0.3 * torch.randn(N, E, generator=gen) / E ** 0.5, dim=1)
+    return x.to(dt).cuda(), w.to(dt).cuda(), gen
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_a_crowd_of_nearly_equal_items(seed):
+    """60 items that differ in their last bits (one text encoded in different batches)."""
+    x, w, _ = crowd(5, 3000, 384, 60, torch.float32, seed)
+    check(x, w, 0.07, 10)
+
+
+@pytest.mark.parametrize("dt,N,V,E,members", [
+    (torch.float32, 1, 200000, 64, 3000),      # many segments of a row
+    (torch.float32, 40, 9001, 100, 1500), (torch.float32, 150, 20000, 64, 700),
+    (torch.bfloat16, 1, 150000, 384, 4000), (torch.bfloat16, 33, 10007, 384, 1000),
+    (torch.bfloat16, 140, 25000, 256, 900),    # tiles of 128
+    (torch.bfloat16, 300, 33000, 64, 1500),    # tiles of 256
+    (torch.bfloat16, 384, 90000, 384, 700)])   # rows kept in registers
+@pytest.mark.parametrize("bias", [False, True])
+def test_large_crowds(dt, N, V, E, members, bias):
+    """More of them than any fixed number of candidates, over the whole catalog."""
+    x, w, gen = crowd(N, V, E, members, dt, N + V)
+    b = None
+    if bias:
+        b = torch.where(torch.rand(V, generator=gen) < 0.3, float("-inf"),
+                        2.0 ** -20 * torch.randint(0, 3, (V,), generator=gen)).cuda()
+    for top in (1, 10, 32):
+        check(x, w, 0.07, top, b)
+
+
+def test_a_crowd_in_a_graph_and_on_another_stream():
+    x, w, _ = crowd(40, 9001, 64, 800, torch.float32, 3)
+    from twotower.losses import catalog_log_probs
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        r = catalog_log_probs(x, w, None, 0.07, top=12)
+    st.synchronize()
+    assert torch.equal(r.top_ids, order(exact(x, w, 0.07), 12))
+    xs = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        r = catalog_log_probs(xs, w, None, 0.07, top=12)
+    for k in range(4):  # replays with and without a crowd among the alternatives
+        xs.copy_(x if k % 2 == 0 else -x)
+        graph.replay()
+        torch.cuda.synchronize()
+        e = catalog_log_probs(xs, w, None, 0.07, top=12)
+        assert torch.equal(r.top_ids, order(exact(xs, w, 0.07), 12))
+        assert torch.equal(r.top_ids, e.top_ids) and torch.equal(r.top_log_probs, e.top_log_probs)

@@ -20,7 +20,9 @@
 //     floats).  The k largest logits lie in the k groups with the largest maxima; k + 8 groups are
 //     taken (32-bit maxima may swap near-equal ones), their items scored again in 64 bits, and
 //     ordered by that, ties by the lower id.  What 32-bit logits are off by at most is known: see
-//     logit_error; the STAT pass also takes the largest item norm that this needs.
+//     logit_error; the STAT pass also takes the largest item norm that this needs.  A row where groups
+//     that were not taken lie within it (a crowd of nearly equal items) is searched again, over all of
+//     its groups that do (k_top_wide).
 // k_logits<COEF>  the same product again, its epilogue writing C for a chunk of the catalog, in x's type:
 //     the products take it as an operand of their matrix instructions.  In bf16 a coefficient is then off
 //     by up to 2^-8 of itself, which makes 2.0e-3 of the gradients of 4096 rows (their own rounding
@@ -1132,31 +1134,127 @@ __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tm
   if (w == 0 && lane < keep) out[(n * nseg + sg) * keep + lane] = fin[lane];
 }
 
-// One block per row: the keep largest groups of all segments, their items scored in 64 bits (16 lanes
-// an item, 16-byte loads, 128 items in flight), the top of them by (score, lower id).
+struct TopEntry {
+  double l;
+  int64_t v;
+};
+struct TopArgs {
+  const uint64_t* segs;
+  int nseg, keep, top;
+  const void *x, *w;
+  int64_t ldx, ldw;
+  int N, E, V;
+  const float* bias;
+  double s;
+  const float *lse, *err;
+  int64_t* ids_out;
+  float* lp_out;
+  // the second search
+  const float* tmax;
+  int64_t M;
+  int seg_len;
+  float* floor;     // [N]
+  uint32_t* state;  // [N] CT_DONE, or the segments that are searched already
+  TopEntry* found;  // [N, nseg, top]
+};
+constexpr uint32_t CT_DONE = 0x80000000u;
+constexpr int CT_GROUPS = CT_TOP_MAX + CT_TOP_EXTRA;  // groups scored at a time
+struct TopList {
+  double l[CT_GROUPS * 16 + CT_TOP_MAX];  // candidates, in any order (ranks do not depend on it)
+  int v[CT_GROUPS * 16 + CT_TOP_MAX];
+  double bl[CT_TOP_MAX];  // the best of them, the first first
+  int bv[CT_TOP_MAX];
+  int n;
+};
+
+// The items of n_grp groups, scored in 64 bits (16 lanes an item, 16-byte loads, NT / 4 items in
+// flight); those not below cut (powers of two) join the list.
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ segs, int nseg, int keep,
-                                                   int top, const T* __restrict__ x, int64_t ldx,
-                                                   const T* __restrict__ w, int64_t ldw, int E, int V,
-                                                   const float* __restrict__ bias, double s,
-                                                   const float* __restrict__ lse, const float* __restrict__ err,
-                                                   int64_t* __restrict__ ids_out, float* __restrict__ lp_out) {
-  constexpr int GMAX = CT_TOP_MAX + CT_TOP_EXTRA;
-  constexpr int PC = 16 / (int)sizeof(T);
-  constexpr int NW = NT / 64, NG = NT / 16;
+__device__ __forceinline__ void top_score(const TopArgs& a, const T* xr, const uint32_t* grp, int n_grp, double cut,
+                                          TopList& o) {
+  constexpr int PC = 16 / (int)sizeof(T), NG = NT / 16;
+  const T* w = (const T*)a.w;
+  const int sub = threadIdx.x >> 4, l16 = threadIdx.x & 15, cand = n_grp * 16, V = a.V, E = a.E;
+  for (int i0 = sub; i0 < cand; i0 += 4 * NG) {
+    int v[4];
+    double d[4];
+    const T* wr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = i0 + i * NG < cand ? i0 + i * NG : i0, it = c & 15;
+      const uint32_t q = grp[c >> 4];
+      v[i] = (int)(q >> 2) * 64 + 16 * (it >> 2) + 4 * (int)(q & 3) + (it & 3);
+      wr[i] = w + (int64_t)(v[i] < V ? v[i] : V - 1) * a.ldw;
+      d[i] = 0.0;
+    }
+#pragma unroll 2
+    for (int e = l16 * PC; e < E; e += 16 * PC) {
+      const u32x4_t xv = *(const u32x4_t*)(xr + e);
+      u32x4_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = *(const u32x4_t*)(wr[i] + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = dot16<T>(xv, y[i], d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int m = 1; m < 16; m <<= 1) d[i] += __shfl_xor(d[i], m, 64);
+      if (l16 == 0 && i0 + i * NG < cand && v[i] < V) {
+        const float b = a.bias ? a.bias[v[i]] : 0.0f;
+        const double l = b <= CT_OUT ? -__builtin_huge_val() : a.s * d[i] + (double)b;
+        if (!(l * 1.4426950408889634 < cut)) {  // (-inf, NaN: only where the cut lets them)
+          const int k = atomicAdd(&o.n, 1);
+          o.l[k] = l;
+          o.v[k] = v[i];
+        }
+      }
+    }
+  }
+}
+// The best of the list, by (score, lower id); NaN scores by id among themselves, below all others.
+template <int NT>
+__device__ __forceinline__ void top_rank(TopList& o, int top) {
+  const int m = o.n;
+  for (int i = threadIdx.x; i < m; i += NT) {
+    const double l = o.l[i];
+    const int v = o.v[i];
+    int rank = 0;
+    for (int q = 0; q < m; ++q) {
+      const double t = o.l[q];
+      const bool gt = t > l || (l != l && t == t);
+      const bool eq = t == l || (t != t && l != l);
+      rank += gt || (eq && o.v[q] < v) ? 1 : 0;
+    }
+    if (rank < top) {
+      o.bl[rank] = l;
+      o.bv[rank] = v;
+    }
+  }
+}
+__device__ __forceinline__ void top_write(const TopArgs& a, const TopList& o, int64_t n) {
+  const int i = threadIdx.x;
+  if (i >= a.top) return;
+  const double l = o.bl[i];
+  a.ids_out[n * a.top + i] = o.bv[i];
+  a.lp_out[n * a.top + i] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : at_most_0((float)(l - (double)a.lse[n]));
+}
+
+// One block per row: the keep largest groups of all segments, their items scored in 64 bits, the top of
+// them by (score, lower id).
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_top_items(const TopArgs a) {
+  constexpr int NW = NT / 64;
   __shared__ __attribute__((aligned(16))) uint64_t red[NW][64];
   __shared__ uint64_t fin[64];
   __shared__ uint32_t grp[64];
   __shared__ int s_groups;
   __shared__ float s_floor;
-  __shared__ double sc[GMAX * 16];
-  __shared__ int vid[GMAX * 16];
-  __shared__ int nlist;
-  __shared__ short list[GMAX * 16];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  __shared__ TopList o;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, keep = a.keep, top = a.top;
   const int64_t n = blockIdx.x;
-  const int total = nseg * keep;
-  const uint64_t* src = segs + n * total;
+  const int total = a.nseg * keep;
+  const uint64_t* src = a.segs + n * total;
   if (total <= NT) {
     red[wv][lane] = tid < total ? src[tid] : 0ull;
   } else {
@@ -1183,96 +1281,121 @@ __global__ __launch_bounds__(NT) void k_top_items(const uint64_t* __restrict__ s
     }
   }
   __syncthreads();
-  const float e0 = err[n];
-  const T* xr = x + n * ldx;
-  const int sub = tid >> 4, l16 = tid & 15;
+  const float e0 = a.err[n];
+  const T* xr = (const T*)a.x + n * a.ldx;
+  bool more = false;  // (wave 0) groups that were not taken may hold some of the top
   for (bool all = false;; all = true) {
     if (wv == 0) {
       const uint64_t k1 = lane < keep ? fin[lane] : 0ull;
       // the top-th largest maximum: top groups hold an item each that is not below it in 32 bits, so the
       // top-th largest exact logit is not below it by more than a 32-bit logit is off.  A group whose
       // maximum is clearly below that holds none of the top, nor is one of the top below it in 64 bits.
-      const uint64_t last = fin[top - 1];
+      const uint64_t last = fin[top - 1], end = fin[keep - 1];
       const float kth = key_score(last);
       float fl = kth - (2.01f * e0 + 2.0e-6f * fabsf(kth));
       // (fewer than top groups, taken-out items among the top, values past 32 bits or not numbers, or
       // fewer than top items found: every item of the groups kept takes part)
-      if (all || last == 0ull || kth < 0.9f * CT_OUT || !(fabsf(fl) < 3.0e38f)) fl = -__builtin_huge_valf();
+      const bool few = last == 0ull || kth < 0.9f * CT_OUT;
+      if (all || few || !(fabsf(fl) < 3.0e38f)) fl = -__builtin_huge_valf();
+      // (few: the groups kept are all that hold anything, and those of the lowest ids besides)
+      more = end != 0ull && !few && e0 == e0 && !(key_score(end) < fl);
       const bool use = k1 != 0ull && !(key_score(k1) < fl);
       const uint64_t bm = __ballot(use);
       if (use) grp[__popcll(bm & ((1ull << lane) - 1))] = key_row(k1);
       if (lane == 0) {
         s_groups = __popcll(bm);
         s_floor = fl;
-        nlist = 0;
+        o.n = 0;
       }
     }
     __syncthreads();
-    const int cand = s_groups * 16;
-    const float floor = s_floor;
-    for (int i0 = sub; i0 < cand; i0 += 4 * NG) {
-      int v[4];
-      double d[4];
-      const T* wr[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = i0 + i * NG < cand ? i0 + i * NG : i0, it = c & 15;
-        const uint32_t q = grp[c >> 4];
-        v[i] = (int)(q >> 2) * 64 + 16 * (it >> 2) + 4 * (int)(q & 3) + (it & 3);
-        wr[i] = w + (int64_t)(v[i] < V ? v[i] : V - 1) * ldw;
-        d[i] = 0.0;
-      }
-#pragma unroll 2
-      for (int e = l16 * PC; e < E; e += 16 * PC) {
-        const u32x4_t xv = *(const u32x4_t*)(xr + e);
-        u32x4_t y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = *(const u32x4_t*)(wr[i] + e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = dot16<T>(xv, y[i], d[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) d[i] += __shfl_xor(d[i], o, 64);
-        const int c = i0 + i * NG;
-        if (l16 == 0 && c < cand) {
-          double l = -__builtin_huge_val();
-          bool in = false;
-          if (v[i] < V) {
-            const float b = bias ? bias[v[i]] : 0.0f;
-            if (!(b <= CT_OUT)) l = s * d[i] + (double)b;
-            in = !(l * 1.4426950408889634 < (double)floor);  // (-inf, NaN: only where the floor lets them)
-          }
-          sc[c] = l;
-          vid[c] = v[i];
-          if (in) list[atomicAdd(&nlist, 1)] = (short)c;
-        }
-      }
-    }
+    top_score<T, NT>(a, xr, grp, s_groups, (double)s_floor, o);
     __syncthreads();
     // (a second round only where sums in 32 bits went past their range: all the groups kept hold at
     // least top items)
-    if (all || nlist >= top) break;
+    if (all || o.n >= top) break;
     __syncthreads();
   }
-  const float ls = lse[n];
-  const int m = nlist;  // (in any order: ranks do not depend on it)
-  for (int i = tid; i < m; i += NT) {
-    const int c = list[i];
-    const double l = sc[c];
-    const int v = vid[c];
-    int rank = 0;  // NaN scores rank by id among themselves, below all others
-    for (int o = 0; o < m; ++o) {
-      const int q = list[o];
-      const double t = sc[q];
-      const bool gt = t > l || (l != l && t == t);
-      const bool eq = t == l || (t != t && l != l);
-      rank += gt || (eq && vid[q] < v) ? 1 : 0;
+  top_rank<NT>(o, top);
+  __syncthreads();
+  top_write(a, o, n);
+  if (a.state && tid == 0) {
+    a.floor[n] = s_floor;
+    a.state[n] = more ? 0u : CT_DONE;
+  }
+}
+
+// The second search: rows whose groups above the floor were more than are kept.  Block = (row, segment):
+// the segment's groups above the floor, 40 at a time, are scored in 64 bits with the best so far; the
+// row's last block joins the segments (no block waits for another).  Without such rows: 2 us of launch.
+template <typename T>
+__global__ __launch_bounds__(256) void k_top_wide(const TopArgs a) {
+  __shared__ TopList o;
+  __shared__ uint32_t pend[256];
+  __shared__ int n_pend, s_last;
+  const int tid = threadIdx.x, top = a.top;
+  auto carry = [&]() __attribute__((always_inline)) {  // the list becomes its best
+    __syncthreads();
+    top_rank<256>(o, top);
+    __syncthreads();
+    const int k = o.n < top ? o.n : top;
+    if (tid < k) {
+      o.l[tid] = o.bl[tid];
+      o.v[tid] = o.bv[tid];
     }
-    if (rank < top) {
-      ids_out[n * top + rank] = v;
-      lp_out[n * top + rank] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : at_most_0((float)(l - (double)ls));
+    __syncthreads();
+    if (tid == 0) o.n = k;
+    __syncthreads();
+  };
+  const int64_t units = (int64_t)a.N * a.nseg;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t n = u / a.nseg;
+    if (a.state[n] & CT_DONE) continue;
+    const int sg = (int)(u % a.nseg);
+    const T* xr = (const T*)a.x + n * a.ldx;
+    const float* row = a.tmax + n * a.M;
+    const float floor = a.floor[n];
+    const int64_t i0 = (int64_t)sg * a.seg_len, i1 = i0 + a.seg_len < a.M ? i0 + a.seg_len : a.M;
+    double cut = (double)floor;
+    if (tid == 0) o.n = 0;
+    for (int64_t b = i0; b < i1; b += 256) {
+      if (tid == 0) n_pend = 0;
+      __syncthreads();
+      const int64_t e = b + tid;
+      if (e < i1 && !(row[e] < floor)) pend[atomicAdd(&n_pend, 1)] = (uint32_t)e;
+      __syncthreads();
+      const int np = n_pend;
+      for (int p = 0; p < np; p += CT_GROUPS) {
+        top_score<T, 256>(a, xr, pend + p, np - p < CT_GROUPS ? np - p : CT_GROUPS, cut, o);
+        carry();
+        // (an equal score passes: the lower id counts)
+        if (o.n == top && o.l[top - 1] * 1.4426950408889634 > cut) cut = o.l[top - 1] * 1.4426950408889634;
+      }
+      __syncthreads();
+    }
+    __syncthreads();
+    if (tid < top) a.found[u * top + tid] = tid < o.n ? TopEntry{o.l[tid], o.v[tid]} : TopEntry{0.0, -1};
+    __threadfence();  // visible before the block counts itself in
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(&a.state[n], 1u) == (uint32_t)a.nseg - 1u;
+    __syncthreads();
+    if (s_last) {
+      __threadfence();
+      const TopEntry* f = a.found + n * a.nseg * top;
+      const int total = a.nseg * top;
+      if (tid == 0) o.n = 0;
+      __syncthreads();
+      for (int b = 0; b < total; b += 512) {
+        for (int i = b + tid; i < total && i < b + 512; i += 256)
+          if (f[i].v >= 0) {
+            const int k = atomicAdd(&o.n, 1);
+            o.l[k] = f[i].l;
+            o.v[k] = (int)f[i].v;
+          }
+        carry();
+      }
+      if (o.n == top) top_write(a, o, n);  // (always: the floor has at least top items above it)
+      __syncthreads();
     }
   }
 }
@@ -1505,7 +1628,7 @@ static void logits_shape(int64_t N, int64_t V, int edge, int& n_tiles, int& v_ti
 struct StatPlan {
   bool ring;
   int edge, n_tiles, v_tiles, splits, keep, nseg, seg_len;
-  int64_t M, off_tmax, off_seg, off_wsq, off_err, bytes;
+  int64_t M, off_tmax, off_seg, off_wsq, off_err, off_floor, off_state, off_found, bytes;
 };
 // Shares: about 512 blocks (two a CU; three of the small tiles).
 static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
@@ -1528,7 +1651,10 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
     p.off_seg = p.off_tmax + up(N * p.M * 4, 256);
     p.off_wsq = p.off_seg + up(N * p.nseg * p.keep * 8, 256);
     p.off_err = p.off_wsq + up((int64_t)p.n_tiles * p.splits * 4, 256);
-    p.bytes = p.off_err + up(N * 4, 256);
+    p.off_floor = p.off_err + up(N * 4, 256);
+    p.off_state = p.off_floor + up(N * 4, 256);
+    p.off_found = p.off_state + up(N * 4, 256);
+    p.bytes = p.off_found + up(p.M > p.keep ? N * p.nseg * top * 16 : 0, 256);
   }
   return p;
 }
@@ -1688,17 +1814,23 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     const unsigned sb = (unsigned)(N * p.nseg);
     hipLaunchKernelGGL(k_top_groups<T>, dim3(sb + cb), dim3(256), 0, st, a.tmax, p.M, p.seg_len, p.nseg,
                        p.keep, seg, sb, ca);
+    TopArgs ta{};
+    ta.segs = seg; ta.nseg = p.nseg; ta.keep = p.keep; ta.top = top;
+    ta.x = x; ta.w = w; ta.ldx = ldx; ta.ldw = ldw; ta.N = (int)N; ta.E = E; ta.V = (int)V;
+    ta.bias = bias; ta.s = s; ta.lse = lse; ta.err = ca.err; ta.ids_out = top_ids; ta.lp_out = top_lp;
+    const bool wide = p.M > p.keep;  // (else no group is left out)
+    if (wide) {
+      ta.tmax = a.tmax; ta.M = p.M; ta.seg_len = p.seg_len;
+      ta.floor = (float*)(ws + p.off_floor);
+      ta.state = (uint32_t*)(ws + p.off_state);
+      ta.found = (TopEntry*)(ws + p.off_found);
+    }
     // more threads a row while rows are few: 33 rows 24 us with 1024 (31 with 512); 2049 rows 53 us with
     // 256 (90 with 512)
-    if (N <= 128)
-      hipLaunchKernelGGL((k_top_items<T, 1024>), dim3((unsigned)N), dim3(1024), 0, st, seg, p.nseg, p.keep, top,
-                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, ca.err, top_ids, top_lp);
-    else if (N <= 512)
-      hipLaunchKernelGGL((k_top_items<T, 512>), dim3((unsigned)N), dim3(512), 0, st, seg, p.nseg, p.keep, top,
-                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, ca.err, top_ids, top_lp);
-    else
-      hipLaunchKernelGGL((k_top_items<T, 256>), dim3((unsigned)N), dim3(256), 0, st, seg, p.nseg, p.keep, top,
-                         (const T*)x, ldx, (const T*)w, ldw, E, (int)V, bias, s, lse, ca.err, top_ids, top_lp);
+    if (N <= 128) hipLaunchKernelGGL((k_top_items<T, 1024>), dim3((unsigned)N), dim3(1024), 0, st, ta);
+    else if (N <= 512) hipLaunchKernelGGL((k_top_items<T, 512>), dim3((unsigned)N), dim3(512), 0, st, ta);
+    else hipLaunchKernelGGL((k_top_items<T, 256>), dim3((unsigned)N), dim3(256), 0, st, ta);
+    if (wide) hipLaunchKernelGGL(k_top_wide<T>, dim3(sb < 1024 ? sb : 1024), dim3(256), 0, st, ta);
   } else {
     hipLaunchKernelGGL(k_combine<T>, dim3(cb), dim3(256), 0, st, ca);
   }
