@@ -309,10 +309,15 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
   float m[FI], L[FI], TT[FI];
   float4 rc[FI];
   int id[FI];
-  // the items' norms (with tmax): a tile's by the block of the row tile that its number falls to; every
-  // lane sums the squares of what it loaded itself (8 lanes a row)
-  constexpr int PW = decltype(sw)::PW;
-  float sq[PW], wmx = 0.0f;
+  // the items' norms (with tmax): a tile's by the block of the row tile that its number falls to, the
+  // blocks of 16 items shared out among the waves that hold them.  A lane has a quarter of an item's
+  // elements; the largest quarters of any items, added at the end, exceed no norm by much.  (1 x 1M x
+  // 384: the same from reads of their own from LDS took 214 us a call instead of 172.)  The 256 tile has
+  // no registers for holding on to the fragments: there every wave reads what it loaded once more (8
+  // lanes a row).
+  constexpr bool OWN_READ = NB == 8;
+  constexpr int JP = OWN_READ ? decltype(sw)::PW : FJ / TL::ROW_WV;
+  float sq[JP], wmx = 0.0f;
 #pragma unroll
   for (int i = 0; i < FI; ++i) {
     m[i] = CT_NONE;
@@ -348,16 +353,16 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const bool nrm = !COEF && a.tmax && vt % a.n_tiles == tn;
 #pragma unroll
-    for (int j = 0; j < PW; ++j) sq[j] = 0.0f;
+    for (int j = 0; j < JP; ++j) sq[j] = 0.0f;
     for (int kt = 0; kt < nk; ++kt, ++gs) {
       ct_wait_vm<0>();
       ct_barrier();  // stage gs complete; every wave is done with the slot refilled next
       issue_next();
       const char* st = smem + (gs & 1) * 2 * TL::OP_B;
-      if constexpr (!COEF) {
+      if constexpr (!COEF && OWN_READ) {
         if (nrm) {
 #pragma unroll
-          for (int j = 0; j < PW; ++j)
+          for (int j = 0; j < JP; ++j)
             sq[j] = sumsq16<T>(*(const u32x4_t*)(st + 1024 * (w + TL::NWV * j) + 16 * lane), sq[j]);
         }
       }
@@ -365,16 +370,28 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       row_frags(st, 16 * FJ * wv, lane, fw);
       row_frags(st + TL::OP_B, nw, lane, fx);
       ct_stage<T>(fw, fx, acc);
+      if constexpr (!COEF && !OWN_READ) {
+        if (nrm) {
+#pragma unroll
+          for (int q = 0; q < TL::ROW_WV; ++q)
+            if (wn == q) {
+#pragma unroll
+              for (int j = 0; j < JP; ++j) sq[j] = sumsq16<T>(fw[1][q * JP + j], sumsq16<T>(fw[0][q * JP + j], sq[j]));
+            }
+        }
+      }
     }
     if constexpr (!COEF) {
       if (nrm) {
 #pragma unroll
-        for (int j = 0; j < PW; ++j) {
-          float t = sq[j];
+        for (int j = 0; j < JP; ++j) {
+          if constexpr (OWN_READ) {
 #pragma unroll
-          for (int o = 1; o < 8; o <<= 1) t += __shfl_xor(t, o, 64);
-          const int v = a.v_base + vt * TL::EDGE + 8 * (w + TL::NWV * j) + (lane >> 3);
-          if (v < v_end && !(a.bias && a.bias[v] <= CT_OUT)) wmx = fmaxf(wmx, t);  // (a NaN: left out)
+            for (int o = 1; o < 8; o <<= 1) sq[j] += __shfl_xor(sq[j], o, 64);
+          }
+          const int v = a.v_base + vt * TL::EDGE +
+                        (OWN_READ ? 8 * (w + TL::NWV * j) + (lane >> 3) : 16 * (FJ * wv + wn * JP + j) + rl);
+          if (v < v_end && !(a.bias && a.bias[v] <= CT_OUT)) wmx = fmaxf(wmx, sq[j]);  // (a NaN: left out)
         }
       }
     }
@@ -517,14 +534,20 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       }
     }
     if (a.tmax) {
-      const float t = __uint_as_float(wave_max_u32(__float_as_uint(wmx)));
-      if (lane == 0) red[TL::EDGE * 3 + w] = t;
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) wmx = fmaxf(wmx, __shfl_xor(wmx, o, 64));
+      if (rl == 0) red[TL::EDGE * 3 + 4 * w + g] = wmx;
     }
     ct_barrier();
     if (a.tmax && tid == 0) {
-      float t = red[TL::EDGE * 3];
+      float t = 0.0f;
 #pragma unroll
-      for (int i = 1; i < TL::NWV; ++i) t = fmaxf(t, red[TL::EDGE * 3 + i]);
+      for (int q = 0; q < 4; ++q) {
+        float mq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TL::NWV; ++i) mq = fmaxf(mq, red[TL::EDGE * 3 + 4 * i + q]);
+        t = OWN_READ ? fmaxf(t, mq) : t + mq;  // (whole norms, or quarters)
+      }
       a.wsq[blockIdx.x] = t;
     }
     if (wv == 0 && g == 0) {
