@@ -691,7 +691,8 @@ int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_
  * g_entropy [N] (either may be NULL), with the forward's lse and entropy.  A row whose gradients
  * are 0 adds nothing, whatever its vector holds; taken-out items and empty rows get 0.
  * E a multiple of 64; rows 16-byte aligned; N < 2^24, V < 2^30; temperature >= 1e-30.  Sums in f32;
- * log_prob and entropy with the given item's logit in 64 bits throughout, lse (what _bwd takes its
+ * log_prob and top_log_prob (one item's two values are the same) and entropy with the item's own logit in
+ * 64 bits, also in the sum where it holds over a sixteenth of the probability; lse (what _bwd takes its
  * probabilities against) with the 32-bit one.  The coefficients of the gradient products are in dtype
  * (bf16 with N <= 64: in two parts).  The results do not depend on timing (no float atomics).
  * --------------------------------------------------------------------------------- */

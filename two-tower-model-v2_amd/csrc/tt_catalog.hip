@@ -869,16 +869,16 @@ __device__ __forceinline__ double wave_dot64(const T* x, const T* w, int E, int 
 }
 
 // x . w as k_logits and k_ring form it, to the bit: the same instructions in the same order (every
-// row and column of the block is the same)
-template <typename T>
+// row and column of the block is the same); Q stages' loads on their way
+template <typename T, int Q>
 __device__ __forceinline__ float mfma_dot(const T* x, const T* w, int E, int lane) {
   const int g = lane >> 4;
   f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
   constexpr int BK = 128 / (int)sizeof(T), PC = 16 / (int)sizeof(T);
-  for (int k0 = 0; k0 < E; k0 += 4 * BK) {  // 4 stages' loads on their way
-    u32x4_t fw[4][2][1], fx[4][2][1];
+  for (int k0 = 0; k0 < E; k0 += Q * BK) {
+    u32x4_t fw[Q][2][1], fx[Q][2][1];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < Q; ++q)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int k = (k0 + q * BK < E ? k0 + q * BK : k0) + PC * (4 * s + g);
@@ -886,7 +886,7 @@ __device__ __forceinline__ float mfma_dot(const T* x, const T* w, int E, int lan
         fx[q][s][0] = *(const u32x4_t*)(x + k);
       }
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < Q; ++q)
       if (k0 + q * BK < E) ct_stage<T>(fw[q], fx[q], acc);
   }
   return acc[0][0][0];
@@ -894,10 +894,12 @@ __device__ __forceinline__ float mfma_dot(const T* x, const T* w, int E, int lan
 // What the statistics' sums change by when one item's logit z (as they have it) is put right: dz =
 // exact - z, in powers of two, d = z - m.  log p of an item that has nearly all the probability is a
 // difference of two logits that both hold its own: they have to be the same one (4 x 50 x 768, p next to
-// 1: log p 2.9e-5 -> 1.1e-6 of itself off; 3 - 7 us of latency a call).
+// 1: log p 2.9e-5 -> 1.1e-6 of itself off; 3 - 7 us of latency a call).  Below a sixteenth of the probability
+// it is left out: the other items' logits are off by as much, with fifteen times its weight.
 __device__ __forceinline__ void put_right(double dz, double d, double& L, double& TT) {
-  if (!(fabs(dz) < 0.125) || !(d > -1000.0)) return;  // (not finite, or without weight)
-  const double e = exp2(d), q = e * expm1(dz * 0.6931471805599453);
+  const double e = exp2(d);
+  if (!(fabs(dz) < 0.125) || !(16.0 * e > L)) return;  // (not finite, or of little weight)
+  const double q = e * expm1(dz * 0.6931471805599453);
   TT += q * (d + dz) + e * dz;
   L += q;
 }
@@ -930,7 +932,17 @@ struct CombineArgs {
   const float* wsq;  // with alternatives: [n_wsq] of the statistics' blocks
   int n_wsq;
   float* err;        // [N] logit_error
+  float2* stat;      // [N] m, L
 };
+// An item's logit as the statistics have it, from its product in 32 bits.
+__device__ __forceinline__ double stat_logit(float dot32, float s2, bool bias, float b, int v, int group, int V) {
+  const bool own = bias || (v / group + 1) * group > V;
+  return own ? (double)fmaf(dot32, s2, b * CT_LOG2E) : (double)dot32 * (double)s2;
+}
+// log p = l - lse (natural; m and log2 of the sum in powers of two)
+__device__ __forceinline__ float log_p(double l, double m, double l2) {
+  return at_most_0((float)(l - (m + l2) * 0.6931471805599453));
+}
 // One wave per row: the shares' statistics joined, the given item's logit.
 template <typename T>
 __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int lane) {
@@ -948,7 +960,7 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   const bool has = id >= 0 && id < V;
   const float b = has && bias ? bias[id] : 0.0f;
   const double dot = has ? wave_dot64(x + n * ldx, w + id * ldw, E, lane) : 0.0;
-  const float dot32 = has ? mfma_dot(x + n * ldx, w + id * ldw, E, lane) : 0.0f;
+  const float dot32 = has ? mfma_dot<T, 4>(x + n * ldx, w + id * ldw, E, lane) : 0.0f;
   for (int i0 = lane; i0 < splits; i0 += 256) {  // 4 loads on their way
     float4 p[4];
 #pragma unroll
@@ -972,7 +984,10 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
       xsq += __shfl_xor(xsq, o, 64);
       wsq = fmaxf(wsq, __shfl_xor(wsq, o, 64));
     }
-    if (lane == 0) a.err[n] = logit_error(a.s2, E, xsq, wsq);
+    if (lane == 0) {
+      a.err[n] = logit_error(a.s2, E, xsq, wsq);
+      a.stat[n] = float2{m, L};
+    }
   }
   const float inf = __builtin_huge_valf();
   const bool empty = m <= CT_OUT && L == L;  // every item taken out (and no NaN)
@@ -980,14 +995,13 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   const double l = s * dot + (double)b;
   double L2 = (double)L, T2 = (double)TT;
   if (has && !(b <= CT_OUT)) {
-    const bool own = bias || ((int)id / a.group + 1) * a.group > V;
-    const double z = own ? (double)fmaf(dot32, a.s2, b * CT_LOG2E) : (double)dot32 * (double)a.s2;
+    const double z = stat_logit(dot32, a.s2, bias != nullptr, b, (int)id, a.group, V);
     put_right(l * 1.4426950408889634 - z, z - (double)m, L2, T2);
   }
   const double l2 = log2(L2);
   if (logp) {
     const float o = !has ? 0.0f : empty || b <= CT_OUT ? -inf
-                    : at_most_0((float)(l - ((double)m + l2) * 0.6931471805599453));
+                    : log_p(l, (double)m, l2);
     if (lane == 0) logp[n] = o;
   }
   if (lane == 0) {
@@ -1169,7 +1183,10 @@ struct TopArgs {
   int N, E, V;
   const float* bias;
   double s;
-  const float *lse, *err;
+  float s2;
+  int group;  // as in CombineArgs
+  const float* err;
+  const float2* stat;
   int64_t* ids_out;
   float* lp_out;
   // the second search
@@ -1255,12 +1272,27 @@ __device__ __forceinline__ void top_rank(TopList& o, int top) {
     }
   }
 }
+// A wave an alternative: the value that log_prob has for it, its own part of the sums put right too.
+template <typename T, int NT>
 __device__ __forceinline__ void top_write(const TopArgs& a, const TopList& o, int64_t n) {
-  const int i = threadIdx.x;
-  if (i >= a.top) return;
-  const double l = o.bl[i];
-  a.ids_out[n * a.top + i] = o.bv[i];
-  a.lp_out[n * a.top + i] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : at_most_0((float)(l - (double)a.lse[n]));
+  const int lane = threadIdx.x & 63;
+  const float2 st = a.stat[n];
+  const double m = (double)st.x, l20 = log2((double)st.y);
+  for (int i = threadIdx.x >> 6; i < a.top; i += NT / 64) {
+    const double l = o.bl[i];
+    const int v = __builtin_amdgcn_readfirstlane(o.bv[i]);
+    double L2 = (double)st.y, T2 = 0.0, l2 = l20;
+    if (l * 1.4426950408889634 - m > l20 - 4.25) {  // (else put_right leaves it)
+      const float dot32 = mfma_dot<T, 1>((const T*)a.x + n * a.ldx, (const T*)a.w + (int64_t)v * a.ldw, a.E, lane);
+      const double z = stat_logit(dot32, a.s2, a.bias != nullptr, a.bias ? a.bias[v] : 0.0f, v, a.group, a.V);
+      put_right(l * 1.4426950408889634 - z, z - m, L2, T2);
+      l2 = log2(L2);
+    }
+    if (lane == 0) {
+      a.ids_out[n * a.top + i] = v;
+      a.lp_out[n * a.top + i] = l == -__builtin_huge_val() ? -__builtin_huge_valf() : log_p(l, m, l2);
+    }
+  }
 }
 
 // One block per row: the keep largest groups of all segments, their items scored in 64 bits, the top of
@@ -1341,7 +1373,7 @@ __global__ __launch_bounds__(NT) void k_top_items(const TopArgs a) {
   }
   top_rank<NT>(o, top);
   __syncthreads();
-  top_write(a, o, n);
+  top_write<T, NT>(a, o, n);
   if (a.state && tid == 0) {
     a.floor[n] = s_floor;
     a.state[n] = more ? 0u : CT_DONE;
@@ -1417,7 +1449,7 @@ __global__ __launch_bounds__(256) void k_top_wide(const TopArgs a) {
           }
         carry();
       }
-      if (o.n == top) top_write(a, o, n);  // (always: the floor has at least top items above it)
+      if (o.n == top) top_write<T, 256>(a, o, n);  // (always: the floor has at least top items above it)
       __syncthreads();
     }
   }
@@ -1651,7 +1683,7 @@ static void logits_shape(int64_t N, int64_t V, int edge, int& n_tiles, int& v_ti
 struct StatPlan {
   bool ring;
   int edge, n_tiles, v_tiles, splits, keep, nseg, seg_len;
-  int64_t M, off_tmax, off_seg, off_wsq, off_err, off_floor, off_state, off_found, bytes;
+  int64_t M, off_tmax, off_seg, off_wsq, off_err, off_stat, off_floor, off_state, off_found, bytes;
 };
 // Shares: about 512 blocks (two a CU; three of the small tiles).
 static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
@@ -1674,7 +1706,8 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
     p.off_seg = p.off_tmax + up(N * p.M * 4, 256);
     p.off_wsq = p.off_seg + up(N * p.nseg * p.keep * 8, 256);
     p.off_err = p.off_wsq + up((int64_t)p.n_tiles * p.splits * 4, 256);
-    p.off_floor = p.off_err + up(N * 4, 256);
+    p.off_stat = p.off_err + up(N * 4, 256);
+    p.off_floor = p.off_stat + up(N * 8, 256);
     p.off_state = p.off_floor + up(N * 4, 256);
     p.off_found = p.off_state + up(N * 4, 256);
     p.bytes = p.off_found + up(p.M > p.keep ? N * p.nseg * top * 16 : 0, 256);
@@ -1830,7 +1863,7 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   else logits_launch<T, false>(a, p.edge, ent != nullptr, st);
   const CombineArgs ca{a.part, p.splits, (int)N, (int)V, E, x, w, ldx, ldw, ids, bias, s, a.s2,
                        p.ring || p.edge == 64 ? 32 : 64, logp, ent, lse, a.wsq, p.n_tiles * p.splits,
-                       top ? (float*)(ws + p.off_err) : nullptr};
+                       top ? (float*)(ws + p.off_err) : nullptr, top ? (float2*)(ws + p.off_stat) : nullptr};
   const unsigned cb = (unsigned)cdiv(N, 4);
   if (top) {
     uint64_t* seg = (uint64_t*)(ws + p.off_seg);
@@ -1840,7 +1873,7 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     TopArgs ta{};
     ta.segs = seg; ta.nseg = p.nseg; ta.keep = p.keep; ta.top = top;
     ta.x = x; ta.w = w; ta.ldx = ldx; ta.ldw = ldw; ta.N = (int)N; ta.E = E; ta.V = (int)V;
-    ta.bias = bias; ta.s = s; ta.lse = lse; ta.err = ca.err; ta.ids_out = top_ids; ta.lp_out = top_lp;
+    ta.bias = bias; ta.s = s; ta.s2 = a.s2; ta.group = ca.group; ta.err = ca.err; ta.stat = ca.stat; ta.ids_out = top_ids; ta.lp_out = top_lp;
     const bool wide = p.M > p.keep;  // (else no group is left out)
     if (wide) {
       ta.tmax = a.tmax; ta.M = p.M; ta.seg_len = p.seg_len;
