@@ -689,7 +689,8 @@ int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_
  * A row with every item taken out: lse -inf, entropy 0, log_prob -inf (0 without an id).
  * _bwd: dx [N, E], dw [V, E] of dtype, contiguous (either may be NULL), for gradients g_log_prob and
  * g_entropy [N] (either may be NULL), with the forward's lse and entropy.  A row whose gradients
- * are 0 adds nothing, whatever its vector holds; taken-out items and empty rows get 0.
+ * are 0 adds nothing, whatever its vector holds; taken-out items and empty rows get 0.  A NaN in another
+ * row or item (or a logit past the range of f32) makes the gradients that it enters NaN.
  * E a multiple of 64; rows 16-byte aligned; N < 2^24, V < 2^30; temperature >= 1e-30.  Sums in f32;
  * log_prob and top_log_prob (one item's two values are the same) and entropy with the item's own logit in
  * 64 bits, also in the sum where it holds over a sixteenth of the probability; lse (what _bwd takes its

@@ -39,7 +39,8 @@
 // coefficients 195 us and the products 152, 150 us per 21888 items, 0.71, 0.91, 0.92 PFLOP/s).
 //
 // Items with a bias at or below -1e30 (-inf, the type's lowest) are taken out: probability 0 and
-// gradient 0 whatever their vectors hold.  Rows whose gradients are both 0 do not reach dw.
+// gradient 0 whatever their vectors hold.  Rows whose gradients are both 0 do not reach dw.  A row whose
+// lse is no number (a NaN in it or in an item, a logit past the range) has gradients that are none.
 #include "tt_common.hpp"
 
 namespace tt {
@@ -261,7 +262,7 @@ struct LogitArgs {
   float4* part;        // STAT [splits, N] (m, L, T, -)
   float* tmax;         // STAT: [N, 4 ceil(V / 64)] or null
   float* wsq;          // STAT with tmax: [blocks] what no |w_v|^2 that the block looked at exceeds
-  const float4* rowc;  // COEF [N] (log2-domain lse, g, e, H)
+  const float4* rowc;  // COEF [N] (log2-domain lse, g, e, H); g and e both 0: the row is dead
   const int64_t* ids;  // COEF
   void* C;             // COEF [Npad, ldc]: items v_base .. of this chunk
   int64_t ldc;
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
               if constexpr (ENT) TT[i] = fmaf(e, d, TT[i]);
             }
         } else {
-          const bool live = rc[i].x < 1.0e30f;
+          const bool live = rc[i].y != 0.0f || rc[i].z != 0.0f;  // (a lse that is no number: NaN)
           const bool two = NB <= 4 && sizeof(T) == 2 && a.two;
           const bool store = n < (two ? a.N : a.Npad) && c0 < a.ldc;
           T* o = (T*)a.C + (int64_t)n * a.ldc + c0;
@@ -729,7 +730,7 @@ __global__ __launch_bounds__(CR_NT, 2) void k_ring(const LogitArgs a) {
       }
     } else {
       const int n = nb + 16 * q + rl, vi = a.v_base + 32 * t + 16 * rb + 4 * g;
-      const bool live = rc[q].x < 1.0e30f;
+      const bool live = rc[q].y != 0.0f || rc[q].z != 0.0f;
       f32x4 c;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
