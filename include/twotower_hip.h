@@ -694,8 +694,8 @@ int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_
  * E a multiple of 64; rows 16-byte aligned; N < 2^24, V < 2^30; temperature >= 1e-30.  Sums in f32;
  * log_prob and top_log_prob (one item's two values are the same) and entropy with the item's own logit in
  * 64 bits, also in the sum where it holds over a sixteenth of the probability; lse (what _bwd takes its
- * probabilities against) with the 32-bit one.  The coefficients of the gradient products are in dtype
- * (bf16 with N <= 64: in two parts).  The results do not depend on timing (no float atomics).
+ * probabilities against) with the 32-bit one.  The coefficients of the gradient products are in dtype;
+ * in bf16 the given items' in two parts, with N <= 64 all.  The results do not depend on timing (no float atomics).
  * --------------------------------------------------------------------------------- */
 int tt_catalog_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t E, int32_t dtype, int32_t top,
                                         int64_t* bytes);

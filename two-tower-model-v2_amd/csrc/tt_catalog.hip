@@ -25,9 +25,11 @@
 //     its groups that do (k_top_wide).
 // k_logits<COEF>  the same product again, its epilogue writing C for a chunk of the catalog, in x's type:
 //     the products take it as an operand of their matrix instructions.  In bf16 a coefficient is then off
-//     by up to 2^-8 of itself, which makes 2.0e-3 of the gradients of 4096 rows (their own rounding
-//     1.7e-3); up to 64 rows, where one coefficient may be all of a sum (2.8e-3 at 7 rows), it is kept in
-//     two parts.
+//     by up to 2^-8 of itself.  The given item's, which is most of its row's gradient, keeps what the
+//     rounding left (k_lost), and the products begin with that: the gradients of 4096 x 32768 x 768 are
+//     1.66e-3 off, their own rounding (2.02e-3 without; 3 in 100 of the call).  The others' roundings
+//     are many and small.  Up to 64 rows, where any coefficient may be all of a sum, all are kept in two
+//     parts.
 // k_product       dx += C w (C rows, w as it lies) and dw = C^T x: operands whose rows run along the
 //     sum are read from LDS transposed (ds_read_b64_tr_b16; 4-byte reads in f32), so neither C nor
 //     w nor x is ever stored transposed.  What the output's tiles leave of the last round of blocks is
@@ -269,6 +271,8 @@ struct LogitArgs {
   int v_base, v_count, Npad;  // v_count: items from v_base on
   bool two;            // COEF in bf16: row n + N of C takes what the rounding of row n leaves
 };
+// what the rounding of c to bf16 leaves
+__device__ __forceinline__ float ct_lost(float c) { return c - __uint_as_float(ct_pack2(c, 0.0f) << 16); }
 
 // A tile of 32 NB rows x 32 NB items: 4 waves of 16 NB x 16 NB, or (NB = 8, bf16) 8 waves of 64 rows x
 // 128 items: half the loads per product, and 3/8 of a fragment read from LDS per matrix instruction
@@ -496,7 +500,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
               for (int j = 0; j < HJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                  c[j][r] -= __uint_as_float(ct_pack2(c[j][r], 0.0f) << 16);
+                  c[j][r] = ct_lost(c[j][r]);
               put(o + (int64_t)a.N * a.ldc, n + a.N < a.Npad && c0 < a.ldc);
             }
           }
@@ -1495,6 +1499,29 @@ __global__ __launch_bounds__(256) void k_items(const T* __restrict__ w, int64_t 
   }
 }
 
+// What the rounding of the given items' coefficients to bf16 left of them (the items of this chunk of C):
+// the coefficient once more, in f32, from the same 32-bit logit that the row's lse holds, less what C has.
+// A wave a row.
+__global__ __launch_bounds__(256) void k_lost(const LogitArgs a, float* __restrict__ delta) {
+  const int lane = threadIdx.x & 63;
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= a.N) return;
+  const int64_t id = a.ids[n];
+  if (id < a.v_base || id >= a.v_base + a.v_count) return;  // (read by the products for this chunk's items alone)
+  const float4 rc = a.rowc[n];
+  const float b = a.bias ? a.bias[id] : 0.0f;
+  float d = 0.0f;
+  if (rc.y != 0.0f && !(b <= CT_OUT)) {
+    const float z = mfma_dot<uint16_t, 4>((const uint16_t*)a.x + (int64_t)n * a.ldx,
+                                          (const uint16_t*)a.w + id * a.ldw, a.E, lane);
+    const float lp = a.bias ? fmaf(z, a.s2, b * CT_LOG2E) - rc.x : fmaf(z, a.s2, -rc.x);
+    const float k = rc.z != 0.0f ? fmaf(rc.z, fmaf(lp, CT_LN2, rc.w), rc.y) : rc.y;
+    const float c = fmaf(-__builtin_amdgcn_exp2f(lp), k, rc.y);
+    d = c - __uint_as_float((uint32_t)((const uint16_t*)a.C)[(int64_t)n * a.ldc + (id - a.v_base)] << 16);
+  }
+  if (lane == 0) delta[n] = d;
+}
+
 // out[m][c] = scale sum_k A[m, k] B[k, c]; B [K rows, cols] as it lies; A rows [m][k] (ACOL false) or
 // as it lies [k][m] (ACOL).  K a multiple of BK (rows past a's or b's end are zero in A).  splits > 1
 // or acc: f32 partial sums part[split][M][cols] (acc: added to what is there), else out.
@@ -1508,7 +1535,19 @@ struct ProductArgs {
   void* out;
   int64_t ldo;
   float* part;        // [block from the first that writes here, tile edge^2]
+  // bf16, or null: what the given items' coefficients of A lost by their rounding ([rows], items ids),
+  // v_base the first item of A; the sums begin with it
+  const float* delta;
+  const int64_t* ids;
+  int v_base;
 };
+__device__ __forceinline__ f32x4 ct_floats(const ct_u32x2& u) {  // 4 bf16 elements
+  return f32x4{__uint_as_float(u[0] << 16), __uint_as_float(u[0] & 0xffff0000u), __uint_as_float(u[1] << 16),
+               __uint_as_float(u[1] & 0xffff0000u)};
+}
+__device__ __forceinline__ f32x4 ct_fma4(float d, const f32x4& x, const f32x4& acc) {
+  return f32x4{fmaf(d, x[0], acc[0]), fmaf(d, x[1], acc[1]), fmaf(d, x[2], acc[2]), fmaf(d, x[3], acc[3])};
+}
 template <typename T, bool ACOL, int NB>
 __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(const ProductArgs a) {
   using TL = Tile<NB>;
@@ -1518,6 +1557,10 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(cons
   // tiles end in long vector work that both should do at once, lost by it: 465 -> 524)
   constexpr bool TURNS = NB == 8;
   __shared__ __attribute__((aligned(16))) char smem[4 * TL::OP_B];
+  constexpr int FOUND = 256 * TL::NWV;  // (dw in bf16) rows that are looked at together for the tile's items
+  __shared__ __attribute__((aligned(16))) uint32_t found[ACOL && sizeof(T) == 2 ? FOUND : 1];  // row << 8 | item
+  __shared__ float lost[ACOL && sizeof(T) == 2 ? FOUND : 1];
+  __shared__ int n_found[TL::NWV];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w % TL::ROW_WV, wc = w / TL::ROW_WV, g = lane >> 4, rl = lane & 15;
@@ -1561,6 +1604,95 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(cons
   };
   const int late = TURNS ? w >> 2 : 0;
   if (k0 < k1) issue(k0);
+  if constexpr (sizeof(T) == 2) {
+    if (a.delta) {
+      // (before the loop, whose registers are not taken yet; after it the 256 tile would spill.)  The
+      // block's part of the sum runs over [kb, ke): items (dx), rows (dw)
+      const int64_t kb = (int64_t)k0 * BK, ke = (int64_t)k1 * BK < a.b_rows ? (int64_t)k1 * BK : a.b_rows;
+      const int cb = c0 + 16 * FJ * wc + 4 * g, cl = a.cols - 4;  // (columns past the end: loaded again)
+      if constexpr (!ACOL) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i) {
+          const int n = m0 + 16 * FI * wm + 16 * i + rl;
+          const int64_t k = n < a.M ? a.ids[n] - a.v_base : -1;
+          if (k >= kb && k < ke) {
+            const float d = a.delta[n];
+            if (d != 0.0f) {
+#pragma unroll
+              for (int j = 0; j < FJ; ++j) {
+                const int c = cb + 16 * j < cl ? cb + 16 * j : cl;
+                acc[i][j] = ct_fma4(d, ct_floats(*(const ct_u32x2*)(B + k * a.ldb + c)), acc[i][j]);
+              }
+            }
+          }
+        }
+      } else {
+        // the rows whose item is one of the tile's, FOUND rows looked at at a time (256 a wave), listed in
+        // their order (the sums do not depend on timing) and multiplied 32 at a time: 4096 rows, 65537
+        // items: 16 a tile, 6 us; a popular item costs 0.1 us a row
+        for (int64_t s0 = kb; s0 < ke; s0 += FOUND) {
+          const int64_t n0 = s0 + (FOUND / TL::NWV) * w;
+          int q[FOUND / TL::NT], np = 0;
+#pragma unroll
+          for (int u = 0; u < FOUND / TL::NT; ++u) {
+            const int64_t n = n0 + 64 * u + lane, v = n < ke ? a.ids[n] - a.v_base - m0 : -1;
+            q[u] = v >= 0 && v < EDGE ? (int)v : -1;
+            np += __popcll(__ballot(q[u] >= 0));
+          }
+          if (lane == 0) n_found[w] = np;
+          __syncthreads();
+          int at = 0, total = 0;
+#pragma unroll
+          for (int i = 0; i < TL::NWV; ++i) {
+            at += i < w ? n_found[i] : 0;
+            total += n_found[i];
+          }
+#pragma unroll
+          for (int u = 0; u < FOUND / TL::NT; ++u) {
+            const uint64_t bm = __ballot(q[u] >= 0);
+            if (q[u] >= 0) {
+              const int k = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(bm >> 32),
+                                                                __builtin_amdgcn_mbcnt_lo((uint32_t)bm, 0u));
+              found[k] = (uint32_t)(n0 - s0 + 64 * u + lane) << 8 | (uint32_t)q[u];
+              lost[k] = a.delta[n0 + 64 * u + lane];
+            }
+            at += __popcll(bm);
+          }
+          __syncthreads();
+          for (int p = 0; p < total; p += 32) {
+            uint32_t e[8];
+            float d[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int o = p + 8 * g + k, in = o < total ? o : p;
+              e[k] = found[in];
+              d[k] = o < total ? lost[in] : 0.0f;
+            }
+            u32x4_t fa[1][FI], fb[1][FJ];
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) {
+              const int c = c0 + 16 * (FJ * wc + j) + rl;
+              const uint16_t* xc = B + s0 * a.ldb + (c < a.cols ? c : 0);  // (columns past the end are not stored)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                fb[0][j][k] = (uint32_t)xc[(int64_t)(e[2 * k] >> 8) * a.ldb] |
+                              (uint32_t)xc[(int64_t)(e[2 * k + 1] >> 8) * a.ldb] << 16;
+            }
+#pragma unroll
+            for (int i = 0; i < FI; ++i) {
+              const uint32_t r = (uint32_t)(16 * (FI * wm + i) + rl);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                fa[0][i][k] = ct_pack2((e[2 * k] & 255u) == r ? d[2 * k] : 0.0f,
+                                       (e[2 * k + 1] & 255u) == r ? d[2 * k + 1] : 0.0f);
+            }
+            ct_mfma<T>(fb, fa, acc);
+          }
+          __syncthreads();
+        }
+      }
+    }
+  }
   if constexpr (TURNS) {
     ct_wait_vm<0>();
     ct_turn();
@@ -1753,7 +1885,7 @@ static ProductPlan product_plan(int64_t M, int64_t cols, int64_t K, int64_t sz, 
   return b;
 }
 struct BwdPlan {
-  int64_t Npad, Vc, n_chunks, off_x, off_w, off_c, off_px, off_pw, bytes;
+  int64_t Npad, Vc, n_chunks, off_x, off_d, off_w, off_c, off_px, off_pw, bytes;
   bool two;  // C in two bf16 rows a row
   ProductPlan px, pw, pw_last;  // dx; dw of a chunk, of the last chunk
 };
@@ -1770,6 +1902,8 @@ static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, 
   int64_t o = up(N * 16, 256);
   p.off_x = o;
   o += up((p.two ? 2 * N : N) * E * sz, 256);
+  p.off_d = o;
+  if (sz == 2 && !p.two) o += up(N * 4, 256);
   p.off_w = o;
   if (bias) o += up(V * E * sz, 256);
   p.off_c = o;
@@ -1902,6 +2036,7 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   const double s = 1.0 / (double)temperature;
   float4* rowc = (float4*)ws;
   T* xz = (T*)(ws + p.off_x);
+  float* delta = sizeof(T) == 2 && !p.two && ids && g ? (float*)(ws + p.off_d) : nullptr;
   hipLaunchKernelGGL(k_rows<T>, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, st, (const T*)x, ldx, (int)N, E, lse,
                      ent, g, e, ids, (int)V, rowc, xz, p.two);
   const T* wz = (const T*)w;
@@ -1933,6 +2068,9 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       logits_shape(p.two ? p.Npad - N : N, vn, edge, a.n_tiles, a.v_tiles, a.splits);
       logits_launch<T, true>(a, edge, e != nullptr, st);
     }
+    if constexpr (sizeof(T) == 2) {
+      if (delta) hipLaunchKernelGGL(k_lost, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, st, a, delta);
+    }
     const int64_t vk = up(vn, 64);
     if (dx) {
       qx.A = C; qx.lda = p.Vc; qx.a_rows = p.Npad;
@@ -1941,6 +2079,7 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       qx.all = p.n_chunks > 1 || p.two; qx.acc = c > 0;
       qx.scale = (float)s; qx.out = dx; qx.ldo = E;
       qx.part = px;
+      qx.delta = delta; qx.ids = ids; qx.v_base = (int)vb;
       product_launch<T, false>(qx, p.px, st);
       if (p.two) {
         qx.A = C + N * p.Vc; qx.a_rows = p.Npad - N;
@@ -1955,6 +2094,7 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
       q.M = (int)vn; q.cols = E; q.K = (int)p.Npad;
       q.scale = (float)s; q.out = (T*)dw + vb * E; q.ldo = E;
       q.part = (float*)(ws + p.off_pw);
+      q.delta = delta; q.ids = ids; q.v_base = (int)vb;
       const ProductPlan& pw = c + 1 < p.n_chunks ? p.pw : p.pw_last;
       product_launch<T, true>(q, pw, st);
       product_sum<T>(q, pw, st);
