@@ -290,12 +290,13 @@ __device__ __forceinline__ void ct_turn() {  // a barrier that no matrix instruc
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <typename T, bool COEF, bool ENT, int NB>
+// (TOP: with the groups' maxima and the norms; without their registers and branches 457 us for 469)
+template <typename T, bool COEF, bool ENT, int NB, bool TOP>
 __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const LogitArgs a) {
   using TL = Tile<NB>;
   constexpr int BK = 128 / (int)sizeof(T), FI = TL::FI, FJ = TL::FJ, HJ = FJ < 4 ? FJ : 4;
   __shared__ __attribute__((aligned(16))) char smem[4 * TL::OP_B];
-  __shared__ float half[NB == 2 && !COEF ? TL::EDGE : 1][4];
+  __shared__ float half[NB == 2 && TOP ? TL::EDGE : 1][4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = w % TL::ROW_WV, wv = w / TL::ROW_WV, g = lane >> 4, rl = lane & 15;
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
     for (int i = 0; i < FI; ++i)
 #pragma unroll
       for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const bool nrm = !COEF && a.tmax && vt % a.n_tiles == tn;
+    const bool nrm = TOP && vt % a.n_tiles == tn;
 #pragma unroll
     for (int j = 0; j < JP; ++j) sq[j] = 0.0f;
     for (int kt = 0; kt < nk; ++kt, ++gs) {
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       ct_barrier();  // stage gs complete; every wave is done with the slot refilled next
       issue_next();
       const char* st = smem + (gs & 1) * 2 * TL::OP_B;
-      if constexpr (!COEF && OWN_READ) {
+      if constexpr (TOP && OWN_READ) {
         if (nrm) {
 #pragma unroll
           for (int j = 0; j < JP; ++j)
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       row_frags(st, 16 * FJ * wv, lane, fw);
       row_frags(st + TL::OP_B, nw, lane, fx);
       ct_stage<T>(fw, fx, acc);
-      if constexpr (!COEF && !OWN_READ) {
+      if constexpr (TOP && !OWN_READ) {
         if (nrm) {
 #pragma unroll
           for (int q = 0; q < TL::ROW_WV; ++q)
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
         }
       }
     }
-    if constexpr (!COEF) {
+    if constexpr (TOP) {
       if (nrm) {
 #pragma unroll
         for (int j = 0; j < JP; ++j) {
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
           for (int j = 1; j < HJ; ++j)
             mx = fmaxf(fmaxf(fmaxf(z[j][0], z[j][1]), fmaxf(z[j][2], z[j][3])), mx);
           const float tm = fmaxf(mx * s2, CT_OUT);
-          if (a.tmax) {
+          if constexpr (TOP) {
             if constexpr (NB >= 4) {
               if (n < a.N && v0 < v_end)
                 a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] = tm;
@@ -506,16 +507,14 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
           }
         }
       }
-      if constexpr (!COEF && NB == 2) {
-        if (a.tmax) {
-          ct_barrier();
-          if (wv == 0) {
+      if constexpr (TOP && NB == 2) {
+        ct_barrier();
+        if (wv == 0) {
 #pragma unroll
-            for (int i = 0; i < FI; ++i) {
-              const int n = n0 + 16 * i + rl;
-              if (n < a.N) a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] =
-                               fmaxf(tmx[i], half[nw + 16 * i + rl][g]);
-            }
+          for (int i = 0; i < FI; ++i) {
+            const int n = n0 + 16 * i + rl;
+            if (n < a.N) a.tmax[(int64_t)n * (4 * (((int64_t)a.V + 63) / 64)) + (v0 >> 6) * 4 + g] =
+                             fmaxf(tmx[i], half[nw + 16 * i + rl][g]);
           }
         }
       }
@@ -538,13 +537,13 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
         r[2] = TT[i];
       }
     }
-    if (a.tmax) {
+    if constexpr (TOP) {
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) wmx = fmaxf(wmx, __shfl_xor(wmx, o, 64));
       if (rl == 0) red[TL::EDGE * 3 + 4 * w + g] = wmx;
     }
     ct_barrier();
-    if (a.tmax && tid == 0) {
+    if (TOP && tid == 0) {
       float t = 0.0f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -1945,23 +1944,26 @@ static void product_sum(const ProductArgs& q, const ProductPlan& p, hipStream_t 
   const dim3 grid((unsigned)(p.edge * p.edge / 1024 * tiles));
   hipLaunchKernelGGL(k_product_sum<T>, grid, dim3(256), 0, st, q, p.edge);
 }
-template <typename T, bool COEF>
-static void logits_launch(const LogitArgs& a, int edge, bool ent, hipStream_t st) {
-  const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits));
-  if constexpr (sizeof(T) == 2) {
-    if (edge == 256) {
-      if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, 8>), grid, dim3(512), 0, st, a);
-      else hipLaunchKernelGGL((k_logits<T, COEF, false, 8>), grid, dim3(512), 0, st, a);
+template <typename T, bool COEF, int NB>
+static void logits_go(const LogitArgs& a, bool ent, hipStream_t st) {
+  const dim3 grid((unsigned)(a.n_tiles * (int64_t)a.splits)), block(Tile<NB>::NT);
+  if constexpr (!COEF) {
+    if (a.tmax) {
+      if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, NB, true>), grid, block, 0, st, a);
+      else hipLaunchKernelGGL((k_logits<T, COEF, false, NB, true>), grid, block, 0, st, a);
       return;
     }
   }
-  if (edge == 64) {
-    if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_logits<T, COEF, false, 2>), grid, dim3(256), 0, st, a);
-  } else {
-    if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, 4>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_logits<T, COEF, false, 4>), grid, dim3(256), 0, st, a);
+  if (ent) hipLaunchKernelGGL((k_logits<T, COEF, true, NB, false>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((k_logits<T, COEF, false, NB, false>), grid, block, 0, st, a);
+}
+template <typename T, bool COEF>
+static void logits_launch(const LogitArgs& a, int edge, bool ent, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (edge == 256) return logits_go<T, COEF, 8>(a, ent, st);
   }
+  if (edge == 64) logits_go<T, COEF, 2>(a, ent, st);
+  else logits_go<T, COEF, 4>(a, ent, st);
 }
 
 static int ct_check(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype, int64_t N,
