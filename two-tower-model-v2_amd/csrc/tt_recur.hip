@@ -275,6 +275,7 @@ __device__ __forceinline__ void gates(const typename Pack<T, VEC>::type (&gp)[U]
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (w[j] == 1.0f || !(w[j] > 0.0f)) continue;
+      const float wj = fminf(w[j], 3.0e38f);  // an infinite weight: h becomes x (and w A is 0, no NaN)
       float sn[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sn[i] = na[j][i];
@@ -285,14 +286,14 @@ __device__ __forceinline__ void gates(const typename Pack<T, VEC>::type (&gp)[U]
         unpack<T, VEC>(gp[j], g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const Gate q = gate_pow(g[i], fminf(w[j], 3.0e38f));  // an infinite weight: h becomes x
+          const Gate q = gate_pow(g[i], wj);
           a[j][i] = q.a;
           na[j][i] = q.na;
         }
       }
       if (KQ) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) kq[j][i] = w[j] * a[j][i] * sn[i];
+        for (int i = 0; i < VEC; ++i) kq[j][i] = wj * a[j][i] * sn[i];
       }
     }
   }
