@@ -565,9 +565,9 @@ class TwoTowerTrainStep:
                         for o, (k, p) in zip(self.adamw.offsets, self.params.items())})
         return out
 
-    # torch.optim.Adam state dict (the reference saves optimizer.state_dict(), trainer.py:330):
-    # 'state' indexed by the position of the parameter in model.parameters(), 'param_groups'
-    # with Adam's defaults.  Parameters the fused step does not train (the frozen text
+    # torch.optim.Adam state dict (the reference saves optimizer.state_dict(), trainer.py:330), AdamW's
+    # with decay: 'state' indexed by the position of the parameter in model.parameters(),
+    # 'param_groups' with the defaults.  Parameters the fused step does not train (the frozen text
     # encoder) have no state entry, as under torch Adam when they never received a gradient.
     def optimizer_state_dict(self, model) -> Dict:
         pos = {p.data_ptr(): i for i, p in enumerate(model.parameters())}
@@ -581,7 +581,8 @@ class TwoTowerTrainStep:
         group = {"lr": self.lr, "betas": tuple(self.betas), "eps": self.eps,
                  "weight_decay": self.weight_decay or 0,
                  "amsgrad": False, "maximize": False, "foreach": None, "capturable": False,
-                 "differentiable": False, "fused": None, "decoupled_weight_decay": False,
+                 "differentiable": False, "fused": None,
+                 "decoupled_weight_decay": self.adamw is not None,
                  "params": list(range(len(pos)))}
         return {"state": state, "param_groups": [group]}
 
@@ -593,12 +594,23 @@ class TwoTowerTrainStep:
         indexes the SentenceTransformer's ~200 frozen parameters first (item_tower.py:38,
         trainer.py:49-50), so its indices do not line up here.  A state dict whose entries do
         not match the trained parameters' shapes, or none of whose entries lands on a trained
-        parameter, raises instead of silently leaving Adam at step 0."""
+        parameter, raises instead of silently leaving Adam at step 0.
+
+        The learning rate, betas, eps and weight decay become the saved ones.  The decay here is
+        decoupled: saved decay that is not marked so (torch.optim.Adam adds it to the gradient) is
+        refused, unless this step was built with the same."""
+        g = sd.get("param_groups", [{}])[0]
+        for key in ("amsgrad", "maximize"):
+            if g.get(key):
+                raise ValueError(f"the saved optimizer has {key}=True, which this step does not do")
+        wd = float(g.get("weight_decay", self.weight_decay))
+        if wd > 0 and not g.get("decoupled_weight_decay", False) and wd != self.weight_decay:
+            raise ValueError(f"the saved optimizer adds weight_decay={wd} to the gradient (it is not "
+                             "marked as decoupled), which this step does not do; if it is decoupled, "
+                             f"build the step with weight_decay={wd}")
         pos = {p.data_ptr(): i for i, p in enumerate(model.parameters())}
         st = sd["state"]
-        steps = set()
-        matched = 0
-        load = {}
+        found = {}
         for k, p in self.params.items():
             i = pos[p.data_ptr()]
             e = st.get(i)
@@ -611,22 +623,24 @@ class TwoTowerTrainStep:
                     f"needs {tuple(p.shape)}: the state dict indexes a different parameter "
                     "list (e.g. a reference checkpoint, whose frozen text-encoder parameters come "
                     "first)")
-            if self.adamw is None:
-                self.m[k].copy_(ea.view_as(self.m[k]))
-                self.v[k].copy_(es.view_as(self.v[k]))
-            else:
-                load[list(self.params).index(k)] = e
-            steps.add(int(float(e["step"])))
-            matched += 1
-        if st and matched == 0:
+            found[k] = e
+        if st and not found:
             raise ValueError("no optimizer state entry matches a trained parameter: the state dict "
                              "indexes a different parameter list")
+        steps = {int(float(e["step"])) for e in found.values()}
         if len(steps) > 1:
             raise ValueError(f"inconsistent Adam step counts in the state dict: {sorted(steps)}")
+        # nothing has changed up to here
+        self.weight_decay = wd
+        if wd > 0 and self.adamw is None:
+            self._flatten()  # the AdamW form's moments
         self.t = steps.pop() if steps else 0
         if self.adamw is not None:
-            self.adamw.load_state(load)
-        g = sd.get("param_groups", [{}])[0]
+            self.adamw.load_state({i: found[k] for i, k in enumerate(self.params) if k in found})
+        else:
+            for k, e in found.items():
+                self.m[k].copy_(torch.as_tensor(e["exp_avg"]).view_as(self.m[k]))
+                self.v[k].copy_(torch.as_tensor(e["exp_avg_sq"]).view_as(self.v[k]))
         self.lr = g.get("lr", self.lr)
         self.betas = tuple(g.get("betas", self.betas))
         self.eps = g.get("eps", self.eps)
