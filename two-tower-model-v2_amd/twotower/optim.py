@@ -19,6 +19,7 @@ from torch.optim.optimizer import _global_optimizer_pre_hooks as _pre_hooks
 from . import _lib
 from ._lib import check, lib, require_device, stream_ptr
 
+_increment_version = torch._C._increment_version  # torch.autograd.graph.increment_version of a list
 MAX_TENSORS = 416  # per launch (TT_ADAMW_MAX_TENSORS)
 _TENSOR = np.dtype([("p", "u8"), ("exp_avg", "u8"), ("exp_avg_sq", "u8"), ("scale_m", "u8"),
                     ("scale_v", "u8"), ("step", "u8"), ("ticket", "u8"), ("n", "i8"),
@@ -127,9 +128,9 @@ class MultiTensorAdamW:
         self.dtypes = [t.dtype for t in tensors]
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], lr: float, betas, eps: float,
-             weight_decay: float, first: int = 0) -> None:
+             weight_decay: float, first: int = 0) -> bool:
         """One step of tensors first .. first + len(grads) - 1 (the others stay); a gradient None
-        leaves its tensor and its step count as they are."""
+        leaves its tensor and its step count as they are.  True if all moved."""
         sizes, dtypes, dev = self.sizes, self.dtypes, self._dev_index
         with _lib.on_device(self._tab):
             keep = []
@@ -156,6 +157,7 @@ class MultiTensorAdamW:
                     self._tab.data_ptr(), self._items.data_ptr() + 8 * i0, i1 - i0, first + a,
                     (ctypes.c_void_p * len(part))(*part), len(part), self.chunk, self.bits, lr,
                     betas[0], betas[1], eps, weight_decay, st), "tt_adamw_step")
+        return None not in ptrs
 
     def moments(self, out=None):
         """(exp_avg, exp_avg_sq) of all tensors as f32 buffers, tensor i's at offsets[i]: the state
@@ -369,8 +371,10 @@ class AdamW(torch.optim.Optimizer):
                 t.bind([p.detach() for _, _, ps in spans for p in ps])  # a storage was replaced
             for gi, first, ps in spans:
                 g = self.param_groups[gi]
-                t.step([p.grad for p in ps], g["lr"], g["betas"], g["eps"], g["weight_decay"],
-                       first)
+                whole = t.step([p.grad for p in ps], g["lr"], g["betas"], g["eps"],
+                               g["weight_decay"], first)
+                # (written by their addresses: autograd refuses a backward pass over the old values)
+                _increment_version(ps if whole else [p for p in ps if p.grad is not None])
         return loss
 
     # ------------------------------------------------------------------ state
