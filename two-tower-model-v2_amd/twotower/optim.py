@@ -7,6 +7,7 @@ captured in a HIP graph advances on every replay (with the learning rate of the 
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 from itertools import chain
 from typing import Dict, List, Optional, Sequence
@@ -28,6 +29,26 @@ _TENSOR = np.dtype([("p", "u8"), ("exp_avg", "u8"), ("exp_avg_sq", "u8"), ("scal
 
 def _round_up(n: int, q: int) -> int:
     return (n + q - 1) // q * q
+
+
+def _check_state(i: int, s: Dict, n: int) -> None:
+    """Refuses entries of a saved state that are not parameter i's, of n elements."""
+    for k in ("step", "exp_avg", "exp_avg_sq"):
+        if k not in s:
+            raise ValueError(f"the state dict is not AdamW's: no {k!r}")
+    codes = not torch.as_tensor(s["exp_avg"]).is_floating_point()
+    for k in ("exp_avg", "exp_avg_sq"):
+        t = torch.as_tensor(s[k])
+        if t.numel() != n:
+            raise ValueError(f"AdamW state: {k} of parameter {i} has {t.numel()} elements, the "
+                             f"parameter {n}")
+        if t.is_floating_point() == codes:
+            raise ValueError(f"AdamW state: of parameter {i}'s moments one is in codes, one is not")
+        if codes:
+            sc = s.get(k + "_scale")
+            if sc is None or torch.as_tensor(sc).numel() != -(-n // 256):
+                raise ValueError(f"AdamW state: {k} of parameter {i} is in codes and needs "
+                                 f"{-(-n // 256)} scales")
 
 
 class MultiTensorAdamW:
@@ -197,6 +218,8 @@ class MultiTensorAdamW:
     def load_state(self, states: Dict[int, Dict]) -> None:
         """Sets the moments and counts of the tensors in ``states`` (index -> entries as state_of
         gives them, or f32 moments as torch.optim.AdamW saves them); the others become zero."""
+        for i, s in states.items():
+            _check_state(i, s, self.sizes[i])
         full = None
         if self.bits == 8 and any(torch.as_tensor(s["exp_avg"]).is_floating_point()
                                   for s in states.values()):
@@ -207,7 +230,6 @@ class MultiTensorAdamW:
                 for t, k in zip(full, ("exp_avg", "exp_avg_sq")):
                     src = torch.as_tensor(s[k])
                     if src.is_floating_point():
-                        self._size_check(i, src, k)
                         t[self.offsets[i]:self.offsets[i] + self.sizes[i]].copy_(src.reshape(-1))
         for t in (self.exp_avg, self.exp_avg_sq, self.scale_m, self.scale_v, self.steps):
             if t is not None:
@@ -225,22 +247,13 @@ class MultiTensorAdamW:
             if codes and self.bits == 32:  # 8-bit state into 32 bits: the values it stands for
                 for k, top, power in (("exp_avg", 127.0, 2), ("exp_avg_sq", 255.0, 4)):
                     q = torch.as_tensor(s[k]).reshape(-1).to(self.device).double()
-                    self._size_check(i, q, k)
                     sc = torch.as_tensor(s[k + "_scale"]).to(self.device).double()
                     val = torch.sign(q) * (q.abs() / top) ** power
                     mine[k].copy_(val * sc.repeat_interleave(256)[:q.numel()])
             elif codes or self.bits == 32:
                 for k, dst in mine.items():
                     if k != "step":
-                        src = torch.as_tensor(s[k])
-                        if k in ("exp_avg", "exp_avg_sq"):
-                            self._size_check(i, src, k)
-                        dst.copy_(src.reshape(dst.shape))
-
-    def _size_check(self, i, t, key):
-        if t.numel() != self.sizes[i]:
-            raise ValueError(f"AdamW state: {key} of parameter {i} has {t.numel()} elements, the "
-                             f"parameter {self.sizes[i]}")
+                        dst.copy_(torch.as_tensor(s[k]).reshape(dst.shape))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -404,27 +417,41 @@ class AdamW(torch.optim.Optimizer):
         raise ValueError("not a parameter of this optimizer")
 
     def load_state_dict(self, state_dict: Dict) -> None:
+        """Moments, counts and groups (all of their entries, as torch restores them) become the saved
+        ones.  A state that does not fit is refused before anything changes."""
+        state_dict = state_dict.copy()
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            new = hook(self, state_dict)
+            if new is not None:
+                state_dict = new
         groups, saved = self.param_groups, state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
             raise ValueError("loaded state dict's parameter groups do not match this optimizer's")
+        restored = []
+        for g, s in zip(groups, saved):
+            for key in ("amsgrad", "maximize"):
+                if s.get(key):
+                    raise ValueError(f"the saved optimizer has {key}=True, which this one does not do")
+            new = {**g, **copy.deepcopy({k: v for k, v in s.items() if k != "params"})}
+            if isinstance(new["lr"], torch.Tensor):
+                new["lr"] = float(new["lr"])
+            self._check_group(new)
+            restored.append(new)
         ids = [i for g in saved for i in g["params"]]
         params = [p for g in groups for p in g["params"]]
-        states = {p: state_dict["state"][i] for i, p in zip(ids, params)
-                  if i in state_dict["state"]}
-        for s in states.values():
-            for k in ("step", "exp_avg", "exp_avg_sq"):
-                if k not in s:
-                    raise ValueError(f"the state dict is not AdamW's: no {k!r}")
-        # (the saved state may be this optimizer's own views: copied before the tables go)
-        states = {p: {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in s.items()}
-                  for p, s in states.items()}
-        for g, s in zip(groups, saved):
-            for k in ("lr", "betas", "eps", "weight_decay"):
-                if k in s:
-                    g[k] = float(s[k]) if isinstance(s[k], torch.Tensor) else s[k]
-            self._check_group(g)
+        # (the saved state may be this optimizer's own views: copied before they are overwritten)
+        states = {p: {k: v.clone() if isinstance(v, torch.Tensor) else v
+                      for k, v in state_dict["state"][i].items()}
+                  for i, p in zip(ids, params) if i in state_dict["state"]}
+        for i, p in enumerate(params):
+            if p in states:
+                _check_state(i, states[p], p.numel())
         if not self._tables:
             self._build()
+        for g, new in zip(groups, restored):
+            g.update(new)
         for t, spans in self._tables:  # in place: a captured step goes on from the loaded state
             at = [p for _, _, ps in spans for p in ps]
             t.load_state({i: states[p] for i, p in enumerate(at) if p in states})
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
