@@ -65,3 +65,21 @@ def test_host_tensors_are_refused():
 
     with pytest.raises(HipUnavailable):
         catalog_log_probs(torch.zeros(2, 64), torch.zeros(3, 64))
+
+
+def test_a_trainable_temperature_is_refused():
+    """Its gradient is not computed: refused, not lost."""
+    from twotower.losses import CatalogSoftmaxLoss, catalog_log_probs
+
+    x, w, ids = torch.zeros(2, 64), torch.zeros(3, 64), torch.zeros(2, dtype=torch.int64)
+    t = torch.tensor(0.07, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="temperature"):
+        catalog_log_probs(x, w, ids, temperature=t)
+    with pytest.raises(NotImplementedError, match="temperature"):
+        CatalogSoftmaxLoss(t)(x, w, ids)
+    from twotower._lib import HipUnavailable
+
+    with torch.no_grad(), pytest.raises(HipUnavailable):  # (a value without a gradient is one)
+        catalog_log_probs(x, w, ids, temperature=t)
+    with pytest.raises(HipUnavailable):
+        catalog_log_probs(x, w, ids, temperature=torch.tensor(0.07))

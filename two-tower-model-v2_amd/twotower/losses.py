@@ -131,6 +131,10 @@ def catalog_log_probs(queries: torch.Tensor, items: torch.Tensor, ids: torch.Ten
     vector may hold anything).  A row with nothing left: log_prob -inf, entropy 0.  Differentiable in
     queries and items (log_prob and entropy); the logits are never stored, so N x V is bounded by
     time alone.  E is padded to a multiple of 64 (a copy) where it is not one."""
+    if (isinstance(temperature, torch.Tensor) and temperature.requires_grad
+            and torch.is_grad_enabled()):
+        raise NotImplementedError("gradients w.r.t. the temperature are not computed: pass a number "
+                                  "(or temperature.detach())")
     if torch.is_grad_enabled() and (queries.requires_grad or items.requires_grad
                                     or (bias is not None and bias.requires_grad)):
         return LogProbs(*_CatalogFn.apply(queries, items, ids, bias, float(temperature), entropy,
