@@ -686,6 +686,9 @@ int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_
  *   entropy[n]  = -sum_v p log p  (NULL: not wanted) ;  lse[n] = log sum_v exp l[n, v]
  *   top_ids / top_log_prob [N, top]: the top (<= 32, <= V) largest logits by the product in 64
  *                 bits, ties to the lower id (taken-out items last, with -inf)
+ *                 The workspace then holds a float per 16 logits, N V / 4 bytes, and N times the
+ *                 segments of a row (one per 65536 items, at most 64) has to be below 2^24: pass the rows
+ *                 in parts
  * A row with every item taken out: lse -inf, entropy 0, log_prob -inf (0 without an id).
  * _bwd: dx [N, E], dw [V, E] of dtype, contiguous (either may be NULL), for gradients g_log_prob and
  * g_entropy [N] (either may be NULL), with the forward's lse and entropy.  A row whose gradients

@@ -132,3 +132,34 @@ def test_a_crowd_in_a_graph_and_on_another_stream():
         e = catalog_log_probs(xs, w, None, 0.07, top=12)
         assert torch.equal(r.top_ids, order(exact(xs, w, 0.07), 12))
         assert torch.equal(r.top_ids, e.top_ids) and torch.equal(r.top_log_probs, e.top_log_probs)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_rows_in_parts(dt, monkeypatch):
+    """More rows than the alternatives' workspace is given memory for: taken in parts, the last a shorter
+    one; each row's result is its own."""
+    from twotower import kernels
+    from twotower.losses import catalog_log_probs
+
+    gen = torch.Generator().manual_seed(0)
+    x = torch.nn.functional.normalize(torch.randn(103, 64, generator=gen), dim=1).to(dt).cuda()
+    w = torch.nn.functional.normalize(torch.randn(1200, 64, generator=gen), dim=1).to(dt).cuda()
+    ids = torch.randint(0, 1200, (206,), generator=gen).cuda()[::2]
+    b = torch.randn(1200, generator=gen).cuda()
+    want = catalog_log_probs(x, w, ids, 0.07, b, entropy=True, top=7)
+    sizes = []
+    make = kernels._catalog_ws_bytes
+    monkeypatch.setattr(kernels, "_catalog_ws_bytes", lambda n, *a: sizes.append(n) or make(n, *a))
+    for limit, part in ((1200 // 4 * 20 + 400, 20), (1, 1)):
+        sizes.clear()
+        monkeypatch.setattr(kernels, "CATALOG_TOP_BYTES", limit)
+        got = catalog_log_probs(x, w, ids, 0.07, b, entropy=True, top=7)
+        assert sorted(sizes) == sorted({part, 103 % part} - {0})
+        assert torch.equal(got.top_ids, want.top_ids)
+        T = U * (68 * 1.02 / 0.07 + 150 + 64)  # (other tiles may sum in another order)
+        for p, q in ((got.log_prob, want.log_prob), (got.top_log_probs, want.top_log_probs)):
+            assert ((p - q).abs() <= 2 * T + 2 * U * q.abs()).all()
+        assert ((got.entropy - want.entropy).abs() <= 4 * T * 40).all()
+    sizes.clear()
+    catalog_log_probs(x, w, ids, 0.07, b)  # (without alternatives: one call)
+    assert sizes == [103]

@@ -744,6 +744,9 @@ def gated_scan_backward(x, gate, weights, saved, dh, dlast, need_h0: bool):
 
 
 CATALOG_TOP_MAX = 32  # alternatives per row of catalog_logprobs
+# Alternatives need a float per 16 logits: rows are taken in parts that stay below this (and below the
+# 2^24 blocks that one launch takes).
+CATALOG_TOP_BYTES = 4 << 30
 
 
 def catalog_rows(t: torch.Tensor) -> torch.Tensor:
@@ -822,11 +825,18 @@ def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entro
         lse = torch.empty(n, dtype=_f32, device=dev)
         ti = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
         tl = torch.empty((n, top), dtype=_f32, device=dev) if top else None
-        ws = torch.empty(_catalog_ws_bytes(n, v, e, dt, top), dtype=torch.uint8, device=dev)
-        check(lib().tt_catalog_logprobs(
-            x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), dt, n, v, e, _addr(ids),
-            _addr(bias), temperature, _addr(lp), _addr(ent), lse.data_ptr(), top, _addr(ti),
-            _addr(tl), ws.data_ptr(), ws.numel(), stream_ptr()), "tt_catalog_logprobs")
+        part = n
+        if top:  # (segments of a row: at most 64)
+            part = min(n, max(1, min(CATALOG_TOP_BYTES // (v // 4 + 16), (1 << 24) // 64 - 1)))
+        need = [_catalog_ws_bytes(m, v, e, dt, top) for m in {part, n % part if part else 0} if m]
+        ws = torch.empty(max(need, default=0), dtype=torch.uint8, device=dev)
+        for a in range(0, n, part or 1):
+            m = min(part, n - a)
+            at = (lambda t: None if t is None else t[a:].data_ptr()) if a else _addr
+            check(lib().tt_catalog_logprobs(
+                at(x), x.stride(0), w.data_ptr(), w.stride(0), dt, m, v, e, at(ids), _addr(bias),
+                temperature, at(lp), at(ent), at(lse), top, at(ti), at(tl), ws.data_ptr(),
+                ws.numel(), stream_ptr()), "tt_catalog_logprobs")
     return lp, ent, lse, ti, tl
 
 
