@@ -275,8 +275,9 @@ class Evaluator:
         for b0 in range(0, len(test_pairs), self.batch_size):
             chunk = test_pairs[b0: b0 + self.batch_size]
             emb = self._encode([inter for _, inter, _ in chunk])
+            at, n = self.vector_db.id_to_index, self.vector_db.index.ntotal
             rows = [(i, p) for i, (_, _, rel) in enumerate(chunk) for p in sorted(rel)
-                    if p in self.vector_db.id_to_index]
+                    if 0 <= at.get(p, -1) < n]
             if rows:
                 v, e, _ = self.vector_db.log_probs(emb[[i for i, _ in rows]],
                                                    [p for _, p in rows], temperature)

@@ -721,16 +721,18 @@ class VectorDatabase:
             return none if product_ids is not None else None, none, []
         from .losses import catalog_log_probs
 
-        with self.index._lock:  # one state of the catalog
-            xb, n = self.index.xb, self.index.ntotal
+        index, rows_of = self.index, self.id_to_index
+        with index._lock:  # one state of the catalog
+            xb, n = index.xb, index.ntotal
         with _lib.on_device(xb):
             dev = xb.device
             rows = self.normalize_queries(
                 torch.from_numpy(np.ascontiguousarray(q, dtype=np.float32)).to(dev))
             ids = None
             if product_ids is not None:
-                ids = torch.tensor([self.id_to_index.get(p, -1) for p in product_ids],
-                                   dtype=torch.int64, device=dev)
+                at = [rows_of.get(p, -1) for p in product_ids]
+                ids = torch.tensor([i if 0 <= i < n else -1 for i in at], dtype=torch.int64,
+                                   device=dev)
             r = catalog_log_probs(rows, xb[:n], ids, temperature, entropy=True, top=min(top, n))
             lp = None
             if ids is not None:
