@@ -135,7 +135,10 @@ class TwoTowerTrainStep:
                  betas=(0.9, 0.999), eps: float = 1e-8, prec: str = "f32", graph: bool = False,
                  weight_decay: float = 0.0, state_bits: int = 32):
         if buyer_tower.aggregation_method not in ("attention", "weighted_avg"):
-            raise ValueError(f"Unknown aggregation method: {buyer_tower.aggregation_method}")
+            raise ValueError("the fused training step computes 'attention' and 'weighted_avg' buyer "
+                             f"towers, not '{buyer_tower.aggregation_method}': train that one "
+                             "through autograd (its forward, InfoNCELoss or CatalogSoftmaxLoss, "
+                             "optim.AdamW)")
         self.attention = buyer_tower.aggregation_method == "attention"
         if prec not in ("f32", "bf16"):
             raise ValueError("prec must be 'f32' or 'bf16'")
