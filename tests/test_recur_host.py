@@ -67,3 +67,16 @@ def test_refusals_on_the_device():
     _, last = gated_scan(x, x, w)
     with pytest.raises(NotImplementedError):
         last.sum().backward()
+
+
+def test_when_histories_are_split(L):
+    """Histories that fill the card are not split (no workspace), few long ones are."""
+    n = ctypes.c_int64(-1)
+
+    def need(B, S, D):
+        assert L.tt_gated_scan_workspace_bytes(B, S, D, ctypes.byref(n)) == 0
+        return n.value
+
+    assert need(639, 1000, 128) > 0 and need(1, 128, 64) > 0
+    assert need(1024, 1000, 64) == 0  # (with one channel a lane as well)
+    assert need(700, 1000, 64) == 0 and need(700, 100000, 64) == 0 and need(3, 127, 64) == 0

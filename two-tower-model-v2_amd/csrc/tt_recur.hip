@@ -645,15 +645,18 @@ struct ScanPlan {
 };
 // VEC: two channels a lane where D, the strides and the addresses allow (4- or 8-byte loads),
 // else one.  Chunks: as many as give the card about 8192 waves (8 a SIMD), none shorter than 32
-// events; one chunk when the histories alone give 1024.
-static ScanPlan scan_plan(int64_t B, int64_t S, int D, bool vec_ok) {
+// events; one chunk when the histories alone give 640 waves in bf16, 512 in f32 (128 channels, forward
+// and backward, us, one chunk : split: bf16 512 x 1000 214 + 265 : 148 + 208, 768 x 1000 205 + 236 :
+// 251 + 336, 1000 x 1000 188 + 273 : 317 + 427; f32 256 x 1000 247 + 311 : 135 + 195, 512 x 1000 253 +
+// 335 : 302 + 416) or have fewer than 128 events (bf16 256 x 128 27 + 32 : 30 + 31).
+static ScanPlan scan_plan(int64_t B, int64_t S, int D, int64_t sz, bool vec_ok) {
   ScanPlan p;
   p.vec = vec_ok && D % 2 == 0 ? 2 : 1;
   p.nw = (D + 64 * p.vec - 1) / (64 * p.vec);
   p.C = 1;
   p.T = S > 0 ? S : 1;
   const int64_t waves = B * p.nw;
-  if (waves < 1024 && S >= 128) {
+  if (waves < (sz == 2 ? 640 : 512) && S >= 128) {
     int64_t c = (8192 + waves - 1) / waves, cmax = (S + 31) / 32;
     c = c < cmax ? c : cmax;
     p.T = ((S + c - 1) / c + RC_CK - 1) / RC_CK * RC_CK;
@@ -661,11 +664,11 @@ static ScanPlan scan_plan(int64_t B, int64_t S, int D, bool vec_ok) {
   }
   return p;
 }
-// workspace for either vector width (the caller of the size does not know the addresses)
+// workspace for either type and vector width (the caller of the size does not know the addresses)
 static int64_t scan_ws(int64_t B, int64_t S, int D) {
   int64_t need = 0;
-  for (int v = 0; v < 2; ++v) {
-    const ScanPlan p = scan_plan(B, S, D, v != 0);
+  for (int v = 0; v < 4; ++v) {
+    const ScanPlan p = scan_plan(B, S, D, v & 2 ? 4 : 2, (v & 1) != 0);
     const int64_t n = p.C > 1 ? 3 * B * p.C * (int64_t)D * 4 : 0;
     need = n > need ? n : need;
   }
@@ -704,7 +707,7 @@ static int scan_setup(ScanArgs& a, int32_t dtype, ScanPlan& p, void* workspace, 
   const int64_t sz = dtype == TT_DTYPE_F32 ? 4 : 2;
   bool vec = a.xsb % 2 == 0 && a.xss % 2 == 0 && a.gsb % 2 == 0 && a.gss % 2 == 0;
   for (const void* r : rows) vec = vec && addr_ok(r, 2 * sz);
-  p = scan_plan(a.B, a.S, a.D, vec);
+  p = scan_plan(a.B, a.S, a.D, sz, vec);
   a.nw = p.nw;
   a.C = p.C;
   a.T = p.T;
