@@ -1522,8 +1522,9 @@ __global__ __launch_bounds__(256) void k_lost(const LogitArgs a, float* __restri
 }
 
 // out[m][c] = scale sum_k A[m, k] B[k, c]; B [K rows, cols] as it lies; A rows [m][k] (ACOL false) or
-// as it lies [k][m] (ACOL).  K a multiple of BK (rows past a's or b's end are zero in A).  splits > 1
-// or acc: f32 partial sums part[split][M][cols] (acc: added to what is there), else out.
+// as it lies [k][m] (ACOL).  K a multiple of BK (rows past a's or b's end are zero in A).  Tiles whose
+// sums are split (or all, acc: added to what is there) write f32 partial sums, a square of the tile's
+// edge a block; the others write out.
 struct ProductArgs {
   const void *A, *B;
   int64_t lda, ldb, a_rows, b_rows;

@@ -40,14 +40,14 @@ struct ScanArgs {
   const void *x, *gate;
   const float *w, *h0;      // w [B, S] rows wsb apart; h0 [B, D]; either may be null
   void* h;                  // [B, S, D] or null
-  float *h_last, *ck;       // [B, D]; [B, ceil(S / 16), D] or null
+  float *h_last, *ck;       // [B, D]; [B, ceil(S / RC_CK), D] or null
   const void* dh;           // backward: [B, S, D] or null
   const float* dlast;       // [B, D] or null
   void *dx, *dgate;
   float* dh0;
   int64_t B, S, xsb, xss, gsb, gss, wsb;
   int D, nw, C;             // waves per row, chunks per history
-  int64_t T;                // events per chunk (a multiple of 16 unless C == 1)
+  int64_t T;                // events per chunk (a multiple of RC_CK unless C == 1)
   float *sumA, *sumH, *carry;  // [B, C, D] each (C > 1)
 };
 
@@ -58,13 +58,9 @@ struct Pack<float, 1> { typedef float type; };
 template <>
 struct Pack<float, 2> { typedef float type __attribute__((ext_vector_type(2))); };
 template <>
-struct Pack<float, 4> { typedef float type __attribute__((ext_vector_type(4))); };
-template <>
 struct Pack<uint16_t, 1> { typedef uint16_t type; };
 template <>
 struct Pack<uint16_t, 2> { typedef uint32_t type; };
-template <>
-struct Pack<uint16_t, 4> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
 
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -80,14 +76,9 @@ __device__ __forceinline__ void unpack(typename Pack<T, VEC>::type p, float (&o)
     }
   } else if constexpr (VEC == 1) {
     o[0] = bf_lo(p);
-  } else if constexpr (VEC == 2) {
+  } else {
     o[0] = bf_lo(p);
     o[1] = bf_hi(p);
-  } else {
-    o[0] = bf_lo(p[0]);
-    o[1] = bf_hi(p[0]);
-    o[2] = bf_lo(p[1]);
-    o[3] = bf_hi(p[1]);
   }
 }
 typedef __bf16 rc_bf16x2 __attribute__((ext_vector_type(2)));
@@ -107,11 +98,8 @@ __device__ __forceinline__ typename Pack<T, VEC>::type pack(const float (&v)[VEC
     }
   } else if constexpr (VEC == 1) {
     p = (uint16_t)rc_pack2(v[0], 0.0f);
-  } else if constexpr (VEC == 2) {
-    p = rc_pack2(v[0], v[1]);
   } else {
-    p[0] = rc_pack2(v[0], v[1]);
-    p[1] = rc_pack2(v[2], v[3]);
+    p = rc_pack2(v[0], v[1]);
   }
   return p;
 }
