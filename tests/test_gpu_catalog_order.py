@@ -150,7 +150,8 @@ def test_rows_in_parts(dt, monkeypatch):
     sizes = []
     make = kernels._catalog_ws_bytes
     monkeypatch.setattr(kernels, "_catalog_ws_bytes", lambda n, *a: sizes.append(n) or make(n, *a))
-    for limit, part in ((1200 // 4 * 20 + 400, 20), (1, 1)):
+    row = 1200 // 4 + 7 * 16 + 64 * 15 * 8
+    for limit, part in ((row * 20 + 40, 20), (1, 1)):
         sizes.clear()
         monkeypatch.setattr(kernels, "CATALOG_TOP_BYTES", limit)
         got = catalog_log_probs(x, w, ids, 0.07, b, entropy=True, top=7)
@@ -163,3 +164,20 @@ def test_rows_in_parts(dt, monkeypatch):
     sizes.clear()
     catalog_log_probs(x, w, ids, 0.07, b)  # (without alternatives: one call)
     assert sizes == [103]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V,share", [(1, 300000, 1.0), (33, 50000, 0.5), (300, 20000, 0.2), (2, 17000, 1.0)])
+def test_many_copies_of_one_item(dt, N, V, share):
+    """Catalogs with thousands of copies of one vector (items without a text): the lowest ids of them."""
+    gen = torch.Generator().manual_seed(V)
+    w = torch.nn.functional.normalize(torch.randn(V, 64, generator=gen), dim=1)
+    same = torch.rand(V, generator=gen) < share
+    same[0] = True  # (the one they are copies of)
+    w[same] = w[0].clone()
+    x = torch.nn.functional.normalize(w[same][:1] + 0.05 * torch.randn(N, 64, generator=gen), dim=1)
+    x, w = x.to(dt).cuda(), w.to(dt).cuda()
+    for top in (1, 32):
+        ids, _ = run(x, w, 0.07, top)
+        # (their 64-bit logits are equal by construction, whatever order a sum takes)
+        assert torch.equal(ids, torch.nonzero(same)[:top, 0].cuda().expand(N, top))

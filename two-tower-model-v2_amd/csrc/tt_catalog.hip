@@ -1090,12 +1090,14 @@ __device__ __forceinline__ int key_rank(const uint64_t* keys, int n, uint64_t mi
 template <typename T>
 __global__ __launch_bounds__(256) void k_top_groups(const float* __restrict__ tmax, int64_t M, int seg_len,
                                                     int nseg, int keep, uint64_t* __restrict__ out,
-                                                    unsigned n_seg_blocks, const CombineArgs ca) {
+                                                    unsigned n_seg_blocks, const CombineArgs ca,
+                                                    uint32_t* __restrict__ n_rows) {
   __shared__ uint64_t red[4][64];
   __shared__ __attribute__((aligned(16))) uint64_t all[258];
   __shared__ uint64_t fin[64];
   __shared__ int cnt[4];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (n_rows && blockIdx.x == 0 && threadIdx.x == 0) *n_rows = 0u;  // (for the next kernel)
   if (blockIdx.x >= n_seg_blocks) {
     const int64_t r = (int64_t)(blockIdx.x - n_seg_blocks) * 4 + w;
     if (r < ca.N) combine_row<T>(ca, r, lane);
@@ -1193,15 +1195,16 @@ struct TopArgs {
   const float2* stat;
   int64_t* ids_out;
   float* lp_out;
-  // the second search
+  // the second search: n_rows rows [N] of it, in parts of part_len groups
   const float* tmax;
   int64_t M;
-  int seg_len;
-  float* floor;     // [N]
-  uint32_t* state;  // [N] CT_DONE, or the segments that are searched already
-  TopEntry* found;  // [N, nseg, top]
+  int parts, part_len;
+  uint32_t *n_rows, *rows;
+  float* floor;     // [N] of the groups' maxima
+  TopEntry* kth;    // [N] the top-th item of the groups kept: a later one is none of the top
+  uint32_t* done;   // [N] parts that are searched
+  TopEntry* found;  // [N, parts, top]
 };
-constexpr uint32_t CT_DONE = 0x80000000u;
 constexpr int CT_GROUPS = CT_TOP_MAX + CT_TOP_EXTRA;  // groups scored at a time
 struct TopList {
   double l[CT_GROUPS * 16 + CT_TOP_MAX];  // candidates, in any order (ranks do not depend on it)
@@ -1211,11 +1214,15 @@ struct TopList {
   int n;
 };
 
+// after k in the order (score, lower id)
+__device__ __forceinline__ bool top_after(const TopEntry& k, double l, int v) {
+  return l < k.l || (l == k.l && v > (int)k.v);
+}
 // The items of n_grp groups, scored in 64 bits (16 lanes an item, 16-byte loads, NT / 4 items in
-// flight); those not below cut (powers of two) join the list.
+// flight); those not below cut (powers of two) and not after kth join the list.
 template <typename T, int NT>
 __device__ __forceinline__ void top_score(const TopArgs& a, const T* xr, const uint32_t* grp, int n_grp, double cut,
-                                          TopList& o) {
+                                          const TopEntry& kth, TopList& o) {
   constexpr int PC = 16 / (int)sizeof(T), NG = NT / 16;
   const T* w = (const T*)a.w;
   const int sub = threadIdx.x >> 4, l16 = threadIdx.x & 15, cand = n_grp * 16, V = a.V, E = a.E;
@@ -1247,7 +1254,8 @@ __device__ __forceinline__ void top_score(const TopArgs& a, const T* xr, const u
       if (l16 == 0 && i0 + i * NG < cand && v[i] < V) {
         const float b = a.bias ? a.bias[v[i]] : 0.0f;
         const double l = b <= CT_OUT ? -__builtin_huge_val() : a.s * d[i] + (double)b;
-        if (!(l * 1.4426950408889634 < cut)) {  // (-inf, NaN: only where the cut lets them)
+        // (-inf, NaN: only where the cut lets them)
+        if (!(l * 1.4426950408889634 < cut) && !top_after(kth, l, v[i])) {
           const int k = atomicAdd(&o.n, 1);
           o.l[k] = l;
           o.v[k] = v[i];
@@ -1368,7 +1376,7 @@ __global__ __launch_bounds__(NT) void k_top_items(const TopArgs a) {
       }
     }
     __syncthreads();
-    top_score<T, NT>(a, xr, grp, s_groups, (double)s_floor, o);
+    top_score<T, NT>(a, xr, grp, s_groups, (double)s_floor, TopEntry{-__builtin_huge_val(), 0x7fffffff}, o);
     __syncthreads();
     // (a second round only where sums in 32 bits went past their range: all the groups kept hold at
     // least top items)
@@ -1378,21 +1386,24 @@ __global__ __launch_bounds__(NT) void k_top_items(const TopArgs a) {
   top_rank<NT>(o, top);
   __syncthreads();
   top_write<T, NT>(a, o, n);
-  if (a.state && tid == 0) {
+  if (a.n_rows && tid == 0 && more) {
     a.floor[n] = s_floor;
-    a.state[n] = more ? 0u : CT_DONE;
+    a.kth[n] = TopEntry{o.bl[top - 1], o.bv[top - 1]};
+    a.done[n] = 0u;
+    a.rows[atomicAdd(a.n_rows, 1u)] = (uint32_t)n;
   }
 }
 
-// The second search: rows whose groups above the floor were more than are kept.  Block = (row, segment):
-// the segment's groups above the floor, 40 at a time, are scored in 64 bits with the best so far; the
-// row's last block joins the segments (no block waits for another).  Without such rows: 2 us of launch.
+// The second search: rows whose groups above the floor were more than are kept.  Block = (row, part): the
+// part's groups above the floor, 40 at a time, are scored in 64 bits, the best of them kept; the row's
+// last block joins the parts (no block waits for another).  Without such rows 3 us.
 template <typename T>
 __global__ __launch_bounds__(256) void k_top_wide(const TopArgs a) {
   __shared__ TopList o;
   __shared__ uint32_t pend[256];
   __shared__ int n_pend, s_last;
   const int tid = threadIdx.x, top = a.top;
+  TopEntry kth;
   auto carry = [&]() __attribute__((always_inline)) {  // the list becomes its best
     __syncthreads();
     top_rank<256>(o, top);
@@ -1405,17 +1416,18 @@ __global__ __launch_bounds__(256) void k_top_wide(const TopArgs a) {
     __syncthreads();
     if (tid == 0) o.n = k;
     __syncthreads();
+    if (o.n == top && !top_after(kth, o.l[top - 1], o.v[top - 1])) kth = TopEntry{o.l[top - 1], o.v[top - 1]};
   };
-  const int64_t units = (int64_t)a.N * a.nseg;
+  const int64_t units = (int64_t)*a.n_rows * a.parts;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int64_t n = u / a.nseg;
-    if (a.state[n] & CT_DONE) continue;
-    const int sg = (int)(u % a.nseg);
+    const int64_t n = a.rows[u / a.parts];
+    const int part = (int)(u % a.parts);
     const T* xr = (const T*)a.x + n * a.ldx;
     const float* row = a.tmax + n * a.M;
     const float floor = a.floor[n];
-    const int64_t i0 = (int64_t)sg * a.seg_len, i1 = i0 + a.seg_len < a.M ? i0 + a.seg_len : a.M;
-    double cut = (double)floor;
+    const int64_t i0 = (int64_t)part * a.part_len, i1 = i0 + a.part_len < a.M ? i0 + a.part_len : a.M;
+    const TopEntry kth0 = a.kth[n];
+    kth = kth0;
     if (tid == 0) o.n = 0;
     for (int64_t b = i0; b < i1; b += 256) {
       if (tid == 0) n_pend = 0;
@@ -1425,35 +1437,36 @@ __global__ __launch_bounds__(256) void k_top_wide(const TopArgs a) {
       __syncthreads();
       const int np = n_pend;
       for (int p = 0; p < np; p += CT_GROUPS) {
-        top_score<T, 256>(a, xr, pend + p, np - p < CT_GROUPS ? np - p : CT_GROUPS, cut, o);
+        top_score<T, 256>(a, xr, pend + p, np - p < CT_GROUPS ? np - p : CT_GROUPS, (double)floor, kth, o);
         carry();
-        // (an equal score passes: the lower id counts)
-        if (o.n == top && o.l[top - 1] * 1.4426950408889634 > cut) cut = o.l[top - 1] * 1.4426950408889634;
       }
       __syncthreads();
     }
     __syncthreads();
-    if (tid < top) a.found[u * top + tid] = tid < o.n ? TopEntry{o.l[tid], o.v[tid]} : TopEntry{0.0, -1};
+    TopEntry* f = a.found + n * a.parts * top;
+    if (tid < top) f[part * top + tid] = tid < o.n ? TopEntry{o.l[tid], o.v[tid]} : TopEntry{0.0, -1};
     __threadfence();  // visible before the block counts itself in
     __syncthreads();
-    if (tid == 0) s_last = atomicAdd(&a.state[n], 1u) == (uint32_t)a.nseg - 1u;
+    if (tid == 0) s_last = atomicAdd(&a.done[n], 1u) == (uint32_t)a.parts - 1u;
     __syncthreads();
     if (s_last) {
       __threadfence();
-      const TopEntry* f = a.found + n * a.nseg * top;
-      const int total = a.nseg * top;
+      const int total = a.parts * top;
+      kth = kth0;
       if (tid == 0) o.n = 0;
       __syncthreads();
       for (int b = 0; b < total; b += 512) {
-        for (int i = b + tid; i < total && i < b + 512; i += 256)
-          if (f[i].v >= 0) {
+        for (int i = b + tid; i < total && i < b + 512; i += 256) {
+          const TopEntry q = f[i];
+          if (q.v >= 0 && !top_after(kth, q.l, (int)q.v)) {
             const int k = atomicAdd(&o.n, 1);
-            o.l[k] = f[i].l;
-            o.v[k] = (int)f[i].v;
+            o.l[k] = q.l;
+            o.v[k] = (int)q.v;
           }
+        }
         carry();
       }
-      if (o.n == top) top_write<T, 256>(a, o, n);  // (always: the floor has at least top items above it)
+      if (o.n == top) top_write<T, 256>(a, o, n);  // (always: what the first search found is among it)
       __syncthreads();
     }
   }
@@ -1816,7 +1829,8 @@ static void logits_shape(int64_t N, int64_t V, int edge, int& n_tiles, int& v_ti
 struct StatPlan {
   bool ring;
   int edge, n_tiles, v_tiles, splits, keep, nseg, seg_len;
-  int64_t M, off_tmax, off_seg, off_wsq, off_err, off_stat, off_floor, off_state, off_found, bytes;
+  int64_t M, off_tmax, off_seg, off_wsq, off_err, off_stat, off_floor, off_rows, off_done, off_kth, off_found, bytes;
+  int parts, part_len;
 };
 // Shares: about 512 blocks (two a CU; three of the small tiles).
 static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
@@ -1841,9 +1855,15 @@ static StatPlan stat_plan(int64_t N, int64_t V, int E, int64_t sz, int top) {
     p.off_err = p.off_wsq + up((int64_t)p.n_tiles * p.splits * 4, 256);
     p.off_stat = p.off_err + up(N * 4, 256);
     p.off_floor = p.off_stat + up(N * 8, 256);
-    p.off_state = p.off_floor + up(N * 4, 256);
-    p.off_found = p.off_state + up(N * 4, 256);
-    p.bytes = p.off_found + up(p.M > p.keep ? N * p.nseg * top * 16 : 0, 256);
+    // the second search: parts of 256 groups, longer ones past 1024 parts a row
+    const int64_t nw = p.M > p.keep ? N : 0;
+    p.part_len = (int)(256 * cdiv(p.M, 256 * 1024));
+    p.parts = (int)cdiv(p.M, p.part_len);
+    p.off_rows = p.off_floor + up(nw * 4, 256);
+    p.off_done = p.off_rows + up((nw + 1) * 4, 256);  // (their number first)
+    p.off_kth = p.off_done + up(nw * 4, 256);
+    p.off_found = p.off_kth + up(nw * 16, 256);
+    p.bytes = p.off_found + up(nw * p.parts * top * 16, 256);
   }
   return p;
 }
@@ -2006,25 +2026,32 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
   if (top) {
     uint64_t* seg = (uint64_t*)(ws + p.off_seg);
     const unsigned sb = (unsigned)(N * p.nseg);
-    hipLaunchKernelGGL(k_top_groups<T>, dim3(sb + cb), dim3(256), 0, st, a.tmax, p.M, p.seg_len, p.nseg,
-                       p.keep, seg, sb, ca);
     TopArgs ta{};
     ta.segs = seg; ta.nseg = p.nseg; ta.keep = p.keep; ta.top = top;
     ta.x = x; ta.w = w; ta.ldx = ldx; ta.ldw = ldw; ta.N = (int)N; ta.E = E; ta.V = (int)V;
-    ta.bias = bias; ta.s = s; ta.s2 = a.s2; ta.group = ca.group; ta.err = ca.err; ta.stat = ca.stat; ta.ids_out = top_ids; ta.lp_out = top_lp;
+    ta.bias = bias; ta.s = s; ta.s2 = a.s2; ta.group = ca.group; ta.err = ca.err; ta.stat = ca.stat;
+    ta.ids_out = top_ids; ta.lp_out = top_lp;
     const bool wide = p.M > p.keep;  // (else no group is left out)
     if (wide) {
-      ta.tmax = a.tmax; ta.M = p.M; ta.seg_len = p.seg_len;
+      ta.tmax = a.tmax; ta.M = p.M; ta.parts = p.parts; ta.part_len = p.part_len;
+      ta.n_rows = (uint32_t*)(ws + p.off_rows);
+      ta.rows = ta.n_rows + 1;
       ta.floor = (float*)(ws + p.off_floor);
-      ta.state = (uint32_t*)(ws + p.off_state);
+      ta.kth = (TopEntry*)(ws + p.off_kth);
+      ta.done = (uint32_t*)(ws + p.off_done);
       ta.found = (TopEntry*)(ws + p.off_found);
     }
+    hipLaunchKernelGGL(k_top_groups<T>, dim3(sb + cb), dim3(256), 0, st, a.tmax, p.M, p.seg_len, p.nseg,
+                       p.keep, seg, sb, ca, ta.n_rows);
     // more threads a row while rows are few: 33 rows 24 us with 1024 (31 with 512); 2049 rows 53 us with
     // 256 (90 with 512)
     if (N <= 128) hipLaunchKernelGGL((k_top_items<T, 1024>), dim3((unsigned)N), dim3(1024), 0, st, ta);
     else if (N <= 512) hipLaunchKernelGGL((k_top_items<T, 512>), dim3((unsigned)N), dim3(512), 0, st, ta);
     else hipLaunchKernelGGL((k_top_items<T, 256>), dim3((unsigned)N), dim3(256), 0, st, ta);
-    if (wide) hipLaunchKernelGGL(k_top_wide<T>, dim3(sb < 1024 ? sb : 1024), dim3(256), 0, st, ta);
+    if (wide) {
+      const int64_t units = N * p.parts;
+      hipLaunchKernelGGL(k_top_wide<T>, dim3((unsigned)(units < 768 ? units : 768)), dim3(256), 0, st, ta);
+    }
   } else {
     hipLaunchKernelGGL(k_combine<T>, dim3(cb), dim3(256), 0, st, ca);
   }

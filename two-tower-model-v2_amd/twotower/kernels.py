@@ -827,7 +827,8 @@ def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entro
         tl = torch.empty((n, top), dtype=_f32, device=dev) if top else None
         part = n
         if top:  # (segments of a row: at most 64)
-            part = min(n, max(1, min(CATALOG_TOP_BYTES // (v // 4 + 16), (1 << 24) // 64 - 1)))
+            per = v // 4 + (v // 4096 + 1) * top * 16 + 64 * (top + 8) * 8
+            part = min(n, max(1, min(CATALOG_TOP_BYTES // per, (1 << 24) // 64 - 1)))
         need = [_catalog_ws_bytes(m, v, e, dt, top) for m in {part, n % part if part else 0} if m]
         ws = torch.empty(max(need, default=0), dtype=torch.uint8, device=dev)
         for a in range(0, n, part or 1):
