@@ -6,8 +6,9 @@
 // Bound: HBM.  f32: p, g, m, v read and p, m, v written, 28 bytes an element; 8-bit moments: 16.
 // Measured: a 1M x 384 f32 table 2.10 ms (5.1 TB/s), an encoder's 117M parameters with 8-bit moments
 // 440 - 510 us (3.7 - 4.3 TB/s) and 247 us (4.8 TB/s) to decode them, a tower's ten tensors 12 us.
-// A small set of tensors (a tower's ten) is bound by the launch: all tensors go in one, a block
-// per chunk of one tensor, tensors and chunks from a table on the device.  Only the gradients'
+// A small set of tensors (a tower's ten) is bound by latency (a block's entry, its tensor's, the step
+// count and the factors from it, then the data: one after another), not by launches: all tensors go in
+// one, a block per chunk of one tensor, tensors and chunks from a table on the device.  Only the gradients'
 // addresses change from step to step: they travel in the kernel's arguments.
 //
 // The step count lives on the device, one per tensor (a tensor without a gradient keeps its

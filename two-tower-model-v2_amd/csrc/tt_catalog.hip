@@ -36,9 +36,9 @@
 //     filled by splitting their sums (f32 partial sums, added in a fixed order: the result does not
 //     depend on timing).
 //
-// Bound: small N by reading w (1 x 1M x 384 bf16: 143 - 160 us, 4.8 - 5.4 TB/s), large N by the matrix
-// pipes with the loads that feed them (4096 x 65537 x 768 bf16: statistics 470 us, 0.88 PFLOP/s;
-// coefficients 195 us and the products 152, 150 us per 21888 items, 0.71, 0.91, 0.92 PFLOP/s).
+// Bound: small N by reading w (1 x 1M x 384 bf16: 150 - 158 us, 4.9 - 5.1 TB/s), large N by the matrix
+// pipes with the loads that feed them (4096 x 65537 x 768 bf16: statistics 465 us, 0.89 PFLOP/s;
+// coefficients 196 us and the products 154, 159 us per 21888 items, 0.70, 0.90, 0.87 PFLOP/s).
 //
 // Items with a bias at or below -1e30 (-inf, the type's lowest) are taken out: probability 0 and
 // gradient 0 whatever their vectors hold.  Rows whose gradients are both 0 do not reach dw.  A row whose
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
 // wave, 8 waves: 384 rows a block; no longer E leaves room for that, and at a shorter one k_logits
 // re-reads less), the catalog streams through LDS in tiles of 32 items, SLOTS - 1 tiles ahead, one
 // barrier a tile, and the previous tile's exponentials run between this tile's MFMAs.  Bound by the
-// two together: 2049 x 100003 with entropy and alternatives 214 us (0.74 PFLOP/s).
+// two together: 2049 x 100003 with entropy and alternatives 223 us (0.71 PFLOP/s).
 constexpr int CR_NT = 512;
 template <int KS>
 struct RingCfg {
@@ -1642,7 +1642,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_product(cons
       } else {
         // the rows whose item is one of the tile's, FOUND rows looked at at a time (256 a wave), listed in
         // their order (the sums do not depend on timing) and multiplied 32 at a time: 4096 rows, 65537
-        // items: 16 a tile, 6 us; a popular item costs 0.1 us a row
+        // items: 16 a tile, 10 us of 155; a popular item costs 0.1 us a row
         for (int64_t s0 = kb; s0 < ke; s0 += FOUND) {
           const int64_t n0 = s0 + (FOUND / TL::NWV) * w;
           int q[FOUND / TL::NT], np = 0;
@@ -1782,7 +1782,7 @@ static int64_t up(int64_t n, int64_t q) { return (n + q - 1) / q * q; }
 static int64_t cdiv(int64_t n, int64_t q) { return (n + q - 1) / q; }
 
 // k_ring against k_logits' 256 x 256 tiles, us: 4096 x 30000 102 : 113 (coefficients 118 : 136), 1024 x
-// 100000 93 : 98 (111 : 122), 2049 x 100003 with entropy 214 : 248; not where blocks of 384 rows leave
+// 100000 93 : 98 (111 : 122), 2049 x 100003 with entropy 214 : 248 (before the norms); not where blocks of 384 rows leave
 // more empty, nor in small problems (200 x 3000 13 : 6).  E = 256: 47 : 46, E = 128: 99 : 107 (108 : 97).
 constexpr int CR_E = 384, CR_ROWS = 384;
 static bool ring_ok(int64_t N, int64_t V, int E, int64_t sz) {
@@ -2043,7 +2043,7 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     }
     hipLaunchKernelGGL(k_top_groups<T>, dim3(sb + cb), dim3(256), 0, st, a.tmax, p.M, p.seg_len, p.nseg,
                        p.keep, seg, sb, ca, ta.n_rows);
-    // more threads a row while rows are few: 33 rows 24 us with 1024 (31 with 512); 2049 rows 53 us with
+    // more threads a row while rows are few: 33 rows 26 us with 1024 (31 with 512); 2049 rows 56 us with
     // 256 (90 with 512)
     if (N <= 128) hipLaunchKernelGGL((k_top_items<T, 1024>), dim3((unsigned)N), dim3(1024), 0, st, ta);
     else if (N <= 512) hipLaunchKernelGGL((k_top_items<T, 512>), dim3((unsigned)N), dim3(512), 0, st, ta);
