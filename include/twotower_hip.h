@@ -683,7 +683,7 @@ int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_
  * at or below -1e30, e.g. -inf: the item is taken out, whatever its vector holds).
  *   log_prob[n] = l[n, ids[n]] - lse[n]   (ids [N]; an id outside [0, V): 0; NULL log_prob: not
  *                 wanted; -inf if the item is taken out)
- *   entropy[n]  = -sum_v p log p  (NULL: not wanted) ;  lse[n] = log sum_v exp l[n, v]
+ *   entropy[n]  = -sum_v p log p  (NULL: not wanted) ;  lse[n] = log sum_v exp l[n, v]  (double)
  *   top_ids / top_log_prob [N, top]: the top (<= 32, <= V) largest logits by the product in 64
  *                 bits, ties to the lower id (taken-out items last, with -inf)
  *                 The workspace then holds a float per 16 logits, N V / 4 bytes, and N times the
@@ -697,14 +697,14 @@ int tt_adamw_encode(const tt_adamw_tensor* tensors, const int32_t* items, int64_
  * E a multiple of 64; rows 16-byte aligned; N < 2^24, V < 2^30; temperature >= 1e-30.  Sums in f32;
  * log_prob and top_log_prob (one item's two values are the same) and entropy with the item's own logit in
  * 64 bits, also in the sum where it holds over a sixteenth of the probability; lse (what _bwd takes its
- * probabilities against) with the 32-bit one.  The coefficients of the gradient products are in dtype;
+ * probabilities against; 64 bits, since a coefficient next to p = 1 is a difference) with the 32-bit one.  The coefficients of the gradient products are in dtype;
  * in bf16 the given items' in two parts, with N <= 64 all.  The results do not depend on timing (no float atomics).
  * --------------------------------------------------------------------------------- */
 int tt_catalog_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t E, int32_t dtype, int32_t top,
                                         int64_t* bytes);
 int tt_catalog_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
                         int64_t N, int64_t V, int32_t E, const int64_t* ids, const float* bias,
-                        float temperature, float* log_prob, float* entropy, float* lse,
+                        float temperature, float* log_prob, float* entropy, double* lse,
                         int32_t top, int64_t* top_ids, float* top_log_prob, void* workspace,
                         int64_t workspace_bytes, void* stream);
 int tt_catalog_logprobs_bwd_workspace_bytes(int64_t N, int64_t V, int32_t E, int32_t dtype,
@@ -712,7 +712,7 @@ int tt_catalog_logprobs_bwd_workspace_bytes(int64_t N, int64_t V, int32_t E, int
                                             int64_t* bytes);
 int tt_catalog_logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
                             int64_t N, int64_t V, int32_t E, const int64_t* ids,
-                            const float* bias, float temperature, const float* lse,
+                            const float* bias, float temperature, const double* lse,
                             const float* entropy, const float* g_log_prob,
                             const float* g_entropy, void* dx, void* dw, void* workspace,
                             int64_t workspace_bytes, void* stream);

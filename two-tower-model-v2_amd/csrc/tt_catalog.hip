@@ -264,7 +264,10 @@ struct LogitArgs {
   float4* part;        // STAT [splits, N] (m, L, T, -)
   float* tmax;         // STAT: [N, 4 ceil(V / 64)] or null
   float* wsq;          // STAT with tmax: [blocks] what no |w_v|^2 that the block looked at exceeds
-  const float4* rowc;  // COEF [N] (log2-domain lse, g, e, H); g and e both 0: the row is dead
+  // COEF [N] (lse in powers of two, rounded; g, e with what its rounding takes out of p put back; H so too);
+  // g and e both 0: the row is dead
+  const float4* rowc;
+  const float* rowg;   // COEF [N] g itself: the given item's
   const int64_t* ids;  // COEF
   void* C;             // COEF [Npad, ldc]: items v_base .. of this chunk
   int64_t ldc;
@@ -315,6 +318,10 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
   float m[FI], L[FI], TT[FI];
   float4 rc[FI];
   int id[FI];
+  // (g itself for the given item; in the 256 tile, whose bf16 coefficients k_lost corrects, there are no
+  // registers for it)
+  constexpr bool OWN_G = NB < 8;
+  float go[FI];
   // the items' norms (with tmax): a tile's by the block of the row tile that its number falls to, the
   // blocks of 16 items shared out among the waves that hold them.  A lane has a quarter of an item's
   // elements; the largest quarters of any items, added at the end, exceed no norm by much.  (1 x 1M x
@@ -333,6 +340,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
       rc[i] = n < a.N ? a.rowc[n] : float4{1.0e30f, 0.f, 0.f, 0.f};
       const int64_t q = n < a.N && a.ids ? a.ids[n] : -1;
       id[i] = q >= 0 && q < a.V ? (int)q : -1;
+      if constexpr (OWN_G) go[i] = n < a.N ? a.rowg[n] : 0.0f;
     }
   }
   // loads run one stage ahead over (tile, k) as one sequence
@@ -475,7 +483,7 @@ __global__ __launch_bounds__(Tile<NB>::NT, Tile<NB>::PER_EU) void k_logits(const
               const float lp = fmaf(z[j][r], s2, -rc[i].x);  // log2 p
               const float p = __builtin_amdgcn_exp2f(lp);
               const float k = ENT ? fmaf(rc[i].z, fmaf(lp, CT_LN2, rc[i].w), rc[i].y) : rc[i].y;
-              const float q = fmaf(-p, k, id[i] == v0 + 16 * j + 4 * g + r ? rc[i].y : 0.0f);
+              const float q = fmaf(-p, k, id[i] == v0 + 16 * j + 4 * g + r ? (OWN_G ? go[i] : rc[i].y) : 0.0f);
               c[j][r] = live && !(sel && z[j][r] == CT_OUT) ? q : 0.0f;
             }
           if constexpr (sizeof(T) == 4) {
@@ -932,7 +940,8 @@ struct CombineArgs {
   double s;
   float s2;   // log2(e) s, as the statistics' kernel has it
   int group;  // items of a wave there: a group that ends past V has its logits rounded on their own
-  float *logp, *ent, *lse;
+  float *logp, *ent;
+  double* lse;
   const float* wsq;  // with alternatives: [n_wsq] of the statistics' blocks
   int n_wsq;
   float* err;        // [N] logit_error
@@ -958,7 +967,7 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   const int64_t* ids = a.ids;
   const float* bias = a.bias;
   const double s = a.s;
-  float *logp = a.logp, *ent = a.ent, *lse = a.lse;
+  float *logp = a.logp, *ent = a.ent;
   float m = CT_NONE, L = 0.0f, TT = 0.0f;
   const int64_t id = logp ? ids[n] : -1;
   const bool has = id >= 0 && id < V;
@@ -1011,7 +1020,7 @@ __device__ __forceinline__ void combine_row(const CombineArgs& a, int64_t n, int
   if (lane == 0) {
     const float h = (float)((l2 - T2 / L2) * 0.6931471805599453);
     if (ent) ent[n] = empty || h < 0.0f ? 0.0f : h;
-    lse[n] = empty ? -inf : (float)ls;
+    a.lse[n] = empty ? -(double)inf : ls;
   }
 }
 template <typename T>
@@ -1477,19 +1486,26 @@ __global__ __launch_bounds__(256) void k_top_wide(const TopArgs a) {
 // more, for the second rows of C).
 template <typename T>
 __global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t ldx, int N, int E,
-                                              const float* __restrict__ lse, const float* __restrict__ ent,
+                                              const double* __restrict__ lse, const float* __restrict__ ent,
                                               const float* __restrict__ g, const float* __restrict__ e,
                                               const int64_t* __restrict__ ids, int V,
-                                              float4* __restrict__ rowc, T* __restrict__ xo, bool two) {
+                                              float4* __restrict__ rowc, float* __restrict__ rowg,
+                                              T* __restrict__ xo, bool two) {
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= N) return;
   const int64_t id = ids ? ids[n] : -1;
   const float gn = g && id >= 0 && id < V ? g[n] : 0.0f, en = e ? e[n] : 0.0f;
-  const bool live = (gn != 0.0f || en != 0.0f) && !(lse[n] == -__builtin_huge_valf());
-  if (lane == 0)
-    rowc[n] = live ? float4{(float)((double)lse[n] * 1.4426950408889634), gn, en, ent ? ent[n] : 0.0f}
+  const bool live = (gn != 0.0f || en != 0.0f) && !(lse[n] == -__builtin_huge_val());
+  if (lane == 0) {
+    // a coefficient is g [v = id] - p k: with lse rounded to 32 bits p would be off by up to 2^-25 |lse| of
+    // itself, which next to 1 is most of 1 - p.  What is lost of it goes into the factors.
+    const double z = lse[n] * 1.4426950408889634, lo = z - (double)(float)z, f = exp2(-lo);
+    rowc[n] = live ? float4{(float)z, (float)((double)gn * f), (float)((double)en * f),
+                            (float)((ent ? (double)ent[n] : 0.0) - lo * 0.6931471805599453)}
                    : float4{1.0e30f, 0.f, 0.f, 0.f};
+    rowg[n] = live ? gn : 0.0f;
+  }
   constexpr int PC = 16 / (int)sizeof(T);
   for (int c = lane * PC; c < E; c += 64 * PC)
   {
@@ -1528,7 +1544,7 @@ __global__ __launch_bounds__(256) void k_lost(const LogitArgs a, float* __restri
                                           (const uint16_t*)a.w + id * a.ldw, a.E, lane);
     const float lp = a.bias ? fmaf(z, a.s2, b * CT_LOG2E) - rc.x : fmaf(z, a.s2, -rc.x);
     const float k = rc.z != 0.0f ? fmaf(rc.z, fmaf(lp, CT_LN2, rc.w), rc.y) : rc.y;
-    const float c = fmaf(-__builtin_amdgcn_exp2f(lp), k, rc.y);
+    const float c = fmaf(-__builtin_amdgcn_exp2f(lp), k, a.rowg[n]);
     d = c - __uint_as_float((uint32_t)((const uint16_t*)a.C)[(int64_t)n * a.ldc + (id - a.v_base)] << 16);
   }
   if (lane == 0) delta[n] = d;
@@ -1905,7 +1921,7 @@ static ProductPlan product_plan(int64_t M, int64_t cols, int64_t K, int64_t sz, 
   return b;
 }
 struct BwdPlan {
-  int64_t Npad, Vc, n_chunks, off_x, off_d, off_w, off_c, off_px, off_pw, bytes;
+  int64_t Npad, Vc, n_chunks, off_g, off_x, off_d, off_w, off_c, off_px, off_pw, bytes;
   bool two;  // C in two bf16 rows a row
   ProductPlan px, pw, pw_last;  // dx; dw of a chunk, of the last chunk
 };
@@ -1920,6 +1936,8 @@ static BwdPlan bwd_plan(int64_t N, int64_t V, int64_t E, int64_t sz, bool bias, 
   p.Vc = up(cdiv(V, cdiv(V, vc)), CT_TILE);  // chunks of like size
   p.n_chunks = cdiv(V, p.Vc);
   int64_t o = up(N * 16, 256);
+  p.off_g = o;
+  o += up(N * 4, 256);
   p.off_x = o;
   o += up((p.two ? 2 * N : N) * E * sz, 256);
   p.off_d = o;
@@ -2005,7 +2023,7 @@ static int ct_check(const void* x, int64_t ldx, const void* w, int64_t ldw, int3
 template <typename T>
 static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int E,
                         const int64_t* ids, const float* bias, float temperature, float* logp, float* ent,
-                        float* lse, int top, int64_t* top_ids, float* top_lp, char* ws, const StatPlan& p,
+                        double* lse, int top, int64_t* top_ids, float* top_lp, char* ws, const StatPlan& p,
                         hipStream_t st) {
   const double s = 1.0 / (double)temperature;
   LogitArgs a{};
@@ -2060,15 +2078,16 @@ static int logprobs_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
 
 template <typename T>
 static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t N, int64_t V, int E,
-                        const int64_t* ids, const float* bias, float temperature, const float* lse,
+                        const int64_t* ids, const float* bias, float temperature, const double* lse,
                         const float* ent, const float* g, const float* e, void* dx, void* dw, char* ws,
                         const BwdPlan& p, hipStream_t st) {
   const double s = 1.0 / (double)temperature;
   float4* rowc = (float4*)ws;
+  float* rowg = (float*)(ws + p.off_g);
   T* xz = (T*)(ws + p.off_x);
   float* delta = sizeof(T) == 2 && !p.two && ids && g ? (float*)(ws + p.off_d) : nullptr;
   hipLaunchKernelGGL(k_rows<T>, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, st, (const T*)x, ldx, (int)N, E, lse,
-                     ent, g, e, ids, (int)V, rowc, xz, p.two);
+                     ent, g, e, ids, (int)V, rowc, rowg, xz, p.two);
   const T* wz = (const T*)w;
   int64_t ldwz = ldw;
   if (bias) {
@@ -2087,7 +2106,7 @@ static int logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, 
     a.x = xz; a.w = wz; a.ldx = E; a.ldw = ldwz; a.bias = bias;
     a.s2 = (float)(s * 1.4426950408889634);
     a.N = (int)N; a.V = (int)V; a.E = E;
-    a.rowc = rowc; a.ids = ids; a.C = C; a.ldc = p.Vc; a.v_base = (int)vb; a.Npad = (int)p.Npad;
+    a.rowc = rowc; a.rowg = rowg; a.ids = ids; a.C = C; a.ldc = p.Vc; a.v_base = (int)vb; a.Npad = (int)p.Npad;
     a.v_count = (int)vn;
     a.two = p.two;
     if (ring_ok(N, vn, E, sizeof(T))) {
@@ -2154,7 +2173,7 @@ extern "C" int tt_catalog_logprobs_workspace_bytes(int64_t N, int64_t V, int32_t
 
 extern "C" int tt_catalog_logprobs(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
                                    int64_t N, int64_t V, int32_t E, const int64_t* ids, const float* bias,
-                                   float temperature, float* log_prob, float* entropy, float* lse, int32_t top,
+                                   float temperature, float* log_prob, float* entropy, double* lse, int32_t top,
                                    int64_t* top_ids, float* top_log_prob, void* workspace,
                                    int64_t workspace_bytes, void* stream) {
   if (int rc = ct_check(x, ldx, w, ldw, dtype, N, V, E, temperature, __func__)) return rc;
@@ -2181,7 +2200,7 @@ extern "C" int tt_catalog_logprobs_bwd_workspace_bytes(int64_t N, int64_t V, int
 
 extern "C" int tt_catalog_logprobs_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype,
                                        int64_t N, int64_t V, int32_t E, const int64_t* ids, const float* bias,
-                                       float temperature, const float* lse, const float* entropy,
+                                       float temperature, const double* lse, const float* entropy,
                                        const float* g_log_prob, const float* g_entropy, void* dx, void* dw,
                                        void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = ct_check(x, ldx, w, ldw, dtype, N, V, E, temperature, __func__)) return rc;

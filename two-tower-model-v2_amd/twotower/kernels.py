@@ -806,7 +806,7 @@ def _catalog_bwd_ws_bytes(n, v, e, dt, bias, need_x, need_w):
 def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entropy: bool = False,
                      top: int = 0, checked: int = None):
     """tt_catalog_logprobs on catalog_rows' x [N, E] and w [V, E] -> (log_prob [N] f32 or None
-    without ids, entropy [N] f32 or None, lse [N] f32, top_ids [N, top] int64 and top_log_prob
+    without ids, entropy [N] f32 or None, lse [N] f64, top_ids [N, top] int64 and top_log_prob
     [N, top] f32 or None).  ``checked``: what catalog_check said of these arguments."""
     dt = catalog_check(x, w, ids, bias) if checked is None else checked
     n, e = x.shape
@@ -822,7 +822,7 @@ def catalog_logprobs(x, w, ids=None, bias=None, temperature: float = 0.07, entro
         dev = x.device
         lp = torch.empty(n, dtype=_f32, device=dev) if ids is not None else None
         ent = torch.empty(n, dtype=_f32, device=dev) if entropy else None
-        lse = torch.empty(n, dtype=_f32, device=dev)
+        lse = torch.empty(n, dtype=torch.float64, device=dev)
         ti = torch.empty((n, top), dtype=torch.int64, device=dev) if top else None
         tl = torch.empty((n, top), dtype=_f32, device=dev) if top else None
         part = n
@@ -848,9 +848,10 @@ def catalog_logprobs_backward(x, w, ids, bias, temperature, lse, ent, g, ge, nee
     dt = catalog_check(x, w, ids, bias) if checked is None else checked
     n, e = x.shape
     v = w.shape[0]
-    for t, name in ((g, "g"), (ge, "ge"), (lse, "lse"), (ent, "entropy")):
-        if t is not None and (t.shape != (n,) or t.dtype is not _f32):
-            raise ValueError(f"catalog_logprobs_backward: {name} must be float32 [{n}]")
+    for t, name, want in ((g, "g", _f32), (ge, "ge", _f32), (lse, "lse", torch.float64),
+                          (ent, "entropy", _f32)):
+        if t is not None and (t.shape != (n,) or t.dtype is not want):
+            raise ValueError(f"catalog_logprobs_backward: {name} must be {want} [{n}]")
     _same_device(x, ((g, "g"), (ge, "ge"), (lse, "lse"), (ent, "entropy")),
                  "catalog_logprobs_backward")
     if lse is None or (ge is not None and ent is None) or (g is not None and ids is None):
