@@ -1048,7 +1048,7 @@ __device__ __forceinline__ int wave_select(const uint64_t (&key)[PER], int keep,
       for (int r = 0; r < PER; ++r) c += __popcll(__ballot((uint32_t)(key[r] >> 32) >= cand));
       if (c >= keep) x = cand;
     }
-  int gt = 0, eq = 0;
+    int gt = 0, eq = 0;
 #pragma unroll
     for (int r = 0; r < PER; ++r) {
       gt += __popcll(__ballot((uint32_t)(key[r] >> 32) > x));

@@ -130,7 +130,9 @@ def catalog_log_probs(queries: torch.Tensor, items: torch.Tensor, ids: torch.Ten
     ``bias`` [V] f32: e.g. -log q of a sampled-softmax correction; -inf takes the item out (its
     vector may hold anything).  A row with nothing left: log_prob -inf, entropy 0.  Differentiable in
     queries and items (log_prob and entropy); the logits are never stored, so N x V is bounded by
-    time alone (with ``top`` a float per 16 of them is, for as many rows at a time as 4 GB hold).  E is padded to a multiple of 64 (a copy) where it is not one."""
+    time alone (with ``top`` a float per 16 of them is, for as many rows at a time as 4 GB hold).  E
+    is padded to a multiple of 64 where it is not one: a copy of the items in every call, which a
+    caller saves by keeping them padded with zeros."""
     if (isinstance(temperature, torch.Tensor) and temperature.requires_grad
             and torch.is_grad_enabled()):
         raise NotImplementedError("gradients w.r.t. the temperature are not computed: pass a number "
